@@ -41,8 +41,27 @@ pub struct MoearcAttnBlock {
     pub corr_hi: c_float,
 }
 
+/// `moearc_moe` (include/moearc_attn.h): one block's experts.
+#[repr(C)]
+pub struct MoearcMoe {
+    pub w_type: [c_uint; 3],
+    pub w: [*const c_void; 3],
+    pub bias: [*const c_float; 3],
+    pub n_expert: c_ulong,
+    pub n_embd: c_ulong,
+    pub n_ff: c_ulong,
+    pub act: c_uint,
+    pub alpha: c_float,
+    pub limit: c_float,
+}
+
 pub const MOEARC_OUT_F32: c_uint = 0;
 pub const MOEARC_OUT_F16: c_uint = 1;
+pub const MOEARC_ROUTE_SOFTMAX_ALL: c_uint = 0;
+pub const MOEARC_ROUTE_SOFTMAX_SELECTED: c_uint = 1;
+pub const MOEARC_NO_EXPERT: c_uint = 0xFFFF_FFFF;
+pub const MOEARC_ACT_SWIGLU: c_uint = 0;
+pub const MOEARC_ACT_SWIGLU_CLAMPED: c_uint = 1;
 
 unsafe extern "C" {
     // ---- the reference's entry points (ffi.rs:20-51, :97-103, :167-173, :188-252) ----------
@@ -301,6 +320,77 @@ unsafe extern "C" {
         attn: *const c_float,
         n_rows: c_ulong,
         n_cols: c_ulong,
+    ) -> c_int;
+    #[allow(clippy::too_many_arguments)]
+    pub fn moearc_norm_residual(
+        c: *mut MoearcCtx,
+        x: *mut c_void,
+        x_type: c_uint,
+        h: *mut c_float,
+        y: *const c_void,
+        y_type: c_uint,
+        w_post: *const c_float,
+        gate: *const c_float,
+        gate_stride: c_ulong,
+        scale: c_float,
+        w_pre: *const c_float,
+        n_rows: c_ulong,
+        n_cols: c_ulong,
+        eps: c_float,
+    ) -> c_int;
+    #[allow(clippy::too_many_arguments)]
+    pub fn moearc_moe_route(
+        c: *mut MoearcCtx,
+        ids: *mut c_uint,
+        weights: *mut c_float,
+        logits: *const c_float,
+        n_tok: c_ulong,
+        n_expert: c_ulong,
+        n_used: c_ulong,
+        mode: c_uint,
+        scale: c_float,
+    ) -> c_int;
+    pub fn moearc_moe_workspace(
+        n_tok: c_ulong,
+        n_used: c_ulong,
+        n_expert: c_ulong,
+        n_embd: c_ulong,
+        n_ff: c_ulong,
+        bytes: *mut c_ulong,
+    ) -> c_int;
+    #[allow(clippy::too_many_arguments)]
+    pub fn moearc_matmul_experts(
+        c: *mut MoearcCtx,
+        type_id: c_uint,
+        y: *mut c_void,
+        w: *const c_void,
+        x: *const c_void,
+        io_type: c_uint,
+        bias: *const c_float,
+        ids: *const c_uint,
+        n_tok: c_ulong,
+        n_used: c_ulong,
+        n_expert: c_ulong,
+        x_per_slot: c_uint,
+        n_rows: c_ulong,
+        n_cols: c_ulong,
+        ws: *mut c_void,
+        ws_bytes: c_ulong,
+    ) -> c_int;
+    #[allow(clippy::too_many_arguments)]
+    pub fn moearc_moe_ffn(
+        c: *mut MoearcCtx,
+        m: *const MoearcMoe,
+        y: *mut c_void,
+        x: *const c_void,
+        io_type: c_uint,
+        ids: *const c_uint,
+        weights: *const c_float,
+        n_tok: c_ulong,
+        n_used: c_ulong,
+        accumulate: c_uint,
+        ws: *mut c_void,
+        ws_bytes: c_ulong,
     ) -> c_int;
     pub fn moearc_ctx_stream(c: *mut MoearcCtx) -> *mut c_void;
 }

@@ -333,6 +333,91 @@ int moearc_attn_block_chunk(moearc_ctx *c, const moearc_attn_block *b, float *h,
 int moearc_attn_out(moearc_ctx *c, unsigned int type_id, float *h, const void *w, const float *bias,
                     const float *attn, unsigned long n_rows, unsigned long n_cols);
 
+/* ---- the expert half of a block ------------------------------------------------------------------
+ * Extensions (the reference runs moearc_rmsnorm, moearc_topk_router, one matvec per expert, the
+ * activations and moearc_moe_combine one token at a time, kernels.cpp:1146-1639): the residual update
+ * with its norms, the router's choice, and the chosen experts' products, for one token or a chunk.
+ * A chunk's block is moearc_attn_block_chunk, moearc_norm_residual, the router's logits (a product
+ * of the entry points above), moearc_moe_route and moearc_moe_ffn. */
+
+/* For each row: z = y, or with w_post y / sqrt(mean(y^2) + eps) * w_post; h += scale * gate * z; and, with
+ * x, x = h / sqrt(mean(h^2) + eps) * w_pre. h f32 [n_rows][n_cols]; y and x f32 or f16 by y_type and x_type
+ * (MOEARC_OUT_F32 / _F16), the same shape; w_post, w_pre [n_cols], each may be NULL (a factor of one; no w_post: y is
+ * not normed); gate: row r's factors at gate + r * gate_stride (0: one row for all), NULL: none. Without y, h
+ * is only read: the plain RMSNorm, of a chunk's rows or of its heads' (n_rows = tokens * heads). Without x, the
+ * residual update alone. x may be y itself when their types are equal; no other buffers may overlap.
+ * Refusals: null c or h, or neither x nor y -> -1; a type not 0/1, w_post or gate without y, w_pre without x,
+ * n_cols 0 or >= 2^30, n_rows >= 2^31, a gate_stride between 1 and n_cols - 1, eps negative or NaN -> -2. No rows -> 0. */
+int moearc_norm_residual(moearc_ctx *c, void *x, unsigned int x_type, float *h, const void *y, unsigned int y_type,
+                         const float *w_post, const float *gate, unsigned long gate_stride, float scale,
+                         const float *w_pre, unsigned long n_rows, unsigned long n_cols, float eps);
+
+/* How moearc_moe_route weighs the chosen experts. */
+#define MOEARC_ROUTE_SOFTMAX_ALL 0u      /* softmax over all of the token's logits */
+#define MOEARC_ROUTE_SOFTMAX_SELECTED 1u /* softmax over the chosen ones (the same as renormalising the former) */
+
+/* For each token the n_used largest of its n_expert logits, largest first, equal ones (-0 and +0 too) by
+ * ascending expert: ids u32 [n_tok][n_used] and their softmax weights times scale, f32 [n_tok][n_used].
+ * logits f32 [n_tok][n_expert]. A logit of -inf masks its expert: it is chosen after all others and weighs 0;
+ * NaN counts as -inf and comes last. A token whose experts are all masked gets ids and weights of 0.
+ * Refusals: a null pointer -> -1; n_expert 0 or above 1024, n_used 0 or above n_expert, another mode,
+ * n_tok >= 2^31 -> -2. No tokens -> 0. */
+int moearc_moe_route(moearc_ctx *c, unsigned int *ids, float *weights, const float *logits, unsigned long n_tok,
+                     unsigned long n_expert, unsigned long n_used, unsigned int mode, float scale);
+
+/* An id that chooses no expert (a padded token, an expert held elsewhere): its slot is skipped. */
+#define MOEARC_NO_EXPERT 0xFFFFFFFFu
+
+/* *bytes = the working memory that moearc_moe_ffn takes at these sizes, and moearc_matmul_experts at n_embd =
+ * its n_cols and n_ff = 0; never less for more tokens. Null bytes -> -1; sizes that they refuse -> -2. */
+int moearc_moe_workspace(unsigned long n_tok, unsigned long n_used, unsigned long n_expert, unsigned long n_embd,
+                         unsigned long n_ff, unsigned long *bytes);
+
+/* Products grouped by expert: y[t][j] = W[ids[t][j]] x[t] (+ bias[ids[t][j]]), with x_per_slot x[t][j] in
+ * place of x[t]; j < n_used. w: the experts' matrices of one GGUF type (F16, Q8_0, Q4_K, Q5_K, Q6_K, MXFP4) one after
+ * another, [n_expert][n_rows][n_cols]; bias f32 [n_expert][n_rows] or NULL; ids u32 [n_tok][n_used] (device;
+ * experts may repeat within a token); x and y f32 or f16 by io_type, y [n_tok][n_used][n_rows]. y must not
+ * overlap x. Each expert's weights are read once for all of its slots, whatever their number.
+ * f32 activations enter as f16 hi + lo (to 2^-22 relative; each |x| below 65504), block sums are scaled in
+ * f32: the bound of moearc_matmul_q; f16 ones as they are, and y is rounded once. The result of a slot does not
+ * change from call to call with the same arguments.
+ * A slot of MOEARC_NO_EXPERT gets a row of zeros; another id >= n_expert too, and the next moearc_sync returns -1.
+ * ws: ws_bytes of 256-byte aligned device memory (moearc_moe_workspace), used until the call's work is done; NULL:
+ * the context's, grown on demand. A captured call needs ws (else -1), and graphs that may run at the same time
+ * need one each. Refusals: a null pointer other than bias and ws -> -1; io_type or x_per_slot not 0/1, n_expert or
+ * n_used 0 or above 1024, another type, n_rows 0 or above 2^20, n_cols below 256, above 2^20, not a multiple of 32 or
+ * of the block, an odd W address, a ws too small or misaligned -> -2. No tokens -> 0. */
+int moearc_matmul_experts(moearc_ctx *c, unsigned int type_id, void *y, const void *w, const void *x, unsigned int io_type,
+                          const float *bias, const unsigned int *ids, unsigned long n_tok, unsigned long n_used,
+                          unsigned long n_expert, unsigned int x_per_slot, unsigned long n_rows, unsigned long n_cols,
+                          void *ws, unsigned long ws_bytes);
+
+#define MOEARC_ACT_SWIGLU 0u         /* g sigmoid(g) u */
+#define MOEARC_ACT_SWIGLU_CLAMPED 1u /* g' sigmoid(alpha g') (u' + 1), g' = min(g, limit), u' = u within +-limit */
+
+/* The experts of one block. */
+typedef struct moearc_moe {
+    unsigned int w_type[3];      /* GGUF type ids of W_gate, W_up (the same) and W_down */
+    const void *w[3];            /* W_gate, W_up [n_expert][n_ff][n_embd], W_down [n_expert][n_embd][n_ff] */
+    const float *bias[3];        /* [n_expert][n_ff] twice, [n_expert][n_embd]; each may be NULL */
+    unsigned long n_expert, n_embd, n_ff;
+    unsigned int act;            /* MOEARC_ACT_* */
+    float alpha, limit;          /* of MOEARC_ACT_SWIGLU_CLAMPED */
+} moearc_moe;
+
+/* y[t] = sum over j of weights[t][j] (W_down[e] act(W_gate[e] x[t] + b_gate[e], W_up[e] x[t] + b_up[e]) + b_down[e]),
+ * e = ids[t][j], in the order of j; accumulate: y[t] += it (the residual stream; f32 only). x and y
+ * [n_tok][n_embd], f32 or f16 by io_type, and must not overlap; ids and weights as moearc_moe_route writes them;
+ * all device memory except m. Precision as moearc_matmul_experts, twice in a row: with f32 the values between the two
+ * products stay f32 (as f16 hi + lo: each |act| below 65504), with f16 they are rounded to f16 once. Slots without an
+ * expert add nothing, and their weights are not read; ids out of range and ws as there. Calls of more than
+ * 32768 slots run in chunks of tokens, one after another.
+ * Refusals: a null pointer other than biases and ws -> -1; those of moearc_matmul_experts for each matrix, gate and
+ * up of different types, another act, a negative or NaN limit, accumulate not 0/1 or with f16 -> -2. No tokens -> 0. */
+int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, unsigned int io_type,
+                   const unsigned int *ids, const float *weights, unsigned long n_tok, unsigned long n_used,
+                   unsigned int accumulate, void *ws, unsigned long ws_bytes);
+
 /* The stream the context enqueues on (a hipStream_t), so a caller can order its own work. */
 void *moearc_ctx_stream(moearc_ctx *c);
 

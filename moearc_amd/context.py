@@ -91,6 +91,21 @@ class RopeScaling:
 RopeScaling.NONE = RopeScaling()
 
 
+class RouteMode(enum.IntEnum):
+    """How the router weighs the chosen experts (MOEARC_ROUTE_*)."""
+    SOFTMAX_ALL = 0
+    SOFTMAX_SELECTED = 1
+
+
+class MoeAct(enum.IntEnum):
+    """The experts' activation (MOEARC_ACT_*)."""
+    SWIGLU = 0
+    SWIGLU_CLAMPED = 1
+
+
+NO_EXPERT = 0xFFFFFFFF  # an id that chooses no expert
+
+
 class DeviceBuffer:
     """An owned device allocation (lib.rs ``DeviceBuffer``)."""
 
@@ -471,6 +486,100 @@ class Context:
         self.finish(self._lib.moearc_attn_qkv(self.raw, tarr, _ptr_array(outs), _ptr_array(ws),
                                               _ptr_array(biases), rarr, x.ptr, n_cols), "attn qkv")
 
+    # ---- the expert half of a block ---------------------------------------------------------
+    def norm_residual(self, x: Optional[DeviceBuffer], h: DeviceBuffer, y: Optional[DeviceBuffer],
+                      w_post: Optional[DeviceBuffer], gate: Optional[DeviceBuffer], gate_stride: int, scale: float,
+                      w_pre: Optional[DeviceBuffer], n_rows: int, n_cols: int, eps: float, x_type: int = OUT_F32,
+                      y_type: int = OUT_F32) -> None:
+        """h += scale * gate * (y or RMSNorm(y) * w_post), then x = RMSNorm(h) * w_pre, in one pass."""
+        n = n_rows * n_cols
+        h.require("residual", n * 4)
+        if x is not None:
+            x.require("normed output", n * (2 if x_type == OUT_F16 else 4))
+        if y is not None:
+            y.require("block output", n * (2 if y_type == OUT_F16 else 4))
+        for w, what in ((w_post, "post-norm weights"), (w_pre, "pre-norm weights")):
+            if w is not None:
+                w.require(what, n_cols * 4)
+        if gate is not None and n_rows:
+            gate.require("gate", ((n_rows - 1) * gate_stride + n_cols) * 4)
+        self.finish(self._lib.moearc_norm_residual(self.raw, _ptr(x), x_type, h.ptr, _ptr(y), y_type, _ptr(w_post),
+                                                   _ptr(gate), gate_stride, float(scale), _ptr(w_pre), n_rows, n_cols,
+                                                   float(eps)), "norm with residual")
+
+    def moe_route(self, ids: DeviceBuffer, weights: DeviceBuffer, logits: DeviceBuffer, n_tok: int, n_expert: int,
+                  n_used: int, mode: RouteMode = RouteMode.SOFTMAX_SELECTED, scale: float = 1.0) -> None:
+        """The n_used largest of each token's logits and their softmax weights times scale."""
+        logits.require("router logits", n_tok * n_expert * 4)
+        ids.require("expert ids", n_tok * n_used * 4)
+        weights.require("expert weights", n_tok * n_used * 4)
+        self.finish(self._lib.moearc_moe_route(self.raw, ids.ptr, weights.ptr, logits.ptr, n_tok, n_expert, n_used,
+                                               int(mode), float(scale)), "expert routing")
+
+    def moe_workspace(self, n_tok: int, n_used: int, n_expert: int, n_embd: int, n_ff: int = 0) -> int:
+        """Bytes of working memory of moe_ffn at these sizes (n_ff 0: of matmul_experts with n_embd columns)."""
+        n = ctypes.c_ulong()
+        _check(self._lib.moearc_moe_workspace(n_tok, n_used, n_expert, n_embd, n_ff, ctypes.byref(n)), "experts' workspace")
+        return n.value
+
+    def matmul_experts(self, ty, y: DeviceBuffer, w: DeviceBuffer, x: DeviceBuffer, bias: Optional[DeviceBuffer],
+                       ids: DeviceBuffer, n_tok: int, n_used: int, n_expert: int, n_rows: int, n_cols: int,
+                       io_type: int = OUT_F32, x_per_slot: bool = False,
+                       workspace: Optional[DeviceBuffer] = None) -> None:
+        """y[t][j] = W[ids[t][j]] x[t] (x[t][j] with x_per_slot) (+ bias), grouped by expert."""
+        ty = QuantType(ty)
+        elem = 2 if io_type == OUT_F16 else 4
+        if n_cols % ty.block_elems:
+            raise BadArgument(f"{ty.name}: {n_cols} columns is not a whole number of blocks")
+        w.require("weights", n_expert * n_rows * ty.row_bytes(n_cols))
+        x.require("activations", n_tok * (n_used if x_per_slot else 1) * n_cols * elem)
+        y.require("output", n_tok * n_used * n_rows * elem)
+        ids.require("expert ids", n_tok * n_used * 4)
+        if bias is not None:
+            bias.require("bias", n_expert * n_rows * 4)
+        self.finish(self._lib.moearc_matmul_experts(self.raw, int(ty), y.ptr, w.ptr, x.ptr, io_type, _ptr(bias), ids.ptr,
+                                                    n_tok, n_used, n_expert, int(x_per_slot), n_rows, n_cols,
+                                                    _ptr(workspace), workspace.len if workspace is not None else 0),
+                    f"experts' product {ty.name}")
+
+    def moe_ffn(self, desc: "MoeDesc", y: DeviceBuffer, x: DeviceBuffer, ids: DeviceBuffer, weights: DeviceBuffer,
+                n_tok: int, n_used: int, io_type: int = OUT_F32, accumulate: bool = False,
+                workspace: Optional[DeviceBuffer] = None) -> None:
+        """y (+)= sum_j weights[t][j] * expert ids[t][j] of x[t]: gate, up, activation and down."""
+        elem = 2 if io_type == OUT_F16 else 4
+        x.require("normed input", n_tok * desc.n_embd * elem)
+        y.require("output", n_tok * desc.n_embd * elem)
+        ids.require("expert ids", n_tok * n_used * 4)
+        weights.require("expert weights", n_tok * n_used * 4)
+        self.finish(self._lib.moearc_moe_ffn(self.raw, ctypes.byref(desc), y.ptr, x.ptr, io_type, ids.ptr, weights.ptr,
+                                             n_tok, n_used, int(accumulate), _ptr(workspace),
+                                             workspace.len if workspace is not None else 0), "experts")
+
+
+class MoeDesc(ctypes.Structure):
+    """``moearc_moe`` (include/moearc_attn.h): one block's experts."""
+    _fields_ = [("w_type", ctypes.c_uint * 3), ("w", ctypes.c_void_p * 3), ("bias", ctypes.c_void_p * 3),
+                ("n_expert", ctypes.c_ulong), ("n_embd", ctypes.c_ulong), ("n_ff", ctypes.c_ulong),
+                ("act", ctypes.c_uint), ("alpha", ctypes.c_float), ("limit", ctypes.c_float)]
+
+    @staticmethod
+    def make(types, ws, biases, n_expert: int, n_embd: int, n_ff: int, act: MoeAct = MoeAct.SWIGLU, alpha: float = 1.702,
+             limit: float = 7.0) -> "MoeDesc":
+        """Gate, up and down: their types, weights and biases (each may be None)."""
+        d = MoeDesc()
+        for i, (ty, w, b) in enumerate(zip(types, ws, biases)):
+            ty = QuantType(ty)
+            rows, cols = (n_ff, n_embd) if i < 2 else (n_embd, n_ff)
+            w.require("weights", n_expert * rows * ty.row_bytes(cols))
+            if b is not None:
+                b.require("bias", n_expert * rows * 4)
+            d.w_type[i], d.w[i], d.bias[i] = int(ty), w.ptr, _ptr(b)
+        d.n_expert, d.n_embd, d.n_ff = n_expert, n_embd, n_ff
+        d.act, d.alpha, d.limit = int(act), alpha, limit
+        # the descriptor holds raw device pointers: keep their buffers alive as long as it lives
+        d._buffers = [b for b in (*ws, *biases) if b is not None]
+        return d
+
 
 class AttnBlockDesc(ctypes.Structure):
     """``moearc_attn_block`` (include/moearc_attn.h): one block's attention weights, cache and RoPE."""
@@ -538,3 +647,7 @@ class DeviceView(DeviceBuffer):
 
 def _ptr_array(bufs) -> ctypes.Array:
     return (ctypes.c_void_p * len(bufs))(*[b.ptr if b is not None else None for b in bufs])
+
+
+def _ptr(buf: Optional[DeviceBuffer]) -> Optional[int]:
+    return buf.ptr if buf is not None else None

@@ -237,3 +237,81 @@ struct MatmulArgs {
                                // (matmul_small.hip: wave w, kb_per * w ..)
     uint32_t pad;
 };
+
+// ---- norms with the residual update (norm.hip) --------------------------------------------------
+// A row of up to 16 * threads columns stays in its threads' registers (16, 64, 256 or 1024 threads).
+#define MOEARC_NORM_PER_THREAD 16u
+struct NormArgs {
+    void *x;               // [n_rows][n_cols] f32 or f16, or null
+    float *h;              // [n_rows][n_cols], updated when y is given
+    const void *y;         // [n_rows][n_cols] f32 or f16, or null
+    const float *w_post;   // [n_cols] or null: y enters as it is
+    const float *gate;     // row r at gate + r * gate_stride, or null
+    const float *w_pre;    // [n_cols] or null
+    uint64_t gate_stride;
+    uint32_t n_rows, n_cols;
+    float scale, eps;
+    uint32_t x_f16, y_f16;
+};
+
+// ---- the router and the experts' products (moe.hip, moe_small.hip, moe_tile.hip) ------------------
+#define MOEARC_NO_EXPERT 0xFFFFFFFFu  // a slot without an expert (moearc_attn.h)
+#define MOEARC_MAX_EXPERTS 1024u
+#define MOEARC_ROUTE_LANES 16u        // lanes per token
+
+struct RouteArgs {
+    const float *logits;   // [n_tok][n_expert]
+    uint32_t *ids;         // [n_tok][n_used]
+    float *weights;        // [n_tok][n_used]
+    uint32_t n_tok, n_expert, n_used, over_all;
+    float scale;
+    uint32_t pad;
+};
+
+// A slot is a token's j-th expert, slot t * n_used + j. The plan groups the slots of a call by expert
+// in tiles of at most `tile` slots: tiles[i] = (expert, first place, count), list[place] = slot, each
+// expert's slots in their order. Slots without a valid expert form a last group, "expert" n_expert.
+struct MoeTile {
+    uint32_t expert, first, count, pad;
+};
+struct MoePlanArgs {
+    const uint32_t *ids;   // [n_slots]
+    MoeTile *tiles;
+    uint32_t *n_tiles;
+    uint32_t *list;        // [n_slots]
+    uint32_t *err;         // set to 1 when an id is neither an expert nor MOEARC_NO_EXPERT
+    uint32_t n_slots, n_expert, tile, pad;
+};
+
+// One grouped product: rows of the experts' matrices times their slots' inputs. With two matrices (gate
+// and up) the output is their activation, else the product itself.
+struct MoeArgs {
+    const uint32_t *ids;       // [n_slots], for launches without a plan (n_slots <= 64)
+    const MoeTile *tiles;      // the plan, or null
+    const uint32_t *n_tiles, *list;
+    const void *x, *x_lo;      // row of slot s: s / x_div; f32 or f16 (x_lo: the f16 halves' low half)
+    const uint8_t *w[2];       // expert e's matrix at w + e * expert_bytes
+    const float *bias[2];      // [n_expert][rows] or null
+    void *y, *y_lo;            // [n_slots][rows]
+    uint32_t *err;
+    uint64_t expert_bytes, row_bytes;
+    uint32_t n_slots, n_expert, x_div, rows, cols;
+    uint32_t kb_per;           // moe_small.hip: k-blocks per wave
+    uint32_t y_f16;
+    uint32_t zero_skipped;     // write zero rows for slots without an expert
+    uint32_t clamped;          // the activation: 0 silu(g) u, 1 min(g, limit) sigmoid(alpha g) (clamp(u) + 1)
+    float alpha, limit;
+    uint32_t pad;
+};
+
+// y[t] (+)= sum_j weights[t][j] part[t * n_used + j] over the slots that have an expert, in order
+struct MoeCombineArgs {
+    const float *part;         // [n_tok * n_used][cols]
+    const float *weights;
+    const uint32_t *ids;
+    void *y;                   // [n_tok][cols] f32 or f16
+    uint32_t n_tok, n_used, n_expert, cols, y_f16, accumulate;
+};
+#define MOEARC_MOE_SMALL_SLOTS 64u  // most slots of a launch without a plan
+#define MOEARC_MOE_SMALL_WAVES 8
+#define MOEARC_MOE_SMALL_TOKENS 16u

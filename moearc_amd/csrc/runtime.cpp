@@ -135,6 +135,11 @@ struct moearc_ctx {
     // alone that a captured 64-channel f16 call may hold
     float *ws_kinds = nullptr;
     size_t ws_kinds_floats = 0;
+    // norms (16, 64, 256, 1024 threads a row x scalar, four floats), router (16 << i experts), experts' products
+    hipFunction_t f_norm[4][2] = {}, f_norm_long = nullptr, f_route[7] = {}, f_moe_plan = nullptr, f_moe_combine[2] = {};
+    hipFunction_t f_moe_small[6][2][2] = {};  // F16 Q8_0 Q4_K Q5_K Q6_K MXFP4 x gate and up, one product x f32, f16
+    float *moe_ws = nullptr;  // the experts' products' working memory, eager calls only
+    size_t moe_ws_floats = 0;
     int decode_variant_override = -1;  // MOEARC_DECODE_VARIANT, e.g. "4x2x4"
     unsigned long split_override = 0;  // MOEARC_DECODE_SPLIT (keys per split)
     float *blk_ws = nullptr;  // attention-block chunk: q, k, v, f16 q, attention output, projection
@@ -152,6 +157,8 @@ struct moearc_ctx {
 };
 
 namespace {
+
+bool moe_load(moearc_ctx *c);  // runtime_moe.h
 
 hipEvent_t take_event(moearc_ctx *c) {
     if (!c->event_pool.empty()) {
@@ -659,7 +666,7 @@ moearc_ctx *release(moearc_ctx *c) {
     }
     for (auto e : c->event_pool) (void) hipEventDestroy(e);
     for (void *p : {(void *) c->ws, (void *) c->ws_kinds, (void *) c->pf_ws, (void *) c->blk_ws, (void *) c->mm_ws, (void *) c->mm_part,
-                    (void *) c->err_word})
+                    (void *) c->moe_ws, (void *) c->err_word})
         if (p) (void) hipFree(p);
     if (c->module) (void) hipModuleUnload(c->module);
     if (c->stream) (void) hipStreamDestroy(c->stream);
@@ -770,6 +777,7 @@ moearc_ctx *moearc_ctx_create(void) {
             return release(c);
         }
     }
+    if (!moe_load(c)) return release(c);
     for (hipFunction_t f : c->f_dec_merge) {
         int merge_threads = 0;
         if (hipFuncGetAttribute(&merge_threads, HIP_FUNC_ATTRIBUTE_MAX_THREADS_PER_BLOCK, f) != hipSuccess ||
@@ -2154,3 +2162,5 @@ int moearc_attn_block_chunk(moearc_ctx *c, const moearc_attn_block *b, float *h,
         jobs.push_back(MvJob{b->w[3], att + t * q_rows, b->bias[3], h + t * E, E, true});
     return mv_launch_all(c, b->w_type[3], jobs, q_rows, "attn_proj_chunk");
 }
+
+#include "runtime_moe.h"

@@ -1,0 +1,327 @@
+// The host side of the norms and of the experts' half of a block (norm.hip, moe*.hip): included at the
+// end of runtime.cpp, whose launch, workspace and profiling helpers it uses.
+#pragma once
+
+namespace {
+
+// Bytes of a chunk's working memory are bounded by cutting long calls into chunks of at most this many
+// slots: 32,768 slots of 2,880 columns hold 0.4 GB per f32 array, and give each of 128 experts 256 slots.
+constexpr unsigned long kMoeChunkSlots = 32768;
+
+constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+// The parts of a call's workspace, in order.
+struct MoeSpace {
+    size_t n_tiles = 0, tiles = 0, list = 0, act = 0, part = 0, bytes = 0;
+};
+
+uint64_t moe_max_tiles(uint64_t slots, uint64_t n_expert, uint64_t tile) {
+    return std::min<uint64_t>(slots, (slots + tile - 1) / tile + n_expert + 1);
+}
+
+// A call of n_tok tokens (one chunk of it) with n_used experts each: n_ff 0 for a product alone.
+MoeSpace moe_space(uint64_t n_tok, uint64_t n_used, uint64_t n_expert, uint64_t n_embd, uint64_t n_ff) {
+    const uint64_t tok = std::min<uint64_t>(n_tok, std::max<uint64_t>(1, kMoeChunkSlots / n_used)), slots = tok * n_used;
+    MoeSpace s;
+    s.tiles = 256;
+    s.list = s.tiles + align256(sizeof(MoeTile) * moe_max_tiles(slots, n_expert, MOEARC_MOE_SMALL_TOKENS));
+    s.act = s.list + align256(4 * slots);
+    s.part = s.act + align256(4 * slots * n_ff);
+    s.bytes = s.part + (n_ff ? align256(4 * slots * n_embd) : 0);
+    return s;
+}
+
+// The call's working memory: the caller's, or the context's, grown on demand. A captured call takes the
+// caller's only: the context's may move with a later call, and is shared by whatever else the context runs.
+int moe_take_space(moearc_ctx *c, size_t need, void *ws, unsigned long ws_bytes, uint8_t **out) {
+    if (ws) {
+        *out = (uint8_t *) ws;
+        return OK;  // the size and alignment were checked before anything was enqueued
+    }
+    if (capturing(c)) return ERR;
+    if (const int rc = ensure_floats(c, c->moe_ws, c->moe_ws_floats, (need + 3) / 4)) return rc;
+    *out = (uint8_t *) c->moe_ws;
+    return OK;
+}
+
+int moe_space_check(size_t need, const void *ws, unsigned long ws_bytes) {
+    return ws && (ws_bytes < need || (uintptr_t) ws % 256 != 0) ? ERR_ARG : OK;
+}
+
+constexpr unsigned kMoeTypes[6] = {1, 8, 12, 13, 14, 39};
+constexpr const char *kMoeNames[6] = {"f16", "q8_0", "q4_k", "q5_k", "q6_k", "mxfp4"};
+int moe_index(unsigned ty) {
+    for (int i = 0; i < 6; ++i)
+        if (kMoeTypes[i] == ty) return i;
+    return -1;
+}
+
+int moe_matrix_check(unsigned ty, const void *w, unsigned long n_rows, unsigned long n_cols) {
+    if (moe_index(ty) < 0 || n_cols < 256 || n_cols % 32 != 0 || n_cols % moearc_mv_be(ty) != 0 || n_cols > 0x100000ul ||
+        n_rows == 0 || n_rows > 0x100000ul || ((uintptr_t) w & 1u))
+        return ERR_ARG;
+    return OK;
+}
+
+int moe_count_check(unsigned long n_tok, unsigned long n_used, unsigned long n_expert, unsigned int io_type) {
+    if (io_type > MOEARC_OUT_F16 || n_expert == 0 || n_expert > MOEARC_MAX_EXPERTS || n_used == 0 ||
+        n_used > MOEARC_MAX_EXPERTS || n_tok >= 0x80000000ul)
+        return ERR_ARG;
+    return OK;
+}
+
+// Groups a chunk's slots by expert. Launches of at most 64 slots need no plan.
+int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slots, uint32_t n_expert, uint32_t tile,
+             uint8_t *ws, const MoeSpace &sp) {
+    a.ids = ids;
+    a.n_slots = n_slots;
+    a.n_expert = n_expert;
+    a.err = c->err_word;
+    c->err_armed = true;
+    if (n_slots <= MOEARC_MOE_SMALL_SLOTS) return OK;
+    MoePlanArgs p{};
+    p.ids = ids;
+    p.n_tiles = (uint32_t *) ws;
+    p.tiles = (MoeTile *) (ws + sp.tiles);
+    p.list = (uint32_t *) (ws + sp.list);
+    p.err = c->err_word;
+    p.n_slots = n_slots;
+    p.n_expert = n_expert;
+    p.tile = tile;
+    a.tiles = p.tiles;
+    a.n_tiles = p.n_tiles;
+    a.list = p.list;
+    return launch(c, c->f_moe_plan, n_expert + 1, 1024, p, nullptr, n_slots, n_expert, "moe_plan");
+}
+
+// One grouped product (two matrices: gate, up and their activation).
+int moe_product(moearc_ctx *c, MoeArgs a, unsigned ty, bool gate_up, bool x_f16) {
+    const uint64_t nb = a.cols / 32, gran = (ty == 12u || ty == 13u || ty == 14u) ? 8 : 1;
+    a.row_bytes = (uint64_t) a.cols / moearc_mv_be(ty) * moearc_mv_bb(ty);
+    a.expert_bytes = a.row_bytes * a.rows;
+    a.kb_per = (uint32_t) (((nb + MOEARC_MOE_SMALL_WAVES - 1) / MOEARC_MOE_SMALL_WAVES + gran - 1) / gran * gran);
+    const unsigned gx = (a.rows + (gate_up ? 15 : 31)) / (gate_up ? 16 : 32);
+    const unsigned gy = a.tiles ? (unsigned) moe_max_tiles(a.n_slots, a.n_expert, MOEARC_MOE_SMALL_TOKENS) : a.n_slots;
+    return launch2d(c, c->f_moe_small[moe_index(ty)][gate_up ? 0 : 1][x_f16 ? 1 : 0], gx, gy, 64 * MOEARC_MOE_SMALL_WAVES, a,
+                    nullptr, a.rows, a.n_slots, 0, gate_up ? "moe_gate_up" : "moe_product");
+}
+
+// Brackets a call of several launches under one key, as a single launch would be.
+struct MoeScope {
+    moearc_ctx *c;
+    const char *what;
+    unsigned long r, m;
+    hipEvent_t start = nullptr;
+    MoeScope(moearc_ctx *c, const char *what, unsigned long r, unsigned long m) : c(c), what(what), r(r), m(m) {
+        if (tracks(c, what) && (start = take_event(c)) && hipEventRecord(start, c->stream) != hipSuccess) {
+            c->event_pool.push_back(start);
+            start = nullptr;
+        }
+        ++c->scope_depth;
+    }
+    ~MoeScope() {
+        --c->scope_depth;
+        if (start) record_bracket(c, start, what, r, m);
+    }
+};
+
+bool moe_load(moearc_ctx *c) {
+    struct {
+        hipFunction_t *slot;
+        const char *name;
+    } fns[] = {
+        {&c->f_norm[0][0], "moearc_norm_r16_v1_k"},   {&c->f_norm[0][1], "moearc_norm_r16_v4_k"},
+        {&c->f_norm[1][0], "moearc_norm_r64_v1_k"},   {&c->f_norm[1][1], "moearc_norm_r64_v4_k"},
+        {&c->f_norm[2][0], "moearc_norm_r256_v1_k"},  {&c->f_norm[2][1], "moearc_norm_r256_v4_k"},
+        {&c->f_norm[3][0], "moearc_norm_r1024_v1_k"}, {&c->f_norm[3][1], "moearc_norm_r1024_v4_k"},
+        {&c->f_norm_long, "moearc_norm_long_k"},
+        {&c->f_route[0], "moearc_moe_route_p1_k"},    {&c->f_route[1], "moearc_moe_route_p2_k"},
+        {&c->f_route[2], "moearc_moe_route_p4_k"},    {&c->f_route[3], "moearc_moe_route_p8_k"},
+        {&c->f_route[4], "moearc_moe_route_p16_k"},   {&c->f_route[5], "moearc_moe_route_p32_k"},
+        {&c->f_route[6], "moearc_moe_route_p64_k"},   {&c->f_moe_plan, "moearc_moe_plan_k"},
+        {&c->f_moe_combine[0], "moearc_moe_combine_k"}, {&c->f_moe_combine[1], "moearc_moe_combine4_k"},
+    };
+    auto get = [&](hipFunction_t *slot, const char *name) {
+        if (hipModuleGetFunction(slot, c->module, name) == hipSuccess) return true;
+        std::fprintf(stderr, "moearc: code object lacks kernel %s\n", name);
+        return false;
+    };
+    for (auto &f : fns)
+        if (!get(f.slot, f.name)) return false;
+    for (int t = 0; t < 6; ++t)
+        for (int i = 0; i < 4; ++i) {
+            char name[64];
+            std::snprintf(name, sizeof(name), "moearc_moe_small_%s_%s_%s_k", kMoeNames[t], i & 2 ? "p" : "gu", i & 1 ? "f16" : "f32");
+            if (!get(&c->f_moe_small[t][i >> 1][i & 1], name)) return false;
+        }
+    return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+int moearc_norm_residual(moearc_ctx *c, void *x, unsigned int x_type, float *h, const void *y, unsigned int y_type,
+                         const float *w_post, const float *gate, unsigned long gate_stride, float scale,
+                         const float *w_pre, unsigned long n_rows, unsigned long n_cols, float eps) {
+    if (!c || !h || (!x && !y)) return ERR;
+    if (x_type > MOEARC_OUT_F16 || y_type > MOEARC_OUT_F16 || (!y && (w_post || gate)) || (!x && w_pre) || n_cols == 0 ||
+        n_cols >= 0x40000000ul || n_rows >= 0x80000000ul || (gate && gate_stride != 0 && gate_stride < n_cols) || !(eps >= 0.f))
+        return ERR_ARG;
+    if (n_rows == 0) return OK;
+    NormArgs a{};
+    a.x = x;
+    a.h = h;
+    a.y = y;
+    a.w_post = w_post;
+    a.gate = gate;
+    a.w_pre = w_pre;
+    a.gate_stride = gate_stride;
+    a.n_rows = (uint32_t) n_rows;
+    a.n_cols = (uint32_t) n_cols;
+    a.scale = scale;
+    a.eps = eps;
+    a.x_f16 = x_type == MOEARC_OUT_F16;
+    a.y_f16 = y_type == MOEARC_OUT_F16;
+    // four floats at a time where every row allows
+    const bool by4 = n_cols % 4 == 0 && gate_stride % 4 == 0 &&
+                     ((uintptr_t) h | (uintptr_t) w_post | (uintptr_t) gate | (uintptr_t) w_pre) % 16 == 0 &&
+                     (uintptr_t) x % (a.x_f16 ? 8 : 16) == 0 && (uintptr_t) y % (a.y_f16 ? 8 : 16) == 0;
+    const int i = n_cols <= 16 * MOEARC_NORM_PER_THREAD ? 0 : n_cols <= 64 * MOEARC_NORM_PER_THREAD ? 1
+                : n_cols <= 256 * MOEARC_NORM_PER_THREAD ? 2 : n_cols <= 1024 * MOEARC_NORM_PER_THREAD ? 3 : 4;
+    if (i == 4) return launch(c, c->f_norm_long, (unsigned) n_rows, 1024, a, "norm_residual", n_rows, n_cols);
+    const unsigned rows = i == 0 ? 16 : i == 1 ? 4 : 1;
+    return launch(c, c->f_norm[i][by4], (unsigned) ((n_rows + rows - 1) / rows), i == 3 ? 1024 : 256, a, "norm_residual", n_rows,
+                  n_cols);
+}
+
+int moearc_moe_route(moearc_ctx *c, unsigned int *ids, float *weights, const float *logits, unsigned long n_tok,
+                     unsigned long n_expert, unsigned long n_used, unsigned int mode, float scale) {
+    if (!c || !ids || !weights || !logits) return ERR;
+    if (n_expert == 0 || n_expert > MOEARC_MAX_EXPERTS || n_used == 0 || n_used > n_expert || n_tok >= 0x80000000ul ||
+        mode > MOEARC_ROUTE_SOFTMAX_SELECTED)
+        return ERR_ARG;
+    if (n_tok == 0) return OK;
+    const RouteArgs a{logits, ids, weights, (uint32_t) n_tok, (uint32_t) n_expert, (uint32_t) n_used,
+                      mode == MOEARC_ROUTE_SOFTMAX_ALL ? 1u : 0u, scale, 0u};
+    int i = 0;
+    while (((unsigned long) MOEARC_ROUTE_LANES << i) < n_expert) ++i;
+    // a wave of four tokens per work-group while those leave compute units idle, else four waves
+    const unsigned threads = n_tok <= 4096 ? 64 : 256, per = threads / MOEARC_ROUTE_LANES;
+    return launch(c, c->f_route[i], (unsigned) ((n_tok + per - 1) / per), threads, a, "moe_route", n_tok, n_expert);
+}
+
+int moearc_moe_workspace(unsigned long n_tok, unsigned long n_used, unsigned long n_expert, unsigned long n_embd,
+                         unsigned long n_ff, unsigned long *bytes) {
+    if (!bytes) return ERR;
+    if (moe_count_check(n_tok, n_used, n_expert, 0) || n_embd == 0 || n_embd > 0x100000ul || n_ff > 0x100000ul) return ERR_ARG;
+    *bytes = moe_space(n_tok, n_used, n_expert, n_embd, n_ff).bytes;
+    return OK;
+}
+
+int moearc_matmul_experts(moearc_ctx *c, unsigned int type_id, void *y, const void *w, const void *x, unsigned int io_type,
+                          const float *bias, const unsigned int *ids, unsigned long n_tok, unsigned long n_used,
+                          unsigned long n_expert, unsigned int x_per_slot, unsigned long n_rows, unsigned long n_cols,
+                          void *ws, unsigned long ws_bytes) {
+    if (!c || !y || !w || !x || !ids) return ERR;
+    if (const int rc = moe_count_check(n_tok, n_used, n_expert, io_type)) return rc;
+    if (const int rc = moe_matrix_check(type_id, w, n_rows, n_cols)) return rc;
+    if (x_per_slot > 1) return ERR_ARG;
+    const MoeSpace sp = moe_space(n_tok, n_used, n_expert, n_cols, 0);
+    if (const int rc = moe_space_check(sp.bytes, ws, ws_bytes)) return rc;
+    if (n_tok == 0) return OK;
+    uint8_t *mem;
+    if (const int rc = moe_take_space(c, sp.bytes, ws, ws_bytes, &mem)) return rc;
+    const unsigned long chunk = std::max<unsigned long>(1, kMoeChunkSlots / n_used);
+    const size_t elem = io_type == MOEARC_OUT_F16 ? 2 : 4;
+    const MoeScope scope(c, "matmul_experts", n_rows, n_tok * n_used);
+    for (unsigned long t = 0; t < n_tok; t += chunk) {
+        const unsigned long n = std::min(chunk, n_tok - t);
+        MoeArgs a{};
+        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) n_expert,
+                                    MOEARC_MOE_SMALL_TOKENS, mem, sp))
+            return rc;
+        a.x = (const uint8_t *) x + (x_per_slot ? t * n_used : t) * n_cols * elem;
+        a.x_div = x_per_slot ? 1u : (uint32_t) n_used;
+        a.w[0] = (const uint8_t *) w;
+        a.bias[0] = bias;
+        a.y = (uint8_t *) y + t * n_used * n_rows * elem;
+        a.y_f16 = io_type == MOEARC_OUT_F16;
+        a.zero_skipped = 1u;
+        a.rows = (uint32_t) n_rows;
+        a.cols = (uint32_t) n_cols;
+        if (const int rc = moe_product(c, a, type_id, false, io_type == MOEARC_OUT_F16)) return rc;
+    }
+    return OK;
+}
+
+int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, unsigned int io_type, const unsigned int *ids,
+                   const float *weights, unsigned long n_tok, unsigned long n_used, unsigned int accumulate, void *ws,
+                   unsigned long ws_bytes) {
+    if (!c || !m || !y || !x || !ids || !weights || !m->w[0] || !m->w[1] || !m->w[2]) return ERR;
+    if (const int rc = moe_count_check(n_tok, n_used, m->n_expert, io_type)) return rc;
+    if (m->w_type[0] != m->w_type[1] || m->act > MOEARC_ACT_SWIGLU_CLAMPED || accumulate > 1 ||
+        (accumulate && io_type != MOEARC_OUT_F32) || (m->act == MOEARC_ACT_SWIGLU_CLAMPED && !(m->limit >= 0.f)))
+        return ERR_ARG;
+    for (int i = 0; i < 3; ++i)
+        if (const int rc = moe_matrix_check(m->w_type[i], m->w[i], i < 2 ? m->n_ff : m->n_embd, i < 2 ? m->n_embd : m->n_ff))
+            return rc;
+    const MoeSpace sp = moe_space(n_tok, n_used, m->n_expert, m->n_embd, m->n_ff);
+    if (const int rc = moe_space_check(sp.bytes, ws, ws_bytes)) return rc;
+    if (n_tok == 0) return OK;
+    uint8_t *mem;
+    if (const int rc = moe_take_space(c, sp.bytes, ws, ws_bytes, &mem)) return rc;
+    const unsigned long chunk = std::max<unsigned long>(1, kMoeChunkSlots / n_used);
+    const bool half = io_type == MOEARC_OUT_F16;
+    const size_t elem = half ? 2 : 4;
+    const MoeScope scope(c, "moe_ffn", m->n_ff, n_tok * n_used);
+    for (unsigned long t = 0; t < n_tok; t += chunk) {
+        const unsigned long n = std::min(chunk, n_tok - t);
+        MoeArgs a{};
+        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) m->n_expert,
+                                    MOEARC_MOE_SMALL_TOKENS, mem, sp))
+            return rc;
+        MoeArgs g = a, d = a;
+        g.x = (const uint8_t *) x + t * m->n_embd * elem;
+        g.x_div = (uint32_t) n_used;
+        for (int i = 0; i < 2; ++i) {
+            g.w[i] = (const uint8_t *) m->w[i];
+            g.bias[i] = m->bias[i];
+        }
+        g.y = mem + sp.act;
+        g.y_f16 = half;
+        g.rows = (uint32_t) m->n_ff;
+        g.cols = (uint32_t) m->n_embd;
+        g.clamped = m->act == MOEARC_ACT_SWIGLU_CLAMPED;
+        g.alpha = m->alpha;
+        g.limit = m->limit;
+        if (const int rc = moe_product(c, g, m->w_type[0], true, half)) return rc;
+        d.x = mem + sp.act;
+        d.x_div = 1u;
+        d.w[0] = (const uint8_t *) m->w[2];
+        d.bias[0] = m->bias[2];
+        d.y = mem + sp.part;
+        d.rows = (uint32_t) m->n_embd;
+        d.cols = (uint32_t) m->n_ff;
+        if (const int rc = moe_product(c, d, m->w_type[2], false, half)) return rc;
+        MoeCombineArgs s{};
+        s.part = (const float *) (mem + sp.part);
+        s.weights = weights + t * n_used;
+        s.ids = ids + t * n_used;
+        s.y = (uint8_t *) y + t * m->n_embd * elem;
+        s.n_tok = (uint32_t) n;
+        s.n_used = (uint32_t) n_used;
+        s.n_expert = (uint32_t) m->n_expert;
+        s.cols = (uint32_t) m->n_embd;
+        s.y_f16 = half;
+        s.accumulate = accumulate;
+        const bool by4 = m->n_embd % 4 == 0;
+        const unsigned lanes = (unsigned) (by4 ? m->n_embd / 4 : m->n_embd);
+        if (const int rc = launch2d(c, c->f_moe_combine[by4], (lanes + 255) / 256, (unsigned) n, 256, s, nullptr, n, m->n_embd, 0,
+                                    "moe_combine"))
+            return rc;
+    }
+    return OK;
+}
+
+}  // extern "C"

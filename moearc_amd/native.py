@@ -69,6 +69,13 @@ SIGNATURES = {
                                                    _c_ulong, ctypes.c_float, ctypes.c_float,
                                                    ctypes.c_float, ctypes.c_float, ctypes.c_float,
                                                    ctypes.c_float, ctypes.c_int, _u32]),
+    "moearc_norm_residual": (ctypes.c_int, [_vp, _vp, _u32, _vp, _vp, _u32, _vp, _vp, _c_ulong, ctypes.c_float,
+                                            _vp, _c_ulong, _c_ulong, ctypes.c_float]),
+    "moearc_moe_route": (ctypes.c_int, [_vp, _vp, _vp, _vp, _c_ulong, _c_ulong, _c_ulong, _u32, ctypes.c_float]),
+    "moearc_moe_workspace": (ctypes.c_int, [_c_ulong, _c_ulong, _c_ulong, _c_ulong, _c_ulong, _vp]),
+    "moearc_matmul_experts": (ctypes.c_int, [_vp, _u32, _vp, _vp, _vp, _u32, _vp, _vp, _c_ulong, _c_ulong,
+                                             _c_ulong, _u32, _c_ulong, _c_ulong, _vp, _c_ulong]),
+    "moearc_moe_ffn": (ctypes.c_int, [_vp, _vp, _vp, _vp, _u32, _vp, _vp, _c_ulong, _c_ulong, _u32, _vp, _c_ulong]),
     # include/moearc_kv.h
     "moearc_kv_pool_create": (ctypes.c_int, [_u32, _u32, _u32, ctypes.POINTER(_vp)]),
     "moearc_kv_pool_destroy": (None, [_vp]),
