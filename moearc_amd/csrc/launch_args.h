@@ -301,7 +301,7 @@ struct MoeArgs {
     uint32_t zero_skipped;     // write zero rows for slots without an expert
     uint32_t clamped;          // the activation: 0 silu(g) u, 1 min(g, limit) sigmoid(alpha g) (clamp(u) + 1)
     float alpha, limit;
-    uint32_t pad;
+    uint32_t row_tiles;        // moe_tile.hip: row tiles per tile of slots
 };
 
 // y[t] (+)= sum_j weights[t][j] part[t * n_used + j] over the slots that have an expert, in order
@@ -315,3 +315,4 @@ struct MoeCombineArgs {
 #define MOEARC_MOE_SMALL_SLOTS 64u  // most slots of a launch without a plan
 #define MOEARC_MOE_SMALL_WAVES 8
 #define MOEARC_MOE_SMALL_TOKENS 16u
+#define MOEARC_MOE_TILE 64u         // most slots of a plan's tile

@@ -7,9 +7,9 @@
 // windows of its rows' bytes through registers and LDS (the next window in flight while the current one
 // is multiplied) and reads MFMA operands from there, as matmul_small.hip does: lane (q, n) holds
 // k 8q .. 8q + 7 of weight row n (B operand of v_mfma_f32_16x16x32_f16) and of token n (A operand).
-// Without a plan (at most 64 slots) each wave finds the expert's slots from the ids by ballots, in the
-// launch of a decode step that saves: grid y is the slot, and the work-groups of slots that are not
-// their expert's first leave at once.
+// The launch has at most 64 slots: each wave finds its expert's from the ids by ballots, which saves a
+// decode step a launch. Grid y is the slot; the work-groups of slots that are not their expert's first
+// leave at once.
 //
 // f32 activations enter as f16 hi + lo (x = hi + lo to 2^-22 |x|), f16 ones as they are; weight payloads
 // as exact f16 integers (E2M1 code points for MXFP4), each block's f32 sum scaled in f32.
@@ -53,26 +53,18 @@ __device__ __forceinline__ void moe_small_body(const MoeArgs &a) {
 
     // the expert and its slots
     uint32_t e, count;
-    if (a.tiles) {
-        if (blockIdx.y >= *a.n_tiles) return;
-        const MoeTile t = a.tiles[blockIdx.y];
-        e = __builtin_amdgcn_readfirstlane(t.expert);
-        count = __builtin_amdgcn_readfirstlane(t.count);
-        if (tid < count) slots[tid] = a.list[t.first + tid];
+    const uint32_t id = lane < a.n_slots ? a.ids[lane] : MOEARC_NO_EXPERT;
+    e = __builtin_amdgcn_readlane(id, blockIdx.y);
+    if (e >= a.n_expert) {
+        if (e != MOEARC_NO_EXPERT && blockIdx.x == 0u && tid == 0u) *(volatile uint32_t *) a.err = 1u;
+        e = a.n_expert;
+        count = 1u;
+        if (tid == 0u) slots[0] = blockIdx.y;
     } else {
-        const uint32_t id = lane < a.n_slots ? a.ids[lane] : MOEARC_NO_EXPERT;
-        e = __builtin_amdgcn_readlane(id, blockIdx.y);
-        if (e >= a.n_expert) {
-            if (e != MOEARC_NO_EXPERT && blockIdx.x == 0u && tid == 0u) *(volatile uint32_t *) a.err = 1u;
-            e = a.n_expert;
-            count = 1u;
-            if (tid == 0u) slots[0] = blockIdx.y;
-        } else {
-            const uint64_t mask = __ballot(id == e);
-            if (mask & ((1ull << blockIdx.y) - 1ull)) return;  // an earlier slot's work-groups have it
-            count = (uint32_t) __popcll(mask);
-            if (tid < 64u && id == e) slots[__popcll(mask & ((1ull << lane) - 1ull))] = lane;
-        }
+        const uint64_t mask = __ballot(id == e);
+        if (mask & ((1ull << blockIdx.y) - 1ull)) return;  // an earlier slot's work-groups have it
+        count = (uint32_t) __popcll(mask);
+        if (tid < 64u && id == e) slots[__popcll(mask & ((1ull << lane) - 1ull))] = lane;
     }
     const uint32_t rbase = (GU ? 16u : 32u) * blockIdx.x;
     if (e == a.n_expert) {  // no expert: no product

@@ -12,7 +12,8 @@ constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 // The parts of a call's workspace, in order.
 struct MoeSpace {
-    size_t n_tiles = 0, tiles = 0, list = 0, act = 0, part = 0, bytes = 0;
+    size_t tiles = 0, list = 0, split = 0, act = 0, part = 0, bytes = 0;
+    size_t split_n = 0, act_n = 0;  // elements of x and of the activations
 };
 
 uint64_t moe_max_tiles(uint64_t slots, uint64_t n_expert, uint64_t tile) {
@@ -24,16 +25,19 @@ MoeSpace moe_space(uint64_t n_tok, uint64_t n_used, uint64_t n_expert, uint64_t 
     const uint64_t tok = std::min<uint64_t>(n_tok, std::max<uint64_t>(1, kMoeChunkSlots / n_used)), slots = tok * n_used;
     MoeSpace s;
     s.tiles = 256;
-    s.list = s.tiles + align256(sizeof(MoeTile) * moe_max_tiles(slots, n_expert, MOEARC_MOE_SMALL_TOKENS));
-    s.act = s.list + align256(4 * slots);
-    s.part = s.act + align256(4 * slots * n_ff);
+    s.list = s.tiles + align256(sizeof(MoeTile) * moe_max_tiles(slots, n_expert, MOEARC_MOE_TILE));
+    s.split = s.list + align256(4 * slots);
+    s.split_n = (n_ff ? tok : slots) * n_embd;  // a product alone may have a row of x for each slot
+    s.act_n = slots * n_ff;
+    s.act = s.split + align256(4 * s.split_n);
+    s.part = s.act + align256(4 * s.act_n);
     s.bytes = s.part + (n_ff ? align256(4 * slots * n_embd) : 0);
     return s;
 }
 
 // The call's working memory: the caller's, or the context's, grown on demand. A captured call takes the
 // caller's only: the context's may move with a later call, and is shared by whatever else the context runs.
-int moe_take_space(moearc_ctx *c, size_t need, void *ws, unsigned long ws_bytes, uint8_t **out) {
+int moe_take_space(moearc_ctx *c, size_t need, void *ws, uint8_t **out) {
     if (ws) {
         *out = (uint8_t *) ws;
         return OK;  // the size and alignment were checked before anything was enqueued
@@ -71,8 +75,8 @@ int moe_count_check(unsigned long n_tok, unsigned long n_used, unsigned long n_e
 }
 
 // Groups a chunk's slots by expert. Launches of at most 64 slots need no plan.
-int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slots, uint32_t n_expert, uint32_t tile,
-             uint8_t *ws, const MoeSpace &sp) {
+int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slots, uint32_t n_expert, uint8_t *ws,
+             const MoeSpace &sp) {
     a.ids = ids;
     a.n_slots = n_slots;
     a.n_expert = n_expert;
@@ -87,23 +91,41 @@ int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slot
     p.err = c->err_word;
     p.n_slots = n_slots;
     p.n_expert = n_expert;
-    p.tile = tile;
+    p.tile = MOEARC_MOE_TILE;
     a.tiles = p.tiles;
     a.n_tiles = p.n_tiles;
     a.list = p.list;
     return launch(c, c->f_moe_plan, n_expert + 1, 1024, p, nullptr, n_slots, n_expert, "moe_plan");
 }
 
-// One grouped product (two matrices: gate, up and their activation).
-int moe_product(moearc_ctx *c, MoeArgs a, unsigned ty, bool gate_up, bool x_f16) {
-    const uint64_t nb = a.cols / 32, gran = (ty == 12u || ty == 13u || ty == 14u) ? 8 : 1;
+// x (n floats, a multiple of 32) as f16 hi + lo for the tiles' matrix cores.
+int moe_split(moearc_ctx *c, const float *x, size_t n, uint16_t *hi, uint16_t *lo) {
+    const bool by8 = (uintptr_t) x % 16 == 0;
+    struct {
+        const float *x;
+        uint16_t *hi, *lo;
+        uint64_t n;
+    } a{x, hi, lo, by8 ? n / 8 : n};
+    return launch(c, by8 ? c->f_split8 : c->f_split, (unsigned) std::min<size_t>((a.n + 255) / 256, 65536), 256, a, nullptr, n, 0,
+                  "split_f16");
+}
+
+// One grouped product (two matrices: gate, up and their activation). Without a plan x is as the caller's
+// (f32, or f16 with `half`), with one always f16.
+int moe_product(moearc_ctx *c, MoeArgs a, unsigned ty, bool gate_up, bool half) {
+    const int i = moe_index(ty), g = gate_up ? 0 : 1;
+    const char *const name = gate_up ? "moe_gate_up" : "moe_product";
     a.row_bytes = (uint64_t) a.cols / moearc_mv_be(ty) * moearc_mv_bb(ty);
     a.expert_bytes = a.row_bytes * a.rows;
+    if (a.tiles) {
+        a.row_tiles = (a.rows + (gate_up ? 127 : 255)) / (gate_up ? 128 : 256);
+        const unsigned grid = (unsigned) (a.row_tiles * moe_max_tiles(a.n_slots, a.n_expert, MOEARC_MOE_TILE));
+        return launch(c, c->f_moe_tile[i][g][half], grid, 256, a, nullptr, a.rows, a.n_slots, name);
+    }
+    const uint64_t nb = a.cols / 32, gran = (ty == 12u || ty == 13u || ty == 14u) ? 8 : 1;
     a.kb_per = (uint32_t) (((nb + MOEARC_MOE_SMALL_WAVES - 1) / MOEARC_MOE_SMALL_WAVES + gran - 1) / gran * gran);
-    const unsigned gx = (a.rows + (gate_up ? 15 : 31)) / (gate_up ? 16 : 32);
-    const unsigned gy = a.tiles ? (unsigned) moe_max_tiles(a.n_slots, a.n_expert, MOEARC_MOE_SMALL_TOKENS) : a.n_slots;
-    return launch2d(c, c->f_moe_small[moe_index(ty)][gate_up ? 0 : 1][x_f16 ? 1 : 0], gx, gy, 64 * MOEARC_MOE_SMALL_WAVES, a,
-                    nullptr, a.rows, a.n_slots, 0, gate_up ? "moe_gate_up" : "moe_product");
+    return launch2d(c, c->f_moe_small[i][g][half], (a.rows + (gate_up ? 15 : 31)) / (gate_up ? 16 : 32), a.n_slots,
+                    64 * MOEARC_MOE_SMALL_WAVES, a, nullptr, a.rows, a.n_slots, 0, name);
 }
 
 // Brackets a call of several launches under one key, as a single launch would be.
@@ -153,6 +175,8 @@ bool moe_load(moearc_ctx *c) {
             char name[64];
             std::snprintf(name, sizeof(name), "moearc_moe_small_%s_%s_%s_k", kMoeNames[t], i & 2 ? "p" : "gu", i & 1 ? "f16" : "f32");
             if (!get(&c->f_moe_small[t][i >> 1][i & 1], name)) return false;
+            std::snprintf(name, sizeof(name), "moearc_moe_tile_%s_%s_%s_k", kMoeNames[t], i & 2 ? "p" : "gu", i & 1 ? "f16" : "f32");
+            if (!get(&c->f_moe_tile[t][i >> 1][i & 1], name)) return false;
         }
     return true;
 }
@@ -231,26 +255,32 @@ int moearc_matmul_experts(moearc_ctx *c, unsigned int type_id, void *y, const vo
     if (const int rc = moe_space_check(sp.bytes, ws, ws_bytes)) return rc;
     if (n_tok == 0) return OK;
     uint8_t *mem;
-    if (const int rc = moe_take_space(c, sp.bytes, ws, ws_bytes, &mem)) return rc;
+    if (const int rc = moe_take_space(c, sp.bytes, ws, &mem)) return rc;
     const unsigned long chunk = std::max<unsigned long>(1, kMoeChunkSlots / n_used);
     const size_t elem = io_type == MOEARC_OUT_F16 ? 2 : 4;
     const MoeScope scope(c, "matmul_experts", n_rows, n_tok * n_used);
     for (unsigned long t = 0; t < n_tok; t += chunk) {
         const unsigned long n = std::min(chunk, n_tok - t);
         MoeArgs a{};
-        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) n_expert,
-                                    MOEARC_MOE_SMALL_TOKENS, mem, sp))
+        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) n_expert, mem, sp))
             return rc;
         a.x = (const uint8_t *) x + (x_per_slot ? t * n_used : t) * n_cols * elem;
         a.x_div = x_per_slot ? 1u : (uint32_t) n_used;
+        const bool half = io_type == MOEARC_OUT_F16;
+        if (a.tiles && !half) {
+            uint16_t *const hi = (uint16_t *) (mem + sp.split), *const lo = hi + sp.split_n;
+            if (const int rc = moe_split(c, (const float *) a.x, (x_per_slot ? n * n_used : n) * n_cols, hi, lo)) return rc;
+            a.x = hi;
+            a.x_lo = lo;
+        }
         a.w[0] = (const uint8_t *) w;
         a.bias[0] = bias;
         a.y = (uint8_t *) y + t * n_used * n_rows * elem;
-        a.y_f16 = io_type == MOEARC_OUT_F16;
+        a.y_f16 = half;
         a.zero_skipped = 1u;
         a.rows = (uint32_t) n_rows;
         a.cols = (uint32_t) n_cols;
-        if (const int rc = moe_product(c, a, type_id, false, io_type == MOEARC_OUT_F16)) return rc;
+        if (const int rc = moe_product(c, a, type_id, false, half)) return rc;
     }
     return OK;
 }
@@ -270,7 +300,7 @@ int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, u
     if (const int rc = moe_space_check(sp.bytes, ws, ws_bytes)) return rc;
     if (n_tok == 0) return OK;
     uint8_t *mem;
-    if (const int rc = moe_take_space(c, sp.bytes, ws, ws_bytes, &mem)) return rc;
+    if (const int rc = moe_take_space(c, sp.bytes, ws, &mem)) return rc;
     const unsigned long chunk = std::max<unsigned long>(1, kMoeChunkSlots / n_used);
     const bool half = io_type == MOEARC_OUT_F16;
     const size_t elem = half ? 2 : 4;
@@ -278,8 +308,7 @@ int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, u
     for (unsigned long t = 0; t < n_tok; t += chunk) {
         const unsigned long n = std::min(chunk, n_tok - t);
         MoeArgs a{};
-        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) m->n_expert,
-                                    MOEARC_MOE_SMALL_TOKENS, mem, sp))
+        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) m->n_expert, mem, sp))
             return rc;
         MoeArgs g = a, d = a;
         g.x = (const uint8_t *) x + t * m->n_embd * elem;
@@ -288,7 +317,15 @@ int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, u
             g.w[i] = (const uint8_t *) m->w[i];
             g.bias[i] = m->bias[i];
         }
+        if (a.tiles && !half) {
+            uint16_t *const hi = (uint16_t *) (mem + sp.split), *const lo = hi + sp.split_n;
+            if (const int rc = moe_split(c, (const float *) g.x, n * m->n_embd, hi, lo)) return rc;
+            g.x = hi;
+            g.x_lo = lo;
+        }
         g.y = mem + sp.act;
+        g.y_lo = (uint16_t *) (mem + sp.act) + sp.act_n;
+        d.x_lo = g.y_lo;
         g.y_f16 = half;
         g.rows = (uint32_t) m->n_ff;
         g.cols = (uint32_t) m->n_embd;
