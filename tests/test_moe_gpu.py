@@ -167,6 +167,30 @@ def test_odd_row_lengths(ctx, ty, cols):
 
 
 @pytest.mark.parametrize("ty", TYPES, ids=lambda t: t.name)
+def test_scales_of_every_size(ctx, ty):
+    """Blocks whose scales are zero, negative, or orders of magnitude from their neighbours'."""
+    e, rows, cols = 3, 70, 1024
+    raw, _ = weights(ty, e, rows, cols, 5)
+    b = raw.reshape(-1, ty.block_bytes).copy()
+    rng = np.random.default_rng(6)
+    pick = rng.integers(0, 4, len(b))
+    at = {QuantType.Q6_K: [208], QuantType.Q8_0: [0], QuantType.Q4_K: [0, 2], QuantType.Q5_K: [0, 2]}.get(ty, [])
+    for i in at:
+        d = b[:, i:i + 2].copy().view(np.float16)[:, 0]
+        d = np.where(pick == 0, 0, np.where(pick == 1, -d, np.where(pick == 2, d * np.float16(100), d))).astype(np.float16)
+        b[:, i:i + 2] = d.view(np.uint8).reshape(-1, 2)
+    if ty == QuantType.MXFP4:  # some windows within f16's normal range, most not; the smallest exponents too
+        b[:, 0] = np.where(np.arange(len(b)) % 32 < 8, rng.integers(114, 140, len(b)), rng.integers(90, 150, len(b)))
+        b[rng.integers(0, len(b), 40), 0] = 0
+        b[:32 * rows // 2, 0] = rng.integers(114, 140, 32 * rows // 2)  # half an expert all within it
+    raw = b.reshape(-1)
+    w = oracle.dequant(int(ty), raw, len(b)).astype(np.float64).reshape(e, rows, cols)
+    for t in (4, 100):
+        for io in (OUT_F32, OUT_F16) if ty != QuantType.MXFP4 else (OUT_F32,):  # f16 could not hold the sums
+            run_linear(ctx, ty, t, 2, e, rows, cols, io, bias=False, made=(raw, w))
+
+
+@pytest.mark.parametrize("ty", TYPES, ids=lambda t: t.name)
 def test_weights_at_any_even_address(ctx, ty):
     for shift in (2, 6, 14):
         run_linear(ctx, ty, 4, 2, 4, 33, 512, shift=shift)
