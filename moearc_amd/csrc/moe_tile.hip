@@ -29,13 +29,16 @@ namespace {
 
 typedef float moe_f32x16 __attribute__((ext_vector_type(16)));
 
-template <uint32_t TY>
+// A row's window in LDS: bytes where they belong but for Q6_K's last piece (bytes 194 .. 209), which goes to
+// 208 .. 223. Lanes read 8 bytes of 32 rows at once, so rows are 2 dwords apart modulo the 32 banks times an odd
+// number (136, 152, 184, 232 bytes); F16's 16-byte reads want 4. Q5_K with f32 inputs has no room for that
+// beside two work-groups per CU.
+template <uint32_t TY, int HALVES>
 struct MoeTileFmt {
     static constexpr uint32_t WB = TY == 1 ? 2 : TY == 8 ? 4 : 8;
     static constexpr uint32_t S = WB * 32u / moearc_mv_be(TY) * moearc_mv_bb(TY);
     static constexpr uint32_t NP = (S + 15u) / 16u;       // 16-byte pieces of a row's window
-    static constexpr uint32_t RS = 16u * (NP | 1u);       // an odd number of them apart: rows on all banks
-    static constexpr bool SPLIT_LAST = TY == 8;           // as MoeFmt
+    static constexpr uint32_t RS = TY == 1 ? 144 : TY == 12 ? 152 : TY == 13 ? (HALVES == 2 ? 176 : 184) : TY == 14 ? 232 : 136;
 };
 
 __device__ __forceinline__ uint32_t moe_swz(uint32_t t) { return (t >> 2) & 3u; }
@@ -79,93 +82,113 @@ __device__ __forceinline__ uint32_t moe_k4_min(u32x4_t hd, uint32_t i) {
     return i < 4u ? (hd[2] >> sh) & 63u : ((hd[3] >> (sh + 4u)) & 15u) | (((hd[2] >> (sh + 6u)) & 3u) << 4);
 }
 
-// Eight elements of k-block i of a row's window in LDS, k 8 lq .. 8 lq + 7: the payload as f16 integers
-// (E2M1 values times `scale` for MXFP4).
+// The eight bytes at p + OFF, p 8-byte aligned, OFF known at compile time.
+__device__ __forceinline__ void moe_get8(uint32_t &d0, uint32_t &d1, const uint8_t *p, uint32_t off) {
+    if (off % 8u == 0u) {
+        const u32x2_t v = *(const u32x2_t *) (p + off);
+        d0 = v[0];
+        d1 = v[1];
+        return;
+    }
+    const uint32_t *w = (const uint32_t *) (p + (off & ~3u));
+    if (off % 4u == 0u) {
+        d0 = w[0];
+        d1 = w[1];
+        return;
+    }
+    const uint32_t w0 = w[0], w1 = w[1], w2 = w[2];
+    d0 = __builtin_amdgcn_alignbyte(w1, w0, off & 3u);
+    d1 = __builtin_amdgcn_alignbyte(w2, w1, off & 3u);
+}
+
+// The lane's elements of k-block i of a row's window in LDS, slices s = 0, 1: k 16 s + 8 h .. + 7, as f16
+// integers (MXFP4: E2M1 values times `scale`; F16: the weights). live: 0 gives zeros (MXFP4, F16).
 template <uint32_t TY>
-__device__ __forceinline__ half8_t moe_payload(const uint8_t *row, uint32_t i, uint32_t lq, float scale) {
-    uint32_t q0, q1;
-    if constexpr (TY == 39) {
-        mms_get8(q0, q1, row, 17u * i + 1u + (i == 7u ? MmsFmt<39>::LAST : 0u), lq & 1u);
-        const uint32_t q[2] = {q0, q1};
-        half8_t r;
+__device__ __forceinline__ void moe_payload(half8_t (&w)[2], const uint8_t *row, uint32_t i, uint32_t h, float scale, uint32_t live) {
+    if constexpr (TY == 1) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint32_t x = (q[j] >> (4u * (lq >> 1))) & 0x0F0F0F0Fu;
-            const uint32_t y = x | (x >> 4);  // pairs in bytes 0 and 2
-            const half2_t p0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(y, scale, 0);
-            const half2_t p1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(y, scale, 2);
-            r[4 * j] = p0[0];
-            r[4 * j + 1] = p0[1];
-            r[4 * j + 2] = p1[0];
-            r[4 * j + 3] = p1[1];
+        for (uint32_t s = 0; s < 2; ++s) {
+            u32x4_t v = *(const u32x4_t *) (row + 64u * i + 32u * s + 16u * h);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] &= live;
+            w[s] = __builtin_bit_cast(half8_t, v);
         }
-        return r;
+    } else if constexpr (TY == 8) {
+#pragma unroll
+        for (uint32_t s = 0; s < 2; ++s) {
+            uint32_t q0, q1;
+            moe_get8(q0, q1, row + 8u * h, 34u * i + 2u + 16u * s);
+            w[s] = mms_bytes<128>(q0 ^ 0x80808080u, q1 ^ 0x80808080u);
+        }
+    } else if constexpr (TY == 39) {
+        uint32_t q[2];  // the low nibbles are slice 0's, the high ones slice 1's
+        moe_get8(q[0], q[1], row + 8u * h, 17u * i + 1u);
+        const uint32_t mask = 0x0F0F0F0Fu & live;
+#pragma unroll
+        for (uint32_t s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t x = (q[j] >> (4u * s)) & mask;
+                const uint32_t y = x | (x >> 4);  // pairs in bytes 0 and 2
+                const half2_t p0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(y, scale, 0);
+                const half2_t p1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(y, scale, 2);
+                w[s][4 * j] = p0[0];
+                w[s][4 * j + 1] = p0[1];
+                w[s][4 * j + 2] = p1[0];
+                w[s][4 * j + 3] = p1[1];
+            }
     } else if constexpr (TY == 12 || TY == 13) {
-        mms_get8(q0, q1, row, (TY == 12 ? 16u : 48u) + 32u * (i >> 1), lq);
         const uint32_t sh = 4u * (i & 1u);
-        q0 = (q0 >> sh) & 0x0F0F0F0Fu;
-        q1 = (q1 >> sh) & 0x0F0F0F0Fu;
-        if constexpr (TY == 13) {
-            uint32_t h0, h1;
-            mms_get8(h0, h1, row, 16u, lq);
-            q0 |= ((h0 >> i) & 0x01010101u) << 4;
-            q1 |= ((h1 >> i) & 0x01010101u) << 4;
+#pragma unroll
+        for (uint32_t s = 0; s < 2; ++s) {
+            uint32_t q0, q1;
+            moe_get8(q0, q1, row + 8u * h, (TY == 12 ? 16u : 48u) + 32u * (i >> 1) + 16u * s);
+            q0 = (q0 >> sh) & 0x0F0F0F0Fu;
+            q1 = (q1 >> sh) & 0x0F0F0F0Fu;
+            if constexpr (TY == 13) {
+                uint32_t h0, h1;
+                moe_get8(h0, h1, row + 8u * h, 16u + 16u * s);
+                q0 |= ((h0 >> i) & 0x01010101u) << 4;
+                q1 |= ((h1 >> i) & 0x01010101u) << 4;
+            }
+            w[s] = mms_bytes<0>(q0, q1);
         }
-        return mms_bytes<0>(q0, q1);
     } else {
-        static_assert(TY == 14, "a format whose scale enters the operand");
+        static_assert(TY == 14, "a weight format");
         const uint32_t n = i >> 2, c = i & 3u, shl = 4u * (c >> 1), shh = 2u * c;
-        uint32_t h0, h1;
-        mms_get8(q0, q1, row, 64u * n + 32u * (c & 1u), lq);
-        mms_get8(h0, h1, row, 128u + 32u * n, lq);
-        return mms_bytes<32>(((q0 >> shl) & 0x0F0F0F0Fu) | (((h0 >> shh) & 0x03030303u) << 4),
-                             ((q1 >> shl) & 0x0F0F0F0Fu) | (((h1 >> shh) & 0x03030303u) << 4));
+#pragma unroll
+        for (uint32_t s = 0; s < 2; ++s) {
+            uint32_t q0, q1, h0, h1;
+            moe_get8(q0, q1, row + 8u * h, 64u * n + 32u * (c & 1u) + 16u * s);
+            moe_get8(h0, h1, row + 8u * h, 128u + 32u * n + 16u * s);
+            w[s] = mms_bytes<32>(((q0 >> shl) & 0x0F0F0F0Fu) | (((h0 >> shh) & 0x03030303u) << 4),
+                                 ((q1 >> shl) & 0x0F0F0F0Fu) | (((h1 >> shh) & 0x03030303u) << 4));
+        }
     }
 }
 
 typedef __bf16 moe_bf8 __attribute__((ext_vector_type(8)));
 
-template <uint32_t TY, bool GU, int HALVES>
-__device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
-    using F = MoeTileFmt<TY>;
+// The reduction of one tile for a wave: acc[slot half][row tile], slots 32 and up only with BOTH. FOLD (MXFP4):
+// the scales enter the operand; returns false where one is out of f16's range, and the sums are not valid then.
+template <uint32_t TY, bool GU, int HALVES, bool BOTH, bool FOLD>
+__device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc)[2][2], uint8_t *xbuf, uint8_t *wbuf, uint16_t *sums,
+                                              uint32_t e, const uint32_t *slots, uint32_t count, uint32_t r0) {
+    using F = MoeTileFmt<TY, HALVES>;
     constexpr uint32_t WB = F::WB, SPW = WB / 2u;
-    constexpr bool Q45 = TY == 12 || TY == 13, Q6 = TY == 14, MX = TY == 39;
-    constexpr bool KQ = Q45 || Q6;
+    constexpr bool Q45 = TY == 12 || TY == 13, Q6 = TY == 14, MX = TY == 39, KQ = Q45 || Q6;
+    constexpr int NT = BOTH ? 2 : 1;
     constexpr uint32_t XB = 4096u, XPAIR = 2u * HALVES * XB;  // one half of a k-block, a pair of k-blocks
-    __shared__ __attribute__((aligned(1024))) uint8_t xbuf[2 * XPAIR];
-    __shared__ __attribute__((aligned(16))) uint8_t wbuf[4][64 * F::RS];
-    // Q4_K, Q5_K: [slot][piece 0 .. 3][block of the super-block] bf16, a block's sum of x in three pieces
-    __shared__ __attribute__((aligned(16))) uint16_t sums[Q45 ? 64 * 32 : 8];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t n = lane & 31u, h = lane >> 5;
-
-    const uint32_t ti = blockIdx.x / a.row_tiles, rt_i = blockIdx.x % a.row_tiles;
-    if (ti >= *a.n_tiles) return;
-    const MoeTile t = a.tiles[ti];
-    const uint32_t e = __builtin_amdgcn_readfirstlane(t.expert), count = __builtin_amdgcn_readfirstlane(t.count);
-    const uint32_t *const slots = a.list + t.first;
-    // this wave's rows: GU: 32 of each matrix from r0, else 64 from r0
-    const uint32_t r0 = rt_i * (GU ? 128u : 256u) + wave * (GU ? 32u : 64u);
-    if (e == a.n_expert) {
-        if (!GU && a.zero_skipped)
-            for (uint32_t u = 0; u < count; ++u) {
-                const uint64_t o = (uint64_t) slots[u] * a.rows + r0 + lane;
-                if (r0 + lane >= a.rows) continue;
-                if (a.y_f16) ((uint16_t *) a.y)[o] = 0;
-                else ((float *) a.y)[o] = 0.f;
-            }
-        return;
-    }
-    const bool both = count > 32u;  // uniform
-    const uint32_t nb = a.cols / 32u, n_win = (nb + WB - 1u) / WB, total = n_win * SPW;
-    // window w starts at block min(w WB, nb - WB): the last one may repeat blocks, which are skipped
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 31u, h = lane >> 5;
+    const uint32_t nb = a.cols / 32u, n_win = (nb + WB - 1u) / WB;
+    // Window w starts at block w WB, the last one at nb - WB: its first `skip` blocks have been done. Whole
+    // pairs of them are left out (skip0), a single one is taken as zero.
+    const uint32_t skip = n_win * WB - nb, skip0 = skip / 2u, total = n_win * SPW - skip0;
     auto wstart = [&](uint32_t w) { return min(w * WB, nb - WB); };
 
     // weights: lane l's pieces l % 32 + 32 j of rows r0 + 32 (l / 32) .. (GU: of matrix l / 32)
-    const uint8_t *wsrc = a.w[GU ? h : 0] + e * a.expert_bytes;
     const uint32_t wr0 = min(r0 + (GU ? 0u : 32u * h), a.rows - 1u), wleft = a.rows - 1u - wr0;
-    wsrc += (uint64_t) wr0 * a.row_bytes;
+    const uint8_t *const wsrc = a.w[GU ? h : 0] + e * a.expert_bytes + (uint64_t) wr0 * a.row_bytes;
     u32x4_t wreg[F::NP];
     auto wload = [&](uint32_t w) {
         const uint8_t *p = wsrc + (uint64_t) wstart(w) * 32u / moearc_mv_be(TY) * moearc_mv_bb(TY);
@@ -179,174 +202,178 @@ __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
 #pragma unroll
         for (uint32_t j = 0; j < F::NP; ++j) {
             const uint32_t q = n + 32u * j, row = q / F::NP, piece = q % F::NP;
-            uint8_t *d = wbuf[wave] + (32u * h + row) * F::RS;
-            if constexpr (F::SPLIT_LAST) {
-                d += min(16u * piece, F::S - 16u);
+            uint8_t *d = wbuf + (32u * h + row) * F::RS + (F::S % 8u ? 16u * piece : min(16u * piece, F::S - 16u));
+            if constexpr (TY == 1) {
+                *(u32x4_t *) d = wreg[j];
+            } else {
                 *(u32x2_t *) d = u32x2_t{wreg[j][0], wreg[j][1]};
                 *(u32x2_t *) (d + 8) = u32x2_t{wreg[j][2], wreg[j][3]};
-            } else {
-                *(u32x4_t *) (d + 16u * piece) = wreg[j];
             }
         }
     };
     // inputs: thread i, load (half, group g): slot i / 8 + 32 g, 16 bytes i % 8 of the pair's 128
-    const uint16_t *xrow[2];
+    const uint16_t *xrow[NT];
 #pragma unroll
-    for (uint32_t g = 0; g < 2; ++g)
+    for (uint32_t g = 0; g < NT; ++g)
         xrow[g] = (const uint16_t *) a.x + (uint64_t) (slots[min((tid >> 3) + 32u * g, count - 1u)] / a.x_div) * a.cols + 8u * (tid & 7u);
     const int64_t xlo = HALVES == 2 ? (const uint16_t *) a.x_lo - (const uint16_t *) a.x : 0;
-    u32x4_t xreg[HALVES][2];
+    u32x4_t xreg[HALVES][NT];
     auto xload = [&](uint32_t step) {
-        const uint32_t b = wstart(step / SPW) + 2u * (step % SPW);
+        const uint32_t w = step / SPW, b = wstart(w) + 2u * (step % SPW + (w + 1u == n_win ? skip0 : 0u));
 #pragma unroll
-        for (uint32_t g = 0; g < 2; ++g)
-            if (g == 0u || both)
+        for (uint32_t g = 0; g < NT; ++g)
 #pragma unroll
-                for (int f = 0; f < HALVES; ++f)
-                    __builtin_memcpy(&xreg[f][g], xrow[g] + (f ? xlo : 0) + 32u * b, 16);
+            for (int f = 0; f < HALVES; ++f) __builtin_memcpy(&xreg[f][g], xrow[g] + (f ? xlo : 0) + 32u * b, 16);
     };
     auto xput = [&](uint32_t buf) {
         const uint32_t blk = (tid >> 2) & 1u, c = tid & 3u;
 #pragma unroll
-        for (uint32_t g = 0; g < 2; ++g)
-            if (g == 0u || both) {
-                const uint32_t u = (tid >> 3) + 32u * g;
+        for (uint32_t g = 0; g < NT; ++g) {
+            const uint32_t u = (tid >> 3) + 32u * g;
 #pragma unroll
-                for (int f = 0; f < HALVES; ++f)
-                    *(u32x4_t *) (xbuf + buf * XPAIR + (blk * HALVES + f) * XB + u * 64u + 16u * (c ^ moe_swz(u))) = xreg[f][g];
-            }
+            for (int f = 0; f < HALVES; ++f)
+                *(u32x4_t *) (xbuf + buf * XPAIR + (blk * HALVES + f) * XB + u * 64u + 16u * (c ^ moe_swz(u))) = xreg[f][g];
+        }
     };
     // The sums of x over the k-blocks of the pair in the registers, as this thread's bf16 piece: piece
     // tid % 4 of block (tid / 4) % 2, slots tid / 8 and + 32. Cut off bits, so that three pieces are exact.
-    auto xsums = [&](uint32_t (&piece)[2]) {
+    auto xsums = [&](uint32_t (&piece)[NT]) {
 #pragma unroll
-        for (uint32_t g = 0; g < 2; ++g)
-            if (g == 0u || both) {
-                float s = 0.f;
+        for (uint32_t g = 0; g < NT; ++g) {
+            float s = 0.f;
 #pragma unroll
-                for (int f = HALVES - 1; f >= 0; --f) {
-                    const half8_t v = __builtin_bit_cast(half8_t, xreg[f][g]);
+            for (int f = HALVES - 1; f >= 0; --f) {
+                const half8_t v = __builtin_bit_cast(half8_t, xreg[f][g]);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) s += (float) v[k];
-                }
-                s += dpp<0xB1>(s);
-                s += dpp<0x4E>(s);
-                const uint32_t p0 = __float_as_uint(s) & 0xFFFF0000u;
-                const float s1 = s - __uint_as_float(p0);
-                const uint32_t p1 = __float_as_uint(s1) & 0xFFFF0000u;
-                const uint32_t p2 = __float_as_uint(s1 - __uint_as_float(p1));
-                const uint32_t c = tid & 3u;
-                piece[g] = (c == 0u ? p0 : c == 1u ? p1 : c == 2u ? p2 : 0u) >> 16;
+                for (int k = 0; k < 8; ++k) s += (float) v[k];
             }
+            s += dpp<0xB1>(s);
+            s += dpp<0x4E>(s);
+            const uint32_t p0 = __float_as_uint(s) & 0xFFFF0000u;
+            const float s1 = s - __uint_as_float(p0);
+            const uint32_t p1 = __float_as_uint(s1) & 0xFFFF0000u;
+            const uint32_t p2 = __float_as_uint(s1 - __uint_as_float(p1));
+            const uint32_t c = tid & 3u;
+            piece[g] = (c == 0u ? p0 : c == 1u ? p1 : c == 2u ? p2 : 0u) >> 16;
+        }
     };
-    auto sput = [&](const uint32_t (&piece)[2], uint32_t pair) {  // `pair` of the window
+    auto sput = [&](const uint32_t (&piece)[NT], uint32_t pair) {  // `pair` of the window
 #pragma unroll
-        for (uint32_t g = 0; g < 2; ++g)
-            if (g == 0u || both)
-                sums[((tid >> 3) + 32u * g) * 32u + (tid & 3u) * 8u + 2u * pair + ((tid >> 2) & 1u)] = (uint16_t) piece[g];
+        for (uint32_t g = 0; g < NT; ++g)
+            sums[((tid >> 3) + 32u * g) * 32u + (tid & 3u) * 8u + 2u * pair + ((tid >> 2) & 1u)] = (uint16_t) piece[g];
     };
 
-    moe_f32x16 acc[2][2];  // [slot half][row tile]
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
+    for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[tt][rt][j] = 0.f;
-
     // K-quants: per row tile, what the accumulators are in units of, and whether the super-block counts at
     // all (d = 0: its scales are taken as 0, and the unit stays)
     float unit[2] = {1.f, 1.f};
     bool counts[2] = {true, true};
 
-    bool fold = false;  // MXFP4: this window's scales are in the operand
     auto mul = [&](const half8_t &x, const half8_t &w, const moe_f32x16 &c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, w, c, 0, 0, 0);
     };
-    // k-block i of the window, block blk of the pair in buffer buf
-    auto compute = [&](uint32_t buf, uint32_t blk, uint32_t i) {
-        half8_t x[HALVES][2][2];
+    // k-block i of the window, block blk of the pair in buffer buf; live 0: taken as zero
+    auto compute = [&](uint32_t buf, uint32_t blk, uint32_t i, uint32_t live) {
+        half8_t x[HALVES][NT][2];
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-            if (tt == 0 || both)
+        for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
-                for (int s = 0; s < 2; ++s)
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int f = 0; f < HALVES; ++f) {
-                        const uint32_t u = 32u * tt + n;
-                        x[f][tt][s] = __builtin_bit_cast(half8_t, *(const u32x4_t *) (xbuf + buf * XPAIR + (blk * HALVES + f) * XB +
-                                                                                      u * 64u + 16u * ((2u * s + h) ^ moe_swz(u))));
-                    }
+                for (int f = 0; f < HALVES; ++f) {
+                    const uint32_t u = 32u * tt + n;
+                    x[f][tt][s] = __builtin_bit_cast(half8_t, *(const u32x4_t *) (xbuf + buf * XPAIR + (blk * HALVES + f) * XB +
+                                                                                  u * 64u + 16u * ((2u * s + h) ^ moe_swz(u))));
+                }
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
-            const uint8_t *row = wbuf[wave] + (32u * rt + n) * F::RS;
-            half8_t w[2], wl[2];
-            float s0 = 0.f, s1 = 0.f;
-            bool lost = false;  // Q6_K: some product of the wave was rounded
-            if constexpr (Q45) {
-                const uint32_t sc = counts[rt] ? moe_k4_scale(*(const u32x4_t *) row, i) : 0u;
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-                    w[s] = moe_times(moe_payload<TY>(row, i, 2u * s + h, 1.f), (_Float16) (uint16_t) sc);
-            } else if constexpr (Q6) {
-                const uint32_t sc = *(const uint16_t *) (row + 192u + 8u * (i >> 2) + 2u * (i & 3u));
+            const uint8_t *row = wbuf + (32u * rt + n) * F::RS;
+            half8_t w[2];
+            if constexpr (KQ) {
+                moe_payload<TY>(w, row, i, h, 1.f, live);
+                half8_t lost[2];
                 uint32_t any = 0u;
+                if constexpr (Q45) {
+                    const u32x2_t h0 = *(const u32x2_t *) row, h1 = *(const u32x2_t *) (row + 8);
+                    const uint32_t sc = counts[rt] ? moe_k4_scale(u32x4_t{h0[0], h0[1], h1[0], h1[1]}, i) : 0u;
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const _Float16 f = counts[rt] ? (_Float16) (int16_t) (int8_t) (sc >> (8 * s)) : (_Float16) 0.f;
-                    const half8_t q = moe_payload<TY>(row, i, 2u * s + h, 1.f);
-                    w[s] = moe_times(q, f);
-                    wl[s] = moe_lost(q, f, w[s]);
-                    const u32x4_t bits = __builtin_bit_cast(u32x4_t, wl[s]);
-                    any |= (bits[0] | bits[1] | bits[2] | bits[3]) & 0x7FFF7FFFu;
-                }
-                lost = __ballot(any != 0u) != 0ull;
-            } else if constexpr (MX) {
-                const uint32_t e8 = row[17u * i];
-                s0 = __uint_as_float(e8 ? e8 << 23 : 0x00400000u);  // 2^(e - 127)
-                const float f = fold ? s0 : 1.f;
+                    for (int s = 0; s < 2; ++s) w[s] = moe_times(w[s], (_Float16) (uint16_t) sc);
+                } else {
+                    const uint32_t sc = *(const uint16_t *) (row + 192u + 8u * (i >> 2) + 2u * (i & 3u));
 #pragma unroll
-                for (int s = 0; s < 2; ++s) w[s] = moe_payload<TY>(row, i, 2u * s + h, f);
-            } else {
-#pragma unroll
-                for (int s = 0; s < 2; ++s) w[s] = mms_operand<TY>(row, i, 2u * s + h, s0, s1);
-            }
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-                if (tt == 0 || both) {
-                    if (TY == 1 || KQ || fold) {
-#pragma unroll
-                        for (int s = 0; s < 2; ++s)
-#pragma unroll
-                            for (int f = 0; f < HALVES; ++f) acc[tt][rt] = mul(x[f][tt][s], w[s], acc[tt][rt]);
-                        if constexpr (Q6)
-                            if (lost) {
-#pragma unroll
-                                for (int s = 0; s < 2; ++s) acc[tt][rt] = mul(x[0][tt][s], wl[s], acc[tt][rt]);
-                            }
-                    } else {
-                        moe_f32x16 d = {};
-#pragma unroll
-                        for (int s = 0; s < 2; ++s)
-#pragma unroll
-                            for (int f = 0; f < HALVES; ++f) d = mul(x[f][tt][s], w[s], d);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) acc[tt][rt][j] = fmaf(s0, d[j], acc[tt][rt][j]);
+                    for (int s = 0; s < 2; ++s) {
+                        const _Float16 f = counts[rt] ? (_Float16) (int16_t) (int8_t) (sc >> (8 * s)) : (_Float16) 0.f;
+                        const half8_t q = w[s];
+                        w[s] = moe_times(q, f);
+                        lost[s] = moe_lost(q, f, w[s]);
+                        const u32x4_t bits = __builtin_bit_cast(u32x4_t, lost[s]);
+                        any |= (bits[0] | bits[1] | bits[2] | bits[3]) & 0x7FFF7FFFu;
                     }
                 }
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int f = 0; f < HALVES; ++f)
+#pragma unroll
+                        for (int tt = 0; tt < NT; ++tt) acc[tt][rt] = mul(x[f][tt][s], w[s], acc[tt][rt]);
+                if constexpr (Q6)
+                    if (__ballot(any != 0u) != 0ull) {  // some product of the wave was rounded
+#pragma unroll
+                        for (int s = 0; s < 2; ++s)
+#pragma unroll
+                            for (int tt = 0; tt < NT; ++tt) acc[tt][rt] = mul(x[0][tt][s], lost[s], acc[tt][rt]);
+                    }
+            } else if constexpr (TY == 1 || FOLD) {
+                float f = 1.f;
+                if constexpr (FOLD) f = __uint_as_float((uint32_t) row[17u * i] << 23);  // 2^(e - 127)
+                moe_payload<TY>(w, row, i, h, f, live);
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int f = 0; f < HALVES; ++f)
+#pragma unroll
+                        for (int tt = 0; tt < NT; ++tt) acc[tt][rt] = mul(x[f][tt][s], w[s], acc[tt][rt]);
+            } else {
+                float f;
+                if constexpr (MX) {
+                    const uint32_t e8 = row[17u * i];
+                    f = __uint_as_float(e8 ? e8 << 23 : 0x00400000u);  // 2^(e - 127)
+                } else {
+                    f = live ? mms_f16(*(const uint16_t *) (row + 34u * i)) : 0.f;
+                }
+                moe_payload<TY>(w, row, i, h, 1.f, live);
+                moe_f32x16 d[NT];
+#pragma unroll
+                for (int tt = 0; tt < NT; ++tt) d[tt] = moe_f32x16{};
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int f = 0; f < HALVES; ++f)
+#pragma unroll
+                        for (int tt = 0; tt < NT; ++tt) d[tt] = mul(x[f][tt][s], w[s], d[tt]);
+#pragma unroll
+                for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) acc[tt][rt][j] = fmaf(f, d[tt][j], acc[tt][rt][j]);
+            }
         }
     };
     // the accumulators from the last super-block's unit to this one's
     auto rescale = [&]() {
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
-            const uint8_t *row = wbuf[wave] + (32u * rt + n) * F::RS;
+            const uint8_t *row = wbuf + (32u * rt + n) * F::RS;
             const float d = mms_f16(*(const uint16_t *) (row + (Q6 ? 208u + MmsFmt<14>::LAST : 0u)));
             counts[rt] = d != 0.f;
             const float ratio = counts[rt] ? unit[rt] / d : 1.f;
             unit[rt] = counts[rt] ? d : unit[rt];
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
+            for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) acc[tt][rt][j] *= ratio;
         }
@@ -354,26 +381,28 @@ __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
     auto mins = [&]() {
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
-            const u32x4_t hd = *(const u32x4_t *) (wbuf[wave] + (32u * rt + n) * F::RS);
+            const uint8_t *row = wbuf + (32u * rt + n) * F::RS;
+            const u32x2_t h0 = *(const u32x2_t *) row, h1 = *(const u32x2_t *) (row + 8);
+            const u32x4_t hd = {h0[0], h0[1], h1[0], h1[1]};
             const float f = -mms_f16(hd[0] >> 16) / unit[rt];
             moe_bf8 m;
 #pragma unroll
             for (uint32_t k = 0; k < 8; ++k) m[k] = (__bf16) (float) moe_k4_min(hd, k);
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-                if (tt == 0 || both) {
-                    moe_f32x16 d = {};
+            for (int tt = 0; tt < NT; ++tt) {
+                moe_f32x16 d = {};
 #pragma unroll
-                    for (uint32_t p = 0; p < 2; ++p)
-                        d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                            __builtin_bit_cast(moe_bf8, *(const u32x4_t *) (sums + (32u * tt + n) * 32u + 16u * p + 8u * h)), m, d, 0, 0, 0);
+                for (uint32_t p = 0; p < 2; ++p)
+                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        __builtin_bit_cast(moe_bf8, *(const u32x4_t *) (sums + (32u * tt + n) * 32u + 16u * p + 8u * h)), m, d, 0, 0, 0);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) acc[tt][rt][j] = fmaf(f, d[j], acc[tt][rt][j]);
-                }
+                for (int j = 0; j < 16; ++j) acc[tt][rt][j] = fmaf(f, d[j], acc[tt][rt][j]);
+            }
         }
     };
 
-    uint32_t piece[2] = {0u, 0u};
+    uint32_t piece[NT] = {};
+    bool ok = true;
     wload(0u);
     xload(0u);
     xput(0u);
@@ -381,11 +410,29 @@ __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
     xload(min(1u, total - 1u));
     moe_barrier();
     uint32_t step = 0;
-    // The steps of a window. Sums: the pair that is stored for the next step has its own stored with it, but
-    // the next window's first pair waits for that window, when the mins of this one have been taken.
-    auto steps = [&](uint32_t skip) {
+    for (uint32_t w = 0; w < n_win; ++w) {
+        __builtin_amdgcn_wave_barrier();
+        wput();
+        __builtin_amdgcn_wave_barrier();
+        wload(min(w + 1u, n_win - 1u));
+        const bool last = w + 1u == n_win;
+        const uint32_t from = last ? skip0 : 0u, live0 = last && (skip & 1u) ? 0u : 0xFFFFFFFFu;
+        if constexpr (KQ) rescale();
+        if constexpr (FOLD) {
+            uint32_t lo = 255u, hi = 0u;  // of row `lane`
 #pragma unroll
-        for (uint32_t j = 0; j < SPW; ++j, ++step) {
+            for (uint32_t i = 0; i < WB; ++i) {
+                const uint32_t e8 = wbuf[lane * F::RS + 17u * i];
+                lo = min(lo, e8);
+                hi = max(hi, e8);
+            }
+            ok = ok && lo >= 114u && hi <= 139u;
+        }
+        // Sums: the pair that is stored for the next step has its own stored with it, but the next window's
+        // first pair waits for that window, when the mins of this one have been taken.
+#pragma unroll
+        for (uint32_t j = 0; j < SPW; ++j) {
+            if (j < from) continue;
             const uint32_t buf = step & 1u;
             if constexpr (Q45)
                 if (j == 0) sput(piece, 0u);
@@ -395,42 +442,34 @@ __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
                 if (j + 1u < SPW) sput(piece, j + 1u);
             }
             xload(min(step + 2u, total - 1u));
-#pragma unroll
-            for (uint32_t b = 0; b < 2; ++b)
-                if (2u * j + b >= skip) compute(buf, b, 2u * j + b);
+            compute(buf, 0u, 2u * j, j == from ? live0 : 0xFFFFFFFFu);
+            compute(buf, 1u, 2u * j + 1u, 0xFFFFFFFFu);
             if constexpr (Q45)
                 if (j + 1u == SPW) mins();
             moe_barrier();
+            ++step;
         }
-    };
-    for (uint32_t w = 0; w < n_win; ++w) {
-        __builtin_amdgcn_wave_barrier();
-        wput();
-        __builtin_amdgcn_wave_barrier();
-        wload(min(w + 1u, n_win - 1u));
-        const uint32_t skip = w * WB - wstart(w);
-        if constexpr (KQ) rescale();
-        if constexpr (MX) {
-            uint32_t lo = 255u, hi = 0u;  // of row `lane`
-#pragma unroll
-            for (uint32_t i = 0; i < WB; ++i) {
-                const uint32_t e8 = wbuf[wave][lane * F::RS + 17u * i];
-                lo = min(lo, e8);
-                hi = max(hi, e8);
-            }
-            fold = __ballot(lo < 114u || hi > 139u) == 0ull;
-        }
-        steps(skip);
     }
     if constexpr (KQ) {
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
+            for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) acc[tt][rt][j] *= unit[rt];
     }
+    return ok;
+}
 
+template <uint32_t TY, bool GU, int HALVES, bool BOTH>
+__device__ __forceinline__ void moe_tile_half(const MoeArgs &a, uint8_t *xbuf, uint8_t *wbuf, uint16_t *sums, uint32_t e,
+                                              const uint32_t *slots, uint32_t count, uint32_t r0) {
+    const uint32_t lane = threadIdx.x & 63u, n = lane & 31u, h = lane >> 5;
+    moe_f32x16 acc[2][2];
+    const bool ok = moe_tile_sums<TY, GU, HALVES, BOTH, TY == 39>(a, acc, xbuf, wbuf, sums, e, slots, count, r0);
+    if constexpr (TY == 39)  // some scale out of range: again, every block's sum scaled by itself
+        if (__syncthreads_or(!ok))
+            (void) moe_tile_sums<TY, GU, HALVES, BOTH, false>(a, acc, xbuf, wbuf, sums, e, slots, count, r0);
 #pragma unroll
     for (int rt = 0; rt < (GU ? 1 : 2); ++rt) {
         const uint32_t r = r0 + 32u * rt + n;
@@ -438,7 +477,7 @@ __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
         const float b0 = a.bias[0] ? a.bias[0][(uint64_t) e * a.rows + r] : 0.f;
         const float b1 = GU && a.bias[1] ? a.bias[1][(uint64_t) e * a.rows + r] : 0.f;
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
+        for (int tt = 0; tt < (BOTH ? 2 : 1); ++tt)
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 const uint32_t u = 32u * tt + 8u * (j >> 2) + 4u * h + (j & 3);
@@ -456,6 +495,35 @@ __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
                 }
             }
     }
+}
+
+template <uint32_t TY, bool GU, int HALVES>
+__device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
+    using F = MoeTileFmt<TY, HALVES>;
+    __shared__ __attribute__((aligned(1024))) uint8_t xbuf[4 * HALVES * 4096];
+    __shared__ __attribute__((aligned(16))) uint8_t wbuf[4][64 * F::RS];
+    // Q4_K, Q5_K: [slot][piece 0 .. 3][block of the super-block] bf16, a block's sum of x in three pieces
+    __shared__ __attribute__((aligned(16))) uint16_t sums[TY == 12 || TY == 13 ? 64 * 32 : 8];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t ti = blockIdx.x / a.row_tiles, rt_i = blockIdx.x % a.row_tiles;
+    if (ti >= *a.n_tiles) return;
+    const MoeTile t = a.tiles[ti];
+    const uint32_t e = __builtin_amdgcn_readfirstlane(t.expert), count = __builtin_amdgcn_readfirstlane(t.count);
+    const uint32_t *const slots = a.list + t.first;
+    // this wave's rows: GU: 32 of each matrix from r0, else 64 from r0
+    const uint32_t r0 = rt_i * (GU ? 128u : 256u) + wave * (GU ? 32u : 64u);
+    if (e == a.n_expert) {
+        if (!GU && a.zero_skipped)
+            for (uint32_t u = 0; u < count; ++u) {
+                const uint64_t o = (uint64_t) slots[u] * a.rows + r0 + lane;
+                if (r0 + lane >= a.rows) continue;
+                if (a.y_f16) ((uint16_t *) a.y)[o] = 0;
+                else ((float *) a.y)[o] = 0.f;
+            }
+        return;
+    }
+    if (count > 32u) moe_tile_half<TY, GU, HALVES, true>(a, xbuf, wbuf[wave], sums, e, slots, count, r0);
+    else moe_tile_half<TY, GU, HALVES, false>(a, xbuf, wbuf[wave], sums, e, slots, count, r0);
 }
 
 }  // namespace
