@@ -415,6 +415,7 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
         wput();
         __builtin_amdgcn_wave_barrier();
         wload(min(w + 1u, n_win - 1u));
+        __builtin_amdgcn_sched_barrier(0);
         const bool last = w + 1u == n_win;
         const uint32_t from = last ? skip0 : 0u, live0 = last && (skip & 1u) ? 0u : 0xFFFFFFFFu;
         if constexpr (KQ) rescale();
@@ -442,6 +443,7 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
                 if (j + 1u < SPW) sput(piece, j + 1u);
             }
             xload(min(step + 2u, total - 1u));
+            __builtin_amdgcn_sched_barrier(0);  // left alone, the loads sink to the step's end, and the next waits for them
             compute(buf, 0u, 2u * j, j == from ? live0 : 0xFFFFFFFFu);
             compute(buf, 1u, 2u * j + 1u, 0xFFFFFFFFu);
             if constexpr (Q45)
