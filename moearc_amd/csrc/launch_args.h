@@ -269,10 +269,13 @@ struct RouteArgs {
 };
 
 // A slot is a token's j-th expert, slot t * n_used + j. The plan groups the slots of a call by expert
-// in tiles of at most `tile` slots: tiles[i] = (expert, first place, count), list[place] = slot, each
-// expert's slots in their order. Slots without a valid expert form a last group, "expert" n_expert.
+// in tiles of at most `tile` slots: tiles[i] = (expert, first place, slots; which of its expert's tiles, and
+// of how many), list[place] = slot, each expert's slots in their order. Slots without a valid expert form a
+// last group, "expert" n_expert.
 struct MoeTile {
-    uint32_t expert, first, count, pad;
+    uint32_t expert, first;
+    uint16_t count, pad;
+    uint16_t index, of;
 };
 struct MoePlanArgs {
     const uint32_t *ids;   // [n_slots]

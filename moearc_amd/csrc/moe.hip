@@ -155,7 +155,7 @@ extern "C" __global__ void __launch_bounds__(1024) moearc_moe_plan_k(MoePlanArgs
     __syncthreads();
     const uint32_t n = count[mine], first = before[0], tile0 = before[1], n_tiles = (n + a.tile - 1u) / a.tile;
     for (uint32_t i = tid; i < n_tiles; i += 1024u)
-        a.tiles[tile0 + i] = MoeTile{mine, first + i * a.tile, min(a.tile, n - i * a.tile), 0u};
+        a.tiles[tile0 + i] = MoeTile{mine, first + i * a.tile, (uint16_t) min(a.tile, n - i * a.tile), 0, (uint16_t) i, (uint16_t) n_tiles};
     if (mine == a.n_expert && tid == 0u) *a.n_tiles = tile0 + n_tiles;
     if (n == 0u) return;
     uint32_t at = first;

@@ -186,29 +186,64 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
     const uint32_t skip = n_win * WB - nb, skip0 = skip / 2u, total = n_win * SPW - skip0;
     auto wstart = [&](uint32_t w) { return min(w * WB, nb - WB); };
 
-    // weights: lane l's pieces l % 32 + 32 j of rows r0 + 32 (l / 32) .. (GU: of matrix l / 32)
-    const uint32_t wr0 = min(r0 + (GU ? 0u : 32u * h), a.rows - 1u), wleft = a.rows - 1u - wr0;
-    const uint8_t *const wsrc = a.w[GU ? h : 0] + e * a.expert_bytes + (uint64_t) wr0 * a.row_bytes;
-    u32x4_t wreg[F::NP];
-    auto wload = [&](uint32_t w) {
-        const uint8_t *p = wsrc + (uint64_t) wstart(w) * 32u / moearc_mv_be(TY) * moearc_mv_bb(TY);
+    // Weights: copies of 16 rows each take four pieces per row, four lanes a row; what is left of a row's pieces is
+    // copied for the 64 rows at once (one piece) or 32 (two). Rows 0 .. 31 are of matrix GU ? 0 : 0 from r0, rows
+    // 32 .. 63 of matrix GU ? 1 : 0 from r0 + (GU ? 0 : 32); rows past the last repeat it. A lane's offset within
+    // the matrix is 32 bits (64 rows of at most 2 MiB), the rest of the address is the wave's.
+    constexpr uint32_t NQ = F::NP % 4u == 3u ? F::NP / 4u + 1u : F::NP / 4u, NR = F::NP % 4u == 3u ? 0u : F::NP % 4u;
+    constexpr uint32_t RB = F::S % 16u == 8u ? 8u : 16u;  // bytes of the last piece that are new
+    static_assert(RB == 16u || NR == 1u, "a short last piece stands alone");
+    const uint32_t wr0 = min(r0, a.rows - 1u), wleft = a.rows - 1u - wr0;
+    const uint8_t *const wrow0 = a.w[0] + e * a.expert_bytes + (uint64_t) wr0 * a.row_bytes;
+    const uint8_t *const wrow1 = GU ? a.w[1] + e * a.expert_bytes + (uint64_t) wr0 * a.row_bytes : wrow0;
+    const uint32_t rbytes = (uint32_t) a.row_bytes;
+    uint32_t woff[4], roff[NR ? NR : 1];
 #pragma unroll
-        for (uint32_t j = 0; j < F::NP; ++j) {
-            const uint32_t q = n + 32u * j, row = q / F::NP, piece = q % F::NP;
-            __builtin_memcpy(&wreg[j], p + (uint64_t) min(row, wleft) * a.row_bytes + min(16u * piece, F::S - 16u), 16);
+    for (uint32_t g = 0; g < 4; ++g) woff[g] = min((lane >> 2) + (GU ? 16u * (g & 1u) : 16u * g), wleft) * rbytes;
+#pragma unroll
+    for (uint32_t g = 0; g < NR; ++g) {
+        const uint32_t row = NR == 1u ? lane : (lane >> 1) + 32u * g;
+        roff[g] = min(GU ? row & 31u : row, wleft) * rbytes + min(64u * NQ + 16u * (NR == 1u ? 0u : lane & 1u), F::S - RB);
+    }
+    u32x4_t wreg[4][NQ], rreg[NR ? NR : 1];
+    auto wload = [&](uint32_t w) {
+        const uint64_t o = (uint64_t) wstart(w) * 32u / moearc_mv_be(TY) * moearc_mv_bb(TY);
+#pragma unroll
+        for (uint32_t g = 0; g < 4; ++g)
+#pragma unroll
+            for (uint32_t k = 0; k < NQ; ++k) {
+                // only the last quad can pass the window's end, by pieces that repeat the one before
+                const uint32_t at = 64u * (k + 1u) <= F::S ? 64u * k + 16u * (lane & 3u) : min(64u * k + 16u * (lane & 3u), F::S - 16u);
+                __builtin_memcpy(&wreg[g][k], (g < 2u ? wrow0 : wrow1) + o + (woff[g] + at), 16);
+            }
+#pragma unroll
+        for (uint32_t g = 0; g < NR; ++g) {
+            // (one piece: lanes 32 .. 63 hold rows 32 .. 63, which with GU are the other matrix's)
+            const uint8_t *p = (NR == 1u ? (lane < 32u ? wrow0 : wrow1) : (g == 0u ? wrow0 : wrow1)) + o + roff[g];
+            __builtin_memcpy(&rreg[g], p, RB);
+        }
+    };
+    auto put16 = [&](uint8_t *d, u32x4_t v) {
+        if constexpr (TY == 1) {
+            *(u32x4_t *) d = v;
+        } else {
+            *(u32x2_t *) d = u32x2_t{v[0], v[1]};
+            *(u32x2_t *) (d + 8) = u32x2_t{v[2], v[3]};
         }
     };
     auto wput = [&]() {
 #pragma unroll
-        for (uint32_t j = 0; j < F::NP; ++j) {
-            const uint32_t q = n + 32u * j, row = q / F::NP, piece = q % F::NP;
-            uint8_t *d = wbuf + (32u * h + row) * F::RS + (F::S % 8u ? 16u * piece : min(16u * piece, F::S - 16u));
-            if constexpr (TY == 1) {
-                *(u32x4_t *) d = wreg[j];
-            } else {
-                *(u32x2_t *) d = u32x2_t{wreg[j][0], wreg[j][1]};
-                *(u32x2_t *) (d + 8) = u32x2_t{wreg[j][2], wreg[j][3]};
+        for (uint32_t g = 0; g < 4; ++g)
+#pragma unroll
+            for (uint32_t k = 0; k < NQ; ++k) {
+                const uint32_t piece = 4u * k + (lane & 3u);
+                put16(wbuf + ((lane >> 2) + 16u * g) * F::RS + 16u * (4u * (k + 1u) <= F::NP ? piece : min(piece, F::NP - 1u)), wreg[g][k]);
             }
+#pragma unroll
+        for (uint32_t g = 0; g < NR; ++g) {
+            uint8_t *d = wbuf + (NR == 1u ? lane : (lane >> 1) + 32u * g) * F::RS + 64u * NQ + 16u * (NR == 1u ? 0u : lane & 1u);
+            if constexpr (RB == 8u) *(u32x2_t *) d = u32x2_t{rreg[g][0], rreg[g][1]};
+            else put16(d, rreg[g]);
         }
     };
     // inputs: thread i, load (half, group g): slot i / 8 + 32 g, 16 bytes i % 8 of the pair's 128
@@ -507,9 +542,16 @@ __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
     // Q4_K, Q5_K: [slot][piece 0 .. 3][block of the super-block] bf16, a block's sum of x in three pieces
     __shared__ __attribute__((aligned(16))) uint16_t sums[TY == 12 || TY == 13 ? 64 * 32 : 8];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t ti = blockIdx.x / a.row_tiles, rt_i = blockIdx.x % a.row_tiles;
-    if (ti >= *a.n_tiles) return;
-    const MoeTile t = a.tiles[ti];
+    // The work in the order (expert, row tile, tile of slots), cut into eight equal runs, one for each XCD
+    // (work-group i is on XCD i % 8): an expert's rows are then read by the L2 that all of its tiles go through, and
+    // a tile's inputs by one or two of them.
+    const uint32_t items = *a.n_tiles * a.row_tiles, run = (items + 7u) / 8u;
+    const uint32_t at = (blockIdx.x & 7u) * run + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= run || at >= items) return;
+    const MoeTile some = a.tiles[at / a.row_tiles];  // a tile of the expert
+    const uint32_t tile0 = at / a.row_tiles - some.index, in = at - tile0 * a.row_tiles;
+    const uint32_t rt_i = __builtin_amdgcn_readfirstlane(in / some.of);
+    const MoeTile t = a.tiles[tile0 + in % some.of];
     const uint32_t e = __builtin_amdgcn_readfirstlane(t.expert), count = __builtin_amdgcn_readfirstlane(t.count);
     const uint32_t *const slots = a.list + t.first;
     // this wave's rows: GU: 32 of each matrix from r0, else 64 from r0

@@ -119,7 +119,8 @@ int moe_product(moearc_ctx *c, MoeArgs a, unsigned ty, bool gate_up, bool half) 
     a.expert_bytes = a.row_bytes * a.rows;
     if (a.tiles) {
         a.row_tiles = (a.rows + (gate_up ? 127 : 255)) / (gate_up ? 128 : 256);
-        const unsigned grid = (unsigned) (a.row_tiles * moe_max_tiles(a.n_slots, a.n_expert, MOEARC_MOE_TILE));
+        const uint64_t most = a.row_tiles * moe_max_tiles(a.n_slots, a.n_expert, MOEARC_MOE_TILE);
+        const unsigned grid = (unsigned) ((most + 7) / 8 * 8);  // eight runs, one per XCD
         return launch(c, c->f_moe_tile[i][g][half], grid, 256, a, nullptr, a.rows, a.n_slots, name);
     }
     const uint64_t nb = a.cols / 32, gran = (ty == 12u || ty == 13u || ty == 14u) ? 8 : 1;
