@@ -305,6 +305,15 @@ struct MoeArgs {
     uint32_t clamped;          // the activation: 0 silu(g) u, 1 min(g, limit) sigmoid(alpha g) (clamp(u) + 1)
     float alpha, limit;
     uint32_t row_tiles;        // moe_tile.hip: row tiles per tile of slots
+    uint32_t y_order, pad;     // with two matrices: the type of the next product's weights, which orders y
+};
+
+// x as moe_tile.hip's products take it: f16 hi (and lo, of f32), each k-block in the order of weights of `type`
+struct MoePrepArgs {
+    const void *x;
+    uint16_t *hi, *lo;
+    uint64_t n;                // elements, a multiple of 32
+    uint32_t type, pad;
 };
 
 // y[t] (+)= sum_j weights[t][j] part[t * n_used + j] over the slots that have an expert, in order
@@ -318,4 +327,5 @@ struct MoeCombineArgs {
 #define MOEARC_MOE_SMALL_SLOTS 64u  // most slots of a launch without a plan
 #define MOEARC_MOE_SMALL_WAVES 8
 #define MOEARC_MOE_SMALL_TOKENS 16u
-#define MOEARC_MOE_TILE 64u         // most slots of a plan's tile
+#define MOEARC_MOE_TILE 64u         // most slots of a plan's tile, and of a light one
+#define MOEARC_MOE_LIGHT 32u

@@ -41,6 +41,17 @@ struct MoeTileFmt {
     static constexpr uint32_t RS = TY == 1 ? 144 : TY == 12 ? 152 : TY == 13 ? (HALVES == 2 ? 176 : 184) : TY == 14 ? 232 : 136;
 };
 
+// The order of a k-block's 32 inputs, the one in which its weights are cheapest to unpack (the sum does not
+// mind): MXFP4 elements j and j + 16 side by side, 4 j's a chunk of 8; K-quants 0 2 1 3 of every four.
+__device__ __forceinline__ uint32_t moe_place(uint32_t ty, uint32_t k) {  // where element k is
+    if (ty == 39u) {
+        const uint32_t j = k & 15u;
+        return 8u * (2u * ((j >> 2) & 1u) + (j >> 3)) + 2u * (j & 3u) + (k >> 4);
+    }
+    if (ty == 12u || ty == 13u || ty == 14u) return (k & ~3u) | ((k & 1u) << 1) | ((k >> 1) & 1u);
+    return k;
+}
+
 __device__ __forceinline__ uint32_t moe_swz(uint32_t t) { return (t >> 2) & 3u; }
 
 // Every LDS access of this wave is done, and then every wave's. Loads into registers stay in flight.
@@ -101,84 +112,116 @@ __device__ __forceinline__ void moe_get8(uint32_t &d0, uint32_t &d1, const uint8
     d1 = __builtin_amdgcn_alignbyte(w2, w1, off & 3u);
 }
 
-// The lane's elements of k-block i of a row's window in LDS, slices s = 0, 1: k 16 s + 8 h .. + 7, as f16
-// integers (MXFP4: E2M1 values times `scale`; F16: the weights). live: 0 gives zeros (MXFP4, F16).
-template <uint32_t TY>
-__device__ __forceinline__ void moe_payload(half8_t (&w)[2], const uint8_t *row, uint32_t i, uint32_t h, float scale, uint32_t live) {
-    if constexpr (TY == 1) {
+// The lane's operands of the pair of k-blocks 2 t, 2 t + 1 of a row's window in LDS, [block][slice s], each 8
+// elements in the order of moe_perm: f16 integers times the scale where the format allows. live 0: block 2 t as zeros.
+__device__ __forceinline__ uint32_t moe_and_or(uint32_t x, uint32_t mask, uint32_t o) { return (x & mask) | o; }
+__device__ __forceinline__ half2_t moe_h2(uint32_t bits) { return __builtin_bit_cast(half2_t, bits); }
+__device__ __forceinline__ void moe_set(half8_t &w, int k, half2_t p) {
+    w[k] = p[0];
+    w[k + 1] = p[1];
+}
+
+__device__ __forceinline__ void moe_f16_pair(half8_t (&w)[2][2], const uint8_t *row, uint32_t h, uint32_t live) {
+#pragma unroll
+    for (uint32_t b = 0; b < 2; ++b)
 #pragma unroll
         for (uint32_t s = 0; s < 2; ++s) {
-            u32x4_t v = *(const u32x4_t *) (row + 64u * i + 32u * s + 16u * h);
+            u32x4_t v = *(const u32x4_t *) (row + 64u * b + 32u * s + 16u * h);
+            if (b == 0u)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] &= live;
-            w[s] = __builtin_bit_cast(half8_t, v);
+                for (int k = 0; k < 4; ++k) v[k] &= live;
+            w[b][s] = __builtin_bit_cast(half8_t, v);
         }
-    } else if constexpr (TY == 8) {
+}
+__device__ __forceinline__ void moe_q8_pair(half8_t (&w)[2][2], const uint8_t *row, uint32_t t, uint32_t h) {
+#pragma unroll
+    for (uint32_t b = 0; b < 2; ++b)
 #pragma unroll
         for (uint32_t s = 0; s < 2; ++s) {
             uint32_t q0, q1;
-            moe_get8(q0, q1, row + 8u * h, 34u * i + 2u + 16u * s);
-            w[s] = mms_bytes<128>(q0 ^ 0x80808080u, q1 ^ 0x80808080u);
+            moe_get8(q0, q1, row + 8u * h, 34u * (2u * t + b) + 2u + 16u * s);
+            w[b][s] = mms_bytes<128>(q0 ^ 0x80808080u, q1 ^ 0x80808080u);
         }
-    } else if constexpr (TY == 39) {
-        uint32_t q[2];  // the low nibbles are slice 0's, the high ones slice 1's
-        moe_get8(q[0], q[1], row + 8u * h, 17u * i + 1u);
-        const uint32_t mask = 0x0F0F0F0Fu & live;
+}
+// A byte holds elements j and j + 16, the pair of one conversion.
+__device__ __forceinline__ void moe_mx_pair(half8_t (&w)[2][2], const uint8_t *row, uint32_t t, uint32_t h, const float (&scale)[2], uint32_t live) {
 #pragma unroll
-        for (uint32_t s = 0; s < 2; ++s)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t x = (q[j] >> (4u * s)) & mask;
-                const uint32_t y = x | (x >> 4);  // pairs in bytes 0 and 2
-                const half2_t p0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(y, scale, 0);
-                const half2_t p1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(y, scale, 2);
-                w[s][4 * j] = p0[0];
-                w[s][4 * j + 1] = p0[1];
-                w[s][4 * j + 2] = p1[0];
-                w[s][4 * j + 3] = p1[1];
-            }
-    } else if constexpr (TY == 12 || TY == 13) {
-        const uint32_t sh = 4u * (i & 1u);
+    for (uint32_t b = 0; b < 2; ++b) {
+        uint32_t q[2];
+        moe_get8(q[0], q[1], row + 8u * h, 17u * (2u * t + b) + 1u);
 #pragma unroll
         for (uint32_t s = 0; s < 2; ++s) {
-            uint32_t q0, q1;
-            moe_get8(q0, q1, row + 8u * h, (TY == 12 ? 16u : 48u) + 32u * (i >> 1) + 16u * s);
-            q0 = (q0 >> sh) & 0x0F0F0F0Fu;
-            q1 = (q1 >> sh) & 0x0F0F0F0Fu;
-            if constexpr (TY == 13) {
-                uint32_t h0, h1;
-                moe_get8(h0, h1, row + 8u * h, 16u + 16u * s);
-                q0 |= ((h0 >> i) & 0x01010101u) << 4;
-                q1 |= ((h1 >> i) & 0x01010101u) << 4;
-            }
-            w[s] = mms_bytes<0>(q0, q1);
-        }
-    } else {
-        static_assert(TY == 14, "a weight format");
-        const uint32_t n = i >> 2, c = i & 3u, shl = 4u * (c >> 1), shh = 2u * c;
-#pragma unroll
-        for (uint32_t s = 0; s < 2; ++s) {
-            uint32_t q0, q1, h0, h1;
-            moe_get8(q0, q1, row + 8u * h, 64u * n + 32u * (c & 1u) + 16u * s);
-            moe_get8(h0, h1, row + 8u * h, 128u + 32u * n + 16u * s);
-            w[s] = mms_bytes<32>(((q0 >> shl) & 0x0F0F0F0Fu) | (((h0 >> shh) & 0x03030303u) << 4),
-                                 ((q1 >> shl) & 0x0F0F0F0Fu) | (((h1 >> shh) & 0x03030303u) << 4));
+            const uint32_t d = b == 0u ? q[s] & live : q[s];
+            moe_set(w[b][s], 0, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, scale[b], 0));
+            moe_set(w[b][s], 2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, scale[b], 1));
+            moe_set(w[b][s], 4, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, scale[b], 2));
+            moe_set(w[b][s], 6, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, scale[b], 3));
         }
     }
+}
+// Block 2 t in the low nibbles, 2 t + 1 in the high ones of the same bytes. Under exponent 0x64 a low nibble q is
+// 1024 + q and a high one in its place 1024 + 16 q: one fused multiply-add leaves q times the scale, exactly.
+template <uint32_t TY>
+__device__ __forceinline__ void moe_q45_pair(half8_t (&w)[2][2], const uint8_t *row, uint32_t t, uint32_t h, const uint32_t (&sc)[2]) {
+    const float f0 = (float) sc[0], f1 = (float) sc[1];
+    const _Float16 m0 = (_Float16) f0, a0 = (_Float16) (-1024.f * f0), m1 = (_Float16) (0.0625f * f1), a1 = (_Float16) (-64.f * f1);
+#pragma unroll
+    for (uint32_t s = 0; s < 2; ++s) {
+        uint32_t q[2], hb[2] = {0u, 0u};
+        moe_get8(q[0], q[1], row + 8u * h, (TY == 12 ? 16u : 48u) + 32u * t + 16u * s);
+        if constexpr (TY == 13) moe_get8(hb[0], hb[1], row + 8u * h, 16u + 16u * s);
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+#pragma unroll
+            for (uint32_t odd = 0; odd < 2; ++odd) {  // bytes 0 and 2, 1 and 3
+                const uint32_t x = odd ? q[d] >> 8 : q[d];
+                uint32_t lo = moe_and_or(x, 0x000F000Fu, 0x64006400u), hi = moe_and_or(x, 0x00F000F0u, 0x64006400u);
+                if constexpr (TY == 13) {  // the fifth bits: bit 2 t (+ 1) of each byte, to bits 4 and 8
+                    const uint32_t at = 2u * t + 8u * odd;
+                    lo = moe_and_or(at < 4u ? hb[d] << (4u - at) : hb[d] >> (at - 4u), 0x00100010u, lo);
+                    hi = moe_and_or(at + 1u < 8u ? hb[d] << (7u - at) : hb[d] >> (at - 7u), 0x01000100u, hi);
+                }
+                const int k = 4 * d + 2 * (int) odd;
+                moe_set(w[0][s], k, __builtin_elementwise_fma(moe_h2(lo), half2_t{m0, m0}, half2_t{a0, a0}));
+                moe_set(w[1][s], k, __builtin_elementwise_fma(moe_h2(hi), half2_t{m1, m1}, half2_t{a1, a1}));
+            }
+        }
+    }
+}
+// Q6_K, without the scales: q - 32
+__device__ __forceinline__ void moe_q6_pair(half8_t (&w)[2][2], const uint8_t *row, uint32_t t, uint32_t h) {
+#pragma unroll
+    for (uint32_t b = 0; b < 2; ++b)
+#pragma unroll
+        for (uint32_t s = 0; s < 2; ++s) {
+            const uint32_t i = 2u * t + b, n = i >> 2, c = i & 3u, shl = 4u * (c >> 1), shh = 2u * c;
+            uint32_t q[2], hb[2];
+            moe_get8(q[0], q[1], row + 8u * h, 64u * n + 32u * (c & 1u) + 16u * s);
+            moe_get8(hb[0], hb[1], row + 8u * h, 128u + 32u * n + 16u * s);
+#pragma unroll
+            for (int d = 0; d < 2; ++d)
+#pragma unroll
+                for (uint32_t odd = 0; odd < 2; ++odd) {
+                    uint32_t x = moe_and_or(q[d] >> (shl + 8u * odd), 0x000F000Fu, 0x64006400u);
+                    const uint32_t at = shh + 8u * odd;
+                    x = moe_and_or(at < 4u ? hb[d] << (4u - at) : hb[d] >> (at - 4u), 0x00300030u, x);
+                    moe_set(w[b][s], 4 * d + 2 * (int) odd, moe_h2(x) - half2_t{(_Float16) 1056.f, (_Float16) 1056.f});
+                }
+        }
 }
 
 typedef __bf16 moe_bf8 __attribute__((ext_vector_type(8)));
 
 // The reduction of one tile for a wave: acc[slot half][row tile], slots 32 and up only with BOTH. FOLD (MXFP4):
 // the scales enter the operand; returns false where one is out of f16's range, and the sums are not valid then.
-template <uint32_t TY, bool GU, int HALVES, bool BOTH, bool FOLD>
+template <uint32_t TY, bool GU, int HALVES, bool LIGHT, bool BOTH, bool FOLD>
 __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc)[2][2], uint8_t *xbuf, uint8_t *wbuf, uint16_t *sums,
                                               uint32_t e, const uint32_t *slots, uint32_t count, uint32_t r0) {
     using F = MoeTileFmt<TY, HALVES>;
     constexpr uint32_t WB = F::WB, SPW = WB / 2u;
     constexpr bool Q45 = TY == 12 || TY == 13, Q6 = TY == 14, MX = TY == 39, KQ = Q45 || Q6;
     constexpr int NT = BOTH ? 2 : 1;
-    constexpr uint32_t XB = 4096u, XPAIR = 2u * HALVES * XB;  // one half of a k-block, a pair of k-blocks
+    constexpr uint32_t XB = LIGHT ? 2048u : 4096u, XPAIR = 2u * HALVES * XB;  // one half of a k-block, a pair of k-blocks
     const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 31u, h = lane >> 5;
     const uint32_t nb = a.cols / 32u, n_win = (nb + WB - 1u) / WB;
     // Window w starts at block w WB, the last one at nb - WB: its first `skip` blocks have been done. Whole
@@ -312,89 +355,98 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
     auto mul = [&](const half8_t &x, const half8_t &w, const moe_f32x16 &c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, w, c, 0, 0, 0);
     };
-    // k-block i of the window, block blk of the pair in buffer buf; live 0: taken as zero
-    auto compute = [&](uint32_t buf, uint32_t blk, uint32_t i, uint32_t live) {
-        half8_t x[HALVES][NT][2];
-#pragma unroll
-        for (int tt = 0; tt < NT; ++tt)
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int f = 0; f < HALVES; ++f) {
-                    const uint32_t u = 32u * tt + n;
-                    x[f][tt][s] = __builtin_bit_cast(half8_t, *(const u32x4_t *) (xbuf + buf * XPAIR + (blk * HALVES + f) * XB +
-                                                                                  u * 64u + 16u * ((2u * s + h) ^ moe_swz(u))));
-                }
+    // pair t of the window, in buffer buf; live 0: its first block taken as zero
+    auto compute = [&](uint32_t buf, uint32_t t, uint32_t live) {
+        half8_t w[2][2][2], lost[Q6 ? 2 : 1][2][2];  // [row tile][block][slice]
+        float f[2][2];
+        bool any[2][2] = {};
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
             const uint8_t *row = wbuf + (32u * rt + n) * F::RS;
-            half8_t w[2];
-            if constexpr (KQ) {
-                moe_payload<TY>(w, row, i, h, 1.f, live);
-                half8_t lost[2];
-                uint32_t any = 0u;
-                if constexpr (Q45) {
-                    const u32x2_t h0 = *(const u32x2_t *) row, h1 = *(const u32x2_t *) (row + 8);
-                    const uint32_t sc = counts[rt] ? moe_k4_scale(u32x4_t{h0[0], h0[1], h1[0], h1[1]}, i) : 0u;
+            if constexpr (TY == 1) {
+                moe_f16_pair(w[rt], row, h, live);
+            } else if constexpr (TY == 8) {
+                moe_q8_pair(w[rt], row, t, h);
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) w[s] = moe_times(w[s], (_Float16) (uint16_t) sc);
-                } else {
-                    const uint32_t sc = *(const uint16_t *) (row + 192u + 8u * (i >> 2) + 2u * (i & 3u));
+                for (uint32_t b = 0; b < 2; ++b) f[rt][b] = mms_f16(*(const uint16_t *) (row + 34u * (2u * t + b)));
+                f[rt][0] = live ? f[rt][0] : 0.f;
+            } else if constexpr (MX) {
+#pragma unroll
+                for (uint32_t b = 0; b < 2; ++b) {
+                    const uint32_t e8 = row[17u * (2u * t + b)];
+                    f[rt][b] = __uint_as_float(FOLD || e8 ? e8 << 23 : 0x00400000u);  // 2^(e - 127)
+                }
+                const float one[2] = {1.f, 1.f};
+                moe_mx_pair(w[rt], row, t, h, FOLD ? f[rt] : one, live);
+            } else if constexpr (Q45) {
+                const u32x2_t h0 = *(const u32x2_t *) row, h1 = *(const u32x2_t *) (row + 8);
+                uint32_t sc[2];
+#pragma unroll
+                for (uint32_t b = 0; b < 2; ++b) sc[b] = counts[rt] ? moe_k4_scale(u32x4_t{h0[0], h0[1], h1[0], h1[1]}, 2u * t + b) : 0u;
+                moe_q45_pair<TY>(w[rt], row, t, h, sc);
+            } else {
+                moe_q6_pair(w[rt], row, t, h);
+                const uint32_t sc = *(const uint32_t *) (row + 192u + 4u * t);  // scales 4 t .. + 3, two per block
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    uint32_t bits = 0u;
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
-                        const _Float16 f = counts[rt] ? (_Float16) (int16_t) (int8_t) (sc >> (8 * s)) : (_Float16) 0.f;
-                        const half8_t q = w[s];
-                        w[s] = moe_times(q, f);
-                        lost[s] = moe_lost(q, f, w[s]);
-                        const u32x4_t bits = __builtin_bit_cast(u32x4_t, lost[s]);
-                        any |= (bits[0] | bits[1] | bits[2] | bits[3]) & 0x7FFF7FFFu;
+                        const _Float16 m = counts[rt] ? (_Float16) (int16_t) (int8_t) (sc >> (16 * b + 8 * s)) : (_Float16) 0.f;
+                        const half8_t q = w[rt][b][s];
+                        w[rt][b][s] = moe_times(q, m);
+                        lost[rt][b][s] = moe_lost(q, m, w[rt][b][s]);
+                        const u32x4_t v = __builtin_bit_cast(u32x4_t, lost[rt][b][s]);
+                        bits |= (v[0] | v[1] | v[2] | v[3]) & 0x7FFF7FFFu;
                     }
+                    any[rt][b] = __ballot(bits != 0u) != 0ull;  // some product of the wave was rounded
                 }
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            half8_t x[HALVES][NT][2];
+#pragma unroll
+            for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int f = 0; f < HALVES; ++f)
-#pragma unroll
-                        for (int tt = 0; tt < NT; ++tt) acc[tt][rt] = mul(x[f][tt][s], w[s], acc[tt][rt]);
-                if constexpr (Q6)
-                    if (__ballot(any != 0u) != 0ull) {  // some product of the wave was rounded
-#pragma unroll
-                        for (int s = 0; s < 2; ++s)
-#pragma unroll
-                            for (int tt = 0; tt < NT; ++tt) acc[tt][rt] = mul(x[0][tt][s], lost[s], acc[tt][rt]);
+                    for (int g = 0; g < HALVES; ++g) {
+                        const uint32_t u = 32u * tt + n;
+                        x[g][tt][s] = __builtin_bit_cast(half8_t, *(const u32x4_t *) (xbuf + buf * XPAIR + (b * HALVES + g) * XB +
+                                                                                      u * 64u + 16u * ((2u * s + h) ^ moe_swz(u))));
                     }
-            } else if constexpr (TY == 1 || FOLD) {
-                float f = 1.f;
-                if constexpr (FOLD) f = __uint_as_float((uint32_t) row[17u * i] << 23);  // 2^(e - 127)
-                moe_payload<TY>(w, row, i, h, f, live);
 #pragma unroll
-                for (int s = 0; s < 2; ++s)
+            for (int rt = 0; rt < 2; ++rt) {
+                if constexpr (TY == 1 || KQ || FOLD) {
 #pragma unroll
-                    for (int f = 0; f < HALVES; ++f)
+                    for (int s = 0; s < 2; ++s)
 #pragma unroll
-                        for (int tt = 0; tt < NT; ++tt) acc[tt][rt] = mul(x[f][tt][s], w[s], acc[tt][rt]);
-            } else {
-                float f;
-                if constexpr (MX) {
-                    const uint32_t e8 = row[17u * i];
-                    f = __uint_as_float(e8 ? e8 << 23 : 0x00400000u);  // 2^(e - 127)
+                        for (int g = 0; g < HALVES; ++g)
+#pragma unroll
+                            for (int tt = 0; tt < NT; ++tt) acc[tt][rt] = mul(x[g][tt][s], w[rt][b][s], acc[tt][rt]);
+                    if constexpr (Q6)
+                        if (any[rt][b]) {
+#pragma unroll
+                            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                                for (int tt = 0; tt < NT; ++tt) acc[tt][rt] = mul(x[0][tt][s], lost[rt][b][s], acc[tt][rt]);
+                        }
                 } else {
-                    f = live ? mms_f16(*(const uint16_t *) (row + 34u * i)) : 0.f;
+                    moe_f32x16 d[NT];
+#pragma unroll
+                    for (int tt = 0; tt < NT; ++tt) d[tt] = moe_f32x16{};
+#pragma unroll
+                    for (int s = 0; s < 2; ++s)
+#pragma unroll
+                        for (int g = 0; g < HALVES; ++g)
+#pragma unroll
+                            for (int tt = 0; tt < NT; ++tt) d[tt] = mul(x[g][tt][s], w[rt][b][s], d[tt]);
+#pragma unroll
+                    for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) acc[tt][rt][j] = fmaf(f[rt][b], d[tt][j], acc[tt][rt][j]);
                 }
-                moe_payload<TY>(w, row, i, h, 1.f, live);
-                moe_f32x16 d[NT];
-#pragma unroll
-                for (int tt = 0; tt < NT; ++tt) d[tt] = moe_f32x16{};
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int f = 0; f < HALVES; ++f)
-#pragma unroll
-                        for (int tt = 0; tt < NT; ++tt) d[tt] = mul(x[f][tt][s], w[s], d[tt]);
-#pragma unroll
-                for (int tt = 0; tt < NT; ++tt)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) acc[tt][rt][j] = fmaf(f, d[tt][j], acc[tt][rt][j]);
             }
         }
     };
@@ -479,8 +531,7 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
             }
             xload(min(step + 2u, total - 1u));
             __builtin_amdgcn_sched_barrier(0);  // left alone, the loads sink to the step's end, and the next waits for them
-            compute(buf, 0u, 2u * j, j == from ? live0 : 0xFFFFFFFFu);
-            compute(buf, 1u, 2u * j + 1u, 0xFFFFFFFFu);
+            compute(buf, j, j == from ? live0 : 0xFFFFFFFFu);
             if constexpr (Q45)
                 if (j + 1u == SPW) mins();
             moe_barrier();
@@ -498,19 +549,22 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
     return ok;
 }
 
-template <uint32_t TY, bool GU, int HALVES, bool BOTH>
+template <uint32_t TY, bool GU, int HALVES, bool LIGHT, bool BOTH>
 __device__ __forceinline__ void moe_tile_half(const MoeArgs &a, uint8_t *xbuf, uint8_t *wbuf, uint16_t *sums, uint32_t e,
                                               const uint32_t *slots, uint32_t count, uint32_t r0) {
     const uint32_t lane = threadIdx.x & 63u, n = lane & 31u, h = lane >> 5;
     moe_f32x16 acc[2][2];
-    const bool ok = moe_tile_sums<TY, GU, HALVES, BOTH, TY == 39>(a, acc, xbuf, wbuf, sums, e, slots, count, r0);
+    const bool ok = moe_tile_sums<TY, GU, HALVES, LIGHT, BOTH, TY == 39>(a, acc, xbuf, wbuf, sums, e, slots, count, r0);
     if constexpr (TY == 39)  // some scale out of range: again, every block's sum scaled by itself
         if (__syncthreads_or(!ok))
-            (void) moe_tile_sums<TY, GU, HALVES, BOTH, false>(a, acc, xbuf, wbuf, sums, e, slots, count, r0);
+            (void) moe_tile_sums<TY, GU, HALVES, LIGHT, BOTH, false>(a, acc, xbuf, wbuf, sums, e, slots, count, r0);
 #pragma unroll
     for (int rt = 0; rt < (GU ? 1 : 2); ++rt) {
         const uint32_t r = r0 + 32u * rt + n;
         if (r >= a.rows) continue;
+        // GU: where the next product, whose weights are of type a.y_order, looks for column r (a short last block
+        // does not occur: that product has whole blocks of columns)
+        const uint32_t rp = GU ? (r & ~31u) | moe_place(a.y_order, r & 31u) : 0u;
         const float b0 = a.bias[0] ? a.bias[0][(uint64_t) e * a.rows + r] : 0.f;
         const float b1 = GU && a.bias[1] ? a.bias[1][(uint64_t) e * a.rows + r] : 0.f;
 #pragma unroll
@@ -519,7 +573,7 @@ __device__ __forceinline__ void moe_tile_half(const MoeArgs &a, uint8_t *xbuf, u
             for (int j = 0; j < 16; ++j) {
                 const uint32_t u = 32u * tt + 8u * (j >> 2) + 4u * h + (j & 3);
                 if (u >= count) continue;
-                const uint64_t o = (uint64_t) slots[u] * a.rows + r;
+                const uint64_t o = (uint64_t) slots[u] * a.rows + (GU ? rp : r);
                 if constexpr (GU) {
                     const float v = moe_activation(a, acc[tt][0][j] + b0, acc[tt][1][j] + b1);
                     const _Float16 hi = (_Float16) v;
@@ -534,13 +588,13 @@ __device__ __forceinline__ void moe_tile_half(const MoeArgs &a, uint8_t *xbuf, u
     }
 }
 
-template <uint32_t TY, bool GU, int HALVES>
+template <uint32_t TY, bool GU, int HALVES, bool LIGHT>
 __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
     using F = MoeTileFmt<TY, HALVES>;
-    __shared__ __attribute__((aligned(1024))) uint8_t xbuf[4 * HALVES * 4096];
+    __shared__ __attribute__((aligned(1024))) uint8_t xbuf[4 * HALVES * (LIGHT ? 2048 : 4096)];
     __shared__ __attribute__((aligned(16))) uint8_t wbuf[4][64 * F::RS];
     // Q4_K, Q5_K: [slot][piece 0 .. 3][block of the super-block] bf16, a block's sum of x in three pieces
-    __shared__ __attribute__((aligned(16))) uint16_t sums[TY == 12 || TY == 13 ? 64 * 32 : 8];
+    __shared__ __attribute__((aligned(16))) uint16_t sums[TY == 12 || TY == 13 ? (LIGHT ? 32 : 64) * 32 : 8];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // The work in the order (expert, row tile, tile of slots), cut into eight equal runs, one for each XCD
     // (work-group i is on XCD i % 8): an expert's rows are then read by the L2 that all of its tiles go through, and
@@ -566,24 +620,64 @@ __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
             }
         return;
     }
-    if (count > 32u) moe_tile_half<TY, GU, HALVES, true>(a, xbuf, wbuf[wave], sums, e, slots, count, r0);
-    else moe_tile_half<TY, GU, HALVES, false>(a, xbuf, wbuf[wave], sums, e, slots, count, r0);
+    if constexpr (!LIGHT)
+        if (count > 32u) return moe_tile_half<TY, GU, HALVES, false, true>(a, xbuf, wbuf[wave], sums, e, slots, count, r0);
+    moe_tile_half<TY, GU, HALVES, LIGHT, false>(a, xbuf, wbuf[wave], sums, e, slots, count, r0);
+}
+
+// x for the tiles: f16 (of f32: hi, and the remainder lo) in the order of the weights' type, eight elements,
+// one chunk, per thread.
+template <bool F32>
+__device__ __forceinline__ void moe_prep_body(const MoePrepArgs &a) {
+    for (uint64_t i = (uint64_t) blockIdx.x * 256u + threadIdx.x; i < a.n / 8u; i += (uint64_t) gridDim.x * 256u) {
+        const uint32_t c = (uint32_t) i & 3u;
+        const uint64_t blk = (i >> 2) * 32u;
+        // the chunk's elements: two runs of four, from k0 and k1
+        const bool mx = a.type == 39u, kq = a.type == 12u || a.type == 13u || a.type == 14u;
+        const uint32_t k0 = mx ? 8u * (c & 1u) + 4u * (c >> 1) : 8u * c, k1 = mx ? k0 + 16u : k0 + 4u;
+        _Float16 vh[8], vl[8];
+        if constexpr (F32) {
+            float v[8];
+            __builtin_memcpy(v, (const float *) a.x + blk + k0, 16);
+            __builtin_memcpy(v + 4, (const float *) a.x + blk + k1, 16);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                vh[k] = (_Float16) v[k];
+                vl[k] = (_Float16) (v[k] - (float) vh[k]);
+            }
+        } else {
+            __builtin_memcpy(vh, (const _Float16 *) a.x + blk + k0, 8);
+            __builtin_memcpy(vh + 4, (const _Float16 *) a.x + blk + k1, 8);
+        }
+        half8_t hi, lo;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            const int q = (p & 4) | ((p & 1) << 1) | ((p >> 1) & 1), m = (p >> 1) | ((p & 1) << 2);
+            hi[p] = mx ? vh[m] : kq ? vh[q] : vh[p];
+            if constexpr (F32) lo[p] = mx ? vl[m] : kq ? vl[q] : vl[p];
+        }
+        *(half8_t *) (a.hi + 8u * i) = hi;
+        if constexpr (F32) *(half8_t *) (a.lo + 8u * i) = lo;
+    }
 }
 
 }  // namespace
 
-#define MOE_TILE(NAME, TY)                                                                                      \
+#define MOE_TILE_KERNEL(NAME, TY, KIND, GU, IO, HALVES)                                                        \
     extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))                \
-    moearc_moe_tile_##NAME##_gu_f32_k(MoeArgs a) { moe_tile_body<TY, true, 2>(a); }                             \
-    extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))                \
-    moearc_moe_tile_##NAME##_gu_f16_k(MoeArgs a) { moe_tile_body<TY, true, 1>(a); }                             \
-    extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))                \
-    moearc_moe_tile_##NAME##_p_f32_k(MoeArgs a) { moe_tile_body<TY, false, 2>(a); }                             \
-    extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))                \
-    moearc_moe_tile_##NAME##_p_f16_k(MoeArgs a) { moe_tile_body<TY, false, 1>(a); }
+    moearc_moe_tile_##NAME##_##KIND##_##IO##_k(MoeArgs a) { moe_tile_body<TY, GU, HALVES, false>(a); }          \
+    extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3)))                \
+    moearc_moe_light_##NAME##_##KIND##_##IO##_k(MoeArgs a) { moe_tile_body<TY, GU, HALVES, true>(a); }
+#define MOE_TILE(NAME, TY)                     \
+    MOE_TILE_KERNEL(NAME, TY, gu, true, f32, 2) \
+    MOE_TILE_KERNEL(NAME, TY, gu, true, f16, 1) \
+    MOE_TILE_KERNEL(NAME, TY, p, false, f32, 2) \
+    MOE_TILE_KERNEL(NAME, TY, p, false, f16, 1)
 MOE_TILE(f16, 1)
 MOE_TILE(q8_0, 8)
 MOE_TILE(q4_k, 12)
 MOE_TILE(q5_k, 13)
 MOE_TILE(q6_k, 14)
 MOE_TILE(mxfp4, 39)
+extern "C" __global__ void __launch_bounds__(256) moearc_moe_prep_f32_k(MoePrepArgs a) { moe_prep_body<true>(a); }
+extern "C" __global__ void __launch_bounds__(256) moearc_moe_prep_f16_k(MoePrepArgs a) { moe_prep_body<false>(a); }

@@ -25,7 +25,7 @@ MoeSpace moe_space(uint64_t n_tok, uint64_t n_used, uint64_t n_expert, uint64_t 
     const uint64_t tok = std::min<uint64_t>(n_tok, std::max<uint64_t>(1, kMoeChunkSlots / n_used)), slots = tok * n_used;
     MoeSpace s;
     s.tiles = 256;
-    s.list = s.tiles + align256(sizeof(MoeTile) * moe_max_tiles(slots, n_expert, MOEARC_MOE_TILE));
+    s.list = s.tiles + align256(sizeof(MoeTile) * moe_max_tiles(slots, n_expert, MOEARC_MOE_LIGHT));
     s.split = s.list + align256(4 * slots);
     s.split_n = (n_ff ? tok : slots) * n_embd;  // a product alone may have a row of x for each slot
     s.act_n = slots * n_ff;
@@ -74,6 +74,12 @@ int moe_count_check(unsigned long n_tok, unsigned long n_used, unsigned long n_e
     return OK;
 }
 
+// Whether a chunk runs on tiles of 32 slots.
+bool moe_light(uint64_t n_slots, uint64_t n_expert) {
+    static const char *const e = std::getenv("MOE_LIGHT");
+    return n_slots <= (e ? std::strtoul(e, nullptr, 10) : 32) * n_expert;
+}
+
 // Groups a chunk's slots by expert. Launches of at most 64 slots need no plan.
 int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slots, uint32_t n_expert, uint8_t *ws,
              const MoeSpace &sp) {
@@ -91,23 +97,26 @@ int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slot
     p.err = c->err_word;
     p.n_slots = n_slots;
     p.n_expert = n_expert;
-    p.tile = MOEARC_MOE_TILE;
+    p.tile = moe_light(n_slots, n_expert) ? MOEARC_MOE_LIGHT : MOEARC_MOE_TILE;
     a.tiles = p.tiles;
     a.n_tiles = p.n_tiles;
     a.list = p.list;
     return launch(c, c->f_moe_plan, n_expert + 1, 1024, p, nullptr, n_slots, n_expert, "moe_plan");
 }
 
-// x (n floats, a multiple of 32) as f16 hi + lo for the tiles' matrix cores.
-int moe_split(moearc_ctx *c, const float *x, size_t n, uint16_t *hi, uint16_t *lo) {
-    const bool by8 = (uintptr_t) x % 16 == 0;
-    struct {
-        const float *x;
-        uint16_t *hi, *lo;
-        uint64_t n;
-    } a{x, hi, lo, by8 ? n / 8 : n};
-    return launch(c, by8 ? c->f_split8 : c->f_split, (unsigned) std::min<size_t>((a.n + 255) / 256, 65536), 256, a, nullptr, n, 0,
-                  "split_f16");
+// x for the tiles' matrix cores, as MoePrepArgs. f16 inputs of types whose order is the natural one are taken as
+// they are.
+int moe_prep(moearc_ctx *c, MoeArgs &a, unsigned ty, bool half, size_t n, uint8_t *space, size_t space_n) {
+    if (half && (ty == 1u || ty == 8u)) return OK;
+    MoePrepArgs p{};
+    p.x = a.x;
+    p.hi = (uint16_t *) space;
+    p.lo = p.hi + space_n;
+    p.n = n;
+    p.type = ty;
+    a.x = p.hi;
+    a.x_lo = p.lo;
+    return launch(c, c->f_moe_prep[half], (unsigned) std::min<size_t>((n / 8 + 255) / 256, 65536), 256, p, nullptr, n, 0, "moe_prep");
 }
 
 // One grouped product (two matrices: gate, up and their activation). Without a plan x is as the caller's
@@ -119,9 +128,10 @@ int moe_product(moearc_ctx *c, MoeArgs a, unsigned ty, bool gate_up, bool half) 
     a.expert_bytes = a.row_bytes * a.rows;
     if (a.tiles) {
         a.row_tiles = (a.rows + (gate_up ? 127 : 255)) / (gate_up ? 128 : 256);
-        const uint64_t most = a.row_tiles * moe_max_tiles(a.n_slots, a.n_expert, MOEARC_MOE_TILE);
+        const bool light = moe_light(a.n_slots, a.n_expert);
+        const uint64_t most = a.row_tiles * moe_max_tiles(a.n_slots, a.n_expert, light ? MOEARC_MOE_LIGHT : MOEARC_MOE_TILE);
         const unsigned grid = (unsigned) ((most + 7) / 8 * 8);  // eight runs, one per XCD
-        return launch(c, c->f_moe_tile[i][g][half], grid, 256, a, nullptr, a.rows, a.n_slots, name);
+        return launch(c, (light ? c->f_moe_light : c->f_moe_tile)[i][g][half], grid, 256, a, nullptr, a.rows, a.n_slots, name);
     }
     const uint64_t nb = a.cols / 32, gran = (ty == 12u || ty == 13u || ty == 14u) ? 8 : 1;
     a.kb_per = (uint32_t) (((nb + MOEARC_MOE_SMALL_WAVES - 1) / MOEARC_MOE_SMALL_WAVES + gran - 1) / gran * gran);
@@ -162,6 +172,7 @@ bool moe_load(moearc_ctx *c) {
         {&c->f_route[2], "moearc_moe_route_p4_k"},    {&c->f_route[3], "moearc_moe_route_p8_k"},
         {&c->f_route[4], "moearc_moe_route_p16_k"},   {&c->f_route[5], "moearc_moe_route_p32_k"},
         {&c->f_route[6], "moearc_moe_route_p64_k"},   {&c->f_moe_plan, "moearc_moe_plan_k"},
+        {&c->f_moe_prep[0], "moearc_moe_prep_f32_k"}, {&c->f_moe_prep[1], "moearc_moe_prep_f16_k"},
         {&c->f_moe_combine[0], "moearc_moe_combine_k"}, {&c->f_moe_combine[1], "moearc_moe_combine4_k"},
     };
     auto get = [&](hipFunction_t *slot, const char *name) {
@@ -178,6 +189,8 @@ bool moe_load(moearc_ctx *c) {
             if (!get(&c->f_moe_small[t][i >> 1][i & 1], name)) return false;
             std::snprintf(name, sizeof(name), "moearc_moe_tile_%s_%s_%s_k", kMoeNames[t], i & 2 ? "p" : "gu", i & 1 ? "f16" : "f32");
             if (!get(&c->f_moe_tile[t][i >> 1][i & 1], name)) return false;
+            std::snprintf(name, sizeof(name), "moearc_moe_light_%s_%s_%s_k", kMoeNames[t], i & 2 ? "p" : "gu", i & 1 ? "f16" : "f32");
+            if (!get(&c->f_moe_light[t][i >> 1][i & 1], name)) return false;
         }
     return true;
 }
@@ -268,12 +281,8 @@ int moearc_matmul_experts(moearc_ctx *c, unsigned int type_id, void *y, const vo
         a.x = (const uint8_t *) x + (x_per_slot ? t * n_used : t) * n_cols * elem;
         a.x_div = x_per_slot ? 1u : (uint32_t) n_used;
         const bool half = io_type == MOEARC_OUT_F16;
-        if (a.tiles && !half) {
-            uint16_t *const hi = (uint16_t *) (mem + sp.split), *const lo = hi + sp.split_n;
-            if (const int rc = moe_split(c, (const float *) a.x, (x_per_slot ? n * n_used : n) * n_cols, hi, lo)) return rc;
-            a.x = hi;
-            a.x_lo = lo;
-        }
+        if (a.tiles)
+            if (const int rc = moe_prep(c, a, type_id, half, (x_per_slot ? n * n_used : n) * n_cols, mem + sp.split, sp.split_n)) return rc;
         a.w[0] = (const uint8_t *) w;
         a.bias[0] = bias;
         a.y = (uint8_t *) y + t * n_used * n_rows * elem;
@@ -318,12 +327,9 @@ int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, u
             g.w[i] = (const uint8_t *) m->w[i];
             g.bias[i] = m->bias[i];
         }
-        if (a.tiles && !half) {
-            uint16_t *const hi = (uint16_t *) (mem + sp.split), *const lo = hi + sp.split_n;
-            if (const int rc = moe_split(c, (const float *) g.x, n * m->n_embd, hi, lo)) return rc;
-            g.x = hi;
-            g.x_lo = lo;
-        }
+        if (a.tiles)
+            if (const int rc = moe_prep(c, g, m->w_type[0], half, n * m->n_embd, mem + sp.split, sp.split_n)) return rc;
+        g.y_order = m->w_type[2];
         g.y = mem + sp.act;
         g.y_lo = (uint16_t *) (mem + sp.act) + sp.act_n;
         d.x_lo = g.y_lo;
