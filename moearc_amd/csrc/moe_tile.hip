@@ -112,102 +112,103 @@ __device__ __forceinline__ void moe_get8(uint32_t &d0, uint32_t &d1, const uint8
     d1 = __builtin_amdgcn_alignbyte(w2, w1, off & 3u);
 }
 
-// The lane's operands of the pair of k-blocks 2 t, 2 t + 1 of a row's window in LDS, [block][slice s], each 8
-// elements in the order of moe_perm: f16 integers times the scale where the format allows. live 0: block 2 t as zeros.
-__device__ __forceinline__ uint32_t moe_and_or(uint32_t x, uint32_t mask, uint32_t o) { return (x & mask) | o; }
+// The lane's operands of k-block i of a row's window in LDS, slices s = 0, 1, 8 elements each in the order of
+// moe_place: f16 integers, times the scale where the format allows. live 0: zeros.
 __device__ __forceinline__ half2_t moe_h2(uint32_t bits) { return __builtin_bit_cast(half2_t, bits); }
 __device__ __forceinline__ void moe_set(half8_t &w, int k, half2_t p) {
     w[k] = p[0];
     w[k + 1] = p[1];
 }
-
-__device__ __forceinline__ void moe_f16_pair(half8_t (&w)[2][2], const uint8_t *row, uint32_t h, uint32_t live) {
+__device__ __forceinline__ void moe_f16_block(half8_t (&w)[2], const uint8_t *row, uint32_t i, uint32_t h, uint32_t live) {
 #pragma unroll
-    for (uint32_t b = 0; b < 2; ++b)
+    for (uint32_t s = 0; s < 2; ++s) {
+        u32x4_t v = *(const u32x4_t *) (row + 64u * i + 32u * s + 16u * h);
 #pragma unroll
-        for (uint32_t s = 0; s < 2; ++s) {
-            u32x4_t v = *(const u32x4_t *) (row + 64u * b + 32u * s + 16u * h);
-            if (b == 0u)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] &= live;
-            w[b][s] = __builtin_bit_cast(half8_t, v);
-        }
-}
-__device__ __forceinline__ void moe_q8_pair(half8_t (&w)[2][2], const uint8_t *row, uint32_t t, uint32_t h) {
-#pragma unroll
-    for (uint32_t b = 0; b < 2; ++b)
-#pragma unroll
-        for (uint32_t s = 0; s < 2; ++s) {
-            uint32_t q0, q1;
-            moe_get8(q0, q1, row + 8u * h, 34u * (2u * t + b) + 2u + 16u * s);
-            w[b][s] = mms_bytes<128>(q0 ^ 0x80808080u, q1 ^ 0x80808080u);
-        }
-}
-// A byte holds elements j and j + 16, the pair of one conversion.
-__device__ __forceinline__ void moe_mx_pair(half8_t (&w)[2][2], const uint8_t *row, uint32_t t, uint32_t h, const float (&scale)[2], uint32_t live) {
-#pragma unroll
-    for (uint32_t b = 0; b < 2; ++b) {
-        uint32_t q[2];
-        moe_get8(q[0], q[1], row + 8u * h, 17u * (2u * t + b) + 1u);
-#pragma unroll
-        for (uint32_t s = 0; s < 2; ++s) {
-            const uint32_t d = b == 0u ? q[s] & live : q[s];
-            moe_set(w[b][s], 0, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, scale[b], 0));
-            moe_set(w[b][s], 2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, scale[b], 1));
-            moe_set(w[b][s], 4, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, scale[b], 2));
-            moe_set(w[b][s], 6, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, scale[b], 3));
-        }
+        for (int k = 0; k < 4; ++k) v[k] &= live;
+        w[s] = __builtin_bit_cast(half8_t, v);
     }
 }
-// Block 2 t in the low nibbles, 2 t + 1 in the high ones of the same bytes. Under exponent 0x64 a low nibble q is
-// 1024 + q and a high one in its place 1024 + 16 q: one fused multiply-add leaves q times the scale, exactly.
+__device__ __forceinline__ void moe_q8_block(half8_t (&w)[2], const uint8_t *row, uint32_t i, uint32_t h) {
+#pragma unroll
+    for (uint32_t s = 0; s < 2; ++s) {
+        uint32_t q0, q1;
+        moe_get8(q0, q1, row + 8u * h, 34u * i + 2u + 16u * s);
+        w[s] = mms_bytes<128>(q0 ^ 0x80808080u, q1 ^ 0x80808080u);
+    }
+}
+// A byte holds elements j and j + 16, the pair of one conversion.
+__device__ __forceinline__ void moe_mx_block(half8_t (&w)[2], const uint8_t *row, uint32_t i, uint32_t h, float scale, uint32_t live) {
+    uint32_t q[2];
+    moe_get8(q[0], q[1], row + 8u * h, 17u * i + 1u);
+#pragma unroll
+    for (uint32_t s = 0; s < 2; ++s) {
+        const uint32_t d = q[s] & live;
+        moe_set(w[s], 0, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, scale, 0));
+        moe_set(w[s], 2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, scale, 1));
+        moe_set(w[s], 4, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, scale, 2));
+        moe_set(w[s], 6, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, scale, 3));
+    }
+}
+// (x & MASK) | over in one instruction, which takes no literal: the mask from a scalar register, which the
+// compiler, left to know its value, puts back as a literal of an instruction of its own.
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t moe_over(uint32_t x, uint32_t over) {
+    uint32_t mask;
+    asm("s_mov_b32 %0, %1" : "=s"(mask) : "i"(MASK));
+    return (x & mask) | over;
+}
+__device__ __forceinline__ uint32_t moe_exponent() {  // under which a half's low bits are 1024 + the integer
+    uint32_t v;
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(v));
+    return v;
+}
+// Even blocks lie in the low nibbles, odd ones in the high nibbles of the same bytes. Under exponent 0x64 a low
+// nibble q is 1024 + q and a high one in its place 1024 + 16 q: one fused multiply-add leaves q times the scale,
+// exactly.
 template <uint32_t TY>
-__device__ __forceinline__ void moe_q45_pair(half8_t (&w)[2][2], const uint8_t *row, uint32_t t, uint32_t h, const uint32_t (&sc)[2]) {
-    const float f0 = (float) sc[0], f1 = (float) sc[1];
-    const _Float16 m0 = (_Float16) f0, a0 = (_Float16) (-1024.f * f0), m1 = (_Float16) (0.0625f * f1), a1 = (_Float16) (-64.f * f1);
+__device__ __forceinline__ void moe_q45_block(half8_t (&w)[2], const uint8_t *row, uint32_t i, uint32_t h, uint32_t sc) {
+    const bool high = i & 1u;
+    const _Float16 f = (_Float16) (uint16_t) sc, m = high ? f * (_Float16) 0.0625f : f, a = f * (_Float16) (high ? -64.f : -1024.f);
+    const uint32_t exponent = moe_exponent();
 #pragma unroll
     for (uint32_t s = 0; s < 2; ++s) {
         uint32_t q[2], hb[2] = {0u, 0u};
-        moe_get8(q[0], q[1], row + 8u * h, (TY == 12 ? 16u : 48u) + 32u * t + 16u * s);
+        moe_get8(q[0], q[1], row + 8u * h, (TY == 12 ? 16u : 48u) + 32u * (i >> 1) + 16u * s);
         if constexpr (TY == 13) moe_get8(hb[0], hb[1], row + 8u * h, 16u + 16u * s);
 #pragma unroll
-        for (int d = 0; d < 2; ++d) {
+        for (int d = 0; d < 2; ++d)
 #pragma unroll
             for (uint32_t odd = 0; odd < 2; ++odd) {  // bytes 0 and 2, 1 and 3
                 const uint32_t x = odd ? q[d] >> 8 : q[d];
-                uint32_t lo = moe_and_or(x, 0x000F000Fu, 0x64006400u), hi = moe_and_or(x, 0x00F000F0u, 0x64006400u);
-                if constexpr (TY == 13) {  // the fifth bits: bit 2 t (+ 1) of each byte, to bits 4 and 8
-                    const uint32_t at = 2u * t + 8u * odd;
-                    lo = moe_and_or(at < 4u ? hb[d] << (4u - at) : hb[d] >> (at - 4u), 0x00100010u, lo);
-                    hi = moe_and_or(at + 1u < 8u ? hb[d] << (7u - at) : hb[d] >> (at - 7u), 0x01000100u, hi);
+                uint32_t v = high ? moe_over<0x00F000F0u>(x, exponent) : moe_over<0x000F000Fu>(x, exponent);
+                if constexpr (TY == 13) {  // the fifth bits: bit i of each byte, to bit 4 (8)
+                    const uint32_t from = i + 8u * odd, to = high ? 8u : 4u;
+                    const uint32_t y = from < to ? hb[d] << (to - from) : hb[d] >> (from - to);
+                    v = high ? moe_over<0x01000100u>(y, v) : moe_over<0x00100010u>(y, v);
                 }
-                const int k = 4 * d + 2 * (int) odd;
-                moe_set(w[0][s], k, __builtin_elementwise_fma(moe_h2(lo), half2_t{m0, m0}, half2_t{a0, a0}));
-                moe_set(w[1][s], k, __builtin_elementwise_fma(moe_h2(hi), half2_t{m1, m1}, half2_t{a1, a1}));
+                moe_set(w[s], 4 * d + 2 * (int) odd, __builtin_elementwise_fma(moe_h2(v), half2_t{m, m}, half2_t{a, a}));
             }
-        }
     }
 }
 // Q6_K, without the scales: q - 32
-__device__ __forceinline__ void moe_q6_pair(half8_t (&w)[2][2], const uint8_t *row, uint32_t t, uint32_t h) {
+__device__ __forceinline__ void moe_q6_block(half8_t (&w)[2], const uint8_t *row, uint32_t i, uint32_t h) {
+    const uint32_t exponent = moe_exponent();
 #pragma unroll
-    for (uint32_t b = 0; b < 2; ++b)
+    for (uint32_t s = 0; s < 2; ++s) {
+        const uint32_t n = i >> 2, c = i & 3u, shl = 4u * (c >> 1), shh = 2u * c;
+        uint32_t q[2], hb[2];
+        moe_get8(q[0], q[1], row + 8u * h, 64u * n + 32u * (c & 1u) + 16u * s);
+        moe_get8(hb[0], hb[1], row + 8u * h, 128u + 32u * n + 16u * s);
 #pragma unroll
-        for (uint32_t s = 0; s < 2; ++s) {
-            const uint32_t i = 2u * t + b, n = i >> 2, c = i & 3u, shl = 4u * (c >> 1), shh = 2u * c;
-            uint32_t q[2], hb[2];
-            moe_get8(q[0], q[1], row + 8u * h, 64u * n + 32u * (c & 1u) + 16u * s);
-            moe_get8(hb[0], hb[1], row + 8u * h, 128u + 32u * n + 16u * s);
+        for (int d = 0; d < 2; ++d)
 #pragma unroll
-            for (int d = 0; d < 2; ++d)
-#pragma unroll
-                for (uint32_t odd = 0; odd < 2; ++odd) {
-                    uint32_t x = moe_and_or(q[d] >> (shl + 8u * odd), 0x000F000Fu, 0x64006400u);
-                    const uint32_t at = shh + 8u * odd;
-                    x = moe_and_or(at < 4u ? hb[d] << (4u - at) : hb[d] >> (at - 4u), 0x00300030u, x);
-                    moe_set(w[b][s], 4 * d + 2 * (int) odd, moe_h2(x) - half2_t{(_Float16) 1056.f, (_Float16) 1056.f});
-                }
-        }
+            for (uint32_t odd = 0; odd < 2; ++odd) {
+                const uint32_t from = shh + 8u * odd;
+                const uint32_t y = from < 4u ? hb[d] << (4u - from) : hb[d] >> (from - 4u);
+                const uint32_t v = moe_over<0x00300030u>(y, moe_over<0x000F000Fu>(q[d] >> (shl + 8u * odd), exponent));
+                moe_set(w[s], 4 * d + 2 * (int) odd, moe_h2(v) - half2_t{(_Float16) 1056.f, (_Float16) 1056.f});
+            }
+    }
 }
 
 typedef __bf16 moe_bf8 __attribute__((ext_vector_type(8)));
@@ -219,16 +220,14 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
                                               uint32_t e, const uint32_t *slots, uint32_t count, uint32_t r0) {
     using F = MoeTileFmt<TY, HALVES>;
     constexpr uint32_t WB = F::WB, SPW = WB / 2u;
-    constexpr bool Q45 = TY == 12 || TY == 13, Q6 = TY == 14, MX = TY == 39, KQ = Q45 || Q6;
+    constexpr bool Q45 = TY == 12 || TY == 13, Q6 = TY == 14, MX = TY == 39, KQ = Q45 || Q6, PIPE = MX && !LIGHT;
     constexpr int NT = BOTH ? 2 : 1;
     constexpr uint32_t XB = LIGHT ? 2048u : 4096u, XPAIR = 2u * HALVES * XB;  // one half of a k-block, a pair of k-blocks
     const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 31u, h = lane >> 5;
     const uint32_t nb = a.cols / 32u, n_win = (nb + WB - 1u) / WB;
-    // Window w starts at block w WB, the last one at nb - WB: its first `skip` blocks have been done. Whole
-    // pairs of them are left out (skip0), a single one is taken as zero.
-    const uint32_t skip = n_win * WB - nb, skip0 = skip / 2u, total = n_win * SPW - skip0;
-    auto wstart = [&](uint32_t w) { return min(w * WB, nb - WB); };
-
+    // Window 0 has the first `head` blocks (it is copied whole, the rest of it belongs to window 1), the others WB each.
+    const uint32_t head = nb - (n_win - 1u) * WB, steps0 = (head + 1u) / 2u, total = steps0 + (n_win - 1u) * SPW;
+    auto wstart = [&](uint32_t w) __attribute__((always_inline)) { return w ? head + (w - 1u) * WB : 0u; };
     // Weights: copies of 16 rows each take four pieces per row, four lanes a row; what is left of a row's pieces is
     // copied for the 64 rows at once (one piece) or 32 (two). Rows 0 .. 31 are of matrix GU ? 0 : 0 from r0, rows
     // 32 .. 63 of matrix GU ? 1 : 0 from r0 + (GU ? 0 : 32); rows past the last repeat it. A lane's offset within
@@ -249,7 +248,7 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
         roff[g] = min(GU ? row & 31u : row, wleft) * rbytes + min(64u * NQ + 16u * (NR == 1u ? 0u : lane & 1u), F::S - RB);
     }
     u32x4_t wreg[4][NQ], rreg[NR ? NR : 1];
-    auto wload = [&](uint32_t w) {
+    auto wload = [&](uint32_t w) __attribute__((always_inline)) {
         const uint64_t o = (uint64_t) wstart(w) * 32u / moearc_mv_be(TY) * moearc_mv_bb(TY);
 #pragma unroll
         for (uint32_t g = 0; g < 4; ++g)
@@ -266,7 +265,7 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
             __builtin_memcpy(&rreg[g], p, RB);
         }
     };
-    auto put16 = [&](uint8_t *d, u32x4_t v) {
+    auto put16 = [&](uint8_t *d, u32x4_t v) __attribute__((always_inline)) {
         if constexpr (TY == 1) {
             *(u32x4_t *) d = v;
         } else {
@@ -274,7 +273,7 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
             *(u32x2_t *) (d + 8) = u32x2_t{v[2], v[3]};
         }
     };
-    auto wput = [&]() {
+    auto wput = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (uint32_t g = 0; g < 4; ++g)
 #pragma unroll
@@ -296,14 +295,14 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
         xrow[g] = (const uint16_t *) a.x + (uint64_t) (slots[min((tid >> 3) + 32u * g, count - 1u)] / a.x_div) * a.cols + 8u * (tid & 7u);
     const int64_t xlo = HALVES == 2 ? (const uint16_t *) a.x_lo - (const uint16_t *) a.x : 0;
     u32x4_t xreg[HALVES][NT];
-    auto xload = [&](uint32_t step) {
-        const uint32_t w = step / SPW, b = wstart(w) + 2u * (step % SPW + (w + 1u == n_win ? skip0 : 0u));
+    auto xload = [&](uint32_t step) __attribute__((always_inline)) {
+        const uint32_t b = min(step < steps0 ? 2u * step : head + 2u * (step - steps0), nb - 2u);
 #pragma unroll
         for (uint32_t g = 0; g < NT; ++g)
 #pragma unroll
             for (int f = 0; f < HALVES; ++f) __builtin_memcpy(&xreg[f][g], xrow[g] + (f ? xlo : 0) + 32u * b, 16);
     };
-    auto xput = [&](uint32_t buf) {
+    auto xput = [&](uint32_t buf) __attribute__((always_inline)) {
         const uint32_t blk = (tid >> 2) & 1u, c = tid & 3u;
 #pragma unroll
         for (uint32_t g = 0; g < NT; ++g) {
@@ -315,15 +314,16 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
     };
     // The sums of x over the k-blocks of the pair in the registers, as this thread's bf16 piece: piece
     // tid % 4 of block (tid / 4) % 2, slots tid / 8 and + 32. Cut off bits, so that three pieces are exact.
-    auto xsums = [&](uint32_t (&piece)[NT]) {
+    auto xsums = [&](uint32_t (&piece)[NT]) __attribute__((always_inline)) {
 #pragma unroll
         for (uint32_t g = 0; g < NT; ++g) {
-            float s = 0.f;
+            float s = 0.f, one = 1.f;
+            asm("" : "+v"(one));  // s + v as a mixed-precision multiply-add, without a conversion
 #pragma unroll
             for (int f = HALVES - 1; f >= 0; --f) {
                 const half8_t v = __builtin_bit_cast(half8_t, xreg[f][g]);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) s += (float) v[k];
+                for (int k = 0; k < 8; ++k) s = fmaf((float) v[k], one, s);
             }
             s += dpp<0xB1>(s);
             s += dpp<0x4E>(s);
@@ -335,7 +335,7 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
             piece[g] = (c == 0u ? p0 : c == 1u ? p1 : c == 2u ? p2 : 0u) >> 16;
         }
     };
-    auto sput = [&](const uint32_t (&piece)[NT], uint32_t pair) {  // `pair` of the window
+    auto sput = [&](const uint32_t (&piece)[NT], uint32_t pair) __attribute__((always_inline)) {  // `pair` of the window
 #pragma unroll
         for (uint32_t g = 0; g < NT; ++g)
             sums[((tid >> 3) + 32u * g) * 32u + (tid & 3u) * 8u + 2u * pair + ((tid >> 2) & 1u)] = (uint16_t) piece[g];
@@ -347,125 +347,136 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
         for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[tt][rt][j] = 0.f;
-    // K-quants: per row tile, what the accumulators are in units of, and whether the super-block counts at
-    // all (d = 0: its scales are taken as 0, and the unit stays)
-    float unit[2] = {1.f, 1.f};
-    bool counts[2] = {true, true};
+    // K-quants: per row tile, what the accumulators are in units of, the factor of the super-block in LDS, and
+    // whether that counts at all (0: its scales are taken as 0, and the unit stays)
+    float unit[2] = {1.f, 1.f}, factor[2] = {1.f, 1.f};
+    bool ok = true;
 
-    auto mul = [&](const half8_t &x, const half8_t &w, const moe_f32x16 &c) {
+    auto mul = [&](const half8_t &x, const half8_t &w, const moe_f32x16 &c) __attribute__((always_inline)) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, w, c, 0, 0, 0);
     };
-    // pair t of the window, in buffer buf; live 0: its first block taken as zero
-    auto compute = [&](uint32_t buf, uint32_t t, uint32_t live) {
-        half8_t w[2][2][2], lost[Q6 ? 2 : 1][2][2];  // [row tile][block][slice]
-        float f[2][2];
-        bool any[2][2] = {};
+    // One k-block's weights for the matrix cores: [row tile][slice], scales that stayed out, and what Q6_K's
+    // rounding lost
+    struct Ops {
+        half8_t w[2][2], lost[Q6 ? 2 : 1][2];
+        float f[2];
+        bool any[2];
+    };
+    auto decode = [&](Ops &o, uint32_t i, uint32_t live) __attribute__((always_inline)) {  // k-block i of the window
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
             const uint8_t *row = wbuf + (32u * rt + n) * F::RS;
             if constexpr (TY == 1) {
-                moe_f16_pair(w[rt], row, h, live);
+                moe_f16_block(o.w[rt], row, i, h, live);
             } else if constexpr (TY == 8) {
-                moe_q8_pair(w[rt], row, t, h);
-#pragma unroll
-                for (uint32_t b = 0; b < 2; ++b) f[rt][b] = mms_f16(*(const uint16_t *) (row + 34u * (2u * t + b)));
-                f[rt][0] = live ? f[rt][0] : 0.f;
+                moe_q8_block(o.w[rt], row, i, h);
+                o.f[rt] = live ? mms_f16(*(const uint16_t *) (row + 34u * i)) : 0.f;
             } else if constexpr (MX) {
-#pragma unroll
-                for (uint32_t b = 0; b < 2; ++b) {
-                    const uint32_t e8 = row[17u * (2u * t + b)];
-                    f[rt][b] = __uint_as_float(FOLD || e8 ? e8 << 23 : 0x00400000u);  // 2^(e - 127)
-                }
-                const float one[2] = {1.f, 1.f};
-                moe_mx_pair(w[rt], row, t, h, FOLD ? f[rt] : one, live);
+                const uint32_t e8 = row[17u * i];
+                o.f[rt] = __uint_as_float(FOLD || e8 ? e8 << 23 : 0x00400000u);  // 2^(e - 127)
+                moe_mx_block(o.w[rt], row, i, h, FOLD ? o.f[rt] : 1.f, live);
             } else if constexpr (Q45) {
                 const u32x2_t h0 = *(const u32x2_t *) row, h1 = *(const u32x2_t *) (row + 8);
-                uint32_t sc[2];
-#pragma unroll
-                for (uint32_t b = 0; b < 2; ++b) sc[b] = counts[rt] ? moe_k4_scale(u32x4_t{h0[0], h0[1], h1[0], h1[1]}, 2u * t + b) : 0u;
-                moe_q45_pair<TY>(w[rt], row, t, h, sc);
+                moe_q45_block<TY>(o.w[rt], row, i, h, factor[rt] != 0.f ? moe_k4_scale(u32x4_t{h0[0], h0[1], h1[0], h1[1]}, i) : 0u);
             } else {
-                moe_q6_pair(w[rt], row, t, h);
-                const uint32_t sc = *(const uint32_t *) (row + 192u + 4u * t);  // scales 4 t .. + 3, two per block
+                moe_q6_block(o.w[rt], row, i, h);
+                const uint32_t sc = *(const uint16_t *) (row + 192u + 2u * i);
+                uint32_t bits = 0u;
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    uint32_t bits = 0u;
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const _Float16 m = counts[rt] ? (_Float16) (int16_t) (int8_t) (sc >> (16 * b + 8 * s)) : (_Float16) 0.f;
-                        const half8_t q = w[rt][b][s];
-                        w[rt][b][s] = moe_times(q, m);
-                        lost[rt][b][s] = moe_lost(q, m, w[rt][b][s]);
-                        const u32x4_t v = __builtin_bit_cast(u32x4_t, lost[rt][b][s]);
-                        bits |= (v[0] | v[1] | v[2] | v[3]) & 0x7FFF7FFFu;
-                    }
-                    any[rt][b] = __ballot(bits != 0u) != 0ull;  // some product of the wave was rounded
+                for (int s = 0; s < 2; ++s) {
+                    const _Float16 m = factor[rt] != 0.f ? (_Float16) (int16_t) (int8_t) (sc >> (8 * s)) : (_Float16) 0.f;
+                    const half8_t q = o.w[rt][s];
+                    o.w[rt][s] = moe_times(q, m);
+                    o.lost[rt][s] = moe_lost(q, m, o.w[rt][s]);
+                    const u32x4_t v = __builtin_bit_cast(u32x4_t, o.lost[rt][s]);
+                    bits |= (v[0] | v[1] | v[2] | v[3]) & 0x7FFF7FFFu;
                 }
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            half8_t x[HALVES][NT][2];
-#pragma unroll
-            for (int tt = 0; tt < NT; ++tt)
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int g = 0; g < HALVES; ++g) {
-                        const uint32_t u = 32u * tt + n;
-                        x[g][tt][s] = __builtin_bit_cast(half8_t, *(const u32x4_t *) (xbuf + buf * XPAIR + (b * HALVES + g) * XB +
-                                                                                      u * 64u + 16u * ((2u * s + h) ^ moe_swz(u))));
-                    }
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
-                if constexpr (TY == 1 || KQ || FOLD) {
-#pragma unroll
-                    for (int s = 0; s < 2; ++s)
-#pragma unroll
-                        for (int g = 0; g < HALVES; ++g)
-#pragma unroll
-                            for (int tt = 0; tt < NT; ++tt) acc[tt][rt] = mul(x[g][tt][s], w[rt][b][s], acc[tt][rt]);
-                    if constexpr (Q6)
-                        if (any[rt][b]) {
-#pragma unroll
-                            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                                for (int tt = 0; tt < NT; ++tt) acc[tt][rt] = mul(x[0][tt][s], lost[rt][b][s], acc[tt][rt]);
-                        }
-                } else {
-                    moe_f32x16 d[NT];
-#pragma unroll
-                    for (int tt = 0; tt < NT; ++tt) d[tt] = moe_f32x16{};
-#pragma unroll
-                    for (int s = 0; s < 2; ++s)
-#pragma unroll
-                        for (int g = 0; g < HALVES; ++g)
-#pragma unroll
-                            for (int tt = 0; tt < NT; ++tt) d[tt] = mul(x[g][tt][s], w[rt][b][s], d[tt]);
-#pragma unroll
-                    for (int tt = 0; tt < NT; ++tt)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) acc[tt][rt][j] = fmaf(f[rt][b], d[tt][j], acc[tt][rt][j]);
-                }
+                o.any[rt] = __ballot(bits != 0u) != 0ull;  // some product of the wave was rounded
             }
         }
     };
-    // the accumulators from the last super-block's unit to this one's
-    auto rescale = [&]() {
+    auto products = [&](uint32_t buf, uint32_t blk, const Ops &o) __attribute__((always_inline)) {  // block blk of the pair in buffer buf
+        half8_t x[HALVES][NT][2];
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int g = 0; g < HALVES; ++g) {
+                    const uint32_t u = 32u * tt + n;
+                    x[g][tt][s] = __builtin_bit_cast(half8_t, *(const u32x4_t *) (xbuf + buf * XPAIR + (blk * HALVES + g) * XB +
+                                                                                  u * 64u + 16u * ((2u * s + h) ^ moe_swz(u))));
+                }
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
-            const uint8_t *row = wbuf + (32u * rt + n) * F::RS;
-            const float d = mms_f16(*(const uint16_t *) (row + (Q6 ? 208u + MmsFmt<14>::LAST : 0u)));
-            counts[rt] = d != 0.f;
-            const float ratio = counts[rt] ? unit[rt] / d : 1.f;
-            unit[rt] = counts[rt] ? d : unit[rt];
+            if constexpr (TY == 1 || KQ || FOLD) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int g = 0; g < HALVES; ++g)
+#pragma unroll
+                        for (int tt = 0; tt < NT; ++tt) acc[tt][rt] = mul(x[g][tt][s], o.w[rt][s], acc[tt][rt]);
+                if constexpr (Q6)
+                    if (o.any[rt]) {
+#pragma unroll
+                        for (int s = 0; s < 2; ++s)
+#pragma unroll
+                            for (int tt = 0; tt < NT; ++tt) acc[tt][rt] = mul(x[0][tt][s], o.lost[rt][s], acc[tt][rt]);
+                    }
+            } else {
+                moe_f32x16 d[NT];
+#pragma unroll
+                for (int tt = 0; tt < NT; ++tt) d[tt] = moe_f32x16{};
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int g = 0; g < HALVES; ++g)
+#pragma unroll
+                        for (int tt = 0; tt < NT; ++tt) d[tt] = mul(x[g][tt][s], o.w[rt][s], d[tt]);
+#pragma unroll
+                for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) acc[tt][rt][j] = fmaf(o.f[rt], d[tt][j], acc[tt][rt][j]);
+            }
+        }
+    };
+    // the next window into LDS, when the last one's weights have all been taken from there, and the one after it
+    // requested
+    auto advance = [&](uint32_t w) __attribute__((always_inline)) {
+        __builtin_amdgcn_wave_barrier();
+        wput();
+        __builtin_amdgcn_wave_barrier();
+        wload(min(w + 1u, n_win - 1u));
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (KQ) {
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt)
+                factor[rt] = mms_f16(*(const uint16_t *) (wbuf + (32u * rt + n) * F::RS + (Q6 ? 208u + MmsFmt<14>::LAST : 0u)));
+        }
+        if constexpr (FOLD) {
+            uint32_t lo = 255u, hi = 0u;  // of row `lane`
+#pragma unroll
+            for (uint32_t i = 0; i < WB; ++i) {
+                const uint32_t e8 = wbuf[lane * F::RS + 17u * i];
+                lo = min(lo, e8);
+                hi = max(hi, e8);
+            }
+            ok = ok && lo >= 114u && hi <= 139u;
+        }
+    };
+    // the accumulators from the last super-block's unit to this one's
+    auto rescale = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+            const float ratio = factor[rt] != 0.f ? unit[rt] / factor[rt] : 1.f;
+            unit[rt] = factor[rt] != 0.f ? factor[rt] : unit[rt];
 #pragma unroll
             for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) acc[tt][rt][j] *= ratio;
         }
     };
-    auto mins = [&]() {
+    auto mins = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
             const uint8_t *row = wbuf + (32u * rt + n) * F::RS;
@@ -488,54 +499,71 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
         }
     };
 
-    uint32_t piece[NT] = {};
-    bool ok = true;
+    uint32_t piece[NT] = {}, step = 0;
+    // the step's copies: the next pair of inputs into the other buffer (after the last: nothing reads it), the one
+    // after it requested
+    auto copies = [&]() __attribute__((always_inline)) {
+        xput((step + 1u) & 1u);
+        if constexpr (Q45) xsums(piece);
+        xload(min(step + 2u, total - 1u));
+        __builtin_amdgcn_sched_barrier(0);  // left alone, the loads sink to the step's end, and the next waits for them
+    };
+    const uint32_t all = 0xFFFFFFFFu;
     wload(0u);
     xload(0u);
     xput(0u);
     if constexpr (Q45) xsums(piece);
     xload(min(1u, total - 1u));
     moe_barrier();
-    uint32_t step = 0;
-    for (uint32_t w = 0; w < n_win; ++w) {
-        __builtin_amdgcn_wave_barrier();
-        wput();
-        __builtin_amdgcn_wave_barrier();
-        wload(min(w + 1u, n_win - 1u));
-        __builtin_amdgcn_sched_barrier(0);
-        const bool last = w + 1u == n_win;
-        const uint32_t from = last ? skip0 : 0u, live0 = last && (skip & 1u) ? 0u : 0xFFFFFFFFu;
-        if constexpr (KQ) rescale();
-        if constexpr (FOLD) {
-            uint32_t lo = 255u, hi = 0u;  // of row `lane`
+    advance(0u);
+    Ops A, B;
+    uint32_t w = 0;
+    // Sums: the pair that is stored for the next step has its own stored with it, but the next window's first pair
+    // waits for that window, when the mins of this one have been taken.
+    if (!PIPE || head < WB) {
+        const uint32_t until = PIPE ? 1u : n_win;
+#pragma unroll 1
+        for (; w < until; ++w) {
+            const uint32_t blocks = w ? WB : head;
+            if constexpr (KQ) rescale();
 #pragma unroll
-            for (uint32_t i = 0; i < WB; ++i) {
-                const uint32_t e8 = wbuf[lane * F::RS + 17u * i];
-                lo = min(lo, e8);
-                hi = max(hi, e8);
+            for (uint32_t j = 0; j < SPW; ++j) {
+                if (!KQ && 2u * j >= blocks) continue;
+                const uint32_t live = KQ || 2u * j + 1u < blocks ? all : 0u;
+                if constexpr (Q45)
+                    if (j == 0) sput(piece, 0u);
+                copies();
+                if constexpr (Q45)
+                    if (j + 1u < SPW) sput(piece, j + 1u);
+                decode(A, 2u * j, all);
+                decode(B, 2u * j + 1u, live);
+                products(step & 1u, 0u, A);
+                products(step & 1u, 1u, B);
+                if constexpr (Q45)
+                    if (j + 1u == SPW) mins();
+                moe_barrier();
+                ++step;
             }
-            ok = ok && lo >= 114u && hi <= 139u;
+            advance(w + 1u);
         }
-        // Sums: the pair that is stored for the next step has its own stored with it, but the next window's
-        // first pair waits for that window, when the mins of this one have been taken.
+    }
+    // MXFP4's whole windows: each block's weights are decoded while the one before is multiplied (the other formats
+    // have no registers left for it: Q4_K 153 -> 167 us, Q8_0 130 -> 154)
+    if constexpr (PIPE) {
+        decode(A, 0u, all);
+#pragma unroll 1
+        for (; w < n_win; ++w) {
 #pragma unroll
-        for (uint32_t j = 0; j < SPW; ++j) {
-            if (j < from) continue;
-            const uint32_t buf = step & 1u;
-            if constexpr (Q45)
-                if (j == 0) sput(piece, 0u);
-            xput(buf ^ 1u);  // the pair after this one (after the last: nothing reads it)
-            if constexpr (Q45) {
-                xsums(piece);
-                if (j + 1u < SPW) sput(piece, j + 1u);
+            for (uint32_t j = 0; j < SPW; ++j) {
+                copies();
+                decode(B, 2u * j + 1u, all);
+                products(step & 1u, 0u, A);
+                if (j + 1u == SPW) advance(w + 1u);
+                decode(A, (2u * j + 2u) % WB, all);
+                products(step & 1u, 1u, B);
+                moe_barrier();
+                ++step;
             }
-            xload(min(step + 2u, total - 1u));
-            __builtin_amdgcn_sched_barrier(0);  // left alone, the loads sink to the step's end, and the next waits for them
-            compute(buf, j, j == from ? live0 : 0xFFFFFFFFu);
-            if constexpr (Q45)
-                if (j + 1u == SPW) mins();
-            moe_barrier();
-            ++step;
         }
     }
     if constexpr (KQ) {
