@@ -308,6 +308,24 @@ struct MoeArgs {
     uint32_t y_order, pad;     // with two matrices: the type of the next product's weights, which orders y
 };
 
+// The two launches of a single token (moe_vec.hip). Wave w of work-group g has rows (g * waves + w) * rpw .. of the
+// n_used slots: grid y with gate and up, one after the other in down (rpw * n_used at most 64 there, else 32).
+struct MoeVecArgs {
+    const uint32_t *ids;       // [n_used], at most 64
+    const float *weights;      // [n_used]
+    const void *x;             // [cols], or [n_used][cols] f32 or f16
+    const uint8_t *w[2];
+    const float *bias[2];
+    void *y;                   // [n_used][rows], or [rows]
+    uint32_t *err;
+    uint64_t expert_bytes, row_bytes;
+    uint32_t n_used, n_expert, rows, cols;
+    uint32_t n_pieces, rpw;
+    uint32_t x_lds_bytes, wave_buf;
+    uint32_t x_f16, y_f16, accumulate, clamped;
+    float alpha, limit;
+};
+
 // x as moe_tile.hip's products take it: f16 hi (and lo, of f32), each k-block in the order of weights of `type`
 struct MoePrepArgs {
     const void *x;

@@ -28,7 +28,8 @@ struct MoeFmt {
     static constexpr bool SPLIT_LAST = TY == 8;
 };
 
-__device__ __forceinline__ float moe_activation(const MoeArgs &a, float g, float u) {
+template <typename Args>
+__device__ __forceinline__ float moe_activation(const Args &a, float g, float u) {
     // exp2 of a large positive argument is +inf and g / inf is 0: no branch needed
     if (a.clamped) {
         g = fminf(g, a.limit);

@@ -139,6 +139,66 @@ int moe_product(moearc_ctx *c, MoeArgs a, unsigned ty, bool gate_up, bool half) 
                     64 * MOEARC_MOE_SMALL_WAVES, a, nullptr, a.rows, a.n_slots, 0, name);
 }
 
+// Whether a product of a single token's slots can run on moe_vec.hip: its row within one pass of a wave's lanes, its
+// inputs in LDS beside the waves' buffers. Sets the launch's shape; rows_most: per wave, what its lanes can hold.
+constexpr unsigned kMoeVecWaves = 8;
+bool moe_vec_shape(MoeVecArgs &a, unsigned ty, unsigned n_rows_of_x, unsigned rows_most, unsigned &ppl, unsigned &lds) {
+    const uint32_t pe = moearc_mv_pe(ty);
+    a.n_pieces = (a.cols + pe - 1) / pe;
+    if (a.n_pieces > 256) return false;
+    ppl = a.n_pieces <= 64 ? 1 : a.n_pieces <= 128 ? 2 : 4;
+    a.row_bytes = (uint64_t) a.cols / moearc_mv_be(ty) * moearc_mv_bb(ty);
+    a.expert_bytes = a.row_bytes * a.rows;
+    a.wave_buf = moearc_mv_wave_buf(a.row_bytes);
+    a.x_lds_bytes = 4u * n_rows_of_x * a.n_pieces * (pe + 4u);
+    lds = a.x_lds_bytes + kMoeVecWaves * a.wave_buf;
+    // about one work-group per CU: a wave's rows share the inputs in its registers
+    const uint64_t slots = n_rows_of_x > 1 ? 1 : a.n_used, waves = 256ul * kMoeVecWaves;
+    a.rpw = (uint32_t) std::min<uint64_t>(rows_most, (a.rows * slots + waves - 1) / waves);
+    return lds <= 65536u && a.rpw > 0;
+}
+
+// One token's expert half, in two launches; ERR_ARG: another kernel's.
+int moe_token(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, bool half, const unsigned int *ids, const float *weights,
+              unsigned long n_used, unsigned accumulate, uint8_t *act) {
+    if (n_used > 64) return ERR_ARG;
+    MoeVecArgs g{};
+    g.ids = ids;
+    g.weights = weights;
+    g.err = c->err_word;
+    g.n_used = (uint32_t) n_used;
+    g.n_expert = (uint32_t) m->n_expert;
+    g.x_f16 = g.y_f16 = half;
+    MoeVecArgs d = g;
+    unsigned gp, gl, dp, dl;
+    g.rows = d.cols = (uint32_t) m->n_ff;
+    g.cols = d.rows = (uint32_t) m->n_embd;
+    if (!moe_vec_shape(g, m->w_type[0], 1, 32, gp, gl) || !moe_vec_shape(d, m->w_type[2], (unsigned) n_used, 64 / (unsigned) n_used, dp, dl))
+        return ERR_ARG;
+    for (int i = 0; i < 2; ++i) {
+        g.w[i] = (const uint8_t *) m->w[i];
+        g.bias[i] = m->bias[i];
+    }
+    g.x = x;
+    g.y = act;
+    g.clamped = m->act == MOEARC_ACT_SWIGLU_CLAMPED;
+    g.alpha = m->alpha;
+    g.limit = m->limit;
+    d.w[0] = (const uint8_t *) m->w[2];
+    d.bias[0] = m->bias[2];
+    d.x = act;
+    d.y = y;
+    d.accumulate = accumulate;
+    const unsigned per_g = kMoeVecWaves * g.rpw, per_d = kMoeVecWaves * d.rpw;
+    auto form = [](unsigned ppl) { return ppl == 1 ? 0 : ppl == 2 ? 1 : 2; };
+    c->err_armed = true;
+    if (const int rc = launch2d(c, c->f_moe_vec[moe_index(m->w_type[0])][0][form(gp)], (g.rows + per_g - 1) / per_g, (unsigned) n_used,
+                                64 * kMoeVecWaves, g, nullptr, g.rows, n_used, gl, "moe_gate_up"))
+        return rc;
+    return launch2d(c, c->f_moe_vec[moe_index(m->w_type[2])][1][form(dp)], (d.rows + per_d - 1) / per_d, 1, 64 * kMoeVecWaves, d, nullptr,
+                    d.rows, n_used, dl, "moe_down");
+}
+
 // Brackets a call of several launches under one key, as a single launch would be.
 struct MoeScope {
     moearc_ctx *c;
@@ -187,6 +247,12 @@ bool moe_load(moearc_ctx *c) {
             char name[64];
             std::snprintf(name, sizeof(name), "moearc_moe_small_%s_%s_%s_k", kMoeNames[t], i & 2 ? "p" : "gu", i & 1 ? "f16" : "f32");
             if (!get(&c->f_moe_small[t][i >> 1][i & 1], name)) return false;
+            if (i < 3) {  // gate and up, down x 1, 2, 4 pieces per lane
+                for (int k = 0; k < 2; ++k) {
+                    std::snprintf(name, sizeof(name), "moearc_moe_vec_%s_%s_p%d_k", kMoeNames[t], k ? "down" : "gu", 1 << i);
+                    if (!get(&c->f_moe_vec[t][k][i], name)) return false;
+                }
+            }
             std::snprintf(name, sizeof(name), "moearc_moe_tile_%s_%s_%s_k", kMoeNames[t], i & 2 ? "p" : "gu", i & 1 ? "f16" : "f32");
             if (!get(&c->f_moe_tile[t][i >> 1][i & 1], name)) return false;
             std::snprintf(name, sizeof(name), "moearc_moe_light_%s_%s_%s_k", kMoeNames[t], i & 2 ? "p" : "gu", i & 1 ? "f16" : "f32");
@@ -315,6 +381,10 @@ int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, u
     const bool half = io_type == MOEARC_OUT_F16;
     const size_t elem = half ? 2 : 4;
     const MoeScope scope(c, "moe_ffn", m->n_ff, n_tok * n_used);
+    if (n_tok == 1) {
+        const int rc = moe_token(c, m, y, x, half, ids, weights, n_used, accumulate, mem + sp.act);
+        if (rc != ERR_ARG) return rc;
+    }
     for (unsigned long t = 0; t < n_tok; t += chunk) {
         const unsigned long n = std::min(chunk, n_tok - t);
         MoeArgs a{};

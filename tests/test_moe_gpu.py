@@ -226,6 +226,18 @@ def test_ffn(ctx, types, io, t, k, e, embd, ff):
     run_ffn(ctx, types, t, k, e, embd, ff, io, bias=False, add=io == OUT_F32, seed=t + 5)
 
 
+@pytest.mark.parametrize("ty", TYPES, ids=lambda t: t.name)
+@pytest.mark.parametrize("io", [OUT_F32, OUT_F16], ids=["f32", "f16"])
+def test_ffn_of_a_single_token(ctx, ty, io):
+    wide = 2304 if ty in (QuantType.Q4_K, QuantType.Q5_K, QuantType.Q6_K) else 2080
+    for k, e, embd, ff in ((1, 3, 256, 512), (4, 9, 768, 256), (8, 8, 512, 768), (13, 20, 256, 256), (2, 3, wide, 256), (2, 3, 256, wide),
+                           (64, 5, 256, 256), (65, 70, 256, 256), (1, 2, 5120, 256), (8, 9, 256, 5120)):
+        run_ffn(ctx, (ty, ty), 1, k, e, embd, ff, io, MoeAct(k % 2), bias=k != 4, add=io == OUT_F32 and k % 2 == 0, seed=k)
+    for k, ids in ((4, [NO_EXPERT, 2, NO_EXPERT, 1]), (4, [NO_EXPERT] * 4), (3, [5, 5, 5]), (8, [NO_EXPERT] * 7 + [3])):
+        for add in (False, True) if io == OUT_F32 else (False,):
+            run_ffn(ctx, (ty, ty), 1, k, 6, 256, 512, io, add=add, ids=np.array([ids], np.uint32))
+
+
 def test_ffn_odd_widths(ctx):
     run_ffn(ctx, (QuantType.MXFP4, QuantType.Q8_0), 3, 2, 5, 288, 352, add=True)
     run_ffn(ctx, (QuantType.Q8_0, QuantType.MXFP4), 77, 2, 5, 352, 288, act=MoeAct.SWIGLU_CLAMPED)
