@@ -19,7 +19,7 @@ __device__ __forceinline__ void moe_vec_body(const MoeVecArgs &a) {
     constexpr uint32_t GMAX = moearc_mv_gmax(TY, PPL);
     constexpr uint32_t XPAD = PE + 4u;                 // LDS floats per piece of an input row
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const uint32_t P = a.n_pieces, total = P * PE;
+    const uint32_t P = a.n_pieces;
     const uint32_t r0 = (blockIdx.x * waves + wave) * a.rpw, n_rows = r0 < a.rows ? min(a.rpw, a.rows - r0) : 0u;
 
     // the experts: lane j holds the j-th id; GU: this work-group's, else those that count, in order
@@ -79,20 +79,26 @@ __device__ __forceinline__ void moe_vec_body(const MoeVecArgs &a) {
     // the inputs, f32, piece p of a row at floats [p * XPAD, + PE): one row, or the slots' that count
     {
         float *xl = (float *) mvx_smem;
-        for (uint32_t q = 0; q < n_slots; ++q) {
-            const uint64_t row = GU ? 0u : slot_of(q);
-            for (uint32_t c0 = threadIdx.x; c0 < total; c0 += 8u * blockDim.x) {
-                float v[8];
+        const uint32_t quads = a.n_pieces * (PE / 4u), n = n_slots * quads;  // four floats at a time, of all rows
+        for (uint32_t c0 = threadIdx.x; c0 < n; c0 += 8u * blockDim.x) {
+            float v[8][4];
 #pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) {
-                    const uint32_t c = min(c0 + k * blockDim.x, a.cols - 1u);
-                    v[k] = a.x_f16 ? (float) ((const _Float16 *) a.x)[row * a.cols + c] : ((const float *) a.x)[row * a.cols + c];
-                }
+            for (uint32_t k = 0; k < 8; ++k) {
+                const uint32_t i = min(c0 + k * blockDim.x, n - 1u), q = GU ? 0u : i / quads;
+                const uint64_t at = (GU ? 0ull : (uint64_t) slot_of(q) * a.cols) + min(4u * (i - q * quads), a.cols - 4u);
+                if (a.x_f16) {
+                    _Float16 h[4];
+                    __builtin_memcpy(h, (const _Float16 *) a.x + at, 8);
 #pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) {
-                    const uint32_t c = c0 + k * blockDim.x;
-                    if (c < total) xl[q * P * XPAD + (c / PE) * XPAD + c % PE] = c < a.cols ? v[k] : 0.f;
+                    for (int j = 0; j < 4; ++j) v[k][j] = (float) h[j];
+                } else {
+                    __builtin_memcpy(v[k], (const float *) a.x + at, 16);
                 }
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                const uint32_t i = c0 + k * blockDim.x, q = GU ? 0u : i / quads, c = 4u * (i - q * quads);
+                if (i < n) *(float4_t *) (xl + q * P * XPAD + (c / PE) * XPAD + c % PE) = c < a.cols ? float4_t{v[k][0], v[k][1], v[k][2], v[k][3]} : float4_t{0.f, 0.f, 0.f, 0.f};
             }
         }
         __syncthreads();

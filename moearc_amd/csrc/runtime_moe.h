@@ -152,8 +152,8 @@ bool moe_vec_shape(MoeVecArgs &a, unsigned ty, unsigned n_rows_of_x, unsigned ro
     a.wave_buf = moearc_mv_wave_buf(a.row_bytes);
     a.x_lds_bytes = 4u * n_rows_of_x * a.n_pieces * (pe + 4u);
     lds = a.x_lds_bytes + kMoeVecWaves * a.wave_buf;
-    // about one work-group per CU: a wave's rows share the inputs in its registers
-    const uint64_t slots = n_rows_of_x > 1 ? 1 : a.n_used, waves = 256ul * kMoeVecWaves;
+    // two work-groups per CU: a wave's rows share the inputs in its registers (one to four measured alike)
+    const uint64_t slots = n_rows_of_x > 1 ? 1 : a.n_used, waves = 512ul * kMoeVecWaves;
     a.rpw = (uint32_t) std::min<uint64_t>(rows_most, (a.rows * slots + waves - 1) / waves);
     return lds <= 65536u && a.rpw > 0;
 }
