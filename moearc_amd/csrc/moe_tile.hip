@@ -216,12 +216,14 @@ typedef __bf16 moe_bf8 __attribute__((ext_vector_type(8)));
 // The reduction of one tile for a wave: acc[slot half][row tile], slots 32 and up only with BOTH. FOLD (MXFP4):
 // the scales enter the operand; returns false where one is out of f16's range, and the sums are not valid then.
 template <uint32_t TY, bool GU, int HALVES, bool LIGHT, bool BOTH, bool FOLD>
-__device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc)[2][2], uint8_t *xbuf, uint8_t *wbuf, uint16_t *sums,
+__device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc)[2][LIGHT ? 1 : 2], uint8_t *xbuf, uint8_t *wbuf, uint16_t *sums,
                                               uint32_t e, const uint32_t *slots, uint32_t count, uint32_t r0) {
     using F = MoeTileFmt<TY, HALVES>;
     constexpr uint32_t WB = F::WB, SPW = WB / 2u;
     constexpr bool Q45 = TY == 12 || TY == 13, Q6 = TY == 14, MX = TY == 39, KQ = Q45 || Q6, PIPE = MX && !LIGHT;
-    constexpr int NT = BOTH ? 2 : 1;
+    // RT row tiles of 32 per wave; windows of weights requested DEPTH ahead
+    constexpr int NT = BOTH ? 2 : 1, RT = LIGHT ? 1 : 2;
+    constexpr uint32_t WG = 2u * RT, DEPTH = LIGHT ? 2u : 1u;
     constexpr uint32_t XB = LIGHT ? 2048u : 4096u, XPAIR = 2u * HALVES * XB;  // one half of a k-block, a pair of k-blocks
     const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 31u, h = lane >> 5;
     const uint32_t nb = a.cols / 32u, n_win = (nb + WB - 1u) / WB;
@@ -229,41 +231,39 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
     const uint32_t head = nb - (n_win - 1u) * WB, steps0 = (head + 1u) / 2u, total = steps0 + (n_win - 1u) * SPW;
     auto wstart = [&](uint32_t w) __attribute__((always_inline)) { return w ? head + (w - 1u) * WB : 0u; };
     // Weights: copies of 16 rows each take four pieces per row, four lanes a row; what is left of a row's pieces is
-    // copied for the 64 rows at once (one piece) or 32 (two). Rows 0 .. 31 are of matrix GU ? 0 : 0 from r0, rows
-    // 32 .. 63 of matrix GU ? 1 : 0 from r0 + (GU ? 0 : 32); rows past the last repeat it. A lane's offset within
-    // the matrix is 32 bits (64 rows of at most 2 MiB), the rest of the address is the wave's.
-    constexpr uint32_t NQ = F::NP % 4u == 3u ? F::NP / 4u + 1u : F::NP / 4u, NR = F::NP % 4u == 3u ? 0u : F::NP % 4u;
+    // copied for all rows at once (one piece), or 32 (two). The first half of the wave's rows are of matrix 0 from r0, the
+    // second of matrix 1 from r0 (GU) or matrix 0 from r0 + 16 RT; rows past the last repeat it. A lane's offset
+    // within the matrix is 32 bits (64 rows of at most 2 MiB), the rest of the address is the wave's.
+    constexpr uint32_t NQ = F::NP % 4u == 3u ? F::NP / 4u + 1u : F::NP / 4u, LEFT = F::NP % 4u == 3u ? 0u : F::NP % 4u;
+    constexpr uint32_t NR = LEFT == 2u ? RT : LEFT;  // copies of what is left
     constexpr uint32_t RB = F::S % 16u == 8u ? 8u : 16u;  // bytes of the last piece that are new
-    static_assert(RB == 16u || NR == 1u, "a short last piece stands alone");
+    static_assert(RB == 16u || LEFT == 1u, "a short last piece stands alone");
     const uint32_t wr0 = min(r0, a.rows - 1u), wleft = a.rows - 1u - wr0;
     const uint8_t *const wrow0 = a.w[0] + e * a.expert_bytes + (uint64_t) wr0 * a.row_bytes;
     const uint8_t *const wrow1 = GU ? a.w[1] + e * a.expert_bytes + (uint64_t) wr0 * a.row_bytes : wrow0;
     const uint32_t rbytes = (uint32_t) a.row_bytes;
-    uint32_t woff[4], roff[NR ? NR : 1];
+    uint32_t woff[WG], roff[NR ? NR : 1];
 #pragma unroll
-    for (uint32_t g = 0; g < 4; ++g) woff[g] = min((lane >> 2) + (GU ? 16u * (g & 1u) : 16u * g), wleft) * rbytes;
+    for (uint32_t g = 0; g < WG; ++g) woff[g] = min((lane >> 2) + 16u * (GU ? g % RT : g), wleft) * rbytes;
+    // row of the wave that a lane copies what is left of
+    auto rrow = [&](uint32_t g) __attribute__((always_inline)) { return LEFT == 1u ? lane % (32u * RT) : (lane >> 1) + 32u * g; };
 #pragma unroll
-    for (uint32_t g = 0; g < NR; ++g) {
-        const uint32_t row = NR == 1u ? lane : (lane >> 1) + 32u * g;
-        roff[g] = min(GU ? row & 31u : row, wleft) * rbytes + min(64u * NQ + 16u * (NR == 1u ? 0u : lane & 1u), F::S - RB);
-    }
-    u32x4_t wreg[4][NQ], rreg[NR ? NR : 1];
-    auto wload = [&](uint32_t w) __attribute__((always_inline)) {
+    for (uint32_t g = 0; g < NR; ++g)
+        roff[g] = min(GU ? rrow(g) % (16u * RT) : rrow(g), wleft) * rbytes + min(64u * NQ + 16u * (LEFT == 1u ? 0u : lane & 1u), F::S - RB);
+    u32x4_t wreg[DEPTH][WG][NQ], rreg[DEPTH][NR ? NR : 1];
+    auto wload = [&](uint32_t w, uint32_t set) __attribute__((always_inline)) {
         const uint64_t o = (uint64_t) wstart(w) * 32u / moearc_mv_be(TY) * moearc_mv_bb(TY);
 #pragma unroll
-        for (uint32_t g = 0; g < 4; ++g)
+        for (uint32_t g = 0; g < WG; ++g)
 #pragma unroll
             for (uint32_t k = 0; k < NQ; ++k) {
                 // only the last quad can pass the window's end, by pieces that repeat the one before
                 const uint32_t at = 64u * (k + 1u) <= F::S ? 64u * k + 16u * (lane & 3u) : min(64u * k + 16u * (lane & 3u), F::S - 16u);
-                __builtin_memcpy(&wreg[g][k], (g < 2u ? wrow0 : wrow1) + o + (woff[g] + at), 16);
+                __builtin_memcpy(&wreg[set][g][k], (g < RT ? wrow0 : wrow1) + o + (woff[g] + at), 16);
             }
 #pragma unroll
-        for (uint32_t g = 0; g < NR; ++g) {
-            // (one piece: lanes 32 .. 63 hold rows 32 .. 63, which with GU are the other matrix's)
-            const uint8_t *p = (NR == 1u ? (lane < 32u ? wrow0 : wrow1) : (g == 0u ? wrow0 : wrow1)) + o + roff[g];
-            __builtin_memcpy(&rreg[g], p, RB);
-        }
+        for (uint32_t g = 0; g < NR; ++g)
+            __builtin_memcpy(&rreg[set][g], (rrow(g) < 16u * RT ? wrow0 : wrow1) + o + roff[g], RB);
     };
     auto put16 = [&](uint8_t *d, u32x4_t v) __attribute__((always_inline)) {
         if constexpr (TY == 1) {
@@ -273,19 +273,19 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
             *(u32x2_t *) (d + 8) = u32x2_t{v[2], v[3]};
         }
     };
-    auto wput = [&]() __attribute__((always_inline)) {
+    auto wput = [&](uint32_t set) __attribute__((always_inline)) {
 #pragma unroll
-        for (uint32_t g = 0; g < 4; ++g)
+        for (uint32_t g = 0; g < WG; ++g)
 #pragma unroll
             for (uint32_t k = 0; k < NQ; ++k) {
                 const uint32_t piece = 4u * k + (lane & 3u);
-                put16(wbuf + ((lane >> 2) + 16u * g) * F::RS + 16u * (4u * (k + 1u) <= F::NP ? piece : min(piece, F::NP - 1u)), wreg[g][k]);
+                put16(wbuf + ((lane >> 2) + 16u * g) * F::RS + 16u * (4u * (k + 1u) <= F::NP ? piece : min(piece, F::NP - 1u)), wreg[set][g][k]);
             }
 #pragma unroll
         for (uint32_t g = 0; g < NR; ++g) {
-            uint8_t *d = wbuf + (NR == 1u ? lane : (lane >> 1) + 32u * g) * F::RS + 64u * NQ + 16u * (NR == 1u ? 0u : lane & 1u);
-            if constexpr (RB == 8u) *(u32x2_t *) d = u32x2_t{rreg[g][0], rreg[g][1]};
-            else put16(d, rreg[g]);
+            uint8_t *d = wbuf + rrow(g) * F::RS + 64u * NQ + 16u * (LEFT == 1u ? 0u : lane & 1u);
+            if constexpr (RB == 8u) *(u32x2_t *) d = u32x2_t{rreg[set][g][0], rreg[set][g][1]};
+            else put16(d, rreg[set][g]);
         }
     };
     // inputs: thread i, load (half, group g): slot i / 8 + 32 g, 16 bytes i % 8 of the pair's 128
@@ -344,7 +344,7 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
 #pragma unroll
     for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt)
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[tt][rt][j] = 0.f;
     // K-quants: per row tile, what the accumulators are in units of, the factor of the super-block in LDS, and
@@ -358,13 +358,13 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
     // One k-block's weights for the matrix cores: [row tile][slice], scales that stayed out, and what Q6_K's
     // rounding lost
     struct Ops {
-        half8_t w[2][2], lost[Q6 ? 2 : 1][2];
+        half8_t w[RT][2], lost[Q6 ? RT : 1][2];
         float f[2];
         bool any[2];
     };
     auto decode = [&](Ops &o, uint32_t i, uint32_t live) __attribute__((always_inline)) {  // k-block i of the window
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
+        for (int rt = 0; rt < RT; ++rt) {
             const uint8_t *row = wbuf + (32u * rt + n) * F::RS;
             if constexpr (TY == 1) {
                 moe_f16_block(o.w[rt], row, i, h, live);
@@ -408,7 +408,7 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
                                                                                   u * 64u + 16u * ((2u * s + h) ^ moe_swz(u))));
                 }
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
+        for (int rt = 0; rt < RT; ++rt) {
             if constexpr (TY == 1 || KQ || FOLD) {
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
@@ -442,22 +442,22 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
     };
     // the next window into LDS, when the last one's weights have all been taken from there, and the one after it
     // requested
-    auto advance = [&](uint32_t w) __attribute__((always_inline)) {
+    auto advance = [&](uint32_t w, uint32_t set) __attribute__((always_inline)) {  // set: w % DEPTH
         __builtin_amdgcn_wave_barrier();
-        wput();
+        wput(set);
         __builtin_amdgcn_wave_barrier();
-        wload(min(w + 1u, n_win - 1u));
+        wload(min(w + DEPTH, n_win - 1u), set);
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (KQ) {
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
+            for (int rt = 0; rt < RT; ++rt)
                 factor[rt] = mms_f16(*(const uint16_t *) (wbuf + (32u * rt + n) * F::RS + (Q6 ? 208u + MmsFmt<14>::LAST : 0u)));
         }
         if constexpr (FOLD) {
-            uint32_t lo = 255u, hi = 0u;  // of row `lane`
+            uint32_t lo = 255u, hi = 0u;  // of one row per lane
 #pragma unroll
             for (uint32_t i = 0; i < WB; ++i) {
-                const uint32_t e8 = wbuf[lane * F::RS + 17u * i];
+                const uint32_t e8 = wbuf[lane % (32u * RT) * F::RS + 17u * i];
                 lo = min(lo, e8);
                 hi = max(hi, e8);
             }
@@ -467,7 +467,7 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
     // the accumulators from the last super-block's unit to this one's
     auto rescale = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
+        for (int rt = 0; rt < RT; ++rt) {
             const float ratio = factor[rt] != 0.f ? unit[rt] / factor[rt] : 1.f;
             unit[rt] = factor[rt] != 0.f ? factor[rt] : unit[rt];
 #pragma unroll
@@ -478,7 +478,7 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
     };
     auto mins = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
+        for (int rt = 0; rt < RT; ++rt) {
             const uint8_t *row = wbuf + (32u * rt + n) * F::RS;
             const u32x2_t h0 = *(const u32x2_t *) row, h1 = *(const u32x2_t *) (row + 8);
             const u32x4_t hd = {h0[0], h0[1], h1[0], h1[1]};
@@ -509,42 +509,48 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
         __builtin_amdgcn_sched_barrier(0);  // left alone, the loads sink to the step's end, and the next waits for them
     };
     const uint32_t all = 0xFFFFFFFFu;
-    wload(0u);
+#pragma unroll
+    for (uint32_t d = 0; d < DEPTH; ++d) wload(min(d, n_win - 1u), d);
     xload(0u);
     xput(0u);
     if constexpr (Q45) xsums(piece);
     xload(min(1u, total - 1u));
     moe_barrier();
-    advance(0u);
+    advance(0u, 0u);
     Ops A, B;
     uint32_t w = 0;
     // Sums: the pair that is stored for the next step has its own stored with it, but the next window's first pair
     // waits for that window, when the mins of this one have been taken.
+    auto window = [&](uint32_t w, uint32_t next_set) __attribute__((always_inline)) {
+        const uint32_t blocks = w ? WB : head;
+        if constexpr (KQ) rescale();
+#pragma unroll
+        for (uint32_t j = 0; j < SPW; ++j) {
+            if (!KQ && 2u * j >= blocks) continue;
+            const uint32_t live = KQ || 2u * j + 1u < blocks ? all : 0u;
+            if constexpr (Q45)
+                if (j == 0) sput(piece, 0u);
+            copies();
+            if constexpr (Q45)
+                if (j + 1u < SPW) sput(piece, j + 1u);
+            decode(A, 2u * j, all);
+            decode(B, 2u * j + 1u, live);
+            products(step & 1u, 0u, A);
+            products(step & 1u, 1u, B);
+            if constexpr (Q45)
+                if (j + 1u == SPW) mins();
+            moe_barrier();
+            ++step;
+        }
+        advance(w + 1u, next_set);
+    };
     if (!PIPE || head < WB) {
         const uint32_t until = PIPE ? 1u : n_win;
 #pragma unroll 1
-        for (; w < until; ++w) {
-            const uint32_t blocks = w ? WB : head;
-            if constexpr (KQ) rescale();
-#pragma unroll
-            for (uint32_t j = 0; j < SPW; ++j) {
-                if (!KQ && 2u * j >= blocks) continue;
-                const uint32_t live = KQ || 2u * j + 1u < blocks ? all : 0u;
-                if constexpr (Q45)
-                    if (j == 0) sput(piece, 0u);
-                copies();
-                if constexpr (Q45)
-                    if (j + 1u < SPW) sput(piece, j + 1u);
-                decode(A, 2u * j, all);
-                decode(B, 2u * j + 1u, live);
-                products(step & 1u, 0u, A);
-                products(step & 1u, 1u, B);
-                if constexpr (Q45)
-                    if (j + 1u == SPW) mins();
-                moe_barrier();
-                ++step;
-            }
-            advance(w + 1u);
+        for (; w < until; w += DEPTH) {
+            window(w, 1u % DEPTH);
+            if constexpr (DEPTH == 2u)
+                if (w + 1u < until) window(w + 1u, 0u);
         }
     }
     // MXFP4's whole windows: each block's weights are decoded while the one before is multiplied (the other formats
@@ -558,7 +564,7 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
                 copies();
                 decode(B, 2u * j + 1u, all);
                 products(step & 1u, 0u, A);
-                if (j + 1u == SPW) advance(w + 1u);
+                if (j + 1u == SPW) advance(w + 1u, 0u);
                 decode(A, (2u * j + 2u) % WB, all);
                 products(step & 1u, 1u, B);
                 moe_barrier();
@@ -568,7 +574,7 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
     }
     if constexpr (KQ) {
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt)
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
@@ -581,7 +587,8 @@ template <uint32_t TY, bool GU, int HALVES, bool LIGHT, bool BOTH>
 __device__ __forceinline__ void moe_tile_half(const MoeArgs &a, uint8_t *xbuf, uint8_t *wbuf, uint16_t *sums, uint32_t e,
                                               const uint32_t *slots, uint32_t count, uint32_t r0) {
     const uint32_t lane = threadIdx.x & 63u, n = lane & 31u, h = lane >> 5;
-    moe_f32x16 acc[2][2];
+    constexpr int RT = LIGHT ? 1 : 2;
+    moe_f32x16 acc[2][RT];
     const bool ok = moe_tile_sums<TY, GU, HALVES, LIGHT, BOTH, TY == 39>(a, acc, xbuf, wbuf, sums, e, slots, count, r0);
     if constexpr (TY == 39)  // some scale out of range: again, every block's sum scaled by itself
         if (__syncthreads_or(!ok))
@@ -590,9 +597,10 @@ __device__ __forceinline__ void moe_tile_half(const MoeArgs &a, uint8_t *xbuf, u
     // were a round trip apiece: a product of 200 tiles of 1536 x 512 Q4_K 69 us, now 61).
     const uint32_t held = slots[min(lane, count - 1u)];
 #pragma unroll
-    for (int rt = 0; rt < (GU ? 1 : 2); ++rt) {
-        const uint32_t r = r0 + 32u * rt + n;
-        const bool in = r < a.rows;
+    for (int rt = 0; rt < (GU ? 1 : RT); ++rt) {
+        // GU: gate and up in the lane's two row tiles, or, of one tile, in lanes 16 apart, the first 16 of which go on
+        const uint32_t r = r0 + (GU && RT == 1 ? n & 15u : 32u * rt + n);
+        const bool in = r < a.rows && (!GU || RT == 2 || n < 16u);
         const uint64_t at_row = (uint64_t) e * a.rows + min(r, a.rows - 1u);
         const float b0 = a.bias[0] ? a.bias[0][at_row] : 0.f, b1 = GU && a.bias[1] ? a.bias[1][at_row] : 0.f;
         // GU: where the next product, whose weights are of type a.y_order, looks for column r (it has whole blocks)
@@ -603,9 +611,10 @@ __device__ __forceinline__ void moe_tile_half(const MoeArgs &a, uint8_t *xbuf, u
             for (int j = 0; j < 16; ++j) {
                 const uint32_t u = 32u * tt + 8u * (j >> 2) + 4u * h + (j & 3);
                 const uint64_t o = (uint64_t) (uint32_t) __shfl((int) held, (int) u) * a.rows + col;
+                const float up = !GU ? 0.f : RT == 2 ? acc[tt][RT - 1][j] : __shfl_xor(acc[tt][0][j], 16);
                 if (!in || u >= count) continue;
                 if constexpr (GU) {
-                    const float v = moe_activation(a, acc[tt][0][j] + b0, acc[tt][1][j] + b1);
+                    const float v = moe_activation(a, acc[tt][0][j] + b0, up + b1);
                     const _Float16 hi = (_Float16) v;
                     ((_Float16 *) a.y)[o] = hi;
                     if constexpr (HALVES == 2) ((_Float16 *) a.y_lo)[o] = (_Float16) (v - (float) hi);
@@ -622,7 +631,7 @@ template <uint32_t TY, bool GU, int HALVES, bool LIGHT>
 __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
     using F = MoeTileFmt<TY, HALVES>;
     __shared__ __attribute__((aligned(1024))) uint8_t xbuf[4 * HALVES * (LIGHT ? 2048 : 4096)];
-    __shared__ __attribute__((aligned(16))) uint8_t wbuf[4][64 * F::RS];
+    __shared__ __attribute__((aligned(16))) uint8_t wbuf[4][(LIGHT ? 32 : 64) * F::RS];
     // Q4_K, Q5_K: [slot][piece 0 .. 3][block of the super-block] bf16, a block's sum of x in three pieces
     __shared__ __attribute__((aligned(16))) uint16_t sums[TY == 12 || TY == 13 ? (LIGHT ? 32 : 64) * 32 : 8];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -638,13 +647,14 @@ __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
     const MoeTile t = a.tiles[tile0 + in % some.of];
     const uint32_t e = __builtin_amdgcn_readfirstlane(t.expert), count = __builtin_amdgcn_readfirstlane(t.count);
     const uint32_t *const slots = a.list + t.first;
-    // this wave's rows: GU: 32 of each matrix from r0, else 64 from r0
-    const uint32_t r0 = rt_i * (GU ? 128u : 256u) + wave * (GU ? 32u : 64u);
+    // this wave's rows: 32 RT from r0, GU: half as many of each matrix
+    constexpr uint32_t ROWS = (LIGHT ? 32u : 64u) / (GU ? 2u : 1u);
+    const uint32_t r0 = (4u * rt_i + wave) * ROWS;
     if (e == a.n_expert) {
         if (!GU && a.zero_skipped)
             for (uint32_t u = 0; u < count; ++u) {
                 const uint64_t o = (uint64_t) slots[u] * a.rows + r0 + lane;
-                if (r0 + lane >= a.rows) continue;
+                if (lane >= ROWS || r0 + lane >= a.rows) continue;
                 if (a.y_f16) ((uint16_t *) a.y)[o] = 0;
                 else ((float *) a.y)[o] = 0.f;
             }
@@ -693,21 +703,23 @@ __device__ __forceinline__ void moe_prep_body(const MoePrepArgs &a) {
 
 }  // namespace
 
-#define MOE_TILE_KERNEL(NAME, TY, KIND, GU, IO, HALVES)                                                        \
+// Waves per SIMD of the light kernels: four where the registers allow it without spilling (MXFP4: 24 tokens of
+// 128 experts 133 + 82 us, with three 135 + 86; Q8_0, 200 tokens of 64 experts: 130 + 78, with three 114 + 62)
+#define MOE_TILE_KERNEL(NAME, TY, KIND, GU, IO, HALVES, WAVES)                                                  \
     extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))                \
     moearc_moe_tile_##NAME##_##KIND##_##IO##_k(MoeArgs a) { moe_tile_body<TY, GU, HALVES, false>(a); }          \
-    extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3)))                \
+    extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))        \
     moearc_moe_light_##NAME##_##KIND##_##IO##_k(MoeArgs a) { moe_tile_body<TY, GU, HALVES, true>(a); }
-#define MOE_TILE(NAME, TY)                     \
-    MOE_TILE_KERNEL(NAME, TY, gu, true, f32, 2) \
-    MOE_TILE_KERNEL(NAME, TY, gu, true, f16, 1) \
-    MOE_TILE_KERNEL(NAME, TY, p, false, f32, 2) \
-    MOE_TILE_KERNEL(NAME, TY, p, false, f16, 1)
-MOE_TILE(f16, 1)
-MOE_TILE(q8_0, 8)
-MOE_TILE(q4_k, 12)
-MOE_TILE(q5_k, 13)
-MOE_TILE(q6_k, 14)
-MOE_TILE(mxfp4, 39)
+#define MOE_TILE(NAME, TY, WAVES)                     \
+    MOE_TILE_KERNEL(NAME, TY, gu, true, f32, 2, WAVES) \
+    MOE_TILE_KERNEL(NAME, TY, gu, true, f16, 1, WAVES) \
+    MOE_TILE_KERNEL(NAME, TY, p, false, f32, 2, WAVES) \
+    MOE_TILE_KERNEL(NAME, TY, p, false, f16, 1, WAVES)
+MOE_TILE(f16, 1, 4)
+MOE_TILE(q8_0, 8, 3)
+MOE_TILE(q4_k, 12, 3)
+MOE_TILE(q5_k, 13, 3)
+MOE_TILE(q6_k, 14, 3)
+MOE_TILE(mxfp4, 39, 4)
 extern "C" __global__ void __launch_bounds__(256) moearc_moe_prep_f32_k(MoePrepArgs a) { moe_prep_body<true>(a); }
 extern "C" __global__ void __launch_bounds__(256) moearc_moe_prep_f16_k(MoePrepArgs a) { moe_prep_body<false>(a); }

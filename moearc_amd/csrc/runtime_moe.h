@@ -127,8 +127,9 @@ int moe_product(moearc_ctx *c, MoeArgs a, unsigned ty, bool gate_up, bool half) 
     a.row_bytes = (uint64_t) a.cols / moearc_mv_be(ty) * moearc_mv_bb(ty);
     a.expert_bytes = a.row_bytes * a.rows;
     if (a.tiles) {
-        a.row_tiles = (a.rows + (gate_up ? 127 : 255)) / (gate_up ? 128 : 256);
         const bool light = moe_light(a.n_slots, a.n_expert);
+        const uint32_t per = (light ? 128u : 256u) / (gate_up ? 2u : 1u);  // rows of a matrix per work-group
+        a.row_tiles = (a.rows + per - 1) / per;
         const uint64_t most = a.row_tiles * moe_max_tiles(a.n_slots, a.n_expert, light ? MOEARC_MOE_LIGHT : MOEARC_MOE_TILE);
         const unsigned grid = (unsigned) ((most + 7) / 8 * 8);  // eight runs, one per XCD
         return launch(c, (light ? c->f_moe_light : c->f_moe_tile)[i][g][half], grid, 256, a, nullptr, a.rows, a.n_slots, name);
