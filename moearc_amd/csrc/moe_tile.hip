@@ -1,12 +1,12 @@
-// The experts' products over a plan (MoeArgs): tiles of up to 64 of one expert's slots times 256 weight rows
-// (128 of gate and the same 128 of up), on v_mfma_f32_32x32x16_f16.
+// The experts' products over a plan (MoeArgs): tiles of up to 64, or 32, of one expert's slots times 256 or 128
+// weight rows (half of them of gate and half of up), on v_mfma_f32_32x32x16_f16.
 //
 // The product is computed transposed, D[slot][row], so that a lane holds one weight row in all of its
-// accumulators and a block's scale is one per-lane factor. Work-group: 4 waves, each the tile's 64 slots
-// times 64 rows of its own as 2 x 2 tiles of 32 x 32 (gate_up: rows of gate beside the same rows of up, so
-// the activation needs no exchange). A weight is thus decoded by one wave only, and the slots' inputs, four
-// bytes an element where the weights have half to one, are shared by 256 rows. Tiles of at most 32 slots
-// skip the second half.
+// accumulators and a block's scale is one per-lane factor. Work-group: 4 waves, each the tile's slots
+// times 64 or 32 rows of its own in tiles of 32 x 32 (gate_up: rows of gate beside the same rows of up, in the
+// lane's two row tiles or 16 lanes apart, so the activation stays in the wave). A weight is thus decoded by one
+// wave only, and the slots' inputs, four bytes an element where the weights have half to one, are shared by all
+// rows. Tiles of at most 32 slots skip the second half.
 // - Weights: windows of WB k-blocks move through registers (the next window in flight while this one is
 //   multiplied) into the wave's LDS; lane l copies 16-byte pieces of rows 32 (l / 32) .. + 31.
 // - Inputs: pairs of k-blocks, f16 (hi and lo), 64 bytes per slot and block, whose 16-byte chunk c (k 8c ..)
@@ -215,16 +215,16 @@ typedef __bf16 moe_bf8 __attribute__((ext_vector_type(8)));
 
 // The reduction of one tile for a wave: acc[slot half][row tile], slots 32 and up only with BOTH. FOLD (MXFP4):
 // the scales enter the operand; returns false where one is out of f16's range, and the sums are not valid then.
-template <uint32_t TY, bool GU, int HALVES, bool LIGHT, bool BOTH, bool FOLD>
-__device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc)[2][LIGHT ? 1 : 2], uint8_t *xbuf, uint8_t *wbuf, uint16_t *sums,
+template <uint32_t TY, bool GU, int HALVES, int TS, int RT, bool BOTH, bool FOLD>
+__device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc)[2][RT], uint8_t *xbuf, uint8_t *wbuf, uint16_t *sums,
                                               uint32_t e, const uint32_t *slots, uint32_t count, uint32_t r0) {
     using F = MoeTileFmt<TY, HALVES>;
     constexpr uint32_t WB = F::WB, SPW = WB / 2u;
-    constexpr bool Q45 = TY == 12 || TY == 13, Q6 = TY == 14, MX = TY == 39, KQ = Q45 || Q6, PIPE = MX && !LIGHT;
-    // RT row tiles of 32 per wave; windows of weights requested DEPTH ahead
-    constexpr int NT = BOTH ? 2 : 1, RT = LIGHT ? 1 : 2;
-    constexpr uint32_t WG = 2u * RT, DEPTH = LIGHT ? 2u : 1u;
-    constexpr uint32_t XB = LIGHT ? 2048u : 4096u, XPAIR = 2u * HALVES * XB;  // one half of a k-block, a pair of k-blocks
+    constexpr bool Q45 = TY == 12 || TY == 13, Q6 = TY == 14, MX = TY == 39, KQ = Q45 || Q6, PIPE = MX && TS == 2;
+    // windows of weights requested DEPTH ahead
+    constexpr int NT = BOTH ? 2 : 1;
+    constexpr uint32_t WG = 2u * RT, DEPTH = TS == 1 ? 2u : 1u;
+    constexpr uint32_t XB = 2048u * TS, XPAIR = 2u * HALVES * XB;  // one half of a k-block, a pair of k-blocks
     const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 31u, h = lane >> 5;
     const uint32_t nb = a.cols / 32u, n_win = (nb + WB - 1u) / WB;
     // Window 0 has the first `head` blocks (it is copied whole, the rest of it belongs to window 1), the others WB each.
@@ -583,16 +583,15 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
     return ok;
 }
 
-template <uint32_t TY, bool GU, int HALVES, bool LIGHT, bool BOTH>
+template <uint32_t TY, bool GU, int HALVES, int TS, int RT, bool BOTH>
 __device__ __forceinline__ void moe_tile_half(const MoeArgs &a, uint8_t *xbuf, uint8_t *wbuf, uint16_t *sums, uint32_t e,
                                               const uint32_t *slots, uint32_t count, uint32_t r0) {
     const uint32_t lane = threadIdx.x & 63u, n = lane & 31u, h = lane >> 5;
-    constexpr int RT = LIGHT ? 1 : 2;
     moe_f32x16 acc[2][RT];
-    const bool ok = moe_tile_sums<TY, GU, HALVES, LIGHT, BOTH, TY == 39>(a, acc, xbuf, wbuf, sums, e, slots, count, r0);
+    const bool ok = moe_tile_sums<TY, GU, HALVES, TS, RT, BOTH, TY == 39>(a, acc, xbuf, wbuf, sums, e, slots, count, r0);
     if constexpr (TY == 39)  // some scale out of range: again, every block's sum scaled by itself
         if (__syncthreads_or(!ok))
-            (void) moe_tile_sums<TY, GU, HALVES, LIGHT, BOTH, false>(a, acc, xbuf, wbuf, sums, e, slots, count, r0);
+            (void) moe_tile_sums<TY, GU, HALVES, TS, RT, BOTH, false>(a, acc, xbuf, wbuf, sums, e, slots, count, r0);
     // Each lane holds one slot of the tile, from where the others take it (read from memory beside each store, they
     // were a round trip apiece: a product of 200 tiles of 1536 x 512 Q4_K 69 us, now 61).
     const uint32_t held = slots[min(lane, count - 1u)];
@@ -627,13 +626,14 @@ __device__ __forceinline__ void moe_tile_half(const MoeArgs &a, uint8_t *xbuf, u
     }
 }
 
-template <uint32_t TY, bool GU, int HALVES, bool LIGHT>
+// Tiles of up to 32 TS slots, RT row tiles of 32 per wave.
+template <uint32_t TY, bool GU, int HALVES, int TS, int RT>
 __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
     using F = MoeTileFmt<TY, HALVES>;
-    __shared__ __attribute__((aligned(1024))) uint8_t xbuf[4 * HALVES * (LIGHT ? 2048 : 4096)];
-    __shared__ __attribute__((aligned(16))) uint8_t wbuf[4][(LIGHT ? 32 : 64) * F::RS];
+    __shared__ __attribute__((aligned(1024))) uint8_t xbuf[4 * HALVES * 2048 * TS];
+    __shared__ __attribute__((aligned(16))) uint8_t wbuf[4][32 * RT * F::RS];
     // Q4_K, Q5_K: [slot][piece 0 .. 3][block of the super-block] bf16, a block's sum of x in three pieces
-    __shared__ __attribute__((aligned(16))) uint16_t sums[TY == 12 || TY == 13 ? (LIGHT ? 32 : 64) * 32 : 8];
+    __shared__ __attribute__((aligned(16))) uint16_t sums[TY == 12 || TY == 13 ? 32 * TS * 32 : 8];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // The work in the order (expert, row tile, tile of slots), cut into eight equal runs, one for each XCD
     // (work-group i is on XCD i % 8): an expert's rows are then read by the L2 that all of its tiles go through, and
@@ -648,7 +648,7 @@ __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
     const uint32_t e = __builtin_amdgcn_readfirstlane(t.expert), count = __builtin_amdgcn_readfirstlane(t.count);
     const uint32_t *const slots = a.list + t.first;
     // this wave's rows: 32 RT from r0, GU: half as many of each matrix
-    constexpr uint32_t ROWS = (LIGHT ? 32u : 64u) / (GU ? 2u : 1u);
+    constexpr uint32_t ROWS = 32u * RT / (GU ? 2u : 1u);
     const uint32_t r0 = (4u * rt_i + wave) * ROWS;
     if (e == a.n_expert) {
         if (!GU && a.zero_skipped)
@@ -660,9 +660,9 @@ __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
             }
         return;
     }
-    if constexpr (!LIGHT)
-        if (count > 32u) return moe_tile_half<TY, GU, HALVES, false, true>(a, xbuf, wbuf[wave], sums, e, slots, count, r0);
-    moe_tile_half<TY, GU, HALVES, LIGHT, false>(a, xbuf, wbuf[wave], sums, e, slots, count, r0);
+    if constexpr (TS == 2)
+        if (count > 32u) return moe_tile_half<TY, GU, HALVES, TS, RT, true>(a, xbuf, wbuf[wave], sums, e, slots, count, r0);
+    moe_tile_half<TY, GU, HALVES, TS, RT, false>(a, xbuf, wbuf[wave], sums, e, slots, count, r0);
 }
 
 // x for the tiles: f16 (of f32: hi, and the remainder lo) in the order of the weights' type, eight elements,
@@ -703,23 +703,29 @@ __device__ __forceinline__ void moe_prep_body(const MoePrepArgs &a) {
 
 }  // namespace
 
-// Waves per SIMD of the light kernels: four where the registers allow it without spilling (MXFP4: 24 tokens of
-// 128 experts 133 + 82 us, with three 135 + 86; Q8_0, 200 tokens of 64 experts: 130 + 78, with three 114 + 62)
-#define MOE_TILE_KERNEL(NAME, TY, KIND, GU, IO, HALVES, WAVES)                                                  \
-    extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))                \
-    moearc_moe_tile_##NAME##_##KIND##_##IO##_k(MoeArgs a) { moe_tile_body<TY, GU, HALVES, false>(a); }          \
-    extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))        \
-    moearc_moe_light_##NAME##_##KIND##_##IO##_k(MoeArgs a) { moe_tile_body<TY, GU, HALVES, true>(a); }
-#define MOE_TILE(NAME, TY, WAVES)                     \
-    MOE_TILE_KERNEL(NAME, TY, gu, true, f32, 2, WAVES) \
-    MOE_TILE_KERNEL(NAME, TY, gu, true, f16, 1, WAVES) \
-    MOE_TILE_KERNEL(NAME, TY, p, false, f32, 2, WAVES) \
-    MOE_TILE_KERNEL(NAME, TY, p, false, f16, 1, WAVES)
-MOE_TILE(f16, 1, 4)
-MOE_TILE(q8_0, 8, 3)
-MOE_TILE(q4_k, 12, 3)
-MOE_TILE(q5_k, 13, 3)
-MOE_TILE(q6_k, 14, 3)
-MOE_TILE(mxfp4, 39, 4)
+// Shapes, as moe_shape (runtime_moe.h) has them. Wide tiles, 64 slots x 64 rows a wave and two waves per SIMD, decode
+// each weight for twice the slots and read the inputs half as often; narrow ones, 32 rows a wave, hold three or four
+// waves per SIMD, which cover each other's waits. Products measured wide, narrow (us):
+//   MXFP4 f32 361 / 369, f16 172 / 162; Q4_K f32 174 / 201, f16 170 / 169; Q5_K 202 / 225; Q6_K f32 390 / 304,
+//   f16 162 / 134; Q8_0 200 / 189; F16 f32 165 / 161, f16 286 / 260
+// Light tiles, of 32 slots, for few slots an expert: four waves where the registers allow it without spilling
+// (MXFP4: 24 tokens of 128 experts 133 + 82 us, with three 135 + 86; Q8_0, 200 tokens of 64 experts: 130 + 78, with
+// three 114 + 62).
+#define MOE_TILE_KERNEL(NAME, TY, KIND, GU, IO, HALVES, RT, WAVES, LIGHT_WAVES)                                     \
+    extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES)))            \
+    moearc_moe_tile_##NAME##_##KIND##_##IO##_k(MoeArgs a) { moe_tile_body<TY, GU, HALVES, 2, RT>(a); }              \
+    extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(LIGHT_WAVES, LIGHT_WAVES))) \
+    moearc_moe_light_##NAME##_##KIND##_##IO##_k(MoeArgs a) { moe_tile_body<TY, GU, HALVES, 1, 1>(a); }
+#define MOE_TILE(NAME, TY, RT32, WAVES32, RT16, WAVES16, LIGHT_WAVES)          \
+    MOE_TILE_KERNEL(NAME, TY, gu, true, f32, 2, RT32, WAVES32, LIGHT_WAVES)    \
+    MOE_TILE_KERNEL(NAME, TY, gu, true, f16, 1, RT16, WAVES16, LIGHT_WAVES)    \
+    MOE_TILE_KERNEL(NAME, TY, p, false, f32, 2, RT32, WAVES32, LIGHT_WAVES)    \
+    MOE_TILE_KERNEL(NAME, TY, p, false, f16, 1, RT16, WAVES16, LIGHT_WAVES)
+MOE_TILE(f16, 1, 1, 4, 1, 4, 4)
+MOE_TILE(q8_0, 8, 1, 3, 1, 3, 3)
+MOE_TILE(q4_k, 12, 2, 2, 2, 2, 3)
+MOE_TILE(q5_k, 13, 2, 2, 2, 2, 3)
+MOE_TILE(q6_k, 14, 1, 3, 1, 3, 3)
+MOE_TILE(mxfp4, 39, 2, 2, 1, 3, 4)
 extern "C" __global__ void __launch_bounds__(256) moearc_moe_prep_f32_k(MoePrepArgs a) { moe_prep_body<true>(a); }
 extern "C" __global__ void __launch_bounds__(256) moearc_moe_prep_f16_k(MoePrepArgs a) { moe_prep_body<false>(a); }

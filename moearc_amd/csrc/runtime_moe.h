@@ -74,14 +74,19 @@ int moe_count_check(unsigned long n_tok, unsigned long n_used, unsigned long n_e
     return OK;
 }
 
-// Whether a chunk runs on tiles of 32 slots.
-bool moe_light(uint64_t n_slots, uint64_t n_expert) {
-    static const char *const e = std::getenv("MOE_LIGHT");
-    return n_slots <= (e ? std::strtoul(e, nullptr, 10) : 32) * n_expert;
+// Whether a chunk runs on tiles of 32 slots, not 64: up to 56 slots an expert, 40 with f16 inputs. (Products of 64
+// slots an expert, 64 and 32 slots a tile: MXFP4 142 and 121 us, Q8_0 88 and 82, Q4_K 84 and 86, Q5_K 97 and 100, f16
+// Q4_K 155 and 166, Q6_K 149 and 157; of 32: MXFP4 87 and 82, Q4_K 69 and 58, Q5_K 80 and 67, f16 Q4_K 111 and 109.)
+bool moe_light(uint64_t n_slots, uint64_t n_expert, bool half) { return n_slots < (half ? 40 : 56) * n_expert; }
+
+// Rows of each matrix that a tile's work-group takes: moe_tile.hip's shapes.
+uint32_t moe_tile_rows(unsigned ty, bool half, bool light, bool gate_up) {
+    const bool wide = !light && (ty == 12u || ty == 13u || (ty == 39u && !half));
+    return (wide ? 256u : 128u) / (gate_up ? 2u : 1u);
 }
 
 // Groups a chunk's slots by expert. Launches of at most 64 slots need no plan.
-int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slots, uint32_t n_expert, uint8_t *ws,
+int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slots, uint32_t n_expert, bool half, uint8_t *ws,
              const MoeSpace &sp) {
     a.ids = ids;
     a.n_slots = n_slots;
@@ -97,7 +102,7 @@ int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slot
     p.err = c->err_word;
     p.n_slots = n_slots;
     p.n_expert = n_expert;
-    p.tile = moe_light(n_slots, n_expert) ? MOEARC_MOE_LIGHT : MOEARC_MOE_TILE;
+    p.tile = moe_light(n_slots, n_expert, half) ? MOEARC_MOE_LIGHT : MOEARC_MOE_TILE;
     a.tiles = p.tiles;
     a.n_tiles = p.n_tiles;
     a.list = p.list;
@@ -127,8 +132,8 @@ int moe_product(moearc_ctx *c, MoeArgs a, unsigned ty, bool gate_up, bool half) 
     a.row_bytes = (uint64_t) a.cols / moearc_mv_be(ty) * moearc_mv_bb(ty);
     a.expert_bytes = a.row_bytes * a.rows;
     if (a.tiles) {
-        const bool light = moe_light(a.n_slots, a.n_expert);
-        const uint32_t per = (light ? 128u : 256u) / (gate_up ? 2u : 1u);  // rows of a matrix per work-group
+        const bool light = moe_light(a.n_slots, a.n_expert, half);
+        const uint32_t per = moe_tile_rows(ty, half, light, gate_up);
         a.row_tiles = (a.rows + per - 1) / per;
         const uint64_t most = a.row_tiles * moe_max_tiles(a.n_slots, a.n_expert, light ? MOEARC_MOE_LIGHT : MOEARC_MOE_TILE);
         const unsigned grid = (unsigned) ((most + 7) / 8 * 8);  // eight runs, one per XCD
@@ -343,7 +348,7 @@ int moearc_matmul_experts(moearc_ctx *c, unsigned int type_id, void *y, const vo
     for (unsigned long t = 0; t < n_tok; t += chunk) {
         const unsigned long n = std::min(chunk, n_tok - t);
         MoeArgs a{};
-        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) n_expert, mem, sp))
+        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) n_expert, io_type == MOEARC_OUT_F16, mem, sp))
             return rc;
         a.x = (const uint8_t *) x + (x_per_slot ? t * n_used : t) * n_cols * elem;
         a.x_div = x_per_slot ? 1u : (uint32_t) n_used;
@@ -389,7 +394,7 @@ int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, u
     for (unsigned long t = 0; t < n_tok; t += chunk) {
         const unsigned long n = std::min(chunk, n_tok - t);
         MoeArgs a{};
-        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) m->n_expert, mem, sp))
+        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) m->n_expert, half, mem, sp))
             return rc;
         MoeArgs g = a, d = a;
         g.x = (const uint8_t *) x + t * m->n_embd * elem;
