@@ -342,6 +342,9 @@ struct MoeCombineArgs {
     void *y;                   // [n_tok][cols] f32 or f16
     uint32_t n_tok, n_used, n_expert, cols, y_f16, accumulate;
 };
+// Working memory is bounded by cutting long calls into chunks of tokens of at most this many slots: 32,768 slots of
+// 2,880 columns hold 0.4 GB per f32 array, and give each of 128 experts 256 slots.
+#define MOEARC_MOE_CHUNK_SLOTS 32768u
 #define MOEARC_MOE_SMALL_SLOTS 64u  // most slots of a launch without a plan
 #define MOEARC_MOE_SMALL_WAVES 8
 #define MOEARC_MOE_SMALL_TOKENS 16u

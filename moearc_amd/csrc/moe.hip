@@ -128,20 +128,33 @@ ROUTE_KERNEL(64)
 
 // The plan (MoePlanArgs). One work-group per expert, and one for the slots without: each counts every
 // group's slots itself (integer adds in LDS, so the order of the adds does not matter), from which it knows
-// its group's first place and first tile, and then collects its own slots in order. No work-group waits for
-// another, and the result does not depend on their order.
+// its group's first place and first tile, and then collects its own slots in order: each wave its share of the
+// slots, counted, then placed. No work-group waits for another, and the result does not depend on their order.
+// The ids are read once, all loads in flight, and kept in LDS (8000 slots: 13 us when they were read twice, with
+// two barriers for every 1024).
 extern "C" __global__ void __launch_bounds__(1024) moearc_moe_plan_k(MoePlanArgs a) {
+    __shared__ uint16_t ids[MOEARC_MOE_CHUNK_SLOTS];
     __shared__ uint32_t count[MOEARC_MAX_EXPERTS + 1];
     __shared__ uint32_t wave_n[16], before[2];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, mine = blockIdx.x;
     for (uint32_t e = tid; e <= a.n_expert; e += 1024u) count[e] = 0u;
     if (tid < 2u) before[tid] = 0u;
     __syncthreads();
-    for (uint32_t s = tid; s < a.n_slots; s += 1024u) {
-        const uint32_t id = a.ids[s];
-        if (id >= a.n_expert && id != MOEARC_NO_EXPERT) *(volatile uint32_t *) a.err = 1u;  // every writer stores the same
-        atomicAdd(&count[min(id, a.n_expert)], 1u);
+    bool wrong = false;
+    for (uint32_t s0 = tid; s0 < a.n_slots; s0 += 8u * 1024u) {
+        uint32_t id[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8u; ++k) id[k] = a.ids[min(s0 + 1024u * k, a.n_slots - 1u)];
+#pragma unroll
+        for (uint32_t k = 0; k < 8u; ++k)
+            if (s0 + 1024u * k < a.n_slots) {
+                wrong = wrong || (id[k] >= a.n_expert && id[k] != MOEARC_NO_EXPERT);
+                const uint32_t e = min(id[k], a.n_expert);
+                ids[s0 + 1024u * k] = (uint16_t) e;
+                atomicAdd(&count[e], 1u);
+            }
     }
+    if (wrong && mine == 0u) *(volatile uint32_t *) a.err = 1u;  // every writer stores the same
     __syncthreads();
     uint32_t slots = 0u, tiles = 0u;
     for (uint32_t e = tid; e < mine; e += 1024u) {
@@ -152,28 +165,24 @@ extern "C" __global__ void __launch_bounds__(1024) moearc_moe_plan_k(MoePlanArgs
         atomicAdd(&before[0], slots);
         atomicAdd(&before[1], tiles);
     }
+    // this wave's share of the slots, 64 at a time
+    const uint32_t share = (a.n_slots + 1023u) / 1024u * 64u, from = min(wave * share, a.n_slots), to = min(from + share, a.n_slots);
+    uint32_t hits = 0u;
+    for (uint32_t s0 = from; s0 < to; s0 += 64u) hits += (uint32_t) __popcll(__ballot(s0 + lane < to && ids[s0 + lane] == mine));
+    if (lane == 0u) wave_n[wave] = hits;
     __syncthreads();
     const uint32_t n = count[mine], first = before[0], tile0 = before[1], n_tiles = (n + a.tile - 1u) / a.tile;
     for (uint32_t i = tid; i < n_tiles; i += 1024u)
         a.tiles[tile0 + i] = MoeTile{mine, first + i * a.tile, (uint16_t) min(a.tile, n - i * a.tile), 0, (uint16_t) i, (uint16_t) n_tiles};
     if (mine == a.n_expert && tid == 0u) *a.n_tiles = tile0 + n_tiles;
-    if (n == 0u) return;
     uint32_t at = first;
-    for (uint32_t s0 = 0; s0 < a.n_slots; s0 += 1024u) {
-        const uint32_t s = s0 + tid;
-        const bool hit = s < a.n_slots && min(a.ids[s], a.n_expert) == mine;
-        const uint64_t mask = __ballot(hit);
-        if (lane == 0u) wave_n[wave] = (uint32_t) __popcll(mask);
-        __syncthreads();
-        uint32_t lead = 0u, sum = 0u;
 #pragma unroll
-        for (uint32_t w = 0; w < 16u; ++w) {
-            if (w < wave) lead += wave_n[w];
-            sum += wave_n[w];
-        }
-        if (hit) a.list[at + lead + (uint32_t) __popcll(mask & ((1ull << lane) - 1ull))] = s;
-        at += sum;
-        __syncthreads();
+    for (uint32_t w = 0; w < 16u; ++w) at += w < wave ? wave_n[w] : 0u;
+    for (uint32_t s0 = from; s0 < to; s0 += 64u) {
+        const bool hit = s0 + lane < to && ids[s0 + lane] == mine;
+        const uint64_t mask = __ballot(hit);
+        if (hit) a.list[at + (uint32_t) __popcll(mask & ((1ull << lane) - 1ull))] = s0 + lane;
+        at += (uint32_t) __popcll(mask);
     }
 }
 

@@ -4,9 +4,7 @@
 
 namespace {
 
-// Bytes of a chunk's working memory are bounded by cutting long calls into chunks of at most this many
-// slots: 32,768 slots of 2,880 columns hold 0.4 GB per f32 array, and give each of 128 experts 256 slots.
-constexpr unsigned long kMoeChunkSlots = 32768;
+constexpr unsigned long kMoeChunkSlots = MOEARC_MOE_CHUNK_SLOTS;
 
 constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 

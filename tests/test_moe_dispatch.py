@@ -127,6 +127,69 @@ def test_ffn_refusals(cx, lib, desc, kw, rc):
     assert cx._lib.moearc_moe_ffn(cx.raw, None, 64, 64, 0, 64, 64, 1, 1, 0, None, 0) == -1
 
 
+def _kernels(lib):
+    return [k[len("moearc_moe_"):-len("_k")] for k in names(lib)]
+
+
+FORMS = [  # slots per expert, type, f16: the product's form
+    (2, 8, 0, "light"), (55, 8, 0, "light"), (56, 8, 0, "tile"), (39, 8, 1, "light"), (40, 8, 1, "tile"), (55, 39, 0, "light"),
+    (56, 39, 0, "tile"), (56, 14, 0, "tile"), (400, 12, 0, "tile")]
+
+
+@pytest.mark.parametrize("each,ty,half,form", FORMS, ids=str)
+def test_product_forms(cx, lib, each, ty, half, form):
+    name = {8: "q8_0", 39: "mxfp4", 14: "q6_k", 12: "q4_k"}[ty]
+    io = "f16" if half else "f32"
+    assert linear(cx, ty=ty, io=half, n_tok=each * 40, n_used=1, n_expert=40) == 0
+    prep = [] if half and ty == 8 else [f"prep_{io}"]
+    assert _kernels(lib) == ["plan", *prep, f"{form}_{name}_p_{io}"]
+    lib.host_hip_reset()
+    assert ffn(cx, {"w_type": [ty] * 3, "n_expert": 40}, io=half, n_tok=each * 40, n_used=1) == 0
+    assert _kernels(lib) == ["plan", *prep, f"{form}_{name}_gu_{io}", f"{form}_{name}_p_{io}", "combine4"]
+
+
+def test_grids_cover_every_tile(cx, lib):
+    # tiles: at most one partly filled for each expert and for the slots without one
+    for tok, used, experts, rows in ((17, 4, 128, 2880), (1000, 8, 128, 768), (8192, 4, 32, 2880), (65, 1, 1, 1)):
+        for io in (0, 1):
+            for ty in (1, 8, 12, 13, 14, 39):
+                lib.host_hip_reset()
+                assert linear(cx, ty=ty, io=io, n_tok=tok, n_used=used, n_expert=experts, n_rows=rows) == 0
+                (name, gx, gy, gz, block) = host_hip.launches(lib)[-1]
+                light = "light" in name
+                wide = not light and (ty in (12, 13) or (ty == 39 and not io))
+                tile, per, slots = 32 if light else 64, 256 if wide else 128, tok * used
+                tiles = min(slots, -(-slots // tile) + experts + 1)
+                assert (gy, gz, block) == (1, 1, 256) and gx % 8 == 0 and tiles * -(-rows // per) <= gx < tiles * -(-rows // per) + 8
+
+
+def test_few_slots_and_single_tokens(cx, lib):
+    assert linear(cx, n_tok=16, n_used=4, n_rows=70) == 0
+    assert host_hip.launches(lib) == [("moearc_moe_small_q8_0_p_f32_k", 3, 64, 1, 512)]
+    lib.host_hip_reset()
+    assert ffn(cx, n_tok=16, n_used=4) == 0
+    assert _kernels(lib) == ["small_q8_0_gu_f32", "small_q8_0_p_f32", "combine4"]
+    for desc, kw, want in (
+            ({}, {}, ["vec_q8_0_gu_p1", "vec_q8_0_down_p1"]),  # 256 and 512 columns: 16 and 32 pieces
+            ({"n_ff": 2880, "n_embd": 2880, "w_type": [39, 39, 39]}, {}, ["vec_mxfp4_gu_p2", "vec_mxfp4_down_p2"]),
+            ({"n_ff": 4096, "w_type": [8, 8, 12]}, dict(n_used=2), ["vec_q8_0_gu_p1", "vec_q4_k_down_p2"]),
+            ({"n_ff": 2048, "n_embd": 2048, "w_type": [14, 14, 14]}, {}, ["vec_q6_k_gu_p2", "vec_q6_k_down_p2"]),
+            ({"n_ff": 4128}, {}, ["small_q8_0_gu_f32", "small_q8_0_p_f32", "combine4"]),  # 258 pieces
+            ({"n_ff": 4096}, dict(n_used=4), ["small_q8_0_gu_f32", "small_q8_0_p_f32", "combine4"])):  # inputs past the LDS
+        lib.host_hip_reset()
+        assert ffn(cx, desc, n_tok=1, **kw) == 0
+        assert _kernels(lib) == want, (desc, kw)
+    lib.host_hip_reset()
+    assert ffn(cx, n_tok=1, n_used=65) == 0  # more than a wave's lanes
+    assert _kernels(lib)[0] == "plan"
+
+
+def test_long_calls_run_in_chunks(cx, lib):
+    assert ffn(cx, n_tok=8192 * 2 + 1, n_used=4) == 0
+    per = ["plan", "prep_f32", "tile_q8_0_gu_f32", "tile_q8_0_p_f32", "combine4"]
+    assert _kernels(lib)[:10] == per * 2 and _kernels(lib)[10:] == ["small_q8_0_gu_f32", "small_q8_0_p_f32", "combine4"]
+
+
 def test_workspace_sizes(lib):
     n = ctypes.c_ulong()
 
