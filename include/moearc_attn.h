@@ -359,7 +359,7 @@ int moearc_norm_residual(moearc_ctx *c, void *x, unsigned int x_type, float *h, 
 /* For each token the n_used largest of its n_expert logits, largest first, equal ones (-0 and +0 too) by
  * ascending expert: ids u32 [n_tok][n_used] and their softmax weights times scale, f32 [n_tok][n_used].
  * logits f32 [n_tok][n_expert]. A logit of -inf masks its expert: it is chosen after all others and weighs 0;
- * NaN counts as -inf and comes last. A token whose experts are all masked gets ids and weights of 0.
+ * NaN counts as -inf and comes last. A token whose experts are all masked has its ids as by this order, and weights 0.
  * Refusals: a null pointer -> -1; n_expert 0 or above 1024, n_used 0 or above n_expert, another mode,
  * n_tok >= 2^31 -> -2. No tokens -> 0. */
 int moearc_moe_route(moearc_ctx *c, unsigned int *ids, float *weights, const float *logits, unsigned long n_tok,
@@ -377,11 +377,12 @@ int moearc_moe_workspace(unsigned long n_tok, unsigned long n_used, unsigned lon
  * place of x[t]; j < n_used. w: the experts' matrices of one GGUF type (F16, Q8_0, Q4_K, Q5_K, Q6_K, MXFP4) one after
  * another, [n_expert][n_rows][n_cols]; bias f32 [n_expert][n_rows] or NULL; ids u32 [n_tok][n_used] (device;
  * experts may repeat within a token); x and y f32 or f16 by io_type, y [n_tok][n_used][n_rows]. y must not
- * overlap x. Each expert's weights are read once for all of its slots, whatever their number.
+ * overlap x. Slots of one expert share what is read of its weights, up to 64 at a time.
  * f32 activations enter as f16 hi + lo (to 2^-22 relative; each |x| below 65504), block sums are scaled in
  * f32: the bound of moearc_matmul_q; f16 ones as they are, and y is rounded once. The result of a slot does not
  * change from call to call with the same arguments.
- * A slot of MOEARC_NO_EXPERT gets a row of zeros; another id >= n_expert too, and the next moearc_sync returns -1.
+ * A slot of MOEARC_NO_EXPERT gets a row of zeros; another id >= n_expert too, and the next moearc_sync returns -1
+ * (after any replay too, when the call was captured).
  * ws: ws_bytes of 256-byte aligned device memory (moearc_moe_workspace), used until the call's work is done; NULL:
  * the context's, grown on demand. A captured call needs ws (else -1), and graphs that may run at the same time
  * need one each. Refusals: a null pointer other than bias and ws -> -1; io_type or x_per_slot not 0/1, n_expert or
@@ -411,7 +412,7 @@ typedef struct moearc_moe {
  * all device memory except m. Precision as moearc_matmul_experts, twice in a row: with f32 the values between the two
  * products stay f32 (as f16 hi + lo: each |act| below 65504), with f16 they are rounded to f16 once. Slots without an
  * expert add nothing, and their weights are not read; ids out of range and ws as there. Calls of more than
- * 32768 slots run in chunks of tokens, one after another.
+ * 32768 slots (fewer when rows are wider than 32768) run in chunks of tokens, one after another.
  * Refusals: a null pointer other than biases and ws -> -1; those of moearc_matmul_experts for each matrix, gate and
  * up of different types, another act, a negative or NaN limit, accumulate not 0/1 or with f16 -> -2. No tokens -> 0. */
 int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, unsigned int io_type,

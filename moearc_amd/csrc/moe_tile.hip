@@ -221,9 +221,8 @@ __device__ __forceinline__ bool moe_tile_sums(const MoeArgs &a, moe_f32x16 (&acc
     using F = MoeTileFmt<TY, HALVES>;
     constexpr uint32_t WB = F::WB, SPW = WB / 2u;
     constexpr bool Q45 = TY == 12 || TY == 13, Q6 = TY == 14, MX = TY == 39, KQ = Q45 || Q6, PIPE = MX && TS == 2;
-    // windows of weights requested DEPTH ahead
     constexpr int NT = BOTH ? 2 : 1;
-    constexpr uint32_t WG = 2u * RT, DEPTH = TS == 1 ? 2u : 1u;
+    constexpr uint32_t WG = 2u * RT, DEPTH = TS == 1 ? 2u : 1u;  // weights are requested DEPTH windows ahead
     constexpr uint32_t XB = 2048u * TS, XPAIR = 2u * HALVES * XB;  // one half of a k-block, a pair of k-blocks
     const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 31u, h = lane >> 5;
     const uint32_t nb = a.cols / 32u, n_win = (nb + WB - 1u) / WB;
@@ -703,7 +702,7 @@ __device__ __forceinline__ void moe_prep_body(const MoePrepArgs &a) {
 
 }  // namespace
 
-// Shapes, as moe_shape (runtime_moe.h) has them. Wide tiles, 64 slots x 64 rows a wave and two waves per SIMD, decode
+// Shapes, as moe_tile_rows (runtime_moe.h) has them. Wide tiles, 64 slots x 64 rows a wave and two waves per SIMD, decode
 // each weight for twice the slots and read the inputs half as often; narrow ones, 32 rows a wave, hold three or four
 // waves per SIMD, which cover each other's waits. Products measured wide, narrow (us):
 //   MXFP4 f32 361 / 369, f16 172 / 162; Q4_K f32 174 / 201, f16 170 / 169; Q5_K 202 / 225; Q6_K f32 390 / 304,

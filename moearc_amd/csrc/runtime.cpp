@@ -115,6 +115,7 @@ struct moearc_ctx {
     // entry point that returns nothing (moearc_free_device).
     uint32_t *err_word = nullptr;
     bool err_armed = false;
+    bool err_in_graph = false;  // a captured call may set it with any replay: every moearc_sync looks
     bool deferred_error = false;
     // The code object's fixed record array (moearc_decode_scratch): its device address in this
     // context's module instance, read once at creation, and its size in floats.
@@ -136,7 +137,7 @@ struct moearc_ctx {
     float *ws_kinds = nullptr;
     size_t ws_kinds_floats = 0;
     // norms (16, 64, 256, 1024 threads a row x scalar, four floats), router (16 << i experts), experts' products
-    hipFunction_t f_norm[4][2] = {}, f_norm_long = nullptr, f_route[7] = {}, f_moe_plan = nullptr, f_moe_combine[2] = {};
+    hipFunction_t f_norm[4][2] = {}, f_norm_long = nullptr, f_route[7] = {}, f_moe_plan = nullptr, f_moe_combine = {};
     hipFunction_t f_moe_small[6][2][2] = {};  // F16 Q8_0 Q4_K Q5_K Q6_K MXFP4 x gate and up, one product x f32, f16
     hipFunction_t f_moe_tile[6][2][2] = {}, f_moe_light[6][2][2] = {}, f_moe_prep[2] = {}, f_moe_vec[6][2][3] = {};
     float *moe_ws = nullptr;  // the experts' products' working memory, eager calls only
@@ -1006,7 +1007,7 @@ int moearc_sync(moearc_ctx *c) {
     if (hipStreamSynchronize(c->stream) != hipSuccess) return ERR;
     bool failed = c->deferred_error;
     c->deferred_error = false;
-    if (c->err_armed) {
+    if (c->err_armed || c->err_in_graph) {
         c->err_armed = false;
         uint32_t word = 0;
         if (hipMemcpyAsync(&word, c->err_word, 4, hipMemcpyDeviceToHost, c->stream) != hipSuccess ||

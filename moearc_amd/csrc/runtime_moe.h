@@ -4,7 +4,7 @@
 
 namespace {
 
-constexpr unsigned long kMoeChunkSlots = MOEARC_MOE_CHUNK_SLOTS;
+constexpr uint64_t kMaxThreads = 1ull << 31;  // of a launch, which may not have 2^32
 
 constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -18,9 +18,14 @@ uint64_t moe_max_tiles(uint64_t slots, uint64_t n_expert, uint64_t tile) {
     return std::min<uint64_t>(slots, (slots + tile - 1) / tile + n_expert + 1);
 }
 
+// Tokens that run at a time: what the plan's LDS holds, and rows no wider than a launch has threads for.
+uint64_t moe_chunk(uint64_t n_used, uint64_t widest) {
+    return std::max<uint64_t>(1, std::min<uint64_t>(MOEARC_MOE_CHUNK_SLOTS, kMaxThreads / 2 / std::max<uint64_t>(widest, 1)) / n_used);
+}
+
 // A call of n_tok tokens (one chunk of it) with n_used experts each: n_ff 0 for a product alone.
-MoeSpace moe_space(uint64_t n_tok, uint64_t n_used, uint64_t n_expert, uint64_t n_embd, uint64_t n_ff) {
-    const uint64_t tok = std::min<uint64_t>(n_tok, std::max<uint64_t>(1, kMoeChunkSlots / n_used)), slots = tok * n_used;
+MoeSpace moe_space(uint64_t n_tok, uint64_t n_used, uint64_t n_expert, uint64_t n_embd, uint64_t n_ff, uint64_t chunk) {
+    const uint64_t tok = std::min<uint64_t>(n_tok, chunk), slots = tok * n_used;
     MoeSpace s;
     s.tiles = 256;
     s.list = s.tiles + align256(sizeof(MoeTile) * moe_max_tiles(slots, n_expert, MOEARC_MOE_LIGHT));
@@ -44,6 +49,12 @@ int moe_take_space(moearc_ctx *c, size_t need, void *ws, uint8_t **out) {
     if (const int rc = ensure_floats(c, c->moe_ws, c->moe_ws_floats, (need + 3) / 4)) return rc;
     *out = (uint8_t *) c->moe_ws;
     return OK;
+}
+
+// The call's kernels may set the error word, and go on doing so when they were captured.
+void moe_arm(moearc_ctx *c, const void *ws) {
+    c->err_armed = true;
+    if (ws && capturing(c)) c->err_in_graph = true;
 }
 
 int moe_space_check(size_t need, const void *ws, unsigned long ws_bytes) {
@@ -90,7 +101,6 @@ int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slot
     a.n_slots = n_slots;
     a.n_expert = n_expert;
     a.err = c->err_word;
-    c->err_armed = true;
     if (n_slots <= MOEARC_MOE_SMALL_SLOTS) return OK;
     MoePlanArgs p{};
     p.ids = ids;
@@ -195,7 +205,6 @@ int moe_token(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, bool h
     d.accumulate = accumulate;
     const unsigned per_g = kMoeVecWaves * g.rpw, per_d = kMoeVecWaves * d.rpw;
     auto form = [](unsigned ppl) { return ppl == 1 ? 0 : ppl == 2 ? 1 : 2; };
-    c->err_armed = true;
     if (const int rc = launch2d(c, c->f_moe_vec[moe_index(m->w_type[0])][0][form(gp)], (g.rows + per_g - 1) / per_g, (unsigned) n_used,
                                 64 * kMoeVecWaves, g, nullptr, g.rows, n_used, gl, "moe_gate_up"))
         return rc;
@@ -204,19 +213,19 @@ int moe_token(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, bool h
 }
 
 // Brackets a call of several launches under one key, as a single launch would be.
-struct MoeScope {
+struct LaunchScope {
     moearc_ctx *c;
     const char *what;
     unsigned long r, m;
     hipEvent_t start = nullptr;
-    MoeScope(moearc_ctx *c, const char *what, unsigned long r, unsigned long m) : c(c), what(what), r(r), m(m) {
+    LaunchScope(moearc_ctx *c, const char *what, unsigned long r, unsigned long m) : c(c), what(what), r(r), m(m) {
         if (tracks(c, what) && (start = take_event(c)) && hipEventRecord(start, c->stream) != hipSuccess) {
             c->event_pool.push_back(start);
             start = nullptr;
         }
         ++c->scope_depth;
     }
-    ~MoeScope() {
+    ~LaunchScope() {
         --c->scope_depth;
         if (start) record_bracket(c, start, what, r, m);
     }
@@ -237,7 +246,7 @@ bool moe_load(moearc_ctx *c) {
         {&c->f_route[4], "moearc_moe_route_p16_k"},   {&c->f_route[5], "moearc_moe_route_p32_k"},
         {&c->f_route[6], "moearc_moe_route_p64_k"},   {&c->f_moe_plan, "moearc_moe_plan_k"},
         {&c->f_moe_prep[0], "moearc_moe_prep_f32_k"}, {&c->f_moe_prep[1], "moearc_moe_prep_f16_k"},
-        {&c->f_moe_combine[0], "moearc_moe_combine_k"}, {&c->f_moe_combine[1], "moearc_moe_combine4_k"},
+        {&c->f_moe_combine, "moearc_moe_combine_k"},
     };
     auto get = [&](hipFunction_t *slot, const char *name) {
         if (hipModuleGetFunction(slot, c->module, name) == hipSuccess) return true;
@@ -297,10 +306,20 @@ int moearc_norm_residual(moearc_ctx *c, void *x, unsigned int x_type, float *h, 
                      (uintptr_t) x % (a.x_f16 ? 8 : 16) == 0 && (uintptr_t) y % (a.y_f16 ? 8 : 16) == 0;
     const int i = n_cols <= 16 * MOEARC_NORM_PER_THREAD ? 0 : n_cols <= 64 * MOEARC_NORM_PER_THREAD ? 1
                 : n_cols <= 256 * MOEARC_NORM_PER_THREAD ? 2 : n_cols <= 1024 * MOEARC_NORM_PER_THREAD ? 3 : 4;
-    if (i == 4) return launch(c, c->f_norm_long, (unsigned) n_rows, 1024, a, "norm_residual", n_rows, n_cols);
-    const unsigned rows = i == 0 ? 16 : i == 1 ? 4 : 1;
-    return launch(c, c->f_norm[i][by4], (unsigned) ((n_rows + rows - 1) / rows), i == 3 ? 1024 : 256, a, "norm_residual", n_rows,
-                  n_cols);
+    const unsigned rows = i == 0 ? 16 : i == 1 ? 4 : 1, threads = i >= 3 ? 1024 : 256;
+    const hipFunction_t f = i == 4 ? c->f_norm_long : c->f_norm[i][by4];
+    const uint64_t most = kMaxThreads / threads * rows;  // rows of one launch
+    if (n_rows <= most) return launch(c, f, (unsigned) ((n_rows + rows - 1) / rows), threads, a, "norm_residual", n_rows, n_cols);
+    const LaunchScope scope(c, "norm_residual", n_rows, n_cols);
+    for (uint64_t r = 0; r < n_rows; r += most) {
+        a.n_rows = (uint32_t) std::min<uint64_t>(most, n_rows - r);
+        if (const int rc = launch(c, f, (unsigned) ((a.n_rows + rows - 1) / rows), threads, a, nullptr, n_rows, n_cols, "norm_residual")) return rc;
+        a.h += a.n_rows * n_cols;
+        if (a.x) a.x = (uint8_t *) a.x + a.n_rows * n_cols * (a.x_f16 ? 2 : 4);
+        if (a.y) a.y = (const uint8_t *) a.y + a.n_rows * n_cols * (a.y_f16 ? 2 : 4);
+        if (a.gate) a.gate += a.n_rows * gate_stride;
+    }
+    return OK;
 }
 
 int moearc_moe_route(moearc_ctx *c, unsigned int *ids, float *weights, const float *logits, unsigned long n_tok,
@@ -310,20 +329,30 @@ int moearc_moe_route(moearc_ctx *c, unsigned int *ids, float *weights, const flo
         mode > MOEARC_ROUTE_SOFTMAX_SELECTED)
         return ERR_ARG;
     if (n_tok == 0) return OK;
-    const RouteArgs a{logits, ids, weights, (uint32_t) n_tok, (uint32_t) n_expert, (uint32_t) n_used,
+    RouteArgs a{logits, ids, weights, (uint32_t) n_tok, (uint32_t) n_expert, (uint32_t) n_used,
                       mode == MOEARC_ROUTE_SOFTMAX_ALL ? 1u : 0u, scale, 0u};
     int i = 0;
     while (((unsigned long) MOEARC_ROUTE_LANES << i) < n_expert) ++i;
     // a wave of four tokens per work-group while those leave compute units idle, else four waves
     const unsigned threads = n_tok <= 4096 ? 64 : 256, per = threads / MOEARC_ROUTE_LANES;
-    return launch(c, c->f_route[i], (unsigned) ((n_tok + per - 1) / per), threads, a, "moe_route", n_tok, n_expert);
+    const uint64_t most = kMaxThreads / MOEARC_ROUTE_LANES;  // tokens of one launch
+    if (n_tok <= most) return launch(c, c->f_route[i], (unsigned) ((n_tok + per - 1) / per), threads, a, "moe_route", n_tok, n_expert);
+    const LaunchScope scope(c, "moe_route", n_tok, n_expert);
+    for (uint64_t t = 0; t < n_tok; t += most) {
+        a.n_tok = (uint32_t) std::min<uint64_t>(most, n_tok - t);
+        if (const int rc = launch(c, c->f_route[i], (a.n_tok + per - 1) / per, threads, a, nullptr, n_tok, n_expert, "moe_route")) return rc;
+        a.logits += (uint64_t) a.n_tok * n_expert;
+        a.ids += (uint64_t) a.n_tok * n_used;
+        a.weights += (uint64_t) a.n_tok * n_used;
+    }
+    return OK;
 }
 
 int moearc_moe_workspace(unsigned long n_tok, unsigned long n_used, unsigned long n_expert, unsigned long n_embd,
                          unsigned long n_ff, unsigned long *bytes) {
     if (!bytes) return ERR;
     if (moe_count_check(n_tok, n_used, n_expert, 0) || n_embd == 0 || n_embd > 0x100000ul || n_ff > 0x100000ul) return ERR_ARG;
-    *bytes = moe_space(n_tok, n_used, n_expert, n_embd, n_ff).bytes;
+    *bytes = moe_space(n_tok, n_used, n_expert, n_embd, n_ff, moe_chunk(n_used, std::max(n_embd, n_ff))).bytes;
     return OK;
 }
 
@@ -335,16 +364,18 @@ int moearc_matmul_experts(moearc_ctx *c, unsigned int type_id, void *y, const vo
     if (const int rc = moe_count_check(n_tok, n_used, n_expert, io_type)) return rc;
     if (const int rc = moe_matrix_check(type_id, w, n_rows, n_cols)) return rc;
     if (x_per_slot > 1) return ERR_ARG;
-    const MoeSpace sp = moe_space(n_tok, n_used, n_expert, n_cols, 0);
+    const unsigned long chunk = moe_chunk(n_used, n_cols);
+    const MoeSpace sp = moe_space(n_tok, n_used, n_expert, n_cols, 0, chunk);
     if (const int rc = moe_space_check(sp.bytes, ws, ws_bytes)) return rc;
     if (n_tok == 0) return OK;
     uint8_t *mem;
     if (const int rc = moe_take_space(c, sp.bytes, ws, &mem)) return rc;
-    const unsigned long chunk = std::max<unsigned long>(1, kMoeChunkSlots / n_used);
+    moe_arm(c, ws);
     const size_t elem = io_type == MOEARC_OUT_F16 ? 2 : 4;
-    const MoeScope scope(c, "matmul_experts", n_rows, n_tok * n_used);
-    for (unsigned long t = 0; t < n_tok; t += chunk) {
-        const unsigned long n = std::min(chunk, n_tok - t);
+    const LaunchScope scope(c, "matmul_experts", n_rows, n_tok * n_used);
+    const unsigned long step = std::min<unsigned long>(chunk, moe_chunk(n_used, n_rows));  // (the workspace does not know n_rows)
+    for (unsigned long t = 0; t < n_tok; t += step) {
+        const unsigned long n = std::min(step, n_tok - t);
         MoeArgs a{};
         if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) n_expert, io_type == MOEARC_OUT_F16, mem, sp))
             return rc;
@@ -376,15 +407,16 @@ int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, u
     for (int i = 0; i < 3; ++i)
         if (const int rc = moe_matrix_check(m->w_type[i], m->w[i], i < 2 ? m->n_ff : m->n_embd, i < 2 ? m->n_embd : m->n_ff))
             return rc;
-    const MoeSpace sp = moe_space(n_tok, n_used, m->n_expert, m->n_embd, m->n_ff);
+    const unsigned long chunk = moe_chunk(n_used, std::max(m->n_embd, m->n_ff));
+    const MoeSpace sp = moe_space(n_tok, n_used, m->n_expert, m->n_embd, m->n_ff, chunk);
     if (const int rc = moe_space_check(sp.bytes, ws, ws_bytes)) return rc;
     if (n_tok == 0) return OK;
     uint8_t *mem;
     if (const int rc = moe_take_space(c, sp.bytes, ws, &mem)) return rc;
-    const unsigned long chunk = std::max<unsigned long>(1, kMoeChunkSlots / n_used);
+    moe_arm(c, ws);
     const bool half = io_type == MOEARC_OUT_F16;
     const size_t elem = half ? 2 : 4;
-    const MoeScope scope(c, "moe_ffn", m->n_ff, n_tok * n_used);
+    const LaunchScope scope(c, "moe_ffn", m->n_ff, n_tok * n_used);
     if (n_tok == 1) {
         const int rc = moe_token(c, m, y, x, half, ids, weights, n_used, accumulate, mem + sp.act);
         if (rc != ERR_ARG) return rc;
@@ -433,10 +465,8 @@ int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, u
         s.cols = (uint32_t) m->n_embd;
         s.y_f16 = half;
         s.accumulate = accumulate;
-        const bool by4 = m->n_embd % 4 == 0;
-        const unsigned lanes = (unsigned) (by4 ? m->n_embd / 4 : m->n_embd);
-        if (const int rc = launch2d(c, c->f_moe_combine[by4], (lanes + 255) / 256, (unsigned) n, 256, s, nullptr, n, m->n_embd, 0,
-                                    "moe_combine"))
+        if (const int rc = launch2d(c, c->f_moe_combine, (unsigned) ((m->n_embd / 4 + 255) / 256), (unsigned) n, 256, s, nullptr, n,
+                                    m->n_embd, 0, "moe_combine"))
             return rc;
     }
     return OK;

@@ -145,7 +145,7 @@ def test_product_forms(cx, lib, each, ty, half, form):
     assert _kernels(lib) == ["plan", *prep, f"{form}_{name}_p_{io}"]
     lib.host_hip_reset()
     assert ffn(cx, {"w_type": [ty] * 3, "n_expert": 40}, io=half, n_tok=each * 40, n_used=1) == 0
-    assert _kernels(lib) == ["plan", *prep, f"{form}_{name}_gu_{io}", f"{form}_{name}_p_{io}", "combine4"]
+    assert _kernels(lib) == ["plan", *prep, f"{form}_{name}_gu_{io}", f"{form}_{name}_p_{io}", "combine"]
 
 
 def test_grids_cover_every_tile(cx, lib):
@@ -168,14 +168,14 @@ def test_few_slots_and_single_tokens(cx, lib):
     assert host_hip.launches(lib) == [("moearc_moe_small_q8_0_p_f32_k", 3, 64, 1, 512)]
     lib.host_hip_reset()
     assert ffn(cx, n_tok=16, n_used=4) == 0
-    assert _kernels(lib) == ["small_q8_0_gu_f32", "small_q8_0_p_f32", "combine4"]
+    assert _kernels(lib) == ["small_q8_0_gu_f32", "small_q8_0_p_f32", "combine"]
     for desc, kw, want in (
             ({}, {}, ["vec_q8_0_gu_p1", "vec_q8_0_down_p1"]),  # 256 and 512 columns: 16 and 32 pieces
             ({"n_ff": 2880, "n_embd": 2880, "w_type": [39, 39, 39]}, {}, ["vec_mxfp4_gu_p2", "vec_mxfp4_down_p2"]),
             ({"n_ff": 4096, "w_type": [8, 8, 12]}, dict(n_used=2), ["vec_q8_0_gu_p1", "vec_q4_k_down_p2"]),
             ({"n_ff": 2048, "n_embd": 2048, "w_type": [14, 14, 14]}, {}, ["vec_q6_k_gu_p2", "vec_q6_k_down_p2"]),
-            ({"n_ff": 4128}, {}, ["small_q8_0_gu_f32", "small_q8_0_p_f32", "combine4"]),  # 258 pieces
-            ({"n_ff": 4096}, dict(n_used=4), ["small_q8_0_gu_f32", "small_q8_0_p_f32", "combine4"])):  # inputs past the LDS
+            ({"n_ff": 4128}, {}, ["small_q8_0_gu_f32", "small_q8_0_p_f32", "combine"]),  # 258 pieces
+            ({"n_ff": 4096}, dict(n_used=4), ["small_q8_0_gu_f32", "small_q8_0_p_f32", "combine"])):  # inputs past the LDS
         lib.host_hip_reset()
         assert ffn(cx, desc, n_tok=1, **kw) == 0
         assert _kernels(lib) == want, (desc, kw)
@@ -186,8 +186,8 @@ def test_few_slots_and_single_tokens(cx, lib):
 
 def test_long_calls_run_in_chunks(cx, lib):
     assert ffn(cx, n_tok=8192 * 2 + 1, n_used=4) == 0
-    per = ["plan", "prep_f32", "tile_q8_0_gu_f32", "tile_q8_0_p_f32", "combine4"]
-    assert _kernels(lib)[:10] == per * 2 and _kernels(lib)[10:] == ["small_q8_0_gu_f32", "small_q8_0_p_f32", "combine4"]
+    per = ["plan", "prep_f32", "tile_q8_0_gu_f32", "tile_q8_0_p_f32", "combine"]
+    assert _kernels(lib)[:10] == per * 2 and _kernels(lib)[10:] == ["small_q8_0_gu_f32", "small_q8_0_p_f32", "combine"]
 
 
 def test_workspace_sizes(lib):
@@ -275,3 +275,25 @@ def test_constants_match_the_header():
     assert [value("MOEARC_ROUTE_SOFTMAX_ALL"), value("MOEARC_ROUTE_SOFTMAX_SELECTED")] == [int(m) for m in RouteMode]
     assert [value("MOEARC_ACT_SWIGLU"), value("MOEARC_ACT_SWIGLU_CLAMPED")] == [int(a) for a in MoeAct]
     assert (OUT_F32, OUT_F16) == (value("MOEARC_OUT_F32"), value("MOEARC_OUT_F16"))
+
+
+def test_launches_stay_below_the_thread_limit(cx, lib):
+    """A launch may not have 2^32 threads: longer calls are cut."""
+    def threads():
+        return [gx * gy * gz * block for _, gx, gy, gz, block in host_hip.launches(lib)]
+    for kw, want in ((dict(n_rows=(1 << 31) - 1, n_cols=1), 16), (dict(n_rows=(1 << 31) - 1, n_cols=2880), 256),
+                     (dict(n_rows=1 << 24, n_cols=16388), 8), (dict(n_rows=1 << 23, n_cols=2880), 1)):
+        lib.host_hip_reset()
+        assert norm(cx, **kw) == 0
+        assert len(names(lib)) == want and max(threads()) < 1 << 32
+    lib.host_hip_reset()
+    assert cx._lib.moearc_moe_route(cx.raw, 64, 64, 64, (1 << 31) - 1, 1024, 4, 1, 1.0) == 0
+    assert len(names(lib)) == 16 and max(threads()) < 1 << 32
+    for rows, cols in ((1 << 20, 256), (256, 1 << 20), (1 << 20, 1 << 20)):
+        for ty in (8, 12):
+            lib.host_hip_reset()
+            assert linear(cx, ty=ty, n_tok=10000, n_used=4, n_expert=1024, n_rows=rows, n_cols=cols, ws=256, ws_bytes=BIG) == 0
+            assert max(threads()) < 1 << 32
+    lib.host_hip_reset()
+    assert ffn(cx, {"n_embd": 1 << 20, "n_ff": 256}, n_tok=2000, ws=256, ws_bytes=BIG) == 0
+    assert max(threads()) < 1 << 32 and _kernels(lib).count("combine") == 8  # 1024 slots at a time
