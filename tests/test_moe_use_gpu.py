@@ -238,3 +238,60 @@ def test_padded_tokens_leave_the_others_alone(ctx):
         got = ctx.download(by, np.float32, (t, k, rows))
         want, tol = product(w, None, x[:t // 2], ids[:t // 2], False)
         assert np.all(np.abs(got[:t // 2] - want) <= tol) and not got[t // 2:].any()
+
+
+@pytest.mark.parametrize("ty", TYPES, ids=lambda t: t.name)
+@pytest.mark.parametrize("io", [OUT_F32, OUT_F16], ids=["f32", "f16"])
+def test_infinities_stay_in_their_token(ctx, ty, io):
+    """A live token of infinities and NaN changes no other token's result, not by a bit."""
+    e, k, embd, ff = 3, 2, 256, 256
+    made = [ctx.upload(weights(ty, e, r, c, 30 + i)[0]) for i, (r, c) in enumerate([(ff, embd), (ff, embd), (embd, ff)])]
+    desc = MoeDesc.make([ty] * 3, made, [None] * 3, e, embd, ff)
+    for t in (7, 40, 150):
+        rng = np.random.default_rng(t)
+        dtype = np.float16 if io == OUT_F16 else np.float32
+        x, ids = rng.standard_normal((t, embd)).astype(dtype), ids_of(rng, t, k, e)
+        bi, bt = ctx.upload(ids), ctx.upload(np.full((t, k), 0.5, np.float32))
+        out = []
+        for spoilt in (False, True):
+            if spoilt:
+                x[3], x[5, ::3] = np.inf, np.nan
+            by = ctx.alloc(t * embd * 4)
+            ctx.moe_ffn(desc, by, ctx.upload(x), bi, bt, t, k, io_type=io)
+            out.append(ctx.download(by, dtype, (t, embd)))
+        rest = [i for i in range(t) if i not in (3, 5)]
+        assert np.array_equal(out[0][rest], out[1][rest]) and np.isfinite(out[0]).all()
+        assert not np.isfinite(out[1][[3, 5]]).any()
+
+
+@pytest.mark.parametrize("io", [OUT_F32, OUT_F16], ids=["f32", "f16"])
+@pytest.mark.parametrize("t", [1, 9, 100])
+def test_tensors_at_any_element(ctx, io, t):
+    """Inputs, outputs, biases, ids and weights one element off the allocation's alignment: the same bits."""
+    e, k, embd, ff = 5, 3, 512, 256
+    elem = 2 if io == OUT_F16 else 4
+    dtype = np.float16 if io == OUT_F16 else np.float32
+    for types in ((QuantType.MXFP4, QuantType.Q8_0), (QuantType.F16, QuantType.Q6_K), (QuantType.Q5_K, QuantType.Q4_K)):
+        rng = np.random.default_rng(t)
+        made = [ctx.upload(weights(types[i > 1], e, r, c, 40 + i)[0]) for i, (r, c) in enumerate([(ff, embd), (ff, embd), (embd, ff)])]
+        data = [rng.standard_normal((t, embd)).astype(dtype), ids_of(rng, t, k, e), rng.random((t, k)).astype(np.float32),
+                *(rng.standard_normal((e, n)).astype(np.float32) for n in (ff, ff, embd))]
+        out = []
+        for off in (0, 1):
+            def place(a):
+                step = off * a.dtype.itemsize
+                return DeviceView(ctx.upload(np.concatenate([np.zeros(step, np.uint8), np.ascontiguousarray(a).view(np.uint8).reshape(-1)])), step)
+            bx, bi, bt, *bs = (place(a) for a in data)
+            desc = MoeDesc.make([types[0], types[0], types[1]], made, bs, e, embd, ff, MoeAct.SWIGLU_CLAMPED)
+            by = ctx.upload(np.full((t * embd + 2) * elem, 0x5A, np.uint8))
+            ctx.moe_ffn(desc, DeviceView(by, off * elem), bx, bi, bt, t, k, io_type=io)
+            raw = ctx.download(by, np.uint8, ((t * embd + 2) * elem,))
+            assert np.all(raw[:off * elem] == 0x5A) and np.all(raw[(t * embd + off) * elem:] == 0x5A)
+            out.append(raw[off * elem:(t * embd + off) * elem].copy().view(dtype))
+        assert np.array_equal(*out)
+
+
+def test_every_expert_of_1024(ctx):
+    for t, per_slot in ((1, False), (2, True)):
+        run_linear(ctx, QuantType.Q8_0, t, 1024, 1024, 33, 256, OUT_F16, per_slot=per_slot, seed=t)
+    run_ffn(ctx, (QuantType.MXFP4, QuantType.MXFP4), 2, 512, 512, 256, 256, add=True, seed=3)
