@@ -277,6 +277,13 @@ struct MoeTile {
     uint16_t count, pad;
     uint16_t index, of;
 };
+// x as moe_tile.hip's products take it: f16 hi (and lo, of f32), each k-block in the order of weights of `type`
+struct MoePrepArgs {
+    const void *x;
+    uint16_t *hi, *lo;
+    uint64_t n;                // elements, a multiple of 32
+    uint32_t type, pad;
+};
 struct MoePlanArgs {
     const uint32_t *ids;   // [n_slots]
     MoeTile *tiles;
@@ -284,6 +291,7 @@ struct MoePlanArgs {
     uint32_t *list;        // [n_slots]
     uint32_t *err;         // set to 1 when an id is neither an expert nor MOEARC_NO_EXPERT
     uint32_t n_slots, n_expert, tile, pad;
+    MoePrepArgs prep;          // for the kernels that do both
 };
 
 // One grouped product: rows of the experts' matrices times their slots' inputs. With two matrices (gate
@@ -324,14 +332,6 @@ struct MoeVecArgs {
     uint32_t x_lds_bytes, wave_buf;
     uint32_t x_f16, y_f16, accumulate, clamped;
     float alpha, limit;
-};
-
-// x as moe_tile.hip's products take it: f16 hi (and lo, of f32), each k-block in the order of weights of `type`
-struct MoePrepArgs {
-    const void *x;
-    uint16_t *hi, *lo;
-    uint64_t n;                // elements, a multiple of 32
-    uint32_t type, pad;
 };
 
 // y[t] (+)= sum_j weights[t][j] part[t * n_used + j] over the slots that have an expert, in order

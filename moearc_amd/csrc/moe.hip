@@ -127,13 +127,15 @@ ROUTE_KERNEL(16)
 ROUTE_KERNEL(32)
 ROUTE_KERNEL(64)
 
+namespace {
+
 // The plan (MoePlanArgs). One work-group per expert, and one for the slots without: each counts every
 // group's slots itself (integer adds in LDS, so the order of the adds does not matter), from which it knows
 // its group's first place and first tile, and then collects its own slots in order: each wave its share of the
 // slots, counted, then placed. No work-group waits for another, and the result does not depend on their order.
 // The ids are read once, all loads in flight, and kept in LDS (8000 slots: 9 us, and 13 when they were read twice,
 // with two barriers for every 1024).
-extern "C" __global__ void __launch_bounds__(1024) moearc_moe_plan_k(MoePlanArgs a) {
+__device__ __forceinline__ void moe_plan_body(const MoePlanArgs &a) {
     __shared__ uint16_t ids[MOEARC_MOE_CHUNK_SLOTS];
     __shared__ uint32_t count[MOEARC_MAX_EXPERTS + 1];
     __shared__ uint32_t wave_n[16], before[2];
@@ -185,6 +187,56 @@ extern "C" __global__ void __launch_bounds__(1024) moearc_moe_plan_k(MoePlanArgs
         if (hit) a.list[at + (uint32_t) __popcll(mask & ((1ull << lane) - 1ull))] = s0 + lane;
         at += (uint32_t) __popcll(mask);
     }
+}
+
+// x for moe_tile.hip: f16 (of f32: hi, and the remainder lo) in the order of the weights' type, eight elements,
+// one chunk, per thread.
+template <bool F32>
+__device__ __forceinline__ void moe_prep_body(const MoePrepArgs &a, uint32_t block, uint32_t blocks) {
+    for (uint64_t i = (uint64_t) block * 1024u + threadIdx.x; i < a.n / 8u; i += (uint64_t) blocks * 1024u) {
+        const uint32_t c = (uint32_t) i & 3u;
+        const uint64_t blk = (i >> 2) * 32u;
+        // the chunk's elements: two runs of four, from k0 and k1
+        const bool mx = a.type == 39u, kq = a.type == 12u || a.type == 13u || a.type == 14u;
+        const uint32_t k0 = mx ? 8u * (c & 1u) + 4u * (c >> 1) : 8u * c, k1 = mx ? k0 + 16u : k0 + 4u;
+        _Float16 vh[8], vl[8];
+        if constexpr (F32) {
+            float v[8];
+            __builtin_memcpy(v, (const float *) a.x + blk + k0, 16);
+            __builtin_memcpy(v + 4, (const float *) a.x + blk + k1, 16);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                vh[k] = (_Float16) v[k];
+                vl[k] = (_Float16) (v[k] - (float) vh[k]);
+            }
+        } else {
+            __builtin_memcpy(vh, (const _Float16 *) a.x + blk + k0, 8);
+            __builtin_memcpy(vh + 4, (const _Float16 *) a.x + blk + k1, 8);
+        }
+        half8_t hi, lo;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            const int q = (p & 4) | ((p & 1) << 1) | ((p >> 1) & 1), m = (p >> 1) | ((p & 1) << 2);
+            hi[p] = mx ? vh[m] : kq ? vh[q] : vh[p];
+            if constexpr (F32) lo[p] = mx ? vl[m] : kq ? vl[q] : vl[p];
+        }
+        *(half8_t *) (a.hi + 8u * i) = hi;
+        if constexpr (F32) *(half8_t *) (a.lo + 8u * i) = lo;
+    }
+}
+
+}  // namespace
+
+// The inputs' order does not depend on the plan, and both are short: one launch, the plan's work-groups first (8000
+// slots and 1000 f16 rows of 2048: 10.1 us, 14 as two).
+extern "C" __global__ void __launch_bounds__(1024) moearc_moe_plan_k(MoePlanArgs a) { moe_plan_body(a); }
+extern "C" __global__ void __launch_bounds__(1024) moearc_moe_plan_f32_k(MoePlanArgs a) {
+    if (blockIdx.x <= a.n_expert) moe_plan_body(a);
+    else moe_prep_body<true>(a.prep, blockIdx.x - a.n_expert - 1u, gridDim.x - a.n_expert - 1u);
+}
+extern "C" __global__ void __launch_bounds__(1024) moearc_moe_plan_f16_k(MoePlanArgs a) {
+    if (blockIdx.x <= a.n_expert) moe_plan_body(a);
+    else moe_prep_body<false>(a.prep, blockIdx.x - a.n_expert - 1u, gridDim.x - a.n_expert - 1u);
 }
 
 // The sum over a token's experts, four columns per thread (rows are whole blocks of 32): bound by reading the slots'

@@ -664,42 +664,6 @@ __device__ __forceinline__ void moe_tile_body(const MoeArgs &a) {
     moe_tile_half<TY, GU, HALVES, TS, RT, false>(a, xbuf, wbuf[wave], sums, e, slots, count, r0);
 }
 
-// x for the tiles: f16 (of f32: hi, and the remainder lo) in the order of the weights' type, eight elements,
-// one chunk, per thread.
-template <bool F32>
-__device__ __forceinline__ void moe_prep_body(const MoePrepArgs &a) {
-    for (uint64_t i = (uint64_t) blockIdx.x * 256u + threadIdx.x; i < a.n / 8u; i += (uint64_t) gridDim.x * 256u) {
-        const uint32_t c = (uint32_t) i & 3u;
-        const uint64_t blk = (i >> 2) * 32u;
-        // the chunk's elements: two runs of four, from k0 and k1
-        const bool mx = a.type == 39u, kq = a.type == 12u || a.type == 13u || a.type == 14u;
-        const uint32_t k0 = mx ? 8u * (c & 1u) + 4u * (c >> 1) : 8u * c, k1 = mx ? k0 + 16u : k0 + 4u;
-        _Float16 vh[8], vl[8];
-        if constexpr (F32) {
-            float v[8];
-            __builtin_memcpy(v, (const float *) a.x + blk + k0, 16);
-            __builtin_memcpy(v + 4, (const float *) a.x + blk + k1, 16);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                vh[k] = (_Float16) v[k];
-                vl[k] = (_Float16) (v[k] - (float) vh[k]);
-            }
-        } else {
-            __builtin_memcpy(vh, (const _Float16 *) a.x + blk + k0, 8);
-            __builtin_memcpy(vh + 4, (const _Float16 *) a.x + blk + k1, 8);
-        }
-        half8_t hi, lo;
-#pragma unroll
-        for (int p = 0; p < 8; ++p) {
-            const int q = (p & 4) | ((p & 1) << 1) | ((p >> 1) & 1), m = (p >> 1) | ((p & 1) << 2);
-            hi[p] = mx ? vh[m] : kq ? vh[q] : vh[p];
-            if constexpr (F32) lo[p] = mx ? vl[m] : kq ? vl[q] : vl[p];
-        }
-        *(half8_t *) (a.hi + 8u * i) = hi;
-        if constexpr (F32) *(half8_t *) (a.lo + 8u * i) = lo;
-    }
-}
-
 }  // namespace
 
 // Shapes, as moe_tile_rows (runtime_moe.h) has them. Wide tiles, 64 slots x 64 rows a wave and two waves per SIMD, decode
@@ -726,5 +690,3 @@ MOE_TILE(q4_k, 12, 2, 2, 2, 2, 3)
 MOE_TILE(q5_k, 13, 2, 2, 2, 2, 3)
 MOE_TILE(q6_k, 14, 1, 3, 1, 3, 3)
 MOE_TILE(mxfp4, 39, 2, 2, 1, 3, 4)
-extern "C" __global__ void __launch_bounds__(256) moearc_moe_prep_f32_k(MoePrepArgs a) { moe_prep_body<true>(a); }
-extern "C" __global__ void __launch_bounds__(256) moearc_moe_prep_f16_k(MoePrepArgs a) { moe_prep_body<false>(a); }

@@ -137,9 +137,9 @@ struct moearc_ctx {
     float *ws_kinds = nullptr;
     size_t ws_kinds_floats = 0;
     // norms (16, 64, 256, 1024 threads a row x scalar, four floats), router (16 << i experts), experts' products
-    hipFunction_t f_norm[4][2] = {}, f_norm_long = nullptr, f_route[7] = {}, f_moe_plan = nullptr, f_moe_combine = {};
+    hipFunction_t f_norm[4][2] = {}, f_norm_long = nullptr, f_route[7] = {}, f_moe_plan[3] = {}, f_moe_combine = {};
     hipFunction_t f_moe_small[6][2][2] = {};  // F16 Q8_0 Q4_K Q5_K Q6_K MXFP4 x gate and up, one product x f32, f16
-    hipFunction_t f_moe_tile[6][2][2] = {}, f_moe_light[6][2][2] = {}, f_moe_prep[2] = {}, f_moe_vec[6][2][3] = {};
+    hipFunction_t f_moe_tile[6][2][2] = {}, f_moe_light[6][2][2] = {}, f_moe_vec[6][2][3] = {};
     float *moe_ws = nullptr;  // the experts' products' working memory, eager calls only
     size_t moe_ws_floats = 0;
     int decode_variant_override = -1;  // MOEARC_DECODE_VARIANT, e.g. "4x2x4"

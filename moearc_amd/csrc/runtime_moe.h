@@ -97,8 +97,10 @@ uint32_t moe_tile_rows(unsigned ty, bool half, bool light, bool gate_up) {
 // Groups a chunk's slots by expert. Launches of at most 64 slots (a wave's lanes search them) need no plan: products
 // of 32 and 64 slots without one and on tiles, us: 64 Q4_K experts of 2048 x 1024 20, 26 and 26, 27; 8 Q8_0 ones of
 // 2048 x 2048 16, 17 and 32, 31; one Q5_K of 4096 x 2048 15, 26 and 34, 64; 128 MXFP4 of 2880 x 2880 61, 70 and 56, 57.
-int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slots, uint32_t n_expert, bool half, uint8_t *ws,
-             const MoeSpace &sp) {
+// x_n elements of x, for weights of type ty, are laid out for the matrix cores in the same launch; f16 ones of types
+// whose order is the natural one are taken as they are.
+int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slots, uint32_t n_expert, bool half, unsigned ty, size_t x_n,
+             uint8_t *ws, const MoeSpace &sp) {
     a.ids = ids;
     a.n_slots = n_slots;
     a.n_expert = n_expert;
@@ -116,22 +118,16 @@ int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slot
     a.tiles = p.tiles;
     a.n_tiles = p.n_tiles;
     a.list = p.list;
-    return launch(c, c->f_moe_plan, n_expert + 1, 1024, p, nullptr, n_slots, n_expert, "moe_plan");
-}
-
-// x for the tiles' matrix cores, as MoePrepArgs. f16 inputs of types whose order is the natural one are taken as
-// they are.
-int moe_prep(moearc_ctx *c, MoeArgs &a, unsigned ty, bool half, size_t n, uint8_t *space, size_t space_n) {
-    if (half && (ty == 1u || ty == 8u)) return OK;
-    MoePrepArgs p{};
-    p.x = a.x;
-    p.hi = (uint16_t *) space;
-    p.lo = p.hi + space_n;
-    p.n = n;
-    p.type = ty;
-    a.x = p.hi;
-    a.x_lo = p.lo;
-    return launch(c, c->f_moe_prep[half], (unsigned) std::min<size_t>((n / 8 + 255) / 256, 65536), 256, p, nullptr, n, 0, "moe_prep");
+    if (half && (ty == 1u || ty == 8u)) return launch(c, c->f_moe_plan[2], n_expert + 1, 1024, p, nullptr, n_slots, n_expert, "moe_plan");
+    p.prep.x = a.x;
+    p.prep.hi = (uint16_t *) (ws + sp.split);
+    p.prep.lo = p.prep.hi + sp.split_n;
+    p.prep.n = x_n;
+    p.prep.type = ty;
+    a.x = p.prep.hi;
+    a.x_lo = p.prep.lo;
+    const unsigned blocks = (unsigned) std::min<size_t>((x_n / 8 + 1023) / 1024, 16384);
+    return launch(c, c->f_moe_plan[half], n_expert + 1 + blocks, 1024, p, nullptr, n_slots, n_expert, "moe_plan");
 }
 
 // One grouped product (two matrices: gate, up and their activation). Without a plan x is as the caller's
@@ -246,8 +242,8 @@ bool moe_load(moearc_ctx *c) {
         {&c->f_route[0], "moearc_moe_route_p1_k"},    {&c->f_route[1], "moearc_moe_route_p2_k"},
         {&c->f_route[2], "moearc_moe_route_p4_k"},    {&c->f_route[3], "moearc_moe_route_p8_k"},
         {&c->f_route[4], "moearc_moe_route_p16_k"},   {&c->f_route[5], "moearc_moe_route_p32_k"},
-        {&c->f_route[6], "moearc_moe_route_p64_k"},   {&c->f_moe_plan, "moearc_moe_plan_k"},
-        {&c->f_moe_prep[0], "moearc_moe_prep_f32_k"}, {&c->f_moe_prep[1], "moearc_moe_prep_f16_k"},
+        {&c->f_route[6], "moearc_moe_route_p64_k"},   {&c->f_moe_plan[2], "moearc_moe_plan_k"},
+        {&c->f_moe_plan[0], "moearc_moe_plan_f32_k"}, {&c->f_moe_plan[1], "moearc_moe_plan_f16_k"},
         {&c->f_moe_combine, "moearc_moe_combine_k"},
     };
     auto get = [&](hipFunction_t *slot, const char *name) {
@@ -379,13 +375,12 @@ int moearc_matmul_experts(moearc_ctx *c, unsigned int type_id, void *y, const vo
     for (unsigned long t = 0; t < n_tok; t += step) {
         const unsigned long n = std::min(step, n_tok - t);
         MoeArgs a{};
-        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) n_expert, io_type == MOEARC_OUT_F16, mem, sp))
-            return rc;
         a.x = (const uint8_t *) x + (x_per_slot ? t * n_used : t) * n_cols * elem;
         a.x_div = x_per_slot ? 1u : (uint32_t) n_used;
         const bool half = io_type == MOEARC_OUT_F16;
-        if (a.tiles)
-            if (const int rc = moe_prep(c, a, type_id, half, (x_per_slot ? n * n_used : n) * n_cols, mem + sp.split, sp.split_n)) return rc;
+        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) n_expert, half, type_id,
+                                    (x_per_slot ? n * n_used : n) * n_cols, mem, sp))
+            return rc;
         a.w[0] = (const uint8_t *) w;
         a.bias[0] = bias;
         a.y = (uint8_t *) y + t * n_used * n_rows * elem;
@@ -426,17 +421,16 @@ int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, u
     for (unsigned long t = 0; t < n_tok; t += chunk) {
         const unsigned long n = std::min(chunk, n_tok - t);
         MoeArgs a{};
-        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) m->n_expert, half, mem, sp))
+        a.x = (const uint8_t *) x + t * m->n_embd * elem;
+        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) m->n_expert, half, m->w_type[0],
+                                    n * m->n_embd, mem, sp))
             return rc;
         MoeArgs g = a, d = a;
-        g.x = (const uint8_t *) x + t * m->n_embd * elem;
         g.x_div = (uint32_t) n_used;
         for (int i = 0; i < 2; ++i) {
             g.w[i] = (const uint8_t *) m->w[i];
             g.bias[i] = m->bias[i];
         }
-        if (a.tiles)
-            if (const int rc = moe_prep(c, g, m->w_type[0], half, n * m->n_embd, mem + sp.split, sp.split_n)) return rc;
         g.y_order = m->w_type[2];
         g.y = mem + sp.act;
         g.y_lo = (uint16_t *) (mem + sp.act) + sp.act_n;

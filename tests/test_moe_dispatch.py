@@ -141,11 +141,11 @@ def test_product_forms(cx, lib, each, ty, half, form):
     name = {8: "q8_0", 39: "mxfp4", 14: "q6_k", 12: "q4_k"}[ty]
     io = "f16" if half else "f32"
     assert linear(cx, ty=ty, io=half, n_tok=each * 40, n_used=1, n_expert=40) == 0
-    prep = [] if half and ty == 8 else [f"prep_{io}"]
-    assert _kernels(lib) == ["plan", *prep, f"{form}_{name}_p_{io}"]
+    plan = "plan" if half and ty == 8 else f"plan_{io}"  # f16 rows of Q8_0 products are taken as they are
+    assert _kernels(lib) == [plan, f"{form}_{name}_p_{io}"]
     lib.host_hip_reset()
     assert ffn(cx, {"w_type": [ty] * 3, "n_expert": 40}, io=half, n_tok=each * 40, n_used=1) == 0
-    assert _kernels(lib) == ["plan", *prep, f"{form}_{name}_gu_{io}", f"{form}_{name}_p_{io}", "combine"]
+    assert _kernels(lib) == [plan, f"{form}_{name}_gu_{io}", f"{form}_{name}_p_{io}", "combine"]
 
 
 def test_grids_cover_every_tile(cx, lib):
@@ -181,13 +181,13 @@ def test_few_slots_and_single_tokens(cx, lib):
         assert _kernels(lib) == want, (desc, kw)
     lib.host_hip_reset()
     assert ffn(cx, n_tok=1, n_used=65) == 0  # more than a wave's lanes
-    assert _kernels(lib)[0] == "plan"
+    assert _kernels(lib)[0] == "plan_f32"
 
 
 def test_long_calls_run_in_chunks(cx, lib):
     assert ffn(cx, n_tok=8192 * 2 + 1, n_used=4) == 0
-    per = ["plan", "prep_f32", "tile_q8_0_gu_f32", "tile_q8_0_p_f32", "combine"]
-    assert _kernels(lib)[:10] == per * 2 and _kernels(lib)[10:] == ["small_q8_0_gu_f32", "small_q8_0_p_f32", "combine"]
+    per = ["plan_f32", "tile_q8_0_gu_f32", "tile_q8_0_p_f32", "combine"]
+    assert _kernels(lib)[:8] == per * 2 and _kernels(lib)[8:] == ["small_q8_0_gu_f32", "small_q8_0_p_f32", "combine"]
 
 
 def test_workspace_sizes(lib):
