@@ -94,18 +94,26 @@ uint32_t moe_tile_rows(unsigned ty, bool half, bool light, bool gate_up) {
     return (wide ? 256u : 128u) / (gate_up ? 2u : 1u);
 }
 
-// Groups a chunk's slots by expert. Launches of at most 64 slots (a wave's lanes search them) need no plan: products
-// of 32 and 64 slots without one and on tiles, us: 64 Q4_K experts of 2048 x 1024 20, 26 and 26, 27; 8 Q8_0 ones of
-// 2048 x 2048 16, 17 and 32, 31; one Q5_K of 4096 x 2048 15, 26 and 34, 64; 128 MXFP4 of 2880 x 2880 61, 70 and 56, 57.
+// Whether a chunk runs without a plan (moe_small.hip): up to 64 slots, which a wave's lanes search, but for more than
+// 24 over 32 or more experts of MXFP4. Products of 32 and 64 slots without a plan and on tiles, us: 64 Q4_K experts of
+// 2048 x 1024 19, 26 and 23, 24; of Q8_0, 2048 x 2048, 31, 40 and 40, 41; eight 16, 17 and 29, 29; f16 ones of F16 33, 44
+// and 34, 44; one of Q5_K, 4096 x 2048, 15, 26 and 34, 64; but MXFP4, 2880 x 2880, 128 experts 59, 70 and 55, 55, 64
+// experts 50, 67 and 42, 54, 32 experts 39, 47 and 40, 40 (16 slots: 39, 34, 28 and 42, 39, 30), 16 experts 32, 35 and
+// 40, 40.
+bool moe_few(uint64_t n_slots, uint64_t n_expert, unsigned ty, unsigned ty2) {
+    return n_slots <= MOEARC_MOE_SMALL_SLOTS && !(ty == 39u && ty2 == 39u && n_slots > 24 && n_expert >= 32);
+}
+
+// Groups a chunk's slots by expert, for weights of type ty, and ty2 in the product after it.
 // x_n elements of x, for weights of type ty, are laid out for the matrix cores in the same launch; f16 ones of types
 // whose order is the natural one are taken as they are.
-int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slots, uint32_t n_expert, bool half, unsigned ty, size_t x_n,
-             uint8_t *ws, const MoeSpace &sp) {
+int moe_plan(moearc_ctx *c, MoeArgs &a, const unsigned int *ids, uint32_t n_slots, uint32_t n_expert, bool half, unsigned ty,
+             unsigned ty2, size_t x_n, uint8_t *ws, const MoeSpace &sp) {
     a.ids = ids;
     a.n_slots = n_slots;
     a.n_expert = n_expert;
     a.err = c->err_word;
-    if (n_slots <= MOEARC_MOE_SMALL_SLOTS) return OK;
+    if (moe_few(n_slots, n_expert, ty, ty2)) return OK;
     MoePlanArgs p{};
     p.ids = ids;
     p.n_tiles = (uint32_t *) ws;
@@ -378,7 +386,7 @@ int moearc_matmul_experts(moearc_ctx *c, unsigned int type_id, void *y, const vo
         a.x = (const uint8_t *) x + (x_per_slot ? t * n_used : t) * n_cols * elem;
         a.x_div = x_per_slot ? 1u : (uint32_t) n_used;
         const bool half = io_type == MOEARC_OUT_F16;
-        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) n_expert, half, type_id,
+        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) n_expert, half, type_id, type_id,
                                     (x_per_slot ? n * n_used : n) * n_cols, mem, sp))
             return rc;
         a.w[0] = (const uint8_t *) w;
@@ -422,7 +430,7 @@ int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, u
         const unsigned long n = std::min(chunk, n_tok - t);
         MoeArgs a{};
         a.x = (const uint8_t *) x + t * m->n_embd * elem;
-        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) m->n_expert, half, m->w_type[0],
+        if (const int rc = moe_plan(c, a, ids + t * n_used, (uint32_t) (n * n_used), (uint32_t) m->n_expert, half, m->w_type[0], m->w_type[2],
                                     n * m->n_embd, mem, sp))
             return rc;
         MoeArgs g = a, d = a;

@@ -184,6 +184,14 @@ def test_few_slots_and_single_tokens(cx, lib):
     assert _kernels(lib)[0] == "plan_f32"
 
 
+@pytest.mark.parametrize("tok,used,experts,types,few", [
+    (16, 4, 128, (8, 8), True), (16, 4, 31, (39, 39), True), (16, 4, 32, (39, 39), False), (6, 4, 128, (39, 39), True),
+    (7, 4, 128, (39, 39), False), (7, 4, 128, (39, 14), True), (17, 4, 8, (39, 39), False)], ids=str)
+def test_few_slots_need_no_plan(cx, lib, tok, used, experts, types, few):
+    assert ffn(cx, {"w_type": [types[0], types[0], types[1]], "n_expert": experts}, n_tok=tok, n_used=used) == 0
+    assert (_kernels(lib)[0] == "small_%s_gu_f32" % {8: "q8_0", 39: "mxfp4"}[types[0]]) == few
+
+
 def test_long_calls_run_in_chunks(cx, lib):
     assert ffn(cx, n_tok=8192 * 2 + 1, n_used=4) == 0
     per = ["plan_f32", "tile_q8_0_gu_f32", "tile_q8_0_p_f32", "combine"]

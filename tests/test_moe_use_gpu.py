@@ -213,7 +213,11 @@ def test_more_rows_than_a_launch_has_threads_for():
 @pytest.mark.parametrize("ty", TYPES, ids=lambda t: t.name)
 @pytest.mark.parametrize("io", [OUT_F32, OUT_F16], ids=["f32", "f16"])
 def test_both_sides_of_each_form(ctx, ty, io):
-    """64 and 65 slots (without and with a plan), and the slots per expert at which tiles grow."""
+    """64 and 65 slots, 24 and 25 over many experts (without and with a plan), and the slots per expert at which tiles
+    grow."""
+    for t in (24, 25):
+        run_linear(ctx, ty, t, 1, 40, 65, 512, io, seed=t)
+        run_ffn(ctx, (ty, ty), t, 1, 32, 256, 256, io, seed=t)
     for t in (64, 65):
         run_linear(ctx, ty, t, 1, 3, 65, 512, io, seed=t)
     for each in (39, 40, 55, 56):
