@@ -394,7 +394,8 @@ int moearc_matmul_experts(moearc_ctx *c, unsigned int type_id, void *y, const vo
                           void *ws, unsigned long ws_bytes);
 
 #define MOEARC_ACT_SWIGLU 0u         /* g sigmoid(g) u */
-#define MOEARC_ACT_SWIGLU_CLAMPED 1u /* g' sigmoid(alpha g') (u' + 1), g' = min(g, limit), u' = u within +-limit */
+#define MOEARC_ACT_SWIGLU_CLAMPED 1u /* g' sigmoid(alpha g') (u' + 1), g' = min(g, limit), u' = u within +-limit;
+                                        a NaN stays one */
 
 /* The experts of one block. */
 typedef struct moearc_moe {

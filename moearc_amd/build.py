@@ -30,8 +30,9 @@ LIBRARY = os.path.join(HERE, "libmoearc_attn.so")
 LAUNCH_OVERHEAD = os.path.join(HERE, "launch_overhead")
 
 # Packed-FP32 instructions stay disabled (v_pk_fma_f32 and friends are not emitted).
-# -fno-honor-nans: no kernel tests for NaN (the f16 codec classifies NaNs by their bits), and
-# without it every fmaxf is preceded by a NaN-quieting v_max x,x.
+# -fno-honor-nans: no kernel tests for NaN (the f16 codec and the router classify NaNs by their bits, and
+# the experts' clamps, which hand them on, are instructions of their own), and without it every fmaxf is
+# preceded by a NaN-quieting v_max x,x.
 # MFMA accumulators stay in VGPRs: with the AGPR form the compiler copies every accumulator to
 # VGPRs and back around each rescale branch of the prefill loop.
 HIPCC_FLAGS = [

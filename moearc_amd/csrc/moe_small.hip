@@ -28,12 +28,25 @@ struct MoeFmt {
     static constexpr bool SPLIT_LAST = TY == 8;
 };
 
+// min and max that hand a NaN on (fminf and fmaxf drop it, and a token whose gate is NaN would come out as the limit). As
+// instructions: the build leaves the compiler free to take a NaN for impossible.
+__device__ __forceinline__ float moe_min(float a, float b) {
+    float r;
+    asm("v_minimum3_f32 %0, %1, %2, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ float moe_max(float a, float b) {
+    float r;
+    asm("v_maximum3_f32 %0, %1, %2, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+
 template <typename Args>
 __device__ __forceinline__ float moe_activation(const Args &a, float g, float u) {
     // exp2 of a large positive argument is +inf and g / inf is 0: no branch needed
     if (a.clamped) {
-        g = fminf(g, a.limit);
-        u = fminf(fmaxf(u, -a.limit), a.limit);
+        g = moe_min(g, a.limit);
+        u = moe_min(moe_max(u, -a.limit), a.limit);
         return g / (1.f + expf(-a.alpha * g)) * (u + 1.f);
     }
     return g / (1.f + expf(-g)) * u;
