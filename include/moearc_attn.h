@@ -272,10 +272,11 @@ int moearc_attn_qkv(moearc_ctx *c, const unsigned int *type_ids, float *const *o
  * (+ bias[r]) for t < n_tok, r < n_rows; x f32 [n_tok][n_cols], y f32 [n_tok][n_rows] (y may overlap
  * x, which is then read before any of y is written). Weights
  * Q8_0 (8), F16 (1), Q4_K (12), Q5_K (13), Q6_K (14) or MXFP4 (39), W 2-byte aligned. x enters as an f16
- * hi + lo pair (to 2^-22 relative; each |x| must stay below 65504), quantised payloads as exact
- * f16 integers / E2M1 values, block scales (and K-quant mins, against f32 block sums of x) in f32:
- * results are within 2 (32 + n_cols/32 + 5) 2^-24 sum|w x| per element (the matvec bound plus the
- * matrix core's 32-wide block sums). MXFP4 exponents of 253 and above (where the reference's
+ * hi + lo pair (to 2^-22 relative, or 2^-25 absolute where that is more, for |x| below 2^-3; each |x| must
+ * stay below 65504), quantised payloads as exact f16 integers / E2M1 values, block scales (and K-quant
+ * mins, against f32 block sums of x) in f32: results are within 2 (32 + n_cols/32 + 5) 2^-24 sum|w x|
+ * + 2^-25 sum|w| per element (the matvec bound plus the matrix core's 32-wide block sums, and the halves'
+ * steps; |w| of Q4_K and Q5_K: |d s q| + |dmin m|). MXFP4 exponents of 253 and above (where the reference's
  * per-element products overflow) are not reproduced. Refusals: null c/y/w/x -> -1; another type,
  * n_cols not a multiple of 32 or of the block, an odd W address, n_rows, n_tok >= 2^31 -> -2.
  * n_rows or n_tok zero -> 0. */
@@ -378,8 +379,9 @@ int moearc_moe_workspace(unsigned long n_tok, unsigned long n_used, unsigned lon
  * another, [n_expert][n_rows][n_cols]; bias f32 [n_expert][n_rows] or NULL; ids u32 [n_tok][n_used] (device;
  * experts may repeat within a token); x and y f32 or f16 by io_type, y [n_tok][n_used][n_rows]. y must not
  * overlap x. Slots of one expert share what is read of its weights, up to 64 at a time.
- * f32 activations enter as f16 hi + lo (to 2^-22 relative; each |x| below 65504), block sums are scaled in
- * f32: the bound of moearc_matmul_q; f16 ones as they are, and y is rounded once. The result of a slot does not
+ * f32 activations enter as f16 hi + lo, block sums are scaled in f32: the bound of moearc_matmul_q, 2^-25 sum|w| for
+ * small activations within it (an x of 1e-6 is left about 5 bits); each |x| below 65504, and from 65520 on the slot's results are
+ * NaN. f16 ones enter as they are, and y is rounded once. The result of a slot does not
  * change from call to call with the same arguments.
  * A slot of MOEARC_NO_EXPERT gets a row of zeros; another id >= n_expert too, and the next moearc_sync returns -1
  * (after any replay too, when the call was captured).
@@ -411,7 +413,9 @@ typedef struct moearc_moe {
  * e = ids[t][j], in the order of j; accumulate: y[t] += it (the residual stream; f32 only). x and y
  * [n_tok][n_embd], f32 or f16 by io_type, and must not overlap; ids and weights as moearc_moe_route writes them;
  * all device memory except m. Precision as moearc_matmul_experts, twice in a row: with f32 the values between the two
- * products stay f32 (as f16 hi + lo: each |act| below 65504), with f16 they are rounded to f16 once. Slots without an
+ * products are hi + lo as well, each to 2^-22 relative or 2^-25 absolute, and below 65504 (a single token's f32 values,
+ * x and these, may be multiplied as they are: it then has no such limits); with f16 they are rounded to f16 once, to
+ * infinity from 65520 on, which halves the second product's work. Slots without an
  * expert add nothing, and their weights are not read; ids out of range and ws as there. Calls of more than
  * 32768 slots (fewer when rows are wider than 32768) run in chunks of tokens, one after another.
  * Refusals: a null pointer other than biases and ws -> -1; those of moearc_matmul_experts for each matrix, gate and

@@ -225,7 +225,7 @@ struct MatmulSeg {
 };
 struct MatmulArgs {
     MatmulSeg seg[MOEARC_MM_MAX_SEG];
-    const uint16_t *xh, *xl;   // [n_tok][cols] f16: x = hi + lo to within 2^-22 |x|
+    const uint16_t *xh, *xl;   // [n_tok][cols] f16: x = hi + lo to within 2^-22 |x| or 2^-25
     const float *xs;           // Q4_K, Q5_K: block sums of x, f32 [n_tok][cols / 32] (matmul.hip) or f16
                                // pieces [n_tok][cols / 256][4][8] (matmul2k.hip); matmul_small.hip: x
                                // itself, f32 [n_tok][cols]; else unread

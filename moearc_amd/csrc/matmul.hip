@@ -3,7 +3,7 @@
 // (moe.rs:1942-1959, 2063-2071; kernels.cpp:1046-1111), W in Q8_0 or F16.
 //
 // Precision matches the matvec path, not f16 arithmetic: X is split into f16 hi + lo
-// (x - hi - lo <= 2^-22 |x|), the Q8_0 payload enters the MFMA as exact f16 integers, each
+// (x - hi - lo <= 2^-22 |x| or 2^-25), the Q8_0 payload enters the MFMA as exact f16 integers, each
 // 32-wide block's f32 sum q . (hi + lo) comes from two chained v_mfma_f32_16x16x32_f16 and is
 // scaled by the block's d in f32. F16 weights enter as they are. Activations must stay below
 // 65504 in magnitude (the f16 range of the hi part).

@@ -2,7 +2,7 @@
 // Q5_K: matmul2k.hip): Y[t][r] = sum_c W[r][c] X[t][c] (+ bias[r]) for the tokens of a prompt chunk -- the GEMM
 // that the reference's prefill performs as one matvec per token (moe.rs:1942-1959, 2063-2071;
 // kernels.cpp:1046-1111). Precision is matmul.hip's: X is split into f16 hi + lo on the host side of
-// the launch (x - hi - lo <= 2^-22 |x|), a block's payload enters the MFMA as exact f16 integers
+// the launch (x - hi - lo <= 2^-22 |x| or 2^-25), a block's payload enters the MFMA as exact f16 integers
 // (E2M1 code points for MXFP4), each 32-wide block's (Q6_K: 16-wide group's) f32 sum q . (hi + lo)
 // is scaled by the block's factor in f32; F16 weights enter as they are. Activations must stay below 65504.
 //

@@ -12,7 +12,7 @@
 // activations through the L2, which is why this form ends where the larger tiles begin (the host's
 // rule).
 //
-// Precision is matmul.hip's: x = hi + lo to 2^-22, payloads as exact f16 integers (E2M1 code points
+// Precision is matmul.hip's: x = hi + lo to 2^-22 |x| or 2^-25, payloads as exact f16 integers (E2M1 code points
 // for MXFP4), each block's f32 sum scaled in f32. The K-quants' mins multiply the block's f32 sum of x.
 #include "common.h"
 

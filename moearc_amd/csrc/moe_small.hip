@@ -11,7 +11,7 @@
 // decode step a launch. Grid y is the slot; the work-groups of slots that are not their expert's first
 // leave at once. Measured: 8 tokens of 4 of 64 Q5_K experts, 2048 x 2048 (75 MB) 23.6 us, 3.2 TB/s.
 //
-// f32 activations enter as f16 hi + lo (x = hi + lo to 2^-22 |x|), f16 ones as they are; weight payloads
+// f32 activations enter as f16 hi + lo (x = hi + lo to 2^-22 |x| or 2^-25), f16 ones as they are; weight payloads
 // as exact f16 integers (E2M1 code points for MXFP4), each block's f32 sum scaled in f32.
 #include "common.h"
 

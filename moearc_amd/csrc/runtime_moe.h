@@ -443,6 +443,8 @@ int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, u
         g.y = mem + sp.act;
         g.y_lo = (uint16_t *) (mem + sp.act) + sp.act_n;
         d.x_lo = g.y_lo;
+        // f16 calls round the activations once: hi + lo would double the down product's MFMAs and its reads of them, to
+        // undo a rounding of the size that x came with
         g.y_f16 = half;
         g.rows = (uint32_t) m->n_ff;
         g.cols = (uint32_t) m->n_embd;
