@@ -417,9 +417,10 @@ typedef struct moearc_moe {
  * x and these, may be multiplied as they are: it then has no such limits); with f16 they are rounded to f16 once, to
  * infinity from 65520 on, which halves the second product's work. Slots without an
  * expert add nothing, and their weights are not read; ids out of range and ws as there. Calls of more than
- * 32768 slots (fewer when rows are wider than 32768) run in chunks of tokens, one after another.
+ * 32768 slots (fewer when n_embd is above 32768 or n_ff above 16384) run in chunks of tokens, one after another.
  * Refusals: a null pointer other than biases and ws -> -1; those of moearc_matmul_experts for each matrix, gate and
- * up of different types, another act, a negative or NaN limit, accumulate not 0/1 or with f16 -> -2. No tokens -> 0. */
+ * up of different types, another act, a negative or NaN limit, accumulate not 0/1 or with f16, n_used of 1024 with
+ * n_ff above 2^20 - 64 (more than a launch's threads) -> -2. No tokens -> 0. */
 int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, unsigned int io_type,
                    const unsigned int *ids, const float *weights, unsigned long n_tok, unsigned long n_used,
                    unsigned int accumulate, void *ws, unsigned long ws_bytes);

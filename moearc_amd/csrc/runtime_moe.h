@@ -18,10 +18,16 @@ uint64_t moe_max_tiles(uint64_t slots, uint64_t n_expert, uint64_t tile) {
     return std::min<uint64_t>(slots, (slots + tile - 1) / tile + n_expert + 1);
 }
 
-// Tokens that run at a time: what the plan's LDS holds, and rows no wider than a launch has threads for.
+// Tokens that run at a time: what the plan's LDS holds, and rows no wider than a launch has threads for (up to two a row in
+// moe_tile.hip; `widest` counts rows of gate and up twice, of which a tile has half as many).
 uint64_t moe_chunk(uint64_t n_used, uint64_t widest) {
     return std::max<uint64_t>(1, std::min<uint64_t>(MOEARC_MOE_CHUNK_SLOTS, kMaxThreads / 2 / std::max<uint64_t>(widest, 1)) / n_used);
 }
+
+uint64_t moe_ffn_chunk(uint64_t n_used, uint64_t n_embd, uint64_t n_ff) { return moe_chunk(n_used, std::max(n_embd, 2 * n_ff)); }
+
+// Whether gate and up of one token's slots, a tile each, fit a launch: all sizes but 1024 slots of the widest rows.
+bool moe_ffn_fits(uint64_t n_used, uint64_t n_ff) { return n_used * ((n_ff + 63) / 64) * 256 < 2 * kMaxThreads; }
 
 // A call of n_tok tokens (one chunk of it) with n_used experts each: n_ff 0 for a product alone.
 MoeSpace moe_space(uint64_t n_tok, uint64_t n_used, uint64_t n_expert, uint64_t n_embd, uint64_t n_ff, uint64_t chunk) {
@@ -357,8 +363,10 @@ int moearc_moe_route(moearc_ctx *c, unsigned int *ids, float *weights, const flo
 int moearc_moe_workspace(unsigned long n_tok, unsigned long n_used, unsigned long n_expert, unsigned long n_embd,
                          unsigned long n_ff, unsigned long *bytes) {
     if (!bytes) return ERR;
-    if (moe_count_check(n_tok, n_used, n_expert, 0) || n_embd == 0 || n_embd > 0x100000ul || n_ff > 0x100000ul) return ERR_ARG;
-    *bytes = moe_space(n_tok, n_used, n_expert, n_embd, n_ff, moe_chunk(n_used, std::max(n_embd, n_ff))).bytes;
+    if (moe_count_check(n_tok, n_used, n_expert, 0) || n_embd == 0 || n_embd > 0x100000ul || n_ff > 0x100000ul ||
+        !moe_ffn_fits(n_used, n_ff))
+        return ERR_ARG;
+    *bytes = moe_space(n_tok, n_used, n_expert, n_embd, n_ff, moe_ffn_chunk(n_used, n_embd, n_ff)).bytes;
     return OK;
 }
 
@@ -407,12 +415,13 @@ int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, u
     if (!c || !m || !y || !x || !ids || !weights || !m->w[0] || !m->w[1] || !m->w[2]) return ERR;
     if (const int rc = moe_count_check(n_tok, n_used, m->n_expert, io_type)) return rc;
     if (m->w_type[0] != m->w_type[1] || m->act > MOEARC_ACT_SWIGLU_CLAMPED || accumulate > 1 ||
-        (accumulate && io_type != MOEARC_OUT_F32) || (m->act == MOEARC_ACT_SWIGLU_CLAMPED && !(m->limit >= 0.f)))
+        (accumulate && io_type != MOEARC_OUT_F32) || (m->act == MOEARC_ACT_SWIGLU_CLAMPED && !(m->limit >= 0.f)) ||
+        !moe_ffn_fits(n_used, m->n_ff))
         return ERR_ARG;
     for (int i = 0; i < 3; ++i)
         if (const int rc = moe_matrix_check(m->w_type[i], m->w[i], i < 2 ? m->n_ff : m->n_embd, i < 2 ? m->n_embd : m->n_ff))
             return rc;
-    const unsigned long chunk = moe_chunk(n_used, std::max(m->n_embd, m->n_ff));
+    const unsigned long chunk = moe_ffn_chunk(n_used, m->n_embd, m->n_ff);
     const MoeSpace sp = moe_space(n_tok, n_used, m->n_expert, m->n_embd, m->n_ff, chunk);
     if (const int rc = moe_space_check(sp.bytes, ws, ws_bytes)) return rc;
     if (n_tok == 0) return OK;
