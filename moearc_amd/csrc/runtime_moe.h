@@ -75,9 +75,10 @@ int moe_index(unsigned ty) {
     return -1;
 }
 
+bool moe_cols_ok(unsigned long n_cols) { return n_cols >= 256 && n_cols % 32 == 0 && n_cols <= 0x100000ul; }
+
 int moe_matrix_check(unsigned ty, const void *w, unsigned long n_rows, unsigned long n_cols) {
-    if (moe_index(ty) < 0 || n_cols < 256 || n_cols % 32 != 0 || n_cols % moearc_mv_be(ty) != 0 || n_cols > 0x100000ul ||
-        n_rows == 0 || n_rows > 0x100000ul || ((uintptr_t) w & 1u))
+    if (moe_index(ty) < 0 || !moe_cols_ok(n_cols) || n_cols % moearc_mv_be(ty) != 0 || n_rows == 0 || n_rows > 0x100000ul || ((uintptr_t) w & 1u))
         return ERR_ARG;
     return OK;
 }
@@ -363,7 +364,7 @@ int moearc_moe_route(moearc_ctx *c, unsigned int *ids, float *weights, const flo
 int moearc_moe_workspace(unsigned long n_tok, unsigned long n_used, unsigned long n_expert, unsigned long n_embd,
                          unsigned long n_ff, unsigned long *bytes) {
     if (!bytes) return ERR;
-    if (moe_count_check(n_tok, n_used, n_expert, 0) || n_embd == 0 || n_embd > 0x100000ul || n_ff > 0x100000ul ||
+    if (moe_count_check(n_tok, n_used, n_expert, 0) || !moe_cols_ok(n_embd) || (n_ff && !moe_cols_ok(n_ff)) ||
         !moe_ffn_fits(n_used, n_ff))
         return ERR_ARG;
     *bytes = moe_space(n_tok, n_used, n_expert, n_embd, n_ff, moe_ffn_chunk(n_used, n_embd, n_ff)).bytes;

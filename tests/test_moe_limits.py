@@ -45,3 +45,15 @@ def test_the_stated_workspace_is_enough(cx, lib, ff):  # noqa: F811
         for less, rc in ((0, 0), (1, -2)):
             assert ffn(cx, {"n_ff": ff}, n_tok=tok, ws=256, ws_bytes=n.value - less) == rc
     assert linear(cx, n_tok=100, ws=256, ws_bytes=BIG) == 0
+
+
+def test_the_workspace_refuses_what_the_calls_refuse(cx, lib):  # noqa: F811
+    n = ctypes.c_ulong()
+    for embd, ff in ((224, 512), (256, 224), (256, 32), (272, 512), (256, 272), (100, 0), (255, 0), (1, 1), ((1 << 20) + 32, 256), (256, (1 << 20) + 32)):
+        for tok in (0, 5):
+            n.value = 7
+            assert cx._lib.moearc_moe_workspace(tok, 4, 8, embd, ff, ctypes.byref(n)) == -2 and n.value == 7
+            call = ffn(cx, {"n_embd": embd, "n_ff": ff}, n_tok=tok) if ff else linear(cx, n_cols=embd, n_tok=tok)
+            assert call == -2
+    for embd, ff in ((256, 0), (288, 0), (256, 288), (1 << 20, 256)):
+        assert cx._lib.moearc_moe_workspace(5, 4, 8, embd, ff, ctypes.byref(n)) == 0
