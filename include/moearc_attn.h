@@ -384,7 +384,7 @@ int moearc_moe_workspace(unsigned long n_tok, unsigned long n_used, unsigned lon
  * NaN. f16 ones enter as they are, and y is rounded once. The result of a slot does not
  * change from call to call with the same arguments.
  * A slot of MOEARC_NO_EXPERT gets a row of zeros; another id >= n_expert too, and the next moearc_sync returns -1
- * (after any replay too, when the call was captured).
+ * (after any replay too, when the call was captured: every moearc_sync of that context then reads a word back, 20 us).
  * ws: ws_bytes of 256-byte aligned device memory (moearc_moe_workspace), used until the call's work is done; NULL:
  * the context's, grown on demand. A captured call needs ws (else -1), and graphs that may run at the same time
  * need one each. Refusals: a null pointer other than bias and ws -> -1; io_type or x_per_slot not 0/1, n_expert or

@@ -15,7 +15,9 @@
 // Scales cost a vector instruction per accumulator and k-block beside 32 cycles of MFMA, so where the
 // formats allow they are part of the operand, exactly, and the accumulators run through:
 // - MXFP4: 2^(e - 127) scales the E2M1 code in the conversion, exact while every product is a normal f16,
-//   which is checked per window (e from 114 to 139); other windows scale each block's f32 sum.
+//   which is checked per window (e from 114 to 139). A work-group that finds another e, a zero block's e = 0 too, runs
+//   its reduction again and scales each block's f32 sum: 2000 tokens of 32 experts 906 us, and 1827 with one zero block
+//   in 4000, which leaves hardly a work-group without.
 // - Q4_K, Q5_K: 6-bit scale times 4- or 5-bit weight is an integer below 2048. The super-block's f16 factor
 //   d stays out: the accumulators hold the sum over d, and are multiplied by d_before / d_now between two
 //   super-blocks (two roundings in 256 elements). The mins are two MFMAs per super-block on the sums of x over

@@ -6,8 +6,9 @@
 // + 64, ... of every row and holds the inputs of its pieces in registers; rows come through LDS, two in flight per
 // wave. A wave's units here are gate and up of one row in turn, whose results meet in it, or the rows of one
 // expert after the other, summed in the order of j: no wave waits for another, and nothing is added in memory.
-// Measured: four MXFP4 experts of 2880 x 2880 (53 MB) in 13.6 and 13.4 us, against 44 for both as products of
-// moe_small.hip with their sum in a launch of its own.
+// Measured: four MXFP4 experts of 2880 x 2880 in 14.0 us (gate and up, 35 MB) and 13.2 (down, 18 MB: one row a wave, and
+// every work-group stages the four inputs), against 44 for both as products of moe_small.hip with their sum in a launch
+// of its own.
 #include "common.h"
 
 extern __shared__ __attribute__((aligned(16))) uint8_t mvx_smem[];

@@ -115,7 +115,7 @@ struct moearc_ctx {
     // entry point that returns nothing (moearc_free_device).
     uint32_t *err_word = nullptr;
     bool err_armed = false;
-    bool err_in_graph = false;  // a captured call may set it with any replay: every moearc_sync looks
+    bool err_in_graph = false;  // a captured call may set it with any replay: every moearc_sync looks (20 us, 0.2 without)
     bool deferred_error = false;
     // The code object's fixed record array (moearc_decode_scratch): its device address in this
     // context's module instance, read once at creation, and its size in floats.

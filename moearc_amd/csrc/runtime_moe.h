@@ -93,6 +93,7 @@ int moe_count_check(unsigned long n_tok, unsigned long n_used, unsigned long n_e
 // Whether a chunk runs on tiles of 32 slots, not 64: up to 56 slots an expert, 40 with f16 inputs. (Products of 64
 // slots an expert, 64 and 32 slots a tile: MXFP4 142 and 121 us, Q8_0 88 and 82, Q4_K 84 and 86, Q5_K 97 and 100, f16
 // Q4_K 155 and 166, Q6_K 149 and 157; of 32: MXFP4 87 and 82, Q4_K 69 and 58, Q5_K 80 and 67, f16 Q4_K 111 and 109.)
+// One threshold for all types: f32 MXFP4's and Q8_0's lie above it, where was not measured.
 bool moe_light(uint64_t n_slots, uint64_t n_expert, bool half) { return n_slots < (half ? 40 : 56) * n_expert; }
 
 // Rows of each matrix that a tile's work-group takes: moe_tile.hip's shapes.
