@@ -55,6 +55,40 @@ pub struct MoearcMoe {
     pub limit: c_float,
 }
 
+/// `moearc_qkv_append` (include/moearc_attn.h): one layer's rows of a ragged batch, its cache and RoPE.
+#[repr(C)]
+pub struct MoearcQkvAppend {
+    pub q: *const c_void,
+    pub k: *const c_void,
+    pub v: *const c_void,
+    pub in_type: c_uint,
+    pub q_stride: c_ulong,
+    pub k_stride: c_ulong,
+    pub v_stride: c_ulong,
+    pub q_norm: *const c_float,
+    pub k_norm: *const c_float,
+    pub eps: c_float,
+    pub q_out: *mut c_void,
+    pub q_type: c_uint,
+    pub k_pages: *mut c_void,
+    pub v_pages: *mut c_void,
+    pub kv_type: c_uint,
+    pub n_pages: c_ulong,
+    pub page_tokens: c_ulong,
+    pub n_heads: c_ulong,
+    pub n_kv_heads: c_ulong,
+    pub head_dim: c_ulong,
+    pub n_rot: c_ulong,
+    pub neox: c_uint,
+    pub freq_base: c_float,
+    pub freq_scale: c_float,
+    pub ext_factor: c_float,
+    pub attn_factor: c_float,
+    pub corr_lo: c_float,
+    pub corr_hi: c_float,
+    pub freq_factors: *const c_float,
+}
+
 pub const MOEARC_OUT_F32: c_uint = 0;
 pub const MOEARC_OUT_F16: c_uint = 1;
 pub const MOEARC_ROUTE_SOFTMAX_ALL: c_uint = 0;
@@ -389,6 +423,52 @@ unsafe extern "C" {
         n_tok: c_ulong,
         n_used: c_ulong,
         accumulate: c_uint,
+        ws: *mut c_void,
+        ws_bytes: c_ulong,
+    ) -> c_int;
+    pub fn moearc_rope_qkv_append_batched(
+        c: *mut MoearcCtx,
+        d: *const MoearcQkvAppend,
+        block_tables: *const c_uint,
+        bt_stride: c_ulong,
+        row_begin: *const c_uint,
+        n_kv: *const c_uint,
+        n_seqs: c_ulong,
+    ) -> c_int;
+    #[allow(clippy::too_many_arguments)]
+    pub fn moearc_attn_prefill_batched_workspace(
+        c: *mut MoearcCtx,
+        row_begin: *const c_uint,
+        n_kv: *const c_uint,
+        n_seqs: c_ulong,
+        n_swa: c_ulong,
+        n_heads: c_ulong,
+        n_kv_heads: c_ulong,
+        head_dim: c_ulong,
+        bytes: *mut c_ulong,
+    ) -> c_int;
+    #[allow(clippy::too_many_arguments)]
+    pub fn moearc_attn_prefill_batched(
+        c: *mut MoearcCtx,
+        out: *mut c_void,
+        out_type: c_uint,
+        q: *const c_void,
+        k_pages: *const c_void,
+        v_pages: *const c_void,
+        n_pages: c_ulong,
+        block_tables: *const c_uint,
+        bt_stride: c_ulong,
+        row_begin: *const c_uint,
+        n_kv: *const c_uint,
+        sinks: *const c_float,
+        n_seqs: c_ulong,
+        n_swa: c_ulong,
+        n_heads: c_ulong,
+        n_kv_heads: c_ulong,
+        head_dim: c_ulong,
+        page_tokens: c_ulong,
+        scale: c_float,
+        kv_type: c_uint,
         ws: *mut c_void,
         ws_bytes: c_ulong,
     ) -> c_int;

@@ -425,6 +425,80 @@ int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, u
                    const unsigned int *ids, const float *weights, unsigned long n_tok, unsigned long n_used,
                    unsigned int accumulate, void *ws, unsigned long ws_bytes);
 
+/* ---- ragged batches ------------------------------------------------------------------------------
+ * Extensions (the reference runs one token of one sequence at a time): the new tokens of many sequences --
+ * a decode step's one, a draft's few, a prompt chunk's many -- in one append and one attention call. Both take
+ * the batch alike: rows row_begin[b] .. row_begin[b + 1] - 1 of q and out are sequence b's n new tokens
+ * (none is allowed), row_begin HOST u32 [n_seqs + 1], ascending; n_kv HOST u32 [n_seqs] its keys with these among
+ * them, below 2^31, so that new token i sits at position n_kv[b] - n + i; block_tables (device) row b at
+ * block_tables + b * bt_stride, ids below n_pages, the pages of each pool. Rows before row_begin[0] and from
+ * row_begin[n_seqs] on are left as they are; at most 2^20 rows. A captured call keeps the lengths that it was
+ * given. A block-table entry >= n_pages is never used as an address, and the next moearc_sync returns -1 (after any
+ * replay too, when the call was captured: every moearc_sync of that context then reads a word back, 20 us).
+ * A windowed layer's ring table serves as a block table. */
+
+/* One layer's rows on their way to the attention. */
+typedef struct moearc_qkv_append {
+    const void *q, *k, *v;        /* row t at q + t * q_stride elements, [n_heads][head_dim]; k, v [n_kv_heads][head_dim].
+                                     One product's rows: the three pointers into it, its row length as each stride */
+    unsigned int in_type;         /* of q, k and v: MOEARC_OUT_F32 / _F16 */
+    unsigned long q_stride, k_stride, v_stride;  /* elements, at least a row's, below 2^40 */
+    const float *q_norm, *k_norm; /* [head_dim]: each head is normed, x / sqrt(mean(x^2) + eps) * w, first; NULL: not */
+    float eps;
+    void *q_out;                  /* [row][n_heads][head_dim]; q itself where rows and type agree */
+    unsigned int q_type;          /* MOEARC_OUT_F32 / _F16 */
+    void *k_pages, *v_pages;      /* [page][slot][n_kv_heads][head_dim] */
+    unsigned int kv_type;         /* 0 f32, 1 f16 */
+    unsigned long n_pages, page_tokens, n_heads, n_kv_heads, head_dim;
+    unsigned long n_rot;          /* rotated channels of a head, the first ones; the others pass through */
+    unsigned int neox;            /* pairs (j, j + n_rot/2), else (2j, 2j + 1) */
+    float freq_base, freq_scale, ext_factor, attn_factor, corr_lo, corr_hi;  /* as moearc_rope */
+    const float *freq_factors;    /* device f32 [n_rot / 2]: pair j's frequency is divided by its factor; NULL: not */
+} moearc_qkv_append;
+
+/* q and k normed and rotated, q written to q_out, K and V to their sequence's page of the position. Pair j of
+ * a token at position p turns by p * freq_base^(-2j / n_rot) / freq_factors[j], scaled as moearc_rope scales it, with the
+ * angle in 64 bits (moearc_rope's is the reference's, f32: at position 65536 it is up to 4e-3 radians off);
+ * everything else is f32 and rounded once on the way out. A token whose position is negative (n_kv below the new
+ * tokens) is passed over; one whose page is out of range has its q written and its K and V dropped (see above).
+ * Two tokens of one place are a caller error. Refusals: a null c, d, block_tables, row_begin or n_kv, or a null q, k,
+ * v, q_out, k_pages or v_pages -> -1; a type not 0/1, n_heads or n_kv_heads 0 or above 1024, head_dim 0 or above 256,
+ * n_rot 0, odd or above head_dim, page_tokens 0 or above 2^30, n_pages 0 or above 2^32 - 1, a stride out of range,
+ * freq_base or freq_scale not positive, eps negative or NaN with a norm, row_begin descending, more rows or keys than
+ * the above, bt_stride < ceil(n_kv[b] / page_tokens) of a sequence with new tokens -> -2. No rows -> 0. */
+int moearc_rope_qkv_append_batched(moearc_ctx *c, const moearc_qkv_append *d, const unsigned int *block_tables,
+                                   unsigned long bt_stride, const unsigned int *row_begin, const unsigned int *n_kv,
+                                   unsigned long n_seqs);
+
+/* *bytes = the working memory of a moearc_attn_prefill_batched of these lengths (0: none). Refusals: null -> -1;
+ * sizes that it refuses -> -2. */
+int moearc_attn_prefill_batched_workspace(moearc_ctx *c, const unsigned int *row_begin, const unsigned int *n_kv,
+                                          unsigned long n_seqs, unsigned long n_swa, unsigned long n_heads,
+                                          unsigned long n_kv_heads, unsigned long head_dim, unsigned long *bytes);
+
+/* Attention of every new token over its sequence's keys up to itself (with n_swa the last n_swa of them), whose K and V
+ * are in the cache: row i of sequence b is moearc_attn_decode at n_kv = p + 1, p its position. q f16
+ * [row][n_heads][head_dim]; out the same, f32 or f16 by out_type; sinks f32 [n_heads] or NULL. A row at a negative position
+ * is zero. K and V of keys that a row does not see do not reach it, infinities and NaN among them; slots from
+ * n_kv[b] on are not read. Any group, any page size, head_dim a multiple of 8 up to 256; q, out and the pools 16-byte
+ * aligned; kv_type 1 (f16).
+ * Precision: exact f16 products summed in f32. An f16 out rounds each softmax weight to f16 once, to 2^-11 of it
+ * (the output's own rounding is as much, of a sum in which these average out); an f32 out carries it as f16 hi + lo,
+ * to 2^-22 of it; either to 2^-32 of the row's largest weight where that is more.
+ * ws: ws_bytes of 16-byte aligned device memory (moearc_attn_prefill_batched_workspace), used until the call's work is
+ * done; NULL: the context's, grown on demand (calls that find none run without it, slower). A captured call whose
+ * workspace is not 0 needs ws (else -1), and graphs that may run at the same time need one each. Refusals: a null
+ * pointer other than sinks and ws -> -1; kv_type not 1, out_type not 0/1, n_heads 0 or above 1024, n_kv_heads 0 or no
+ * divisor of it, head_dim as above, n_swa >= 2^31, page_tokens 0 or above 2^30, n_pages 0 or above 2^32 - 1, a scale that is
+ * not finite (times log2 e), an address off its alignment, row_begin descending, more rows or keys than the above,
+ * bt_stride < ceil(n_kv[b] / page_tokens) of a sequence with new tokens, a ws too small or misaligned -> -2. No rows -> 0. */
+int moearc_attn_prefill_batched(moearc_ctx *c, void *out, unsigned int out_type, const void *q, const void *k_pages,
+                                const void *v_pages, unsigned long n_pages, const unsigned int *block_tables,
+                                unsigned long bt_stride, const unsigned int *row_begin, const unsigned int *n_kv,
+                                const float *sinks, unsigned long n_seqs, unsigned long n_swa, unsigned long n_heads,
+                                unsigned long n_kv_heads, unsigned long head_dim, unsigned long page_tokens, float scale,
+                                unsigned int kv_type, void *ws, unsigned long ws_bytes);
+
 /* The stream the context enqueues on (a hipStream_t), so a caller can order its own work. */
 void *moearc_ctx_stream(moearc_ctx *c);
 

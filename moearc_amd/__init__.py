@@ -6,4 +6,4 @@ mirror of the reference wrapper (context.py), the ctypes binding (native.py), th
 """
 from .context import (BadArgument, BufferTooSmall, Context, DeviceBuffer, Failed, KernelError,  # noqa: F401
                       AttnBlockDesc, DeviceView, KvType, MoeAct, MoeDesc, NO_EXPERT, NoDevice, OutOfMemory, OUT_F16,
-                      OUT_F32, QuantType, RopeKind, RopeScaling, RouteMode)
+                      OUT_F32, QkvAppendDesc, QuantType, RopeKind, RopeScaling, RouteMode)

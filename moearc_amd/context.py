@@ -379,6 +379,55 @@ class Context:
                                            float(scale), int(KvType(kv)))
         self.finish(rc, "chunked prefill attention")
 
+    # ---- ragged batches -----------------------------------------------------------------------
+    def _batch(self, block_tables: DeviceBuffer, bt_stride: int, row_begin, n_kv):
+        rb, nk = np.ascontiguousarray(row_begin, np.uint32), np.ascontiguousarray(n_kv, np.uint32)
+        if rb.size != nk.size + 1:
+            raise BadArgument("row_begin has one entry more than n_kv")
+        block_tables.require("block tables", nk.size * bt_stride * 4)
+        return rb, nk, int(rb[-1])
+
+    def rope_qkv_append_batched(self, desc: "QkvAppendDesc", block_tables: DeviceBuffer, bt_stride: int, row_begin,
+                                n_kv) -> None:
+        """New tokens of many sequences: q, k normed and rotated, q written, K and V into their pages."""
+        rb, nk, rows = self._batch(block_tables, bt_stride, row_begin, n_kv)
+        desc.require(rows)
+        self.finish(self._lib.moearc_rope_qkv_append_batched(self.raw, ctypes.byref(desc), block_tables.ptr, bt_stride,
+                                                             rb.ctypes.data, nk.ctypes.data, nk.size),
+                    "batched RoPE + KV append")
+
+    def attn_prefill_batched_workspace(self, row_begin, n_kv, n_swa: int, n_heads: int, n_kv_heads: int,
+                                       head_dim: int) -> int:
+        """Bytes of working memory of attn_prefill_batched at these lengths (0: none)."""
+        rb, nk = np.ascontiguousarray(row_begin, np.uint32), np.ascontiguousarray(n_kv, np.uint32)
+        if rb.size != nk.size + 1:
+            raise BadArgument("row_begin has one entry more than n_kv")
+        n = ctypes.c_ulong()
+        _check(self._lib.moearc_attn_prefill_batched_workspace(self.raw, rb.ctypes.data, nk.ctypes.data, nk.size, n_swa,
+                                                               n_heads, n_kv_heads, head_dim, ctypes.byref(n)),
+               "batched attention's workspace")
+        return n.value
+
+    def attn_prefill_batched(self, out: DeviceBuffer, q: DeviceBuffer, k_pages: DeviceBuffer, v_pages: DeviceBuffer,
+                             n_pages: int, block_tables: DeviceBuffer, bt_stride: int, row_begin, n_kv,
+                             sinks: Optional[DeviceBuffer], n_swa: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                             page_tokens: int, scale: float, kv: KvType = KvType.F16, out_type: int = OUT_F32,
+                             workspace: Optional[DeviceBuffer] = None) -> None:
+        """Every new token's attention over its sequence's keys; row_begin, n_kv: host sequences of ints."""
+        rb, nk, rows = self._batch(block_tables, bt_stride, row_begin, n_kv)
+        row = n_heads * head_dim
+        q.require("query (f16)", rows * row * 2)
+        out.require("attention output", rows * row * (2 if out_type == OUT_F16 else 4))
+        for pages, what in ((k_pages, "key pages"), (v_pages, "value pages")):
+            pages.require(what, n_pages * page_tokens * n_kv_heads * head_dim * 2)
+        if sinks is not None:
+            sinks.require("attention sinks", n_heads * 4)
+        self.finish(self._lib.moearc_attn_prefill_batched(
+            self.raw, out.ptr, out_type, q.ptr, k_pages.ptr, v_pages.ptr, n_pages, block_tables.ptr, bt_stride,
+            rb.ctypes.data, nk.ctypes.data, _ptr(sinks), nk.size, n_swa, n_heads, n_kv_heads, head_dim, page_tokens,
+            float(scale), int(KvType(kv)), _ptr(workspace), workspace.len if workspace is not None else 0),
+            "batched chunk attention")
+
     # ---- attention projections -------------------------------------------------------------
     def matvec_q(self, ty, out: DeviceBuffer, w: DeviceBuffer, x: DeviceBuffer, n_rows: int,
                   n_cols: int) -> None:
@@ -554,6 +603,61 @@ class Context:
         self.finish(self._lib.moearc_moe_ffn(self.raw, ctypes.byref(desc), y.ptr, x.ptr, io_type, ids.ptr, weights.ptr,
                                              n_tok, n_used, int(accumulate), _ptr(workspace),
                                              workspace.len if workspace is not None else 0), "experts")
+
+
+class QkvAppendDesc(ctypes.Structure):
+    """``moearc_qkv_append`` (include/moearc_attn.h): one layer's rows of a ragged batch, its cache and RoPE."""
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("in_type", ctypes.c_uint),
+                ("q_stride", ctypes.c_ulong), ("k_stride", ctypes.c_ulong), ("v_stride", ctypes.c_ulong),
+                ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float),
+                ("q_out", ctypes.c_void_p), ("q_type", ctypes.c_uint), ("k_pages", ctypes.c_void_p),
+                ("v_pages", ctypes.c_void_p), ("kv_type", ctypes.c_uint), ("n_pages", ctypes.c_ulong),
+                ("page_tokens", ctypes.c_ulong), ("n_heads", ctypes.c_ulong), ("n_kv_heads", ctypes.c_ulong),
+                ("head_dim", ctypes.c_ulong), ("n_rot", ctypes.c_ulong), ("neox", ctypes.c_uint),
+                ("freq_base", ctypes.c_float), ("freq_scale", ctypes.c_float), ("ext_factor", ctypes.c_float),
+                ("attn_factor", ctypes.c_float), ("corr_lo", ctypes.c_float), ("corr_hi", ctypes.c_float),
+                ("freq_factors", ctypes.c_void_p)]
+
+    @staticmethod
+    def make(q, k, v, q_out, k_pages, v_pages, n_pages: int, n_heads: int, n_kv_heads: int, head_dim: int,
+             page_tokens: int, n_rot: int, freq_base: float, scaling: Optional[RopeScaling] = None,
+             kind: RopeKind = RopeKind.NEOX, in_type: int = OUT_F32, q_type: int = OUT_F16, kv: KvType = KvType.F16,
+             q_stride: Optional[int] = None, k_stride: Optional[int] = None, v_stride: Optional[int] = None,
+             q_norm=None, k_norm=None, eps: float = 1e-6, freq_factors=None) -> "QkvAppendDesc":
+        """Strides in elements; None: rows without a gap."""
+        s, kv, row = scaling or RopeScaling.NONE, KvType(kv), n_kv_heads * head_dim
+        for pages, what in ((k_pages, "key pages"), (v_pages, "value pages")):
+            pages.require(what, n_pages * page_tokens * row * kv.elem_bytes)
+        for w, what in ((q_norm, "query norm"), (k_norm, "key norm")):
+            if w is not None:
+                w.require(what, head_dim * 4)
+        if freq_factors is not None:
+            freq_factors.require("frequency factors", n_rot // 2 * 4)
+        d = QkvAppendDesc()
+        d.q, d.k, d.v, d.q_out, d.k_pages, d.v_pages = q.ptr, k.ptr, v.ptr, q_out.ptr, k_pages.ptr, v_pages.ptr
+        d.in_type, d.q_type, d.kv_type = in_type, q_type, int(kv)
+        d.q_stride = n_heads * head_dim if q_stride is None else q_stride
+        d.k_stride, d.v_stride = (row if n is None else n for n in (k_stride, v_stride))
+        d.q_norm, d.k_norm, d.eps, d.freq_factors = _ptr(q_norm), _ptr(k_norm), eps, _ptr(freq_factors)
+        d.n_pages, d.page_tokens, d.n_heads, d.n_kv_heads, d.head_dim = n_pages, page_tokens, n_heads, n_kv_heads, head_dim
+        d.n_rot, d.neox, d.freq_base = n_rot, int(RopeKind(kind)), freq_base
+        d.freq_scale, d.ext_factor, d.attn_factor = s.freq_scale, s.ext_factor, s.attn_factor
+        d.corr_lo, d.corr_hi = s.corr_lo, s.corr_hi
+        # the descriptor holds raw device pointers: keep their buffers alive as long as it lives
+        d._rows = (q, k, v, q_out)
+        d._buffers = [b for b in (k_pages, v_pages, q_norm, k_norm, freq_factors) if b is not None]
+        return d
+
+    def require(self, rows: int) -> None:
+        """That q, k, v and q_out hold `rows` rows."""
+        if rows == 0:
+            return
+        size = 2 if self.in_type == OUT_F16 else 4
+        q, k, v, q_out = self._rows
+        for buf, stride, heads, what in ((q, self.q_stride, self.n_heads, "query rows"), (k, self.k_stride, self.n_kv_heads, "key rows"),
+                                         (v, self.v_stride, self.n_kv_heads, "value rows")):
+            buf.require(what, ((rows - 1) * stride + heads * self.head_dim) * size)
+        q_out.require("rotated queries", rows * self.n_heads * self.head_dim * (2 if self.q_type == OUT_F16 else 4))
 
 
 class MoeDesc(ctypes.Structure):

@@ -350,3 +350,62 @@ struct MoeCombineArgs {
 #define MOEARC_MOE_SMALL_TOKENS 16u
 #define MOEARC_MOE_TILE 64u         // most slots of a plan's tile, and of a light one
 #define MOEARC_MOE_LIGHT 32u
+
+// ---- ragged batches (append.hip, attn_batch.hip) -------------------------------------------------
+//
+// Sequences one launch carries in its kernel arguments; the host splits larger batches.
+#define MOEARC_BATCH_SEQS 64
+
+// New tokens' q, k and v rows: norm, rotation, q out, K and V into their pages. Row t of the launch (t counts
+// from its first sequence's first row) belongs to sequence b, the last one with row_begin[b] <= t.
+struct QkvAppendArgs {
+    const void *q, *k, *v;          // of the launch's first row, f32 or f16
+    const float *q_norm, *k_norm;   // [head_dim] or null
+    const float *factors;           // [n_rot / 2] or null
+    void *q_out, *k_pages, *v_pages;
+    const uint32_t *block_tables;   // of the launch's first sequence
+    uint32_t *err;
+    uint64_t q_stride, k_stride, v_stride, bt_stride;
+    double log2_step;               // -2 log2(freq_base) / n_rot: pair p turns at 2^(p log2_step) radians a position
+    float freq_scale, ext_factor, mscale, corr_lo, corr_hi, eps;
+    uint32_t n_heads, n_kv_heads, head_dim, n_rot, neox;
+    uint32_t in_f16, q_f16, kv_f16, n_pages, page_tokens;
+    uint32_t row_off;               // the first work-group's row
+    uint32_t pad;
+    uint32_t row_begin[MOEARC_BATCH_SEQS];  // entries n_seqs .. the end: 2^32 - 1
+    uint32_t n_new[MOEARC_BATCH_SEQS];
+    uint32_t n_kv[MOEARC_BATCH_SEQS];
+};
+
+// Attention of a ragged batch. A sequence's rows (token, head of the KV head's group) are cut into tiles of
+// `tile_rows`, a tile's keys into pieces of `piece` keys; a work-group takes one piece of one tile for one KV head.
+// Slot b's work items (tiles x pieces) start at item_begin[b]; a slot with more than one piece to a tile leaves
+// records that the merge kernel joins:
+//   rec_o[((rec_begin[b] + tile * pieces + piece) * n_kv_heads + kvh) * tile_rows + row][head_dim]  un-normalised (f32)
+//   rec_ml[the same row index][2]   reference max (log2 domain), row sum in its frame
+#define MOEARC_AB_ROWS 128        // rows of a tile: 32 to a wave
+#define MOEARC_AB_PT 1024u        // block-table entries that a work-group holds at a time
+#define MOEARC_AB_LOG2_PSCALE 7.0f  // weights are 2^7 at the reference max: f16 keeps 21 bits below it
+struct AttnBatchArgs {
+    const uint16_t *q, *k_pages, *v_pages;
+    const uint32_t *block_tables;
+    const float *sinks;
+    void *out;
+    float *rec_o, *rec_ml;
+    uint32_t *err;
+    uint64_t bt_stride;
+    uint32_t n_swa, n_heads, n_kv_heads, group, head_dim;
+    uint32_t page_tokens, page_magic, page_shift;  // key / page_tokens = key * magic >> shift for key < 2^31
+    uint32_t n_pages, out_f16;
+    float scale_log2e;
+    uint32_t piece;                 // keys, a multiple of 32
+    uint32_t n_slots, rows_per_block;  // (the merge's: rows of a tile that a work-group joins)
+    uint32_t item_begin[MOEARC_BATCH_SEQS + 1];   // entries n_slots .. the end: the item count
+    uint32_t merge_begin[MOEARC_BATCH_SEQS + 1];  // tiles that need a merge
+    uint32_t seq[MOEARC_BATCH_SEQS];      // block-table row
+    uint32_t row0[MOEARC_BATCH_SEQS];     // first token's row of q and out
+    uint32_t n_new[MOEARC_BATCH_SEQS];
+    uint32_t n_kv[MOEARC_BATCH_SEQS];
+    uint32_t n_tiles[MOEARC_BATCH_SEQS];
+    uint32_t rec_begin[MOEARC_BATCH_SEQS];
+};

@@ -142,6 +142,10 @@ struct moearc_ctx {
     hipFunction_t f_moe_tile[6][2][2] = {}, f_moe_light[6][2][2] = {}, f_moe_vec[6][2][3] = {};
     float *moe_ws = nullptr;  // the experts' products' working memory, eager calls only
     size_t moe_ws_floats = 0;
+    hipFunction_t f_qkv_append[4] = {};  // 8, 16, 32 lanes a head, any head
+    hipFunction_t f_attn_batch[3][2] = {}, f_attn_batch_merge = nullptr;  // up to 64, 128, 256 channels x default, precise
+    float *ab_ws = nullptr;  // the records of a ragged batch's cut tiles, eager calls only
+    size_t ab_ws_floats = 0;
     int decode_variant_override = -1;  // MOEARC_DECODE_VARIANT, e.g. "4x2x4"
     unsigned long split_override = 0;  // MOEARC_DECODE_SPLIT (keys per split)
     float *blk_ws = nullptr;  // attention-block chunk: q, k, v, f16 q, attention output, projection
@@ -160,7 +164,8 @@ struct moearc_ctx {
 
 namespace {
 
-bool moe_load(moearc_ctx *c);  // runtime_moe.h
+bool moe_load(moearc_ctx *c);    // runtime_moe.h
+bool batch_load(moearc_ctx *c);  // runtime_batch.h
 
 hipEvent_t take_event(moearc_ctx *c) {
     if (!c->event_pool.empty()) {
@@ -668,7 +673,7 @@ moearc_ctx *release(moearc_ctx *c) {
     }
     for (auto e : c->event_pool) (void) hipEventDestroy(e);
     for (void *p : {(void *) c->ws, (void *) c->ws_kinds, (void *) c->pf_ws, (void *) c->blk_ws, (void *) c->mm_ws, (void *) c->mm_part,
-                    (void *) c->moe_ws, (void *) c->err_word})
+                    (void *) c->moe_ws, (void *) c->ab_ws, (void *) c->err_word})
         if (p) (void) hipFree(p);
     if (c->module) (void) hipModuleUnload(c->module);
     if (c->stream) (void) hipStreamDestroy(c->stream);
@@ -779,7 +784,7 @@ moearc_ctx *moearc_ctx_create(void) {
             return release(c);
         }
     }
-    if (!moe_load(c)) return release(c);
+    if (!moe_load(c) || !batch_load(c)) return release(c);
     for (hipFunction_t f : c->f_dec_merge) {
         int merge_threads = 0;
         if (hipFuncGetAttribute(&merge_threads, HIP_FUNC_ATTRIBUTE_MAX_THREADS_PER_BLOCK, f) != hipSuccess ||
@@ -2166,3 +2171,4 @@ int moearc_attn_block_chunk(moearc_ctx *c, const moearc_attn_block *b, float *h,
 }
 
 #include "runtime_moe.h"
+#include "runtime_batch.h"

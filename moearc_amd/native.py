@@ -76,6 +76,12 @@ SIGNATURES = {
     "moearc_matmul_experts": (ctypes.c_int, [_vp, _u32, _vp, _vp, _vp, _u32, _vp, _vp, _c_ulong, _c_ulong,
                                              _c_ulong, _u32, _c_ulong, _c_ulong, _vp, _c_ulong]),
     "moearc_moe_ffn": (ctypes.c_int, [_vp, _vp, _vp, _vp, _u32, _vp, _vp, _c_ulong, _c_ulong, _u32, _vp, _c_ulong]),
+    "moearc_rope_qkv_append_batched": (ctypes.c_int, [_vp, _vp, _vp, _c_ulong, _vp, _vp, _c_ulong]),
+    "moearc_attn_prefill_batched_workspace": (ctypes.c_int, [_vp, _vp, _vp, _c_ulong, _c_ulong, _c_ulong, _c_ulong,
+                                                             _c_ulong, _vp]),
+    "moearc_attn_prefill_batched": (ctypes.c_int, [_vp, _vp, _u32, _vp, _vp, _vp, _c_ulong, _vp, _c_ulong, _vp, _vp, _vp,
+                                                   _c_ulong, _c_ulong, _c_ulong, _c_ulong, _c_ulong, _c_ulong,
+                                                   ctypes.c_float, _u32, _vp, _c_ulong]),
     # include/moearc_kv.h
     "moearc_kv_pool_create": (ctypes.c_int, [_u32, _u32, _u32, ctypes.POINTER(_vp)]),
     "moearc_kv_pool_destroy": (None, [_vp]),
