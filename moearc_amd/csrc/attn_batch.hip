@@ -27,7 +27,7 @@
 // averaging); precise ones, for f32 outputs, carry it as f16 hi + lo (2^-22).
 //
 // Infinities and NaN in V of keys that a row does not see must not reach it, but 0 * NaN would in the matrix cores.
-// A work-group that ends with a non-finite accumulator runs once more with the tiles that cross a mask done key by key.
+// A work-group that ends with a non-finite accumulator runs once more, with the tiles that cross a mask done key by key.
 #include "common.h"
 
 namespace {
@@ -54,13 +54,21 @@ typedef short short4v_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v_t lds_short4_t;
 typedef __attribute__((address_space(3))) uint8_t lds_u8_t;
 
-// LDS DMA of 16 bytes per active lane from p to LDS address lds + 16 * lane. Through asm: for the builtin the compiler,
-// which cannot tell the buffer being read from the one being filled, would wait for the copy before every LDS read.
-__device__ __forceinline__ void ab_copy16(const uint8_t *p, uint32_t lds) {
-    uint32_t m0_saved;  // m0 is the compiler's
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
-                 "s_mov_b32 m0, %0"
-                 : "=&s"(m0_saved) : "v"(p), "s"(lds) : "memory");
+// LDS DMA of 16 bytes per lane of `mask` to LDS address lds + 16 * lane, from a lane's own address or from a
+// wave-uniform one plus a lane's offset. Through asm: for the builtin the compiler, which cannot tell the buffer being
+// read from the one being filled, would wait for the copy before every LDS read, and branch around it for the mask.
+// m0 and exec are the compiler's: saved and restored; every lane is active where these are called.
+__device__ __forceinline__ void ab_copy16(const uint8_t *p, uint32_t lds, uint64_t mask) {
+    uint32_t m0_saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_mov_b64 exec, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
+                 "s_mov_b64 exec, -1\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0_saved) : "v"(p), "s"(lds), "s"(mask) : "memory");
+}
+__device__ __forceinline__ void ab_copy16(const uint8_t *base, uint32_t off, uint32_t lds, uint64_t mask) {
+    uint32_t m0_saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_mov_b64 exec, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
+                 "s_mov_b64 exec, -1\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0_saved) : "v"(off), "s"(base), "s"(lds), "s"(mask) : "memory");
 }
 
 // The slot whose work items (begin[] ascending, entries n .. the end: the count) hold `item`.
@@ -86,6 +94,7 @@ __device__ __forceinline__ AbSpan ab_span(const AttnBatchArgs &a, uint32_t b, ui
     AbSpan s;
     s.hi = last < 0 ? 0u : (uint32_t) last + 1u;
     s.lo = a.n_swa && (uint32_t) first + 1u > a.n_swa ? (uint32_t) first + 1u - a.n_swa : 0u;
+    if (a.page_tokens % 8u == 0u) s.lo &= ~7u;  // in the same page
     return s;
 }
 
@@ -94,7 +103,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     using S = AbShape<DB>;
     constexpr int NBUF = 4;
     __shared__ __attribute__((aligned(1024))) uint8_t tiles[NBUF * S::BUF];
-    __shared__ uint32_t table[MOEARC_AB_PT];
+    __shared__ uint32_t table[MOEARC_AB_PT];  // places in the pools (page * page_tokens + slot) of eight keys each, or of each key
     __shared__ uint32_t again;
 
     const uint32_t tid = threadIdx.x, lane = tid & 63u, h = lane >> 5, n = lane & 31u;
@@ -106,7 +115,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     const uint32_t pieces = (a.item_begin[b + 1] - a.item_begin[b]) / nt;
     const uint32_t pc = in_slot / nt, tile = nt - 1u - in_slot % nt;  // the latest tile, which has the most keys, first
     const AbSpan span = ab_span(a, b, tile);
-    const uint32_t lo = span.lo + pc * a.piece;
+    const uint32_t lo = span.lo + pc * a.piece;  // with pages of eights a multiple of 8
     const uint32_t hi = pieces > 1 ? min(span.hi, lo + a.piece) : span.hi;
     if (pc && lo >= span.hi) return;  // an earlier tile's span has fewer pieces
 
@@ -137,8 +146,11 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     if (c == 0.f) {  // every score 0, and masked ones still -inf: q = 0
         c = 1.f;
 #pragma unroll
-        for (int t = 0; t < 2 * DB; ++t) qop[t] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+            for (int t = 0; t < 2 * DB; ++t) qop[t] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
     }
+    // q has arrived: the compiler would wait for its loads in the key loop, and so for the copies issued after them
+#pragma unroll
+    for (int t = 0; t < 2 * DB; ++t) asm volatile("" : "+v"(qop[t]));
     // positions of the wave's first and last row: which tiles it skips, which cross a mask
     const uint32_t wr0 = tile * MOEARC_AB_ROWS + wave * 32u;
     const bool wave_ok = wr0 < rows;
@@ -157,8 +169,21 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     }
     const uint32_t k_at = S::k_at(n, h);  // of MFMA t: ^ t << 5
     const uint32_t lds0 = (uint32_t) (uintptr_t) (lds_u8_t *) tiles;
-    const uint32_t ld_key = 8u * wave + lane / S::CHUNKS, ld_slot = lane % S::CHUNKS;
-    const uint64_t key_bytes = (uint64_t) G * D * 2u, head_bytes = (uint64_t) kvh * D * 2u;
+    const uint32_t ld_key = lane / S::CHUNKS, ld_slot = lane % S::CHUNKS;  // of a copy's KEYS keys, and where in their rows
+    const uint32_t key_bytes = G * D * 2u, head_bytes = kvh * D * 2u;
+    const bool eights = a.page_tokens % 8u == 0u;
+    // Byte offsets from its first key's row in the pool of what this lane copies of a wave's eight keys, and whether there
+    // is such a chunk in a head.
+    uint32_t off_k[S::COPIES], off_v[S::COPIES];
+    uint64_t has_k[S::COPIES], has_v[S::COPIES];
+#pragma unroll
+    for (uint32_t i = 0; i < S::COPIES; ++i) {
+        const uint32_t key = ld_key + i * S::KEYS, ck = ld_slot ^ S::fk(8u * wave + key), cv = ld_slot ^ S::fv(8u * wave + key);
+        off_k[i] = key * key_bytes + head_bytes + 16u * ck;
+        off_v[i] = key * key_bytes + head_bytes + 16u * cv;
+        has_k[i] = __builtin_amdgcn_ballot_w64(8u * ck < D);
+        has_v[i] = __builtin_amdgcn_ballot_w64(8u * cv < D);
+    }
     if (D < 32u * DB) {  // chunks behind the head's channels are never copied: zeros for the products
         for (uint32_t i = tid; i < NBUF * S::BUF / 16u; i += 256u) ((u32x4_t *) tiles)[i] = u32x4_t{0u, 0u, 0u, 0u};
     }
@@ -168,7 +193,8 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     const half2_t ones2 = {1, 1};
     const uint32_t *row_table = a.block_tables + a.seq[b] * a.bt_stride;
 
-    for (int round = 0; round < 2; ++round) {  // a second one where an accumulator is not finite
+    auto all_keys = [&](auto by_key_c) {
+        constexpr bool BY_KEY = decltype(by_key_c)::value;
         m_run = PF_M_INIT;
         l_run = 0.f;
 #pragma unroll
@@ -230,7 +256,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
                     for (int i = 0; i < 8; i += 2) l = __builtin_amdgcn_fdot2((half2_t){plo[q][i], plo[q][i + 1]}, ones2, l, false);
             }
             l_run = l;
-            if (round && masked) {  // key by key: weight and visibility from the lane that holds them
+            if (BY_KEY && masked) {  // weight and visibility from the lane that holds them
                 for (uint32_t k = 0; k < 32u; ++k) {
                     const uint32_t i = 4u * (k >> 3) + (k & 3u);  // register of lane half (k >> 2) & 1
                     float w = 0.f;
@@ -265,36 +291,45 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
                 }
         };
 
-        // Keys whose block-table entries fit `table` at a time; one step computes a 32-key tile.
-        const uint64_t seg_keys64 = (uint64_t) (MOEARC_AB_PT - 1u) * a.page_tokens / 32u * 32u;  // a segment may begin inside a page
-        const uint32_t seg_keys = seg_keys64 == 0 ? 32u : (uint32_t) min(seg_keys64, (uint64_t) 0x40000000u);
+        // Keys whose places fit `table` at a time; one step computes a 32-key tile.
+        const uint32_t seg_keys = eights ? 8u * MOEARC_AB_PT : MOEARC_AB_PT;
         for (uint32_t seg = lo; seg < hi; seg += seg_keys) {
             const uint32_t seg_hi = min(hi, seg + seg_keys), last_key = seg_hi - 1u;
-            auto page_of = [&](uint32_t key) { return (uint32_t) ((uint64_t) key * a.page_magic >> a.page_shift); };
-            const uint32_t page0 = page_of(seg), n_ids = page_of(last_key) - page0 + 1u;
+            const uint32_t n_places = eights ? (last_key - seg) / 8u + 1u : last_key - seg + 1u;
             __syncthreads();
-            for (uint32_t i = tid; i < n_ids; i += 256u) {
-                uint32_t id = row_table[page0 + i];
+            for (uint32_t i = tid; i < n_places; i += 256u) {
+                const uint32_t key = seg + (eights ? 8u * i : i);
+                const uint32_t page = (uint32_t) ((uint64_t) key * a.page_magic >> a.page_shift);
+                uint32_t id = row_table[page];
                 if (id >= a.n_pages) {  // reported; what is read instead lies in the pool
                     *(volatile uint32_t *) a.err = 1u;
                     id = 0u;
                 }
-                table[i] = id;
+                table[i] = id * a.page_tokens + (key - page * a.page_tokens);
             }
             __syncthreads();
-            // a wave's copies of tile r: its eight keys of K and of V. Keys behind the last are that one: their scores are
-            // masked, and no slot is read that the cache has not written.
+            // A wave's copies of a tile: its eight keys of K and of V. With pages of eights these share a page, and their
+            // base is wave-uniform. Keys behind the last are that one: their scores are masked, and no slot is read that the
+            // cache has not written.
             auto copy_tile = [&](uint32_t j0, uint32_t buf) {
+                const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + buf * S::BUF + 8u * wave * S::ROW), j = j0 + 8u * wave;
+                if (eights && j + 7u <= last_key) {
+                    const uint64_t at = (uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) table[(j - seg) / 8u]) * key_bytes;
 #pragma unroll
-                for (uint32_t i = 0; i < S::COPIES; ++i) {
-                    const uint32_t in_tile = ld_key + i * S::KEYS;
-                    const uint32_t key = min(j0 + in_tile, last_key);
-                    const uint32_t page = page_of(key);
-                    const uint64_t at = ((uint64_t) table[page - page0] * a.page_tokens + (key - page * a.page_tokens)) * key_bytes + head_bytes;
-                    const uint32_t ck = ld_slot ^ S::fk(in_tile), cv = ld_slot ^ S::fv(in_tile);
-                    const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + buf * S::BUF + (8u * wave + i * S::KEYS) * S::ROW);
-                    if (8u * ck < D) ab_copy16((const uint8_t *) a.k_pages + at + 16u * ck, dst);
-                    if (8u * cv < D) ab_copy16((const uint8_t *) a.v_pages + at + 16u * cv, dst + S::TILE);
+                    for (uint32_t i = 0; i < S::COPIES; ++i) {
+                        ab_copy16((const uint8_t *) a.k_pages + at, off_k[i], dst + i * 1024u, has_k[i]);
+                        ab_copy16((const uint8_t *) a.v_pages + at, off_v[i], dst + S::TILE + i * 1024u, has_v[i]);
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < S::COPIES; ++i) {
+                        const uint32_t key = ld_key + i * S::KEYS, at_key = min(j + key, last_key) - seg;
+                        const uint32_t place = eights ? table[at_key / 8u] + at_key % 8u : table[at_key];
+                        const uint64_t at = (uint64_t) place * key_bytes;
+                        const uint32_t less = key * key_bytes;
+                        ab_copy16((const uint8_t *) a.k_pages + at + (off_k[i] - less), dst + i * 1024u, has_k[i]);
+                        ab_copy16((const uint8_t *) a.v_pages + at + (off_v[i] - less), dst + S::TILE + i * 1024u, has_v[i]);
+                    }
                 }
             };
             // Step r: this wave's copies of tile r are done (those of r + 1 and r + 2, issued later, may be in flight),
@@ -312,21 +347,21 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");  // before the buffers are filled again, or released
         }
 
-        if (round) break;
-        bool finite = true;
-        if (row_ok) {
+    };
+    all_keys(std::false_type{});
+    bool finite = true;
+    if (row_ok) {
 #pragma unroll
-            for (int mb = 0; mb < DB; ++mb)
+        for (int mb = 0; mb < DB; ++mb)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) finite = finite && (__float_as_uint(O[mb][i]) & 0x7F800000u) != 0x7F800000u;
-        }
-        __syncthreads();
-        if (tid == 0) again = 0u;
-        __syncthreads();
-        if (!finite) again = 1u;
-        __syncthreads();
-        if (!again) break;
+            for (int i = 0; i < 16; ++i) finite = finite && (__float_as_uint(O[mb][i]) & 0x7F800000u) != 0x7F800000u;
     }
+    __syncthreads();
+    if (tid == 0) again = 0u;
+    __syncthreads();
+    if (!finite) again = 1u;
+    __syncthreads();
+    if (again) all_keys(std::true_type{});
 
     const float L = l_run + __shfl_xor(l_run, 32);
     if (!row_ok) return;

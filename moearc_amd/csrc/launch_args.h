@@ -384,7 +384,7 @@ struct QkvAppendArgs {
 //   rec_o[((rec_begin[b] + tile * pieces + piece) * n_kv_heads + kvh) * tile_rows + row][head_dim]  un-normalised (f32)
 //   rec_ml[the same row index][2]   reference max (log2 domain), row sum in its frame
 #define MOEARC_AB_ROWS 128        // rows of a tile: 32 to a wave
-#define MOEARC_AB_PT 1024u        // block-table entries that a work-group holds at a time
+#define MOEARC_AB_PT 2048u        // keys' places that a work-group holds at a time (of eight keys each where pages allow)
 #define MOEARC_AB_LOG2_PSCALE 7.0f  // weights are 2^7 at the reference max: f16 keeps 21 bits below it
 struct AttnBatchArgs {
     const uint16_t *q, *k_pages, *v_pages;

@@ -238,6 +238,7 @@ int moearc_attn_prefill_batched(moearc_ctx *c, void *out, unsigned int out_type,
     if (kv_type != 1u || out_type > 1u) return ERR_ARG;
     if (const int rc = attn_batch_check(n_heads, n_kv_heads, head_dim, n_swa)) return rc;
     if (page_tokens == 0 || page_tokens > (1ul << 30) || n_pages == 0 || n_pages > (1ul << 32) - 1) return ERR_ARG;
+    if (n_pages > 0xFFFFFFFFul / page_tokens) return ERR_ARG;  // places in a pool are 32-bit numbers
     const float c2 = scale * 1.4426950408889634f;
     if (!(std::fabs(c2) <= 3.0e38f)) return ERR_ARG;
     if (((uintptr_t) out | (uintptr_t) q | (uintptr_t) k_pages | (uintptr_t) v_pages) % 16 != 0) return ERR_ARG;
