@@ -151,12 +151,10 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     // q has arrived: the compiler would wait for its loads in the key loop, and so for the copies issued after them
 #pragma unroll
     for (int t = 0; t < 2 * DB; ++t) asm volatile("" : "+v"(qop[t]));
-    // positions of the wave's first and last row: which tiles it skips, which cross a mask
+    // positions of the wave's first and last row: which tiles cross a mask
     const uint32_t wr0 = tile * MOEARC_AB_ROWS + wave * 32u;
-    const bool wave_ok = wr0 < rows;
     const int32_t w_first = shift + (int32_t) (min(wr0, rows - 1u) / group);
     const int32_t w_last = shift + (int32_t) (min(wr0 + 31u, rows - 1u) / group);
-    const int32_t w_lo_first = a.n_swa ? max(0, w_first + 1 - (int32_t) a.n_swa) : 0;
     const int32_t w_lo_last = a.n_swa ? max(0, w_last + 1 - (int32_t) a.n_swa) : 0;
 
     // ---- LDS addresses and copies ----------------------------------------------------------------
@@ -218,8 +216,8 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
             return l;
         };
 
-        auto compute = [&](uint32_t j0, uint32_t buf) {
-            if (!wave_ok || (int32_t) j0 > w_last || (int32_t) j0 + 31 < w_lo_first) return;
+        // S^T of the tile in buffer buf.
+        auto scores = [&](uint32_t buf) {
             const uint8_t *const kt = tiles + buf * S::BUF;
             float16_t s;
 #pragma unroll
@@ -227,6 +225,12 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
 #pragma unroll
             for (int t = 0; t < 2 * DB; ++t)
                 s = pf_mfma(*(const half8_t *) (kt + (k_at ^ (uint32_t) t << 5)), qop[t], s);
+            return s;
+        };
+        // The tile of keys j0 .. in buffer buf, s its scores; the next tile's scores, whose products run beside the
+        // weights' arithmetic.
+        auto compute = [&](float16_t s, uint32_t j0, uint32_t buf, uint32_t next_buf) -> float16_t {
+            const uint8_t *const kt = tiles + buf * S::BUF;
             const bool masked = (int32_t) j0 + 31 > w_first || (int32_t) j0 < w_lo_last;
             if (masked) {
                 const uint32_t off = j0 + 4u * h - row_lo;
@@ -234,6 +238,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
                 for (int i = 0; i < 16; ++i)
                     if (off + (uint32_t) (8 * (i >> 2) + (i & 3)) > row_len) s[i] = -INFINITY;
             }
+            const float16_t next = scores(next_buf);
             half8_t phi[2], plo[2];
             float l = weights(s, MOEARC_AB_LOG2_PSCALE - m_run, l_run, phi, plo);
             if (__builtin_amdgcn_ballot_w64(l == INFINITY) != 0) {
@@ -274,7 +279,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
                             if (sees) O[mb][r] = fmaf(w, v, O[mb][r]);
                         }
                 }
-                return;
+                return next;
             }
 #pragma unroll
             for (int mb = 0; mb < DB; ++mb)
@@ -289,6 +294,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
                     O[mb] = pf_mfma(va, phi[q], O[mb]);
                     if constexpr (PRECISE) O[mb] = pf_mfma(va, plo[q], O[mb]);
                 }
+            return next;
         };
 
         // Keys whose places fit `table` at a time; one step computes a 32-key tile.
@@ -332,17 +338,19 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
                     }
                 }
             };
-            // Step r: this wave's copies of tile r are done (those of r + 1 and r + 2, issued later, may be in flight),
-            // every wave meets, so all copies of r are in and nobody reads tile r - 1's buffer, which r + 3 then takes.
-            // Tiles behind the last are copied again, into buffers that no step reads, so the count is always the same.
+            // Step r: this wave's copies of tile r + 1 are done (those of r + 2, issued later, may be in flight), every
+            // wave meets, so all copies of r + 1 are in and nobody reads tile r - 1's buffer, which r + 3 then takes.
+            // Tiles behind the last are copied again, into buffers whose scores nobody uses, so the count is always the same.
             const uint32_t steps = (seg_hi - seg + 31u) / 32u;
             auto first_key = [&](uint32_t r) { return seg + 32u * min(r, steps - 1u); };
 #pragma unroll
             for (uint32_t r = 0; r < NBUF - 1; ++r) copy_tile(first_key(r), r);
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((NBUF - 2) * 2 * S::COPIES) : "memory");
+            float16_t s = scores(0);
             for (uint32_t r = 0; r < steps; ++r) {
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((NBUF - 2) * 2 * S::COPIES) : "memory");
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((NBUF - 3) * 2 * S::COPIES) : "memory");
                 copy_tile(first_key(r + NBUF - 1u), (r + NBUF - 1u) % NBUF);
-                compute(first_key(r), r % NBUF);
+                s = compute(s, first_key(r), r % NBUF, (r + 1u) % NBUF);
             }
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");  // before the buffers are filled again, or released
         }
