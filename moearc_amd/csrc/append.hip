@@ -8,7 +8,8 @@
 // and its sine and cosine are f32, once per work-group and pair, through LDS; every head of the token uses them.
 // Bound by HBM for chunks, by latency for a decode step. A head takes LPH lanes of eight channels, held as the two
 // quads that rotate into each other, so a head's norm is a sum over neighbouring lanes and every access is 16
-// bytes a lane (8 of f16). Work-groups are (token, group of 256 / LPH heads of q, k and v).
+// bytes a lane (8 of f16). Work-groups are (token, group of 256 / LPH heads of q, k and v), or of three times as many
+// heads where there are more of these than the device holds at once: a work-group's life is mostly latency.
 #include "common.h"
 
 #define AP_MAX_PAIRS 128  // head_dim <= 256
@@ -120,77 +121,85 @@ __device__ __forceinline__ float ap_sum(float s) {
     return s;
 }
 
-template <int LPH>
+// NH heads to a thread, 256 / LPH apart: their loads are in flight together.
+template <int LPH, int NH>
 __device__ __forceinline__ void ap_body(const QkvAppendArgs &a) {
     __shared__ float2_t trig[AP_MAX_PAIRS];
     constexpr uint32_t HEADS = 256 / LPH;
     const uint32_t t = a.row_off + blockIdx.x, u = threadIdx.x % LPH;
-    const uint32_t head = blockIdx.y * HEADS + threadIdx.x / LPH;
     const uint32_t D = a.head_dim, nq = a.n_heads, nk = a.n_kv_heads;
-    const uint32_t kind = head < nq ? 0u : head < nq + nk ? 1u : 2u;  // q, k, v
-    const uint32_t own = kind == 0 ? head : kind == 1 ? head - nq : head - nq - nk;
-    const bool live = head < nq + 2 * nk && 8 * u < D, half = a.in_f16;
-    const bool turned = 8 * u < a.n_rot;
+    const bool half = a.in_f16, turned = 8 * u < a.n_rot;
     const uint32_t c0 = turned && a.neox ? 4 * u : 8 * u, c1 = turned && a.neox ? a.n_rot / 2 + 4 * u : 8 * u + 4;
-    ApQuad x0{}, x1{};
-    if (live) {
-        const void *src = (const void *) ap_pick(kind, (uint64_t) a.q, (uint64_t) a.k, (uint64_t) a.v);
-        const uint64_t at = t * ap_pick(kind, a.q_stride, a.k_stride, a.v_stride) + (uint64_t) own * D;
-        x0 = ap_load(src, at + c0, half);
-        x1 = ap_load(src, at + c1, half);
+    uint32_t kind[NH], own[NH];  // q, k, v; the head among its kind's
+    bool live[NH];
+    ApQuad x0[NH] = {}, x1[NH] = {};
+#pragma unroll
+    for (int i = 0; i < NH; ++i) {
+        const uint32_t head = (blockIdx.y * NH + i) * HEADS + threadIdx.x / LPH;
+        kind[i] = head < nq ? 0u : head < nq + nk ? 1u : 2u;
+        own[i] = kind[i] == 0 ? head : kind[i] == 1 ? head - nq : head - nq - nk;
+        live[i] = head < nq + 2 * nk && 8 * u < D;
+        if (live[i]) {
+            const void *src = (const void *) ap_pick(kind[i], (uint64_t) a.q, (uint64_t) a.k, (uint64_t) a.v);
+            const uint64_t at = t * ap_pick(kind[i], a.q_stride, a.k_stride, a.v_stride) + (uint64_t) own[i] * D;
+            x0[i] = ap_load(src, at + c0, half);
+            x1[i] = ap_load(src, at + c1, half);
+        }
     }
     const ApPlace place = ap_place(a, t);
     if (!place.has_pos) return;
     if (!place.has_page && threadIdx.x == 0) *(volatile uint32_t *) a.err = 1u;  // every writer stores the same value
     if (2 * threadIdx.x < a.n_rot) trig[threadIdx.x] = ap_angle(a, threadIdx.x, place.pos);
     __syncthreads();
-    const float *w = (const float *) ap_pick(kind, (uint64_t) a.q_norm, (uint64_t) a.k_norm, 0);
-    if (w) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s = fmaf(x0.v[i], x0.v[i], fmaf(x1.v[i], x1.v[i], s));
-        s = 1.f / sqrtf(ap_sum<LPH>(s) / (float) D + a.eps);
-        if (live) {
-            const ApQuad w0 = ap_load(w, c0, false), w1 = ap_load(w, c1, false);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x0.v[i] = x0.v[i] * s * w0.v[i];
-                x1.v[i] = x1.v[i] * s * w1.v[i];
-            }
-        }
-    }
-    if (kind < 2 && live && turned) {
-        float2_t cs[4];
+    float2_t cs[4] = {};
+    if (turned) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) cs[i] = trig[4 * u + i];
-        if (a.neox) {
+    }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float r0 = x0.v[i], r1 = x1.v[i];
-                x0.v[i] = r0 * cs[i][0] - r1 * cs[i][1];
-                x1.v[i] = r0 * cs[i][1] + r1 * cs[i][0];
-            }
-        } else {
+    for (int i = 0; i < NH; ++i) {
+        ApQuad &y0 = x0[i], &y1 = x1[i];
+        const float *w = (const float *) ap_pick(kind[i], (uint64_t) a.q_norm, (uint64_t) a.k_norm, 0);
+        if (w) {
+            float s = 0.f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float r0 = x0.v[2 * i], r1 = x0.v[2 * i + 1], r2 = x1.v[2 * i], r3 = x1.v[2 * i + 1];
-                x0.v[2 * i] = r0 * cs[i][0] - r1 * cs[i][1];
-                x0.v[2 * i + 1] = r0 * cs[i][1] + r1 * cs[i][0];
-                x1.v[2 * i] = r2 * cs[2 + i][0] - r3 * cs[2 + i][1];
-                x1.v[2 * i + 1] = r2 * cs[2 + i][1] + r3 * cs[2 + i][0];
+            for (int k = 0; k < 4; ++k) s = fmaf(y0.v[k], y0.v[k], fmaf(y1.v[k], y1.v[k], s));
+            s = 1.f / sqrtf(ap_sum<LPH>(s) / (float) D + a.eps);
+            if (live[i]) {
+                const ApQuad w0 = ap_load(w, c0, false), w1 = ap_load(w, c1, false);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    y0.v[k] = y0.v[k] * s * w0.v[k];
+                    y1.v[k] = y1.v[k] * s * w1.v[k];
+                }
             }
         }
-    }
-    if (!live) return;
-    if (kind == 0) {
-        const uint64_t at = ((uint64_t) t * nq + own) * D;
-        ap_store(a.q_out, at + c0, a.q_f16, x0);
-        ap_store(a.q_out, at + c1, a.q_f16, x1);
-    } else if (place.has_page) {
-        void *dst = (void *) ap_pick(kind, 0, (uint64_t) a.k_pages, (uint64_t) a.v_pages);
-        const uint64_t at = (place.token * nk + own) * D;
-        ap_store(dst, at + c0, a.kv_f16, x0);
-        ap_store(dst, at + c1, a.kv_f16, x1);
+        if (kind[i] < 2 && turned) {
+            if (a.neox) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float r0 = y0.v[k], r1 = y1.v[k];
+                    y0.v[k] = r0 * cs[k][0] - r1 * cs[k][1];
+                    y1.v[k] = r0 * cs[k][1] + r1 * cs[k][0];
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float r0 = y0.v[2 * k], r1 = y0.v[2 * k + 1], r2 = y1.v[2 * k], r3 = y1.v[2 * k + 1];
+                    y0.v[2 * k] = r0 * cs[k][0] - r1 * cs[k][1];
+                    y0.v[2 * k + 1] = r0 * cs[k][1] + r1 * cs[k][0];
+                    y1.v[2 * k] = r2 * cs[2 + k][0] - r3 * cs[2 + k][1];
+                    y1.v[2 * k + 1] = r2 * cs[2 + k][1] + r3 * cs[2 + k][0];
+                }
+            }
+        }
+        if (live[i] && (kind[i] == 0 || place.has_page)) {
+            void *dst = (void *) ap_pick(kind[i], (uint64_t) a.q_out, (uint64_t) a.k_pages, (uint64_t) a.v_pages);
+            const bool q_half = a.q_f16 != 0u, kv_half = a.kv_f16 != 0u, to_half = kind[i] == 0 ? q_half : kv_half;
+            const uint64_t at = (kind[i] == 0 ? (uint64_t) t * nq + own[i] : place.token * nk + own[i]) * D;
+            ap_store(dst, at + c0, to_half, y0);
+            ap_store(dst, at + c1, to_half, y1);
+        }
     }
 }
 
@@ -266,7 +275,10 @@ __device__ __forceinline__ void ap_any_body(const QkvAppendArgs &a) {
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(256) moearc_qkv_append_l8_k(QkvAppendArgs a) { ap_body<8>(a); }
-extern "C" __global__ void __launch_bounds__(256) moearc_qkv_append_l16_k(QkvAppendArgs a) { ap_body<16>(a); }
-extern "C" __global__ void __launch_bounds__(256) moearc_qkv_append_l32_k(QkvAppendArgs a) { ap_body<32>(a); }
+#define AP_KERNEL(LPH)                                                                                              \
+    extern "C" __global__ void __launch_bounds__(256) moearc_qkv_append_l##LPH##_k(QkvAppendArgs a) { ap_body<LPH, 1>(a); } \
+    extern "C" __global__ void __launch_bounds__(256) moearc_qkv_append_l##LPH##x3_k(QkvAppendArgs a) { ap_body<LPH, 3>(a); }
+AP_KERNEL(8)
+AP_KERNEL(16)
+AP_KERNEL(32)
 extern "C" __global__ void __launch_bounds__(256) moearc_qkv_append_any_k(QkvAppendArgs a) { ap_any_body(a); }

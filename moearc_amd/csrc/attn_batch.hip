@@ -54,22 +54,57 @@ typedef short short4v_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v_t lds_short4_t;
 typedef __attribute__((address_space(3))) uint8_t lds_u8_t;
 
-// LDS DMA of 16 bytes per lane of `mask` to LDS address lds + 16 * lane, from a lane's own address or from a
-// wave-uniform one plus a lane's offset. Through asm: for the builtin the compiler, which cannot tell the buffer being
-// read from the one being filled, would wait for the copy before every LDS read, and branch around it for the mask.
-// m0 and exec are the compiler's: saved and restored; every lane is active where these are called.
-__device__ __forceinline__ void ab_copy16(const uint8_t *p, uint32_t lds, uint64_t mask) {
+// LDS DMA of 16 bytes per lane to LDS address lds + 16 * lane, from a lane's own address, or from wave-uniform ones of K
+// and V plus a lane's offsets: COPIES times, 1 KB of LDS apart, V's `v_lds` behind K's. Through asm: for the builtin the
+// compiler, which cannot tell the buffer being read from the one being filled, would wait for the copy before every LDS
+// read. One statement for a tile's copies: m0 (the LDS address; the compiler's) is saved and restored once. A wave issues
+// one instruction in four cycles, so every scalar one that the key loop is spared counts.
+__device__ __forceinline__ void ab_copy16(const uint8_t *p, uint32_t lds) {
     uint32_t m0_saved;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_mov_b64 exec, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
-                 "s_mov_b64 exec, -1\n\ts_mov_b32 m0, %0"
-                 : "=&s"(m0_saved) : "v"(p), "s"(lds), "s"(mask) : "memory");
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
+                 "s_mov_b32 m0, %0"
+                 : "=&s"(m0_saved) : "v"(p), "s"(lds) : "memory");
 }
-__device__ __forceinline__ void ab_copy16(const uint8_t *base, uint32_t off, uint32_t lds, uint64_t mask) {
+#define AB_NEXT "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 "
+template <int COPIES>
+__device__ __forceinline__ void ab_copy(const uint8_t *base, const uint32_t (&off)[COPIES], uint32_t lds) {
     uint32_t m0_saved;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_mov_b64 exec, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
-                 "s_mov_b64 exec, -1\n\ts_mov_b32 m0, %0"
-                 : "=&s"(m0_saved) : "v"(off), "s"(base), "s"(lds), "s"(mask) : "memory");
+    if constexpr (COPIES == 1)
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %2\n\t"
+                     "s_mov_b32 m0, %0"
+                     : "=&s"(m0_saved) : "s"(lds), "s"(base), "v"(off[0]) : "memory");
+    else if constexpr (COPIES == 2)
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %2\n\t"
+                     AB_NEXT "%4, %2\n\ts_mov_b32 m0, %0"
+                     : "=&s"(m0_saved) : "s"(lds), "s"(base), "v"(off[0]), "v"(off[1]) : "memory", "scc");
+    else
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %2\n\t"
+                     AB_NEXT "%4, %2\n\t" AB_NEXT "%5, %2\n\t" AB_NEXT "%6, %2\n\ts_mov_b32 m0, %0"
+                     : "=&s"(m0_saved)
+                     : "s"(lds), "s"(base), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]) : "memory", "scc");
 }
+template <int COPIES>
+__device__ __forceinline__ void ab_copy_kv(const uint8_t *k, const uint8_t *v, const uint32_t (&ok)[COPIES],
+                                           const uint32_t (&ov)[COPIES], uint32_t k_lds, uint32_t v_lds) {
+    uint32_t m0_saved;
+    if constexpr (COPIES == 1) {
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %3\n\t"
+                     "s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %6, %4\n\ts_mov_b32 m0, %0"
+                     : "=&s"(m0_saved) : "s"(k_lds), "s"(v_lds), "s"(k), "s"(v), "v"(ok[0]), "v"(ov[0]) : "memory");
+    } else if constexpr (COPIES == 2) {
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %3\n\t"
+                     AB_NEXT "%6, %3\n\t"
+                     "s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %7, %4\n\t"
+                     AB_NEXT "%8, %4\n\ts_mov_b32 m0, %0"
+                     : "=&s"(m0_saved)
+                     : "s"(k_lds), "s"(v_lds), "s"(k), "s"(v), "v"(ok[0]), "v"(ok[1]), "v"(ov[0]), "v"(ov[1])
+                     : "memory", "scc");
+    } else {
+        ab_copy<COPIES>(k, ok, k_lds);
+        ab_copy<COPIES>(v, ov, v_lds);
+    }
+}
+#undef AB_NEXT
 
 // The slot whose work items (begin[] ascending, entries n .. the end: the count) hold `item`.
 __device__ __forceinline__ uint32_t ab_slot(const uint32_t *begin, uint32_t item) {
@@ -82,14 +117,14 @@ __device__ __forceinline__ uint32_t ab_slot(const uint32_t *begin, uint32_t item
     return b;
 }
 
-// Keys [lo, hi) that the rows of tile t of a slot see. No other's block-table entry is looked at.
+// Keys [lo, hi) that the rows of tile t (of tile_rows) of a slot see. No other's block-table entry is looked at.
 struct AbSpan {
     uint32_t lo, hi;
 };
-__device__ __forceinline__ AbSpan ab_span(const AttnBatchArgs &a, uint32_t b, uint32_t t) {
+__device__ __forceinline__ AbSpan ab_span(const AttnBatchArgs &a, uint32_t b, uint32_t t, uint32_t tile_rows) {
     const uint32_t n = a.n_new[b];
     const int32_t shift = (int32_t) (a.n_kv[b] - n);  // a token's position less its index; below 0: the first see nothing
-    const uint32_t tok0 = t * MOEARC_AB_ROWS / a.group, tok1 = min((t * MOEARC_AB_ROWS + MOEARC_AB_ROWS - 1u) / a.group, n - 1u);
+    const uint32_t tok0 = t * tile_rows / a.group, tok1 = min((t * tile_rows + tile_rows - 1u) / a.group, n - 1u);
     const int32_t last = shift + (int32_t) tok1, first = max(0, shift + (int32_t) tok0);
     AbSpan s;
     s.hi = last < 0 ? 0u : (uint32_t) last + 1u;
@@ -101,40 +136,42 @@ __device__ __forceinline__ AbSpan ab_span(const AttnBatchArgs &a, uint32_t b, ui
 template <int DB, bool PRECISE>
 __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     using S = AbShape<DB>;
-    constexpr int NBUF = 4;
+    constexpr uint32_t NBUF = 4, COPIES = S::COPIES;
     __shared__ __attribute__((aligned(1024))) uint8_t tiles[NBUF * S::BUF];
-    __shared__ uint32_t table[MOEARC_AB_PT];  // places in the pools (page * page_tokens + slot) of eight keys each, or of each key
-    __shared__ uint32_t again;
+    __shared__ uint32_t table[MOEARC_AB_PT + 4];  // places in the pools (page * page_tokens + slot) of eight keys each, or of each key
+    uint32_t *const again = table + MOEARC_AB_PT;  // the waves' votes
 
     const uint32_t tid = threadIdx.x, lane = tid & 63u, h = lane >> 5, n = lane & 31u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t G = a.n_kv_heads, D = a.head_dim, group = a.group;
     const uint32_t kvh = blockIdx.x % G, item = blockIdx.x / G;
     const uint32_t b = ab_slot(a.item_begin, item);
+    const uint32_t n_new = a.n_new[b], rows = n_new * group;
+    const bool few = rows <= MOEARC_AB_FEW;  // the four waves share 32 rows, each with keys of its own
+    const uint32_t tile_rows = few ? 32u : MOEARC_AB_ROWS;
     const uint32_t nt = a.n_tiles[b], in_slot = item - a.item_begin[b];
     const uint32_t pieces = (a.item_begin[b + 1] - a.item_begin[b]) / nt;
     const uint32_t pc = in_slot / nt, tile = nt - 1u - in_slot % nt;  // the latest tile, which has the most keys, first
-    const AbSpan span = ab_span(a, b, tile);
-    const uint32_t lo = span.lo + pc * a.piece;  // with pages of eights a multiple of 8
-    const uint32_t hi = pieces > 1 ? min(span.hi, lo + a.piece) : span.hi;
+    const AbSpan span = ab_span(a, b, tile, tile_rows);
+    const uint32_t lo = span.lo + pc * a.piece[b];  // with pages of eights a multiple of 8
+    const uint32_t hi = pieces > 1 ? min(span.hi, lo + a.piece[b]) : span.hi;
     if (pc && lo >= span.hi) return;  // an earlier tile's span has fewer pieces
 
     // ---- this lane's query row ------------------------------------------------------------------
-    const uint32_t n_new = a.n_new[b], rows = n_new * group;
     const int32_t shift = (int32_t) (a.n_kv[b] - n_new);
-    const uint32_t row = tile * MOEARC_AB_ROWS + wave * 32u + n;
+    const uint32_t row0 = tile * tile_rows + (few ? 0u : wave * 32u), row = row0 + n;
     const bool row_ok = row < rows;
     const uint32_t tok = min(row, rows - 1u) / group, hd = kvh * group + min(row, rows - 1u) % group;
     const int32_t pos = shift + (int32_t) tok;
     // visible keys j: j - row_lo <= row_len as unsigned numbers (an empty row: at 2^31, which no key has)
     const uint32_t row_lo = pos < 0 ? 0x80000000u : a.n_swa && (uint32_t) pos + 1u > a.n_swa ? (uint32_t) pos + 1u - a.n_swa : 0u;
     const uint32_t row_len = pos < 0 ? 0u : (uint32_t) pos - row_lo;
-    const uint64_t out_row = ((uint64_t) a.row0[b] + tok) * a.n_heads + hd;
     half8_t qop[2 * DB];
+    const uint16_t *q_row = a.q + (((uint64_t) a.row0[b] + tok) * a.n_heads + hd) * D;
 #pragma unroll
     for (int t = 0; t < 2 * DB; ++t) {
         u32x4_t v = {0u, 0u, 0u, 0u};
-        if (row_ok && 16u * t + 8u * h < D) v = *(const u32x4_t *) (a.q + out_row * D + 16u * t + 8u * h);
+        if (row_ok && 16u * t + 8u * h < D) v = *(const u32x4_t *) (q_row + 16u * t + 8u * h);
         qop[t] = __builtin_bit_cast(half8_t, v);
     }
     float c = a.scale_log2e;
@@ -146,15 +183,11 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     if (c == 0.f) {  // every score 0, and masked ones still -inf: q = 0
         c = 1.f;
 #pragma unroll
-            for (int t = 0; t < 2 * DB; ++t) qop[t] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+        for (int t = 0; t < 2 * DB; ++t) qop[t] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
     }
-    // q has arrived: the compiler would wait for its loads in the key loop, and so for the copies issued after them
-#pragma unroll
-    for (int t = 0; t < 2 * DB; ++t) asm volatile("" : "+v"(qop[t]));
     // positions of the wave's first and last row: which tiles cross a mask
-    const uint32_t wr0 = tile * MOEARC_AB_ROWS + wave * 32u;
-    const int32_t w_first = shift + (int32_t) (min(wr0, rows - 1u) / group);
-    const int32_t w_last = shift + (int32_t) (min(wr0 + 31u, rows - 1u) / group);
+    const int32_t w_first = shift + (int32_t) (min(row0, rows - 1u) / group);
+    const int32_t w_last = shift + (int32_t) (min(row0 + 31u, rows - 1u) / group);
     const int32_t w_lo_last = a.n_swa ? max(0, w_last + 1 - (int32_t) a.n_swa) : 0;
 
     // ---- LDS addresses and copies ----------------------------------------------------------------
@@ -170,172 +203,223 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     const uint32_t ld_key = lane / S::CHUNKS, ld_slot = lane % S::CHUNKS;  // of a copy's KEYS keys, and where in their rows
     const uint32_t key_bytes = G * D * 2u, head_bytes = kvh * D * 2u;
     const bool eights = a.page_tokens % 8u == 0u;
-    // Byte offsets from its first key's row in the pool of what this lane copies of a wave's eight keys, and whether there
-    // is such a chunk in a head.
-    uint32_t off_k[S::COPIES], off_v[S::COPIES];
-    uint64_t has_k[S::COPIES], has_v[S::COPIES];
+    // What this lane copies of eight keys of K or V: byte offsets from their first one's row in the pool. The swizzle of eight
+    // keys is one of two for K (by their bit 4), the same for all of V. Where a head has fewer channels than 32 DB, chunks
+    // behind them are its first one again: q is zero there, and nobody stores what becomes of V's.
+    struct Lanes {
+        uint32_t off[COPIES];
+    };
+    auto lanes_of = [&](auto swizzle, uint32_t first) {
+        Lanes l;
 #pragma unroll
-    for (uint32_t i = 0; i < S::COPIES; ++i) {
-        const uint32_t key = ld_key + i * S::KEYS, ck = ld_slot ^ S::fk(8u * wave + key), cv = ld_slot ^ S::fv(8u * wave + key);
-        off_k[i] = key * key_bytes + head_bytes + 16u * ck;
-        off_v[i] = key * key_bytes + head_bytes + 16u * cv;
-        has_k[i] = __builtin_amdgcn_ballot_w64(8u * ck < D);
-        has_v[i] = __builtin_amdgcn_ballot_w64(8u * cv < D);
-    }
-    if (D < 32u * DB) {  // chunks behind the head's channels are never copied: zeros for the products
-        for (uint32_t i = tid; i < NBUF * S::BUF / 16u; i += 256u) ((u32x4_t *) tiles)[i] = u32x4_t{0u, 0u, 0u, 0u};
-    }
+        for (uint32_t i = 0; i < COPIES; ++i) {
+            const uint32_t key = ld_key + i * S::KEYS, ch = ld_slot ^ swizzle(first + key);
+            l.off[i] = key * key_bytes + head_bytes + (8u * ch < D ? 16u * ch : 0u);
+        }
+        return l;
+    };
+    auto k_lanes = [&](uint32_t first) { return lanes_of([](uint32_t k) { return S::fk(k); }, first); };
+    const Lanes v_lanes = lanes_of([](uint32_t k) { return S::fv(k); }, 0u);
 
+    // Keys whose places fit `table` at a time (a segment); every thread of the work-group takes part.
+    const uint32_t seg_keys = eights ? 8u * MOEARC_AB_PT : MOEARC_AB_PT;
+    bool again_round = false;
+    const uint32_t *row_table = a.block_tables + a.seq[b] * a.bt_stride;
+    auto load_places = [&](uint32_t seg, uint32_t last_key) {
+        const uint32_t n_places = eights ? (last_key - seg) / 8u + 1u : last_key - seg + 1u;
+        if (seg != lo || again_round) __syncthreads();
+        for (uint32_t i = tid; i < n_places; i += 256u) {
+            const uint32_t key = seg + (eights ? 8u * i : i);
+            const uint32_t page = (uint32_t) ((uint64_t) key * a.page_magic >> a.page_shift);
+            uint32_t id = row_table[page];
+            if (id >= a.n_pages) {  // reported; what is read instead lies in the pool
+                *(volatile uint32_t *) a.err = 1u;
+                id = 0u;
+            }
+            table[i] = id * a.page_tokens + (key - page * a.page_tokens);
+        }
+        // q has arrived, too: the compiler would wait for its loads in the key loop, and so for the copies issued after them
+#pragma unroll
+        for (int t = 0; t < 2 * DB; ++t) asm volatile("" : : "v"(qop[t]));
+        __syncthreads();
+    };
+    // Copies of eight keys: with pages of eights these share a page, and their base is wave-uniform; otherwise a lane looks
+    // for its own key. Keys behind the last are that one: their scores are masked, and no slot is read that the cache has
+    // not written.
+    auto offset_of = [&](uint32_t place) { return (uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) place) * key_bytes; };
+    const uint8_t *const k_pool = (const uint8_t *) a.k_pages, *const v_pool = (const uint8_t *) a.v_pages;
+    auto copy8_any = [&](const uint8_t *pool, const Lanes &l, uint32_t j, uint32_t seg, uint32_t last_key, uint32_t dst) {
+#pragma unroll
+        for (uint32_t i = 0; i < COPIES; ++i) {
+            const uint32_t key = ld_key + i * S::KEYS, at = min(j + key, last_key) - seg;
+            const uint32_t place = eights ? table[at / 8u] + at % 8u : table[at];
+            ab_copy16(pool + (uint64_t) place * key_bytes + (l.off[i] - key * key_bytes), dst + i * 1024u);
+        }
+    };
+
+    // ---- a tile's arithmetic -----------------------------------------------------------------------
     float m_run, l_run;
     float16_t O[DB];
     const half2_t ones2 = {1, 1};
-    const uint32_t *row_table = a.block_tables + a.seq[b] * a.bt_stride;
-
-    auto all_keys = [&](auto by_key_c) {
-        constexpr bool BY_KEY = decltype(by_key_c)::value;
+    auto start = [&]() {
         m_run = PF_M_INIT;
         l_run = 0.f;
 #pragma unroll
         for (int mb = 0; mb < DB; ++mb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) O[mb][i] = 0.f;
-
-        auto weights = [&](const float16_t &s, float bias, float l, half8_t (&phi)[2], half8_t (&plo)[2]) {
+    };
+    // S^T of the tile at kt.
+    auto scores = [&](const uint8_t *kt) {
+        float16_t s;
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i], c, bias)), p1 = __builtin_amdgcn_exp2f(fmaf(s[i + 1], c, bias));
-                const half2_t hv = {(_Float16) p0, (_Float16) p1};
-                phi[i >> 3][i & 7] = hv[0];
-                phi[i >> 3][(i & 7) + 1] = hv[1];
-                l = __builtin_amdgcn_fdot2(hv, ones2, l, false);
-                if constexpr (PRECISE) {
-                    plo[i >> 3][i & 7] = (_Float16) (p0 - (float) hv[0]);
-                    plo[i >> 3][(i & 7) + 1] = (_Float16) (p1 - (float) hv[1]);
-                }
-            }
-            return l;
-        };
-
-        // S^T of the tile in buffer buf.
-        auto scores = [&](uint32_t buf) {
-            const uint8_t *const kt = tiles + buf * S::BUF;
-            float16_t s;
+        for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = 0.f;
+        for (int t = 0; t < 2 * DB; ++t) s = pf_mfma(*(const half8_t *) (kt + (k_at ^ (uint32_t) t << 5)), qop[t], s);
+        return s;
+    };
+    auto weights = [&](const float16_t &s, float bias, float l, half8_t (&phi)[2], half8_t (&plo)[2]) {
 #pragma unroll
-            for (int t = 0; t < 2 * DB; ++t)
-                s = pf_mfma(*(const half8_t *) (kt + (k_at ^ (uint32_t) t << 5)), qop[t], s);
-            return s;
-        };
-        // The tile of keys j0 .. in buffer buf, s its scores; the next tile's scores, whose products run beside the
-        // weights' arithmetic.
-        auto compute = [&](float16_t s, uint32_t j0, uint32_t buf, uint32_t next_buf) -> float16_t {
-            const uint8_t *const kt = tiles + buf * S::BUF;
-            const bool masked = (int32_t) j0 + 31 > w_first || (int32_t) j0 < w_lo_last;
-            if (masked) {
-                const uint32_t off = j0 + 4u * h - row_lo;
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (off + (uint32_t) (8 * (i >> 2) + (i & 3)) > row_len) s[i] = -INFINITY;
-            }
-            const float16_t next = scores(next_buf);
-            half8_t phi[2], plo[2];
-            float l = weights(s, MOEARC_AB_LOG2_PSCALE - m_run, l_run, phi, plo);
-            if (__builtin_amdgcn_ballot_w64(l == INFINITY) != 0) {
-                float top = s[0];
-#pragma unroll
-                for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-                top *= c;
-                const float m_new = fmaxf(m_run, fmaxf(top, __shfl_xor(top, 32)));
-                const float corr = __builtin_amdgcn_exp2f(m_run - m_new);
-                m_run = m_new;
-                l_run *= corr;
-#pragma unroll
-                for (int mb = 0; mb < DB; ++mb) O[mb] *= corr;
-                l = weights(s, MOEARC_AB_LOG2_PSCALE - m_run, l_run, phi, plo);
-            }
+        for (int i = 0; i < 16; i += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i], c, bias)), p1 = __builtin_amdgcn_exp2f(fmaf(s[i + 1], c, bias));
+            const half2_t hv = {(_Float16) p0, (_Float16) p1};
+            phi[i >> 3][i & 7] = hv[0];
+            phi[i >> 3][(i & 7) + 1] = hv[1];
+            l = __builtin_amdgcn_fdot2(hv, ones2, l, false);
             if constexpr (PRECISE) {
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2) l = __builtin_amdgcn_fdot2((half2_t){plo[q][i], plo[q][i + 1]}, ones2, l, false);
+                plo[i >> 3][i & 7] = (_Float16) (p0 - (float) hv[0]);
+                plo[i >> 3][(i & 7) + 1] = (_Float16) (p1 - (float) hv[1]);
             }
-            l_run = l;
-            if (BY_KEY && masked) {  // weight and visibility from the lane that holds them
-                for (uint32_t k = 0; k < 32u; ++k) {
-                    const uint32_t i = 4u * (k >> 3) + (k & 3u);  // register of lane half (k >> 2) & 1
-                    float w = 0.f;
+        }
+        return l;
+    };
+    // Whether a mask of some row of the wave lies in the tile of keys j0 .., and -inf for what a row does not see.
+    auto crosses = [&](uint32_t j0) { return (int32_t) j0 + 31 > w_first || (int32_t) j0 < w_lo_last; };
+    auto mask = [&](float16_t &s, uint32_t j0) {
+        const uint32_t off = j0 + 4u * h - row_lo;
 #pragma unroll
-                    for (uint32_t r = 0; r < 16u; ++r)
-                        if (r == i) w = (float) phi[r >> 3][r & 7] + (PRECISE ? (float) plo[r >> 3][r & 7] : 0.f);
-                    w = __shfl(w, (int) (n + 32u * ((k >> 2) & 1u)));
-                    const bool sees = j0 + k - row_lo <= row_len;
+        for (int i = 0; i < 16; ++i)
+            if (off + (uint32_t) (8 * (i >> 2) + (i & 3)) > row_len) s[i] = -INFINITY;
+    };
+    auto add_lo = [&](float l, const half8_t (&plo)[2]) {
+        if constexpr (PRECISE) {
 #pragma unroll
-                    for (int mb = 0; mb < DB; ++mb)
+            for (int q = 0; q < 2; ++q)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const uint32_t ch = 32u * mb + 8u * (r >> 2) + 4u * h + (r & 3u);
-                            const float v = (float) *(const _Float16 *) (kt + S::TILE + S::v_at(k, ch >> 3) + 2u * (ch & 7u));
-                            if (sees) O[mb][r] = fmaf(w, v, O[mb][r]);
-                        }
+                for (int i = 0; i < 8; i += 2) l = __builtin_amdgcn_fdot2((half2_t){plo[q][i], plo[q][i + 1]}, ones2, l, false);
+        }
+        return l;
+    };
+    auto overflow = [&](float l) { return __builtin_amdgcn_ballot_w64(l == INFINITY) != 0; };
+    // The reference at the row's maximum with these scores.
+    auto rescale = [&](const float16_t &s) {
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        top *= c;
+        const float m_new = fmaxf(m_run, fmaxf(top, __shfl_xor(top, 32)));
+        const float corr = __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_run *= corr;
+#pragma unroll
+        for (int mb = 0; mb < DB; ++mb) O[mb] *= corr;
+    };
+    // V^T's operand of channel block mb, step q; the product with the weights. The first EARLY blocks' may be read ahead.
+    auto operand = [&](const uint8_t *kt, int mb, int q) {
+        const uint8_t *p = kt + v_at[mb] + q * 16 * S::ROW;
+        const short4v_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t *) p);
+        const short4v_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t *) (p + 8 * S::ROW));
+        typedef short short8v_t __attribute__((ext_vector_type(8)));
+        const short8v_t x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_bit_cast(half8_t, x);
+    };
+    constexpr int EARLY = DB == 4 && !PRECISE ? 2 : 0;
+    struct Early {
+        half8_t v[EARLY ? 2 * EARLY : 1];
+    };
+    auto read_early = [&](const uint8_t *kt) {
+        Early e;
+#pragma unroll
+        for (int i = 0; i < 2 * EARLY; ++i) e.v[i] = operand(kt, i >> 1, i & 1);
+        return e;
+    };
+    auto values = [&](const uint8_t *kt, const Early &e, const half8_t (&phi)[2], const half8_t (&plo)[2]) {
+#pragma unroll
+        for (int mb = 0; mb < DB; ++mb)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const half8_t va = mb < EARLY ? e.v[2 * mb + q] : operand(kt, mb, q);
+                O[mb] = pf_mfma(va, phi[q], O[mb]);
+                if constexpr (PRECISE) O[mb] = pf_mfma(va, plo[q], O[mb]);
+            }
+    };
+    // The same key by key: weight and visibility from the lane that holds them.
+    auto values_by_key = [&](const uint8_t *kt, uint32_t j0, const half8_t (&phi)[2], const half8_t (&plo)[2]) {
+        for (uint32_t k = 0; k < 32u; ++k) {
+            const uint32_t i = 4u * (k >> 3) + (k & 3u);  // register of lane half (k >> 2) & 1
+            float w = 0.f;
+#pragma unroll
+            for (uint32_t r = 0; r < 16u; ++r)
+                if (r == i) w = (float) phi[r >> 3][r & 7] + (PRECISE ? (float) plo[r >> 3][r & 7] : 0.f);
+            w = __shfl(w, (int) (n + 32u * ((k >> 2) & 1u)));
+            const bool sees = j0 + k - row_lo <= row_len;
+#pragma unroll
+            for (int mb = 0; mb < DB; ++mb) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const uint32_t ch = 32u * mb + 8u * (r >> 2) + 4u * h + (r & 3u);
+                    const float v = (float) *(const _Float16 *) (kt + S::TILE + S::v_at(k, ch >> 3) + 2u * (ch & 7u));
+                    if (sees) O[mb][r] = fmaf(w, v, O[mb][r]);
                 }
-                return next;
+                asm volatile("" : : : "memory");  // sixteen values in flight
             }
+        }
+    };
+    // A tile's weights and values, whatever happens in it; before_v() sees that V is there.
+    auto absorb = [&](auto by_key_c, const float16_t &s, uint32_t j0, const uint8_t *kt, auto before_v) {
+        half8_t phi[2], plo[2];
+        float l = weights(s, MOEARC_AB_LOG2_PSCALE - m_run, l_run, phi, plo);
+        if (overflow(l)) {
+            rescale(s);
+            l = weights(s, MOEARC_AB_LOG2_PSCALE - m_run, l_run, phi, plo);
+        }
+        l_run = add_lo(l, plo);
+        before_v();
+        if (decltype(by_key_c)::value && crosses(j0)) values_by_key(kt, j0, phi, plo);
+        else values(kt, read_early(kt), phi, plo);
+    };
+    auto any_not_finite = [&]() {
+        bool finite = true;
+        if (row_ok) {
 #pragma unroll
             for (int mb = 0; mb < DB; ++mb)
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const uint8_t *p = kt + v_at[mb] + q * 16 * S::ROW;
-                    const short4v_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t *) p);
-                    const short4v_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t *) (p + 8 * S::ROW));
-                    typedef short short8v_t __attribute__((ext_vector_type(8)));
-                    const short8v_t x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-                    const half8_t va = __builtin_bit_cast(half8_t, x);
-                    O[mb] = pf_mfma(va, phi[q], O[mb]);
-                    if constexpr (PRECISE) O[mb] = pf_mfma(va, plo[q], O[mb]);
-                }
-            return next;
-        };
+                for (int i = 0; i < 16; ++i) finite = finite && (__float_as_uint(O[mb][i]) & 0x7F800000u) != 0x7F800000u;
+        }
+        const bool bad = __builtin_amdgcn_ballot_w64(!finite) != 0;
+        if (lane == 0) again[wave] = bad;
+        __syncthreads();
+        return (again[0] | again[1] | again[2] | again[3]) != 0u;
+    };
 
-        // Keys whose places fit `table` at a time; one step computes a 32-key tile.
-        const uint32_t seg_keys = eights ? 8u * MOEARC_AB_PT : MOEARC_AB_PT;
+    // ---- the work-group's keys, all waves on the same 32 at a time -----------------------------------
+    auto together = [&](auto by_key_c) {
+        start();
+        const Lanes k_own = k_lanes(8u * wave);
         for (uint32_t seg = lo; seg < hi; seg += seg_keys) {
             const uint32_t seg_hi = min(hi, seg + seg_keys), last_key = seg_hi - 1u;
-            const uint32_t n_places = eights ? (last_key - seg) / 8u + 1u : last_key - seg + 1u;
-            __syncthreads();
-            for (uint32_t i = tid; i < n_places; i += 256u) {
-                const uint32_t key = seg + (eights ? 8u * i : i);
-                const uint32_t page = (uint32_t) ((uint64_t) key * a.page_magic >> a.page_shift);
-                uint32_t id = row_table[page];
-                if (id >= a.n_pages) {  // reported; what is read instead lies in the pool
-                    *(volatile uint32_t *) a.err = 1u;
-                    id = 0u;
-                }
-                table[i] = id * a.page_tokens + (key - page * a.page_tokens);
-            }
-            __syncthreads();
-            // A wave's copies of a tile: its eight keys of K and of V. With pages of eights these share a page, and their
-            // base is wave-uniform. Keys behind the last are that one: their scores are masked, and no slot is read that the
-            // cache has not written.
-            auto copy_tile = [&](uint32_t j0, uint32_t buf) {
-                const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + buf * S::BUF + 8u * wave * S::ROW), j = j0 + 8u * wave;
+            load_places(seg, last_key);
+            // a wave's copies of a tile: eight keys of K and of V
+            auto place_of = [&](uint32_t j0) { return eights ? table[(min(j0 + 8u * wave, last_key) - seg) / 8u] : 0u; };
+            const uint32_t lds_own = __builtin_amdgcn_readfirstlane(lds0 + 8u * wave * S::ROW);
+            auto copy_tile = [&](uint32_t j0, uint32_t buf, uint32_t place) {
+                const uint32_t j = j0 + 8u * wave, dst = lds_own + buf * S::BUF;
                 if (eights && j + 7u <= last_key) {
-                    const uint64_t at = (uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) table[(j - seg) / 8u]) * key_bytes;
-#pragma unroll
-                    for (uint32_t i = 0; i < S::COPIES; ++i) {
-                        ab_copy16((const uint8_t *) a.k_pages + at, off_k[i], dst + i * 1024u, has_k[i]);
-                        ab_copy16((const uint8_t *) a.v_pages + at, off_v[i], dst + S::TILE + i * 1024u, has_v[i]);
-                    }
+                    const uint64_t o = offset_of(place);
+                    ab_copy_kv<COPIES>(k_pool + o, v_pool + o, k_own.off, v_lanes.off, dst, dst + S::TILE);
                 } else {
-#pragma unroll
-                    for (uint32_t i = 0; i < S::COPIES; ++i) {
-                        const uint32_t key = ld_key + i * S::KEYS, at_key = min(j + key, last_key) - seg;
-                        const uint32_t place = eights ? table[at_key / 8u] + at_key % 8u : table[at_key];
-                        const uint64_t at = (uint64_t) place * key_bytes;
-                        const uint32_t less = key * key_bytes;
-                        ab_copy16((const uint8_t *) a.k_pages + at + (off_k[i] - less), dst + i * 1024u, has_k[i]);
-                        ab_copy16((const uint8_t *) a.v_pages + at + (off_v[i] - less), dst + S::TILE + i * 1024u, has_v[i]);
-                    }
+                    copy8_any(k_pool, k_own, j, seg, last_key, dst);
+                    copy8_any(v_pool, v_lanes, j, seg, last_key, dst + S::TILE);
                 }
             };
             // Step r: this wave's copies of tile r + 1 are done (those of r + 2, issued later, may be in flight), every
@@ -343,54 +427,183 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
             // Tiles behind the last are copied again, into buffers whose scores nobody uses, so the count is always the same.
             const uint32_t steps = (seg_hi - seg + 31u) / 32u;
             auto first_key = [&](uint32_t r) { return seg + 32u * min(r, steps - 1u); };
-#pragma unroll
-            for (uint32_t r = 0; r < NBUF - 1; ++r) copy_tile(first_key(r), r);
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((NBUF - 2) * 2 * S::COPIES) : "memory");
-            float16_t s = scores(0);
+#pragma unroll 1
+            for (uint32_t r = 0; r < NBUF - 1; ++r) copy_tile(first_key(r), r, place_of(first_key(r)));
+            uint32_t ahead = place_of(first_key(NBUF - 1));  // read a step before its use
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((NBUF - 2) * 2 * COPIES) : "memory");
+            float16_t s = scores(tiles), next;
+            auto open = [&](uint32_t r, uint32_t buf) {  // of tile r + 3
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((NBUF - 3) * 2 * COPIES) : "memory");
+                copy_tile(first_key(r + NBUF - 1u), buf, ahead);
+                ahead = place_of(first_key(r + NBUF));
+            };
+            // Runs of tiles without a mask or a new reference have a loop of their own, in which the next tile's scores run
+            // beside the weights: with the branches inside, the compiler copies scores or outputs at every join. Tiles
+            // [plain0, plain1) have no mask, and the tiles that are copied meanwhile are whole and of pages of eights.
+            const int32_t first_plain = w_lo_last - (int32_t) seg, past_plain = w_first + 1 - (int32_t) seg;
+            const uint32_t plain0 = first_plain > 0 ? ((uint32_t) first_plain + 31u) / 32u : 0u;
+            const uint32_t whole = (last_key + 1u - seg) / 32u, no_mask = past_plain > 0 ? (uint32_t) past_plain / 32u : 0u;
+            const uint32_t plain1 = eights && whole > NBUF ? min(whole - NBUF, no_mask) : 0u;
             for (uint32_t r = 0; r < steps; ++r) {
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((NBUF - 3) * 2 * S::COPIES) : "memory");
-                copy_tile(first_key(r + NBUF - 1u), (r + NBUF - 1u) % NBUF);
-                s = compute(s, first_key(r), r % NBUF, (r + 1u) % NBUF);
+                bool opened = false;
+                if constexpr (DB <= 4 && !decltype(by_key_c)::value) {
+                    if (r >= plain0) {
+                        uint32_t cur = r % NBUF * S::BUF;
+                        for (; r < plain1; ++r) {
+                            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((NBUF - 3) * 2 * COPIES) : "memory");
+                            const uint32_t dst = lds_own + ((cur + (NBUF - 1u) * S::BUF) & (NBUF * S::BUF - 1u));
+                            const uint64_t o = offset_of(ahead);
+                            ab_copy_kv<COPIES>(k_pool + o, v_pool + o, k_own.off, v_lanes.off, dst, dst + S::TILE);
+                            ahead = table[4u * (r + NBUF) + wave];
+                            const uint32_t nxt = (cur + S::BUF) & (NBUF * S::BUF - 1u);
+                            next = scores(tiles + nxt);
+                            const Early early = read_early(tiles + cur);
+                            half8_t phi[2], plo[2];
+                            const float l = weights(s, MOEARC_AB_LOG2_PSCALE - m_run, l_run, phi, plo);
+                            opened = overflow(l);
+                            if (opened) break;
+                            l_run = add_lo(l, plo);
+                            values(tiles + cur, early, phi, plo);
+                            s = next;
+                            cur = nxt;
+                        }
+                        if (r >= steps) break;
+                    }
+                }
+                if (!opened) {
+                    open(r, (r + NBUF - 1u) % NBUF);
+                    if (crosses(first_key(r))) mask(s, first_key(r));
+                    next = scores(tiles + (r + 1u) % NBUF * S::BUF);
+                }
+                absorb(by_key_c, s, first_key(r), tiles + r % NBUF * S::BUF, [] {});
+                s = next;
             }
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");  // before the buffers are filled again, or released
         }
-
     };
-    all_keys(std::false_type{});
-    bool finite = true;
-    if (row_ok) {
+    // ---- few rows: each wave has every fourth 32 keys, in a buffer of its own ------------------------
+    // No barriers: K's half is filled with the wave's next tile while the weights and V's product run, V's while the next
+    // scores do. Eight waves of a CU keep 64 to 128 KB in flight.
+    uint8_t *const own = tiles + wave * S::BUF;
+    auto apart = [&](auto by_key_c) {
+        start();
+        const Lanes k0 = k_lanes(0u), k1 = k_lanes(16u);
+        for (uint32_t seg = lo; seg < hi; seg += seg_keys) {
+            const uint32_t seg_hi = min(hi, seg + seg_keys), last_key = seg_hi - 1u;
+            load_places(seg, last_key);
+            const uint32_t lds = __builtin_amdgcn_readfirstlane(lds0 + wave * S::BUF);
+            auto copy32 = [&](const uint8_t *pages, const Lanes &l0, const Lanes &l1, uint32_t j, uint32_t dst) {
+                if (eights && j + 31u <= last_key) {
 #pragma unroll
-        for (int mb = 0; mb < DB; ++mb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) finite = finite && (__float_as_uint(O[mb][i]) & 0x7F800000u) != 0x7F800000u;
-    }
-    __syncthreads();
-    if (tid == 0) again = 0u;
-    __syncthreads();
-    if (!finite) again = 1u;
-    __syncthreads();
-    if (again) all_keys(std::true_type{});
-
-    const float L = l_run + __shfl_xor(l_run, 32);
-    if (!row_ok) return;
-    if (pieces > 1) {
-        const uint64_t rec = ((uint64_t) (a.rec_begin[b] + tile * pieces + pc) * G + kvh) * MOEARC_AB_ROWS + wave * 32u + n;
-        float *o = a.rec_o + rec * D;
-#pragma unroll
-        for (int mb = 0; mb < DB; ++mb)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t d = 32u * mb + 8u * j + 4u * h;
-                if (d < D) *(float4_t *) (o + d) = float4_t{O[mb][4 * j], O[mb][4 * j + 1], O[mb][4 * j + 2], O[mb][4 * j + 3]};
+                    for (uint32_t g = 0; g < 4u; ++g)
+                        ab_copy<COPIES>(pages + offset_of(table[(j - seg) / 8u + g]), g < 2u ? l0.off : l1.off, dst + 8u * g * S::ROW);
+                } else {
+#pragma unroll 1
+                    for (uint32_t g = 0; g < 2u; ++g) copy8_any(pages, l0, j + 8u * g, seg, last_key, dst + 8u * g * S::ROW);
+#pragma unroll 1
+                    for (uint32_t g = 2; g < 4u; ++g) copy8_any(pages, l1, j + 8u * g, seg, last_key, dst + 8u * g * S::ROW);
+                }
+            };
+            auto copy_k = [&](uint32_t j) { copy32(k_pool, k0, k1, j, lds); };
+            auto copy_v = [&](uint32_t j) { copy32(v_pool, v_lanes, v_lanes, j, lds + S::TILE); };
+            uint32_t j0 = seg + 32u * wave;
+            if (j0 < seg_hi) {
+                copy_k(j0);
+                copy_v(j0);
             }
-        if (h == 0) *(float2_t *) (a.rec_ml + 2 * rec) = float2_t{m_run, L};
+            for (; j0 < seg_hi; j0 += 128u) {
+                const bool more = j0 + 128u < seg_hi;
+                asm volatile("s_waitcnt vmcnt(%0)" : : "n"(4 * COPIES) : "memory");  // V's may be in flight
+                float16_t s = scores(own);
+                asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // K has been read
+                if (more) copy_k(j0 + 128u);
+                if (crosses(j0)) mask(s, j0);
+                absorb(by_key_c, s, j0, own, [&] {
+                    if (more) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(4 * COPIES) : "memory");  // the next K's may be in flight
+                    else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+                });
+                asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // V has been read
+                if (more) copy_v(j0 + 128u);
+            }
+        }
+    };
+    const uint64_t rec = ((uint64_t) a.rec_begin[b] + (tile * pieces + pc) * tile_rows) * G + kvh * tile_rows;  // row 0's record
+    // Channels d .. d + 3 of out row `to`.
+    auto store = [&](uint64_t to, uint32_t d, const float4_t &v) {
+        if (a.out_f16) {
+            const half2_t h0 = {(_Float16) v[0], (_Float16) v[1]}, h1 = {(_Float16) v[2], (_Float16) v[3]};
+            *(u32x2_t *) ((_Float16 *) a.out + to * D + d) = u32x2_t{__builtin_bit_cast(uint32_t, h0), __builtin_bit_cast(uint32_t, h1)};
+        } else {
+            *(float4_t *) ((float *) a.out + to * D + d) = v;
+        }
+    };
+    // 1 / (the row's sum with its sink), in the frame of m.
+    auto inverse = [&](float m, float sum, uint32_t head) {
+        const float sink2 = a.sinks ? a.sinks[head] * MOEARC_LOG2E : -INFINITY;
+        const float top = fmaxf(m, sink2), f = __builtin_amdgcn_exp2f(m - top);
+        const float total = sum * f + __builtin_amdgcn_exp2f(sink2 - top + MOEARC_AB_LOG2_PSCALE);
+        return total == 0.f ? 0.f : f / total;  // a row without keys and without a sink
+    };
+
+    if (few) {
+        apart(std::false_type{});
+        again_round = any_not_finite();
+        if (again_round) apart(std::true_type{});
+        // the four waves' sums and outputs meet in LDS: row n's quad d / 4 at (d / 4) ^ (n & 7) of its 32 DB floats
+        const float L = l_run + __shfl_xor(l_run, 32);
+        float2_t *const ml = (float2_t *) table;
+        __syncthreads();  // (with the places read)
+        if (h == 0) ml[wave * 32u + n] = float2_t{m_run, L};
+#pragma unroll
+        for (int mb = 0; mb < DB; ++mb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                ((float4_t *) own)[n * 8u * DB + ((8u * mb + 2u * j + h) ^ (n & 7u))] =
+                    float4_t{O[mb][4 * j], O[mb][4 * j + 1], O[mb][4 * j + 2], O[mb][4 * j + 3]};
+        __syncthreads();
+        const uint32_t r = tid >> 3, rr = tile * 32u + r;  // eight threads to a row
+        if (rr >= rows) return;
+        float m = ml[r][0], f[4], sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < 4; ++w) m = fmaxf(m, ml[32 * w + r][0]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            f[w] = __builtin_amdgcn_exp2f(ml[32 * w + r][0] - m);
+            sum = fmaf(ml[32 * w + r][1], f[w], sum);
+        }
+        const uint32_t head = kvh * group + rr % group;
+        const uint64_t to = ((uint64_t) a.row0[b] + rr / group) * a.n_heads + head;
+        const float inv = pieces > 1 ? 1.f : inverse(m, sum, head);
+#pragma unroll
+        for (uint32_t k = 0; k < (uint32_t) DB; ++k) {
+            const uint32_t quad = (tid & 7u) + 8u * k;
+            if (4u * quad >= D) continue;
+            float4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float4_t x = ((const float4_t *) (tiles + w * S::BUF))[r * 8u * DB + (quad ^ (r & 7u))];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f[w], o[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] *= inv;
+            if (pieces > 1) *(float4_t *) (a.rec_o + (rec + r) * D + 4u * quad) = o;
+            else store(to, 4u * quad, o);
+        }
+        if (pieces > 1 && (tid & 7u) == 0u) *(float2_t *) (a.rec_ml + 2 * (rec + r)) = float2_t{m, sum};
         return;
     }
-    const float sink2 = a.sinks ? a.sinks[hd] * MOEARC_LOG2E : -INFINITY;
-    const float top = fmaxf(m_run, sink2);
-    const float fm = __builtin_amdgcn_exp2f(m_run - top);
-    const float total = L * fm + __builtin_amdgcn_exp2f(sink2 - top + MOEARC_AB_LOG2_PSCALE);
-    const float inv = total == 0.f ? 0.f : fm / total;  // a row without keys and without a sink
+    together(std::false_type{});
+    again_round = any_not_finite();
+    if (again_round) together(std::true_type{});
+    const float L = l_run + __shfl_xor(l_run, 32);
+    uint32_t r = wave * 32u + n;  // the row again, computed anew: its registers are the key loop's until here
+    asm volatile("" : "+v"(r));
+    const uint32_t rr = tile * MOEARC_AB_ROWS + r;
+    if (rr >= rows) return;
+    const uint32_t head = kvh * group + rr % group;
+    const uint64_t to = ((uint64_t) a.row0[b] + rr / group) * a.n_heads + head;
+    const float inv = pieces > 1 ? 1.f : inverse(m_run, L, head);
 #pragma unroll
     for (int mb = 0; mb < DB; ++mb)
 #pragma unroll
@@ -398,54 +611,63 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
             const uint32_t d = 32u * mb + 8u * j + 4u * h;
             if (d >= D) continue;
             const float4_t v = {O[mb][4 * j] * inv, O[mb][4 * j + 1] * inv, O[mb][4 * j + 2] * inv, O[mb][4 * j + 3] * inv};
-            if (a.out_f16) {
-                const half2_t h0 = {(_Float16) v[0], (_Float16) v[1]}, h1 = {(_Float16) v[2], (_Float16) v[3]};
-                *(u32x2_t *) ((_Float16 *) a.out + out_row * D + d) =
-                    u32x2_t{__builtin_bit_cast(uint32_t, h0), __builtin_bit_cast(uint32_t, h1)};
-            } else {
-                *(float4_t *) ((float *) a.out + out_row * D + d) = v;
-            }
+            if (pieces > 1) *(float4_t *) (a.rec_o + (rec + r) * D + d) = v;
+            else store(to, d, v);
         }
+    if (pieces > 1 && h == 0) *(float2_t *) (a.rec_ml + 2 * (rec + r)) = float2_t{m_run, L};
 }
 
-// Joins the records of the tiles that were cut: a work-group takes rows_per_block rows of one tile and KV head, a row
-// its head_dim / 4 neighbouring lanes' worth of work, float4 each.
+// Joins the records of the tiles that were cut, in one pass over a row's pieces with the running maximum. A thread has
+// four channels of a row; work-groups are (tile and KV head, 256 / (head_dim / 4) rows of it).
 __device__ __forceinline__ void ab_merge_body(const AttnBatchArgs &a) {
     const uint32_t G = a.n_kv_heads, D = a.head_dim, kvh = blockIdx.x % G, at = blockIdx.x / G;
     const uint32_t b = ab_slot(a.merge_begin, at);
     const uint32_t nt = a.n_tiles[b], tile = at - a.merge_begin[b], pieces = (a.item_begin[b + 1] - a.item_begin[b]) / nt;
-    const AbSpan span = ab_span(a, b, tile);
-    const uint32_t np = span.hi > span.lo ? (span.hi - span.lo + a.piece - 1u) / a.piece : 1u;
-    const uint32_t rows = min((uint32_t) MOEARC_AB_ROWS, a.n_new[b] * a.group - tile * MOEARC_AB_ROWS);
-    const uint32_t quads = D / 4u;
-    const uint64_t rec0 = ((uint64_t) (a.rec_begin[b] + tile * pieces) * G + kvh) * MOEARC_AB_ROWS;
-    const uint64_t step = (uint64_t) G * MOEARC_AB_ROWS;  // records from piece to piece
-    const uint32_t r_end = min(rows, (blockIdx.y + 1u) * a.rows_per_block);
-    for (uint32_t i = threadIdx.x + blockIdx.y * a.rows_per_block * quads; i < r_end * quads; i += 256u) {
-        const uint32_t r = i / quads, d = 4u * (i % quads);
-        const uint32_t row = tile * MOEARC_AB_ROWS + r, tok = row / a.group, hd = kvh * a.group + row % a.group;
-        const float sink2 = a.sinks ? a.sinks[hd] * MOEARC_LOG2E : -INFINITY;
-        float top = fmaxf(sink2, PF_M_INIT);
-        for (uint32_t k = 0; k < np; ++k) top = fmaxf(top, a.rec_ml[2 * (rec0 + k * step + r)]);
-        float total = __builtin_amdgcn_exp2f(sink2 - top + MOEARC_AB_LOG2_PSCALE);
-        float4_t o = {0.f, 0.f, 0.f, 0.f};
-        for (uint32_t k = 0; k < np; ++k) {
-            const uint64_t rec = rec0 + k * step + r;
-            const float2_t ml = *(const float2_t *) (a.rec_ml + 2 * rec);
-            const float f = __builtin_amdgcn_exp2f(ml[0] - top);
-            const float4_t x = *(const float4_t *) (a.rec_o + rec * D + d);
-            total = fmaf(ml[1], f, total);
+    const uint32_t rows = a.n_new[b] * a.group, tile_rows = rows <= MOEARC_AB_FEW ? 32u : MOEARC_AB_ROWS;
+    const uint32_t quads = D / 4u, r = blockIdx.y * (256u / quads) + threadIdx.x / quads, d = 4u * (threadIdx.x % quads);
+    const uint32_t row = tile * tile_rows + r;
+    if (threadIdx.x / quads >= 256u / quads || r >= tile_rows || row >= rows) return;
+    const AbSpan span = ab_span(a, b, tile, tile_rows);
+    const uint32_t np = span.hi > span.lo ? (span.hi - span.lo + a.piece[b] - 1u) / a.piece[b] : 1u;
+    const uint64_t rec0 = ((uint64_t) a.rec_begin[b] + tile * pieces * tile_rows) * G + kvh * tile_rows + r;
+    const uint64_t step = (uint64_t) G * tile_rows;  // records from piece to piece
+    const uint32_t tok = row / a.group, hd = kvh * a.group + row % a.group;
+    const float sink2 = a.sinks ? a.sinks[hd] * MOEARC_LOG2E : -INFINITY;
+    float top = fmaxf(sink2, PF_M_INIT), total = __builtin_amdgcn_exp2f(sink2 - top + MOEARC_AB_LOG2_PSCALE);
+    float4_t o = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t k0 = 0; k0 < np; k0 += 8u) {  // eight records' loads at a time
+        float2_t ml[8];
+        float4_t x[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+        for (uint32_t k = 0; k < 8u; ++k) {
+            const uint64_t rec = rec0 + min(k0 + k, np - 1u) * step;
+            ml[k] = *(const float2_t *) (a.rec_ml + 2 * rec);
+            x[k] = *(const float4_t *) (a.rec_o + rec * D + d);
+            if (k0 + k >= np) ml[k] = float2_t{PF_M_INIT, 0.f}, x[k] = float4_t{0.f, 0.f, 0.f, 0.f};
         }
-        const float inv = total == 0.f ? 0.f : 1.f / total;
-        const uint64_t to = (((uint64_t) a.row0[b] + tok) * a.n_heads + hd) * D + d;
-        if (a.out_f16) {
-            const half2_t h0 = {(_Float16) (o[0] * inv), (_Float16) (o[1] * inv)}, h1 = {(_Float16) (o[2] * inv), (_Float16) (o[3] * inv)};
-            *(u32x2_t *) ((_Float16 *) a.out + to) = u32x2_t{__builtin_bit_cast(uint32_t, h0), __builtin_bit_cast(uint32_t, h1)};
-        } else {
-            *(float4_t *) ((float *) a.out + to) = float4_t{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+        float m = top;
+#pragma unroll
+        for (uint32_t k = 0; k < 8u; ++k) m = fmaxf(m, ml[k][0]);
+        const float corr = __builtin_amdgcn_exp2f(top - m);
+        top = m;
+        total *= corr;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= corr;
+#pragma unroll
+        for (uint32_t k = 0; k < 8u; ++k) {
+            const float f = __builtin_amdgcn_exp2f(ml[k][0] - m);
+            total = fmaf(ml[k][1], f, total);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[k][e], f, o[e]);
         }
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const uint64_t to = (((uint64_t) a.row0[b] + tok) * a.n_heads + hd) * D + d;
+    if (a.out_f16) {
+        const half2_t h0 = {(_Float16) (o[0] * inv), (_Float16) (o[1] * inv)}, h1 = {(_Float16) (o[2] * inv), (_Float16) (o[3] * inv)};
+        *(u32x2_t *) ((_Float16 *) a.out + to) = u32x2_t{__builtin_bit_cast(uint32_t, h0), __builtin_bit_cast(uint32_t, h1)};
+    } else {
+        *(float4_t *) ((float *) a.out + to) = float4_t{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
     }
 }
 

@@ -377,14 +377,15 @@ struct QkvAppendArgs {
     uint32_t n_kv[MOEARC_BATCH_SEQS];
 };
 
-// Attention of a ragged batch. A sequence's rows (token, head of the KV head's group) are cut into tiles of
-// `tile_rows`, a tile's keys into pieces of `piece` keys; a work-group takes one piece of one tile for one KV head.
-// Slot b's work items (tiles x pieces) start at item_begin[b]; a slot with more than one piece to a tile leaves
-// records that the merge kernel joins:
-//   rec_o[((rec_begin[b] + tile * pieces + piece) * n_kv_heads + kvh) * tile_rows + row][head_dim]  un-normalised (f32)
+// Attention of a ragged batch. A sequence's rows (token, head of the KV head's group) are cut into tiles -- of 128
+// rows, or of 32 where there are at most MOEARC_AB_FEW -- and a tile's keys into pieces of piece[b]; a work-group takes one
+// piece of one tile for one KV head. Slot b's work items (tiles x pieces) start at item_begin[b]; a slot with more
+// than one piece to a tile leaves records that the merge kernel joins (rows of a tile: tr):
+//   rec_o[(rec_begin[b] + (tile * pieces + piece) * tr) * n_kv_heads + kvh * tr + row][head_dim]  un-normalised (f32)
 //   rec_ml[the same row index][2]   reference max (log2 domain), row sum in its frame
-#define MOEARC_AB_ROWS 128        // rows of a tile: 32 to a wave
-#define MOEARC_AB_PT 2048u        // keys' places that a work-group holds at a time (of eight keys each where pages allow)
+#define MOEARC_AB_ROWS 128u       // rows of a tile: 32 to a wave
+#define MOEARC_AB_FEW 64u
+#define MOEARC_AB_PT 2044u        // keys' places that a work-group holds at a time (of eight keys each where pages allow)
 #define MOEARC_AB_LOG2_PSCALE 7.0f  // weights are 2^7 at the reference max: f16 keeps 21 bits below it
 struct AttnBatchArgs {
     const uint16_t *q, *k_pages, *v_pages;
@@ -398,8 +399,6 @@ struct AttnBatchArgs {
     uint32_t page_tokens, page_magic, page_shift;  // key / page_tokens = key * magic >> shift for key < 2^31
     uint32_t n_pages, out_f16;
     float scale_log2e;
-    uint32_t piece;                 // keys, a multiple of 32
-    uint32_t n_slots, rows_per_block;  // (the merge's: rows of a tile that a work-group joins)
     uint32_t item_begin[MOEARC_BATCH_SEQS + 1];   // entries n_slots .. the end: the item count
     uint32_t merge_begin[MOEARC_BATCH_SEQS + 1];  // tiles that need a merge
     uint32_t seq[MOEARC_BATCH_SEQS];      // block-table row
@@ -407,5 +406,6 @@ struct AttnBatchArgs {
     uint32_t n_new[MOEARC_BATCH_SEQS];
     uint32_t n_kv[MOEARC_BATCH_SEQS];
     uint32_t n_tiles[MOEARC_BATCH_SEQS];
-    uint32_t rec_begin[MOEARC_BATCH_SEQS];
+    uint32_t rec_begin[MOEARC_BATCH_SEQS];  // rows of records, per KV head
+    uint32_t piece[MOEARC_BATCH_SEQS];      // keys, a multiple of 32
 };

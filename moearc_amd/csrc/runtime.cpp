@@ -142,7 +142,7 @@ struct moearc_ctx {
     hipFunction_t f_moe_tile[6][2][2] = {}, f_moe_light[6][2][2] = {}, f_moe_vec[6][2][3] = {};
     float *moe_ws = nullptr;  // the experts' products' working memory, eager calls only
     size_t moe_ws_floats = 0;
-    hipFunction_t f_qkv_append[4] = {};  // 8, 16, 32 lanes a head, any head
+    hipFunction_t f_qkv_append[3][2] = {}, f_qkv_append_any = nullptr;  // 8, 16, 32 lanes a head x one, three heads a thread
     hipFunction_t f_attn_batch[3][2] = {}, f_attn_batch_merge = nullptr;  // up to 64, 128, 256 channels x default, precise
     float *ab_ws = nullptr;  // the records of a ragged batch's cut tiles, eager calls only
     size_t ab_ws_floats = 0;

@@ -6,14 +6,17 @@ namespace {
 
 constexpr unsigned long kBatchRows = 1ul << 20;  // new tokens of a call: launches stay below 2^32 threads
 constexpr unsigned long kBatchHeads = 1024;
+#define MOEARC_AB_MIN_CHUNKS 16  // of a piece of few rows' keys: four tiles a wave
 
 bool batch_load(moearc_ctx *c) {
     struct {
         hipFunction_t *slot;
         const char *name;
     } fns[] = {
-        {&c->f_qkv_append[0], "moearc_qkv_append_l8_k"},   {&c->f_qkv_append[1], "moearc_qkv_append_l16_k"},
-        {&c->f_qkv_append[2], "moearc_qkv_append_l32_k"},  {&c->f_qkv_append[3], "moearc_qkv_append_any_k"},
+        {&c->f_qkv_append[0][0], "moearc_qkv_append_l8_k"},  {&c->f_qkv_append[0][1], "moearc_qkv_append_l8x3_k"},
+        {&c->f_qkv_append[1][0], "moearc_qkv_append_l16_k"}, {&c->f_qkv_append[1][1], "moearc_qkv_append_l16x3_k"},
+        {&c->f_qkv_append[2][0], "moearc_qkv_append_l32_k"}, {&c->f_qkv_append[2][1], "moearc_qkv_append_l32x3_k"},
+        {&c->f_qkv_append_any, "moearc_qkv_append_any_k"},
         {&c->f_attn_batch[0][0], "moearc_attn_batch_d2_k"}, {&c->f_attn_batch[0][1], "moearc_attn_batch_precise_d2_k"},
         {&c->f_attn_batch[1][0], "moearc_attn_batch_d4_k"}, {&c->f_attn_batch[1][1], "moearc_attn_batch_precise_d4_k"},
         {&c->f_attn_batch[2][0], "moearc_attn_batch_d8_k"}, {&c->f_attn_batch[2][1], "moearc_attn_batch_precise_d8_k"},
@@ -57,19 +60,19 @@ struct BatchSeq {
 };
 
 struct BatchPlan {
-    uint32_t n = 0, items = 0, tiles = 0, records = 0, merge_tiles = 0;
-    uint32_t piece = 0x40000000u;
+    uint32_t n = 0, items = 0, merge_tiles = 0, merge_rows = 0;
+    uint64_t records = 0;  // rows of records, per KV head
     BatchSeq s[MOEARC_BATCH_SEQS];
-    uint32_t n_tiles[MOEARC_BATCH_SEQS], pieces[MOEARC_BATCH_SEQS];
+    uint32_t tile_rows[MOEARC_BATCH_SEQS], n_tiles[MOEARC_BATCH_SEQS], pieces[MOEARC_BATCH_SEQS], piece[MOEARC_BATCH_SEQS];
 };
 
-// Keys of tile t's span, in 32-key chunks (attn_batch.hip's ab_span).
-uint64_t batch_chunks(const BatchSeq &s, const BatchShape &sh, uint64_t t) {
+// Keys of tile t's span, in 32-key chunks (attn_batch.hip's ab_span; it may start up to seven keys earlier).
+uint64_t batch_chunks(const BatchSeq &s, const BatchShape &sh, uint64_t tile_rows, uint64_t t) {
     const int64_t shift = (int64_t) s.n_kv - s.n_new;
-    const int64_t tok0 = (int64_t) (t * MOEARC_AB_ROWS / sh.group);
-    const int64_t tok1 = std::min<int64_t>((int64_t) ((t * MOEARC_AB_ROWS + MOEARC_AB_ROWS - 1) / sh.group), (int64_t) s.n_new - 1);
+    const int64_t tok0 = (int64_t) (t * tile_rows / sh.group);
+    const int64_t tok1 = std::min<int64_t>((int64_t) ((t * tile_rows + tile_rows - 1) / sh.group), (int64_t) s.n_new - 1);
     const int64_t hi = std::max<int64_t>(0, shift + tok1 + 1), first = std::max<int64_t>(0, shift + tok0);
-    const int64_t lo = sh.n_swa && first + 1 > (int64_t) sh.n_swa ? first + 1 - (int64_t) sh.n_swa : 0;
+    const int64_t lo = sh.n_swa && first + 1 > (int64_t) sh.n_swa ? (first + 1 - (int64_t) sh.n_swa) / 8 * 8 : 0;
     return hi > lo ? (uint64_t) (hi - lo + 31) / 32 : 0;
 }
 
@@ -85,35 +88,58 @@ unsigned long batch_take(BatchPlan &p, const unsigned int *row_begin, const unsi
 }
 
 // Tiles, and pieces where a tile's keys would keep one work-group longer than the whole work keeps the device: with
-// fewer, all work-groups run at once and the longest decides.
+// fewer, all work-groups run at once and the longest decides. Work is counted in 32-key chunks of a tile of few rows, whose
+// work-group takes four at a time; a full tile's takes one.
 void batch_plan(BatchPlan &p, const BatchShape &sh, bool may_split) {
-    uint64_t total = 0, longest[MOEARC_BATCH_SEQS], most = 0;
+    uint64_t total = 0, most = 0, longest[MOEARC_BATCH_SEQS];
     for (uint32_t i = 0; i < p.n; ++i) {
-        p.n_tiles[i] = (uint32_t) (((uint64_t) p.s[i].n_new * sh.group + MOEARC_AB_ROWS - 1) / MOEARC_AB_ROWS);
+        const uint64_t rows = (uint64_t) p.s[i].n_new * sh.group;
+        p.tile_rows[i] = rows <= MOEARC_AB_FEW ? 32u : MOEARC_AB_ROWS;
+        p.n_tiles[i] = (uint32_t) ((rows + p.tile_rows[i] - 1) / p.tile_rows[i]);
         longest[i] = 1;
+        uint64_t sum = 0;
         for (uint64_t t = 0; t < p.n_tiles[i]; ++t) {
-            const uint64_t n = batch_chunks(p.s[i], sh, t);
-            total += n;
+            const uint64_t n = batch_chunks(p.s[i], sh, p.tile_rows[i], t);
+            sum += n;
             longest[i] = std::max(longest[i], n);
         }
-        most = std::max(most, longest[i]);
+        const uint64_t cost = p.tile_rows[i] == MOEARC_AB_ROWS ? 4 : 1;
+        total += sum * cost;
+        most = std::max(most, longest[i] * cost);
     }
-    const uint64_t even = std::max<uint64_t>(8, (total * sh.n_kv_heads + sh.wgs - 1) / sh.wgs);
-    p.piece = may_split && most > even + even / 4 ? (uint32_t) std::min<uint64_t>(even * 32, 0x40000000u) : 0x40000000u;
-    p.items = p.tiles = p.records = p.merge_tiles = 0;
+    static const uint64_t mn = getenv("AB_MIN") ? atoi(getenv("AB_MIN")) : MOEARC_AB_MIN_CHUNKS;
+    static const uint64_t R = getenv("AB_R") ? atoi(getenv("AB_R")) : 100;
+    uint64_t even = std::max<uint64_t>(mn, (total * sh.n_kv_heads + sh.wgs * R / 100 - 1) / (sh.wgs * R / 100));
+    const bool split = may_split && most > even + even / 4;
+    // Pieces that together are a few more than the device holds at once would run in a second round: longer ones.
+    auto cut = [&](uint32_t i) {
+        const bool full = p.tile_rows[i] == MOEARC_AB_ROWS;
+        const uint64_t chunks = full ? std::max<uint64_t>((even + 3) / 4, 16) : (even + 3) / 4 * 4;
+        const bool whole = !split || longest[i] <= chunks + chunks / 4;
+        p.piece[i] = whole ? 0x40000000u : (uint32_t) std::min<uint64_t>(chunks * 32, 0x40000000u);
+        p.pieces[i] = whole ? 1u : (uint32_t) ((longest[i] * 32 + p.piece[i] - 1) / p.piece[i]);
+        return (uint64_t) p.n_tiles[i] * p.pieces[i];
+    };
+    for (int k = 0; k < 8; ++k) {
+        uint64_t wgs = 0;
+        for (uint32_t i = 0; i < p.n; ++i) wgs += cut(i) * sh.n_kv_heads;
+        if (!split || R != 100 || wgs <= sh.wgs || wgs >= 2 * sh.wgs) break;
+        even += even / 16 + 1;
+    }
+    p.items = p.merge_tiles = p.merge_rows = 0;
+    p.records = 0;
     for (uint32_t i = 0; i < p.n; ++i) {
-        p.pieces[i] = p.piece == 0x40000000u ? 1u : (uint32_t) ((longest[i] * 32 + p.piece - 1) / p.piece);
-        p.tiles += p.n_tiles[i];
         p.items += p.n_tiles[i] * p.pieces[i];
         if (p.pieces[i] > 1) {
-            p.records += p.n_tiles[i] * p.pieces[i];
+            p.records += (uint64_t) p.n_tiles[i] * p.pieces[i] * p.tile_rows[i];
             p.merge_tiles += p.n_tiles[i];
+            p.merge_rows = std::max(p.merge_rows, p.tile_rows[i]);
         }
     }
 }
 
 size_t batch_record_bytes(const BatchPlan &p, const BatchShape &sh) {
-    return (size_t) p.records * sh.n_kv_heads * MOEARC_AB_ROWS * (sh.head_dim + 2) * sizeof(float);
+    return (size_t) p.records * sh.n_kv_heads * (sh.head_dim + 2) * sizeof(float);
 }
 
 // The checks that the attention and its workspace share.
@@ -183,9 +209,13 @@ int moearc_rope_qkv_append_batched(moearc_ctx *c, const moearc_qkv_append *d, co
     const bool wide = D % 8 == 0 && d->n_rot % 8 == 0 && d->q_stride % 4 == 0 && d->k_stride % 4 == 0 && d->v_stride % 4 == 0 &&
                       quads(d->q, in_size) && quads(d->k, in_size) && quads(d->v, in_size) && quads(d->q_out, q_size) &&
                       quads(d->k_pages, kv_size) && quads(d->v_pages, kv_size) && quads(d->q_norm, 4) && quads(d->k_norm, 4);
-    const int kind = !wide ? 3 : D <= 64 ? 0 : D <= 128 ? 1 : 2;
-    const unsigned per_wg = kind == 3 ? 4u : 32u >> kind;  // heads
-    const unsigned groups = (unsigned) ((d->n_heads + 2 * d->n_kv_heads + per_wg - 1) / per_wg);
+    const int kind = D <= 64 ? 0 : D <= 128 ? 1 : 2;
+    const uint64_t heads = d->n_heads + 2 * d->n_kv_heads, per_wg = wide ? 32u >> kind : 4u;
+    uint64_t groups = (heads + per_wg - 1) / per_wg;
+    // A work-group of three heads a thread where those of one would be more than the device holds (eight to a CU).
+    const bool many = wide && groups * (row_begin[n_seqs] - row_begin[0]) > 8ull * (c->n_cu ? c->n_cu : 256u);
+    if (many) groups = (groups + 2) / 3;
+    const hipFunction_t kernel = wide ? c->f_qkv_append[kind][many] : c->f_qkv_append_any;
     const LaunchScope scope(c, "rope_qkv_append", d->n_heads, D);
     batch_arm(c);
     const uint32_t step = (uint32_t) (kMaxThreads / 256 / groups);
@@ -204,7 +234,7 @@ int moearc_rope_qkv_append_batched(moearc_ctx *c, const moearc_qkv_append *d, co
         a.q_out = (uint8_t *) d->q_out + (size_t) first * d->n_heads * D * q_size;
         a.block_tables = block_tables + at * bt_stride;
         for (a.row_off = 0; a.row_off < rows; a.row_off += step)
-            if (const int rc = launch2d(c, c->f_qkv_append[kind], std::min(step, rows - a.row_off), groups, 256, a, nullptr,
+            if (const int rc = launch2d(c, kernel, std::min(step, rows - a.row_off), (unsigned) groups, 256, a, nullptr,
                                         d->n_heads, D, 0, "rope_qkv_append"))
                 return rc;
     }
@@ -287,9 +317,8 @@ int moearc_attn_prefill_batched(moearc_ctx *c, void *out, unsigned int out_type,
         at = batch_take(p, row_begin, n_kv, n_seqs, at);
         if (p.n == 0) continue;
         batch_plan(p, sh, split);
-        a.piece = p.piece;
-        a.n_slots = p.n;
-        uint32_t item = 0, rec = 0, merge = 0;
+        uint32_t item = 0, merge = 0;
+        uint64_t rec = 0;
         for (uint32_t i = 0; i <= MOEARC_BATCH_SEQS; ++i) {
             a.item_begin[i] = item;
             a.merge_begin[i] = merge;
@@ -299,22 +328,24 @@ int moearc_attn_prefill_batched(moearc_ctx *c, void *out, unsigned int out_type,
             a.n_new[i] = p.s[i].n_new;
             a.n_kv[i] = p.s[i].n_kv;
             a.n_tiles[i] = p.n_tiles[i];
-            a.rec_begin[i] = rec;
+            a.rec_begin[i] = (uint32_t) rec;
+            a.piece[i] = p.piece[i];
             item += p.n_tiles[i] * p.pieces[i];
             if (p.pieces[i] > 1) {
-                rec += p.n_tiles[i] * p.pieces[i];
+                rec += (uint64_t) p.n_tiles[i] * p.pieces[i] * p.tile_rows[i];
                 merge += p.n_tiles[i];
             }
         }
         a.rec_o = (float *) ws;
-        a.rec_ml = (float *) ws + (size_t) p.records * n_kv_heads * MOEARC_AB_ROWS * head_dim;
+        a.rec_ml = (float *) ws + (size_t) p.records * n_kv_heads * head_dim;
         if (const int rc = launch(c, c->f_attn_batch[kind][out_type == MOEARC_OUT_F32], (unsigned) (p.items * n_kv_heads), 256, a,
                                   nullptr, n_heads, head_dim, "attn_prefill_batched"))
             return rc;
         if (p.merge_tiles) {
-            a.rows_per_block = 16;
-            if (const int rc = launch2d(c, c->f_attn_batch_merge, (unsigned) (p.merge_tiles * n_kv_heads), MOEARC_AB_ROWS / 16, 256, a,
-                                        nullptr, n_heads, head_dim, 0, "attn_prefill_batched.merge"))
+            const unsigned at_a_time = 256u / ((unsigned) head_dim / 4u);
+            if (const int rc = launch2d(c, c->f_attn_batch_merge, (unsigned) (p.merge_tiles * n_kv_heads),
+                                        (p.merge_rows + at_a_time - 1) / at_a_time, 256, a, nullptr, n_heads, head_dim, 0,
+                                        "attn_prefill_batched.merge"))
                 return rc;
         }
     }

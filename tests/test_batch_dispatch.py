@@ -98,8 +98,11 @@ def test_append_grids(cx, lib):
     assert [r[1:] for r in launches(lib)] == [(4, 1, 1, 256)]
     lib.host_hip_reset()
     assert append(cx, rows=(0, 1 << 20), n_kv=(1 << 20,), bt_stride=1 << 20, n_heads=1024, q_stride=1 << 16) == 0
-    rows = launches(lib)
-    assert sum(r[1] for r in rows) == 1 << 20 and all(r[2] == 33 and r[1] * 33 * 256 <= 1 << 31 for r in rows)
+    rows = launches(lib)  # 1028 heads, 96 to a work-group
+    assert sum(r[1] for r in rows) == 1 << 20 and all(r[0] == "moearc_qkv_append_l8x3_k" and r[2] == 11 and r[1] * 11 * 256 <= 1 << 31 for r in rows)
+    lib.host_hip_reset()
+    assert append(cx, rows=(0, 2049), n_kv=(2049,), bt_stride=1 << 20) == 0 and append(cx, rows=(0, 2048), n_kv=(2049,), bt_stride=1 << 20) == 0
+    assert names(lib) == ["moearc_qkv_append_l8x3_k", "moearc_qkv_append_l8_k"]
 
 
 def attend(cx, rows=(0, 1, 3), n_kv=(5, 9), **kw):
