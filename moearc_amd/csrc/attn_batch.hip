@@ -117,6 +117,11 @@ __device__ __forceinline__ uint32_t ab_slot(const uint32_t *begin, uint32_t item
     return b;
 }
 
+// x / group for x < 2^31 (the host's factor and shift).
+__device__ __forceinline__ uint32_t ab_token(const AttnBatchArgs &a, uint32_t x) {
+    return (uint32_t) ((uint64_t) x * a.group_magic >> a.group_shift);
+}
+
 // Keys [lo, hi) that the rows of tile t (of tile_rows) of a slot see. No other's block-table entry is looked at.
 struct AbSpan {
     uint32_t lo, hi;
@@ -124,12 +129,12 @@ struct AbSpan {
 __device__ __forceinline__ AbSpan ab_span(const AttnBatchArgs &a, uint32_t b, uint32_t t, uint32_t tile_rows) {
     const uint32_t n = a.n_new[b];
     const int32_t shift = (int32_t) (a.n_kv[b] - n);  // a token's position less its index; below 0: the first see nothing
-    const uint32_t tok0 = t * tile_rows / a.group, tok1 = min((t * tile_rows + tile_rows - 1u) / a.group, n - 1u);
+    const uint32_t tok0 = ab_token(a, t * tile_rows), tok1 = min(ab_token(a, t * tile_rows + tile_rows - 1u), n - 1u);
     const int32_t last = shift + (int32_t) tok1, first = max(0, shift + (int32_t) tok0);
     AbSpan s;
     s.hi = last < 0 ? 0u : (uint32_t) last + 1u;
     s.lo = a.n_swa && (uint32_t) first + 1u > a.n_swa ? (uint32_t) first + 1u - a.n_swa : 0u;
-    if (a.page_tokens % 8u == 0u) s.lo &= ~7u;  // in the same page
+    if (a.eights) s.lo &= ~7u;  // in the same page
     return s;
 }
 
@@ -145,13 +150,13 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t G = a.n_kv_heads, D = a.head_dim, group = a.group;
     const uint32_t kvh = blockIdx.x % G, item = blockIdx.x / G;
-    const uint32_t b = ab_slot(a.item_begin, item);
+    const uint32_t b = a.n_slots > 1u ? ab_slot(a.item_begin, item) : 0u;
     const uint32_t n_new = a.n_new[b], rows = n_new * group;
     const bool few = rows <= MOEARC_AB_FEW;  // the four waves share 32 rows, each with keys of its own
     const uint32_t tile_rows = few ? 32u : MOEARC_AB_ROWS;
     const uint32_t nt = a.n_tiles[b], in_slot = item - a.item_begin[b];
-    const uint32_t pieces = (a.item_begin[b + 1] - a.item_begin[b]) / nt;
-    const uint32_t pc = in_slot / nt, tile = nt - 1u - in_slot % nt;  // the latest tile, which has the most keys, first
+    const uint32_t pieces = a.pieces[b], pc = pieces > 1u ? in_slot / nt : 0u;
+    const uint32_t tile = nt - 1u - (in_slot - pc * nt);  // the latest tile, which has the most keys, first
     const AbSpan span = ab_span(a, b, tile, tile_rows);
     const uint32_t lo = span.lo + pc * a.piece[b];  // with pages of eights a multiple of 8
     const uint32_t hi = pieces > 1 ? min(span.hi, lo + a.piece[b]) : span.hi;
@@ -161,7 +166,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     const int32_t shift = (int32_t) (a.n_kv[b] - n_new);
     const uint32_t row0 = tile * tile_rows + (few ? 0u : wave * 32u), row = row0 + n;
     const bool row_ok = row < rows;
-    const uint32_t tok = min(row, rows - 1u) / group, hd = kvh * group + min(row, rows - 1u) % group;
+    const uint32_t tok = ab_token(a, min(row, rows - 1u)), hd = kvh * group + min(row, rows - 1u) - tok * group;
     const int32_t pos = shift + (int32_t) tok;
     // visible keys j: j - row_lo <= row_len as unsigned numbers (an empty row: at 2^31, which no key has)
     const uint32_t row_lo = pos < 0 ? 0x80000000u : a.n_swa && (uint32_t) pos + 1u > a.n_swa ? (uint32_t) pos + 1u - a.n_swa : 0u;
@@ -186,8 +191,8 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
         for (int t = 0; t < 2 * DB; ++t) qop[t] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
     }
     // positions of the wave's first and last row: which tiles cross a mask
-    const int32_t w_first = shift + (int32_t) (min(row0, rows - 1u) / group);
-    const int32_t w_last = shift + (int32_t) (min(row0 + 31u, rows - 1u) / group);
+    const int32_t w_first = shift + (int32_t) ab_token(a, min(row0, rows - 1u));
+    const int32_t w_last = shift + (int32_t) ab_token(a, min(row0 + 31u, rows - 1u));
     const int32_t w_lo_last = a.n_swa ? max(0, w_last + 1 - (int32_t) a.n_swa) : 0;
 
     // ---- LDS addresses and copies ----------------------------------------------------------------
@@ -202,7 +207,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     const uint32_t lds0 = (uint32_t) (uintptr_t) (lds_u8_t *) tiles;
     const uint32_t ld_key = lane / S::CHUNKS, ld_slot = lane % S::CHUNKS;  // of a copy's KEYS keys, and where in their rows
     const uint32_t key_bytes = G * D * 2u, head_bytes = kvh * D * 2u;
-    const bool eights = a.page_tokens % 8u == 0u;
+    const bool eights = a.eights;
     // What this lane copies of eight keys of K or V: byte offsets from their first one's row in the pool. The swizzle of eight
     // keys is one of two for K (by their bit 4), the same for all of V. Where a head has fewer channels than 32 DB, chunks
     // behind them are its first one again: q is zero there, and nobody stores what becomes of V's.
@@ -251,9 +256,11 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     auto copy8_any = [&](const uint8_t *pool, const Lanes &l, uint32_t j, uint32_t seg, uint32_t last_key, uint32_t dst) {
 #pragma unroll
         for (uint32_t i = 0; i < COPIES; ++i) {
+            uint32_t off = l.off[i];
+            asm volatile("" : "+v"(off));  // computed here: the loop that hardly takes this path has no registers for it
             const uint32_t key = ld_key + i * S::KEYS, at = min(j + key, last_key) - seg;
             const uint32_t place = eights ? table[at / 8u] + at % 8u : table[at];
-            ab_copy16(pool + (uint64_t) place * key_bytes + (l.off[i] - key * key_bytes), dst + i * 1024u);
+            ab_copy16(pool + ((uint64_t) place * key_bytes + (off - key * key_bytes)), dst + i * 1024u);
         }
     };
 
@@ -324,7 +331,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
 #pragma unroll
         for (int mb = 0; mb < DB; ++mb) O[mb] *= corr;
     };
-    // V^T's operand of channel block mb, step q; the product with the weights. The first EARLY blocks' may be read ahead.
+    // V^T's operand of channel block mb, step q; the product with the weights.
     auto operand = [&](const uint8_t *kt, int mb, int q) {
         const uint8_t *p = kt + v_at[mb] + q * 16 * S::ROW;
         const short4v_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t *) p);
@@ -333,22 +340,12 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
         const short8v_t x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
         return __builtin_bit_cast(half8_t, x);
     };
-    constexpr int EARLY = DB == 4 && !PRECISE ? 2 : 0;
-    struct Early {
-        half8_t v[EARLY ? 2 * EARLY : 1];
-    };
-    auto read_early = [&](const uint8_t *kt) {
-        Early e;
-#pragma unroll
-        for (int i = 0; i < 2 * EARLY; ++i) e.v[i] = operand(kt, i >> 1, i & 1);
-        return e;
-    };
-    auto values = [&](const uint8_t *kt, const Early &e, const half8_t (&phi)[2], const half8_t (&plo)[2]) {
+    auto values = [&](const uint8_t *kt, const half8_t (&phi)[2], const half8_t (&plo)[2]) {
 #pragma unroll
         for (int mb = 0; mb < DB; ++mb)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const half8_t va = mb < EARLY ? e.v[2 * mb + q] : operand(kt, mb, q);
+                const half8_t va = operand(kt, mb, q);
                 O[mb] = pf_mfma(va, phi[q], O[mb]);
                 if constexpr (PRECISE) O[mb] = pf_mfma(va, plo[q], O[mb]);
             }
@@ -386,7 +383,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
         l_run = add_lo(l, plo);
         before_v();
         if (decltype(by_key_c)::value && crosses(j0)) values_by_key(kt, j0, phi, plo);
-        else values(kt, read_early(kt), phi, plo);
+        else values(kt, phi, plo);
     };
     auto any_not_finite = [&]() {
         bool finite = true;
@@ -423,58 +420,32 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
                 }
             };
             // Step r: this wave's copies of tile r + 1 are done (those of r + 2, issued later, may be in flight), every
-            // wave meets, so all copies of r + 1 are in and nobody reads tile r - 1's buffer, which r + 3 then takes.
-            // Tiles behind the last are copied again, into buffers whose scores nobody uses, so the count is always the same.
+            // wave meets, so all copies of r + 1 are in and nobody reads tile r - 1's buffer, which r + 3 then takes. Behind the
+            // last tile there is nothing to wait for, and the scores beside the last weights are nobody's.
             const uint32_t steps = (seg_hi - seg + 31u) / 32u;
-            auto first_key = [&](uint32_t r) { return seg + 32u * min(r, steps - 1u); };
+            auto first_key = [&](uint32_t r) { return seg + 32u * r; };
+            constexpr int ONE = 2 * COPIES;  // a tile's copies
 #pragma unroll 1
-            for (uint32_t r = 0; r < NBUF - 1; ++r) copy_tile(first_key(r), r, place_of(first_key(r)));
-            uint32_t ahead = place_of(first_key(NBUF - 1));  // read a step before its use
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((NBUF - 2) * 2 * COPIES) : "memory");
+            for (uint32_t r = 0; r < min(steps, NBUF - 1u); ++r) copy_tile(first_key(r), r, place_of(first_key(r)));
+            uint32_t ahead = steps >= NBUF ? place_of(first_key(NBUF - 1)) : 0u;  // read a step before its use
+            if (steps > 2u) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * ONE) : "memory");
+            else if (steps > 1u) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(ONE) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
             float16_t s = scores(tiles), next;
             auto open = [&](uint32_t r, uint32_t buf) {  // of tile r + 3
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((NBUF - 3) * 2 * COPIES) : "memory");
-                copy_tile(first_key(r + NBUF - 1u), buf, ahead);
-                ahead = place_of(first_key(r + NBUF));
+                if (r + 2u < steps) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(ONE) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
+                if (r + NBUF - 1u < steps) {
+                    copy_tile(first_key(r + NBUF - 1u), buf, ahead);
+                    if (r + NBUF < steps) ahead = place_of(first_key(r + NBUF));
+                }
             };
-            // Runs of tiles without a mask or a new reference have a loop of their own, in which the next tile's scores run
-            // beside the weights: with the branches inside, the compiler copies scores or outputs at every join. Tiles
-            // [plain0, plain1) have no mask, and the tiles that are copied meanwhile are whole and of pages of eights.
-            const int32_t first_plain = w_lo_last - (int32_t) seg, past_plain = w_first + 1 - (int32_t) seg;
-            const uint32_t plain0 = first_plain > 0 ? ((uint32_t) first_plain + 31u) / 32u : 0u;
-            const uint32_t whole = (last_key + 1u - seg) / 32u, no_mask = past_plain > 0 ? (uint32_t) past_plain / 32u : 0u;
-            const uint32_t plain1 = eights && whole > NBUF ? min(whole - NBUF, no_mask) : 0u;
             for (uint32_t r = 0; r < steps; ++r) {
-                bool opened = false;
-                if constexpr (DB <= 4 && !decltype(by_key_c)::value) {
-                    if (r >= plain0) {
-                        uint32_t cur = r % NBUF * S::BUF;
-                        for (; r < plain1; ++r) {
-                            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((NBUF - 3) * 2 * COPIES) : "memory");
-                            const uint32_t dst = lds_own + ((cur + (NBUF - 1u) * S::BUF) & (NBUF * S::BUF - 1u));
-                            const uint64_t o = offset_of(ahead);
-                            ab_copy_kv<COPIES>(k_pool + o, v_pool + o, k_own.off, v_lanes.off, dst, dst + S::TILE);
-                            ahead = table[4u * (r + NBUF) + wave];
-                            const uint32_t nxt = (cur + S::BUF) & (NBUF * S::BUF - 1u);
-                            next = scores(tiles + nxt);
-                            const Early early = read_early(tiles + cur);
-                            half8_t phi[2], plo[2];
-                            const float l = weights(s, MOEARC_AB_LOG2_PSCALE - m_run, l_run, phi, plo);
-                            opened = overflow(l);
-                            if (opened) break;
-                            l_run = add_lo(l, plo);
-                            values(tiles + cur, early, phi, plo);
-                            s = next;
-                            cur = nxt;
-                        }
-                        if (r >= steps) break;
-                    }
-                }
-                if (!opened) {
-                    open(r, (r + NBUF - 1u) % NBUF);
-                    if (crosses(first_key(r))) mask(s, first_key(r));
-                    next = scores(tiles + (r + 1u) % NBUF * S::BUF);
-                }
+                open(r, (r + NBUF - 1u) % NBUF);
+                if (crosses(first_key(r))) mask(s, first_key(r));
+                next = scores(tiles + (r + 1u) % NBUF * S::BUF);  // beside the weights of this one
                 absorb(by_key_c, s, first_key(r), tiles + r % NBUF * S::BUF, [] {});
                 s = next;
             }
@@ -571,8 +542,8 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
             f[w] = __builtin_amdgcn_exp2f(ml[32 * w + r][0] - m);
             sum = fmaf(ml[32 * w + r][1], f[w], sum);
         }
-        const uint32_t head = kvh * group + rr % group;
-        const uint64_t to = ((uint64_t) a.row0[b] + rr / group) * a.n_heads + head;
+        const uint32_t rt = ab_token(a, rr), head = kvh * group + rr - rt * group;
+        const uint64_t to = ((uint64_t) a.row0[b] + rt) * a.n_heads + head;
         const float inv = pieces > 1 ? 1.f : inverse(m, sum, head);
 #pragma unroll
         for (uint32_t k = 0; k < (uint32_t) DB; ++k) {
@@ -601,8 +572,8 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     asm volatile("" : "+v"(r));
     const uint32_t rr = tile * MOEARC_AB_ROWS + r;
     if (rr >= rows) return;
-    const uint32_t head = kvh * group + rr % group;
-    const uint64_t to = ((uint64_t) a.row0[b] + rr / group) * a.n_heads + head;
+    const uint32_t rt = ab_token(a, rr), head = kvh * group + rr - rt * group;
+    const uint64_t to = ((uint64_t) a.row0[b] + rt) * a.n_heads + head;
     const float inv = pieces > 1 ? 1.f : inverse(m_run, L, head);
 #pragma unroll
     for (int mb = 0; mb < DB; ++mb)
@@ -621,8 +592,8 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
 // four channels of a row; work-groups are (tile and KV head, 256 / (head_dim / 4) rows of it).
 __device__ __forceinline__ void ab_merge_body(const AttnBatchArgs &a) {
     const uint32_t G = a.n_kv_heads, D = a.head_dim, kvh = blockIdx.x % G, at = blockIdx.x / G;
-    const uint32_t b = ab_slot(a.merge_begin, at);
-    const uint32_t nt = a.n_tiles[b], tile = at - a.merge_begin[b], pieces = (a.item_begin[b + 1] - a.item_begin[b]) / nt;
+    const uint32_t b = a.n_slots > 1u ? ab_slot(a.merge_begin, at) : 0u;
+    const uint32_t tile = at - a.merge_begin[b], pieces = a.pieces[b];
     const uint32_t rows = a.n_new[b] * a.group, tile_rows = rows <= MOEARC_AB_FEW ? 32u : MOEARC_AB_ROWS;
     const uint32_t quads = D / 4u, r = blockIdx.y * (256u / quads) + threadIdx.x / quads, d = 4u * (threadIdx.x % quads);
     const uint32_t row = tile * tile_rows + r;
@@ -631,7 +602,7 @@ __device__ __forceinline__ void ab_merge_body(const AttnBatchArgs &a) {
     const uint32_t np = span.hi > span.lo ? (span.hi - span.lo + a.piece[b] - 1u) / a.piece[b] : 1u;
     const uint64_t rec0 = ((uint64_t) a.rec_begin[b] + tile * pieces * tile_rows) * G + kvh * tile_rows + r;
     const uint64_t step = (uint64_t) G * tile_rows;  // records from piece to piece
-    const uint32_t tok = row / a.group, hd = kvh * a.group + row % a.group;
+    const uint32_t tok = ab_token(a, row), hd = kvh * a.group + row - tok * a.group;
     const float sink2 = a.sinks ? a.sinks[hd] * MOEARC_LOG2E : -INFINITY;
     float top = fmaxf(sink2, PF_M_INIT), total = __builtin_amdgcn_exp2f(sink2 - top + MOEARC_AB_LOG2_PSCALE);
     float4_t o = {0.f, 0.f, 0.f, 0.f};

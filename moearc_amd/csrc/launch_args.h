@@ -396,8 +396,10 @@ struct AttnBatchArgs {
     uint32_t *err;
     uint64_t bt_stride;
     uint32_t n_swa, n_heads, n_kv_heads, group, head_dim;
-    uint32_t page_tokens, page_magic, page_shift;  // key / page_tokens = key * magic >> shift for key < 2^31
-    uint32_t n_pages, out_f16;
+    uint32_t page_tokens, page_magic, page_shift;  // x / page_tokens = x * magic >> shift for x < 2^31; so the group
+    uint32_t group_magic, group_shift;
+    uint32_t eights;                // pages of a multiple of eight tokens
+    uint32_t n_pages, out_f16, n_slots, pad;
     float scale_log2e;
     uint32_t item_begin[MOEARC_BATCH_SEQS + 1];   // entries n_slots .. the end: the item count
     uint32_t merge_begin[MOEARC_BATCH_SEQS + 1];  // tiles that need a merge
@@ -408,4 +410,5 @@ struct AttnBatchArgs {
     uint32_t n_tiles[MOEARC_BATCH_SEQS];
     uint32_t rec_begin[MOEARC_BATCH_SEQS];  // rows of records, per KV head
     uint32_t piece[MOEARC_BATCH_SEQS];      // keys, a multiple of 32
+    uint32_t pieces[MOEARC_BATCH_SEQS];
 };

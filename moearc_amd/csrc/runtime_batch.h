@@ -142,6 +142,14 @@ size_t batch_record_bytes(const BatchPlan &p, const BatchShape &sh) {
     return (size_t) p.records * sh.n_kv_heads * (sh.head_dim + 2) * sizeof(float);
 }
 
+// x / d for x below 2^31 as x * magic >> shift: with 2^s >= d, ceil(2^(31 + s) / d) is off by less than 2^-s
+// relative, so the quotient is exact.
+void batch_divisor(unsigned long d, uint32_t &magic, uint32_t &shift) {
+    const uint32_t s = log2u(d);
+    magic = (uint32_t) (((1ull << (31 + s)) + d - 1) / d);
+    shift = 31 + s;
+}
+
 // The checks that the attention and its workspace share.
 int attn_batch_check(unsigned long n_heads, unsigned long n_kv_heads, unsigned long head_dim, unsigned long n_swa) {
     if (n_heads == 0 || n_heads > kBatchHeads || n_kv_heads == 0 || n_heads % n_kv_heads != 0) return ERR_ARG;
@@ -300,12 +308,10 @@ int moearc_attn_prefill_batched(moearc_ctx *c, void *out, unsigned int out_type,
     a.n_kv_heads = (uint32_t) n_kv_heads;
     a.group = (uint32_t) sh.group;
     a.head_dim = (uint32_t) head_dim;
-    // key / page_tokens for keys below 2^31: with 2^s >= d, m = ceil(2^(31 + s) / d) is off by less than 2^-s
-    // relative, so key * m >> (31 + s) is exact
-    const uint32_t s2 = log2u(page_tokens);
     a.page_tokens = (uint32_t) page_tokens;
-    a.page_magic = (uint32_t) (((1ull << (31 + s2)) + page_tokens - 1) / page_tokens);
-    a.page_shift = 31 + s2;
+    batch_divisor(page_tokens, a.page_magic, a.page_shift);
+    batch_divisor(sh.group, a.group_magic, a.group_shift);
+    a.eights = page_tokens % 8 == 0;
     a.n_pages = (uint32_t) n_pages;
     a.out_f16 = out_type;
     a.scale_log2e = c2;
@@ -317,6 +323,7 @@ int moearc_attn_prefill_batched(moearc_ctx *c, void *out, unsigned int out_type,
         at = batch_take(p, row_begin, n_kv, n_seqs, at);
         if (p.n == 0) continue;
         batch_plan(p, sh, split);
+        a.n_slots = p.n;
         uint32_t item = 0, merge = 0;
         uint64_t rec = 0;
         for (uint32_t i = 0; i <= MOEARC_BATCH_SEQS; ++i) {
@@ -330,6 +337,7 @@ int moearc_attn_prefill_batched(moearc_ctx *c, void *out, unsigned int out_type,
             a.n_tiles[i] = p.n_tiles[i];
             a.rec_begin[i] = (uint32_t) rec;
             a.piece[i] = p.piece[i];
+            a.pieces[i] = p.pieces[i];
             item += p.n_tiles[i] * p.pieces[i];
             if (p.pieces[i] > 1) {
                 rec += (uint64_t) p.n_tiles[i] * p.pieces[i] * p.tile_rows[i];

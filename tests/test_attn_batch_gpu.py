@@ -118,6 +118,13 @@ def test_shapes(cx, heads, kv_heads, dim, page, out_type):
     check(cx, Batch(new, np.add(new, cached), heads, kv_heads, dim, page, dim + page), out_type=out_type)
 
 
+@pytest.mark.parametrize("n_kv", [32, 64, 96, 128, 160, 192, 224, 256, 288, 320, 321, 351])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_spans_of_whole_tiles(cx, dim, n_kv):
+    # what is copied ahead ends where the keys do
+    check(cx, Batch([20, 1], [n_kv, n_kv], 8, 1, dim, 32, n_kv), out_type=OUT_F32)
+
+
 @pytest.mark.parametrize("window", [1, 2, 31, 32, 33, 100, 1000])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_windows(cx, window, dim):
