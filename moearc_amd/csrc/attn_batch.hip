@@ -126,9 +126,8 @@ __device__ __forceinline__ uint32_t ab_token(const AttnBatchArgs &a, uint32_t x)
 struct AbSpan {
     uint32_t lo, hi;
 };
-__device__ __forceinline__ AbSpan ab_span(const AttnBatchArgs &a, uint32_t b, uint32_t t, uint32_t tile_rows) {
-    const uint32_t n = a.n_new[b];
-    const int32_t shift = (int32_t) (a.n_kv[b] - n);  // a token's position less its index; below 0: the first see nothing
+__device__ __forceinline__ AbSpan ab_span(const AttnBatchArgs &a, uint32_t n, uint32_t n_kv, uint32_t t, uint32_t tile_rows) {
+    const int32_t shift = (int32_t) (n_kv - n);  // a token's position less its index; below 0: the first see nothing
     const uint32_t tok0 = ab_token(a, t * tile_rows), tok1 = min(ab_token(a, t * tile_rows + tile_rows - 1u), n - 1u);
     const int32_t last = shift + (int32_t) tok1, first = max(0, shift + (int32_t) tok0);
     AbSpan s;
@@ -137,6 +136,10 @@ __device__ __forceinline__ AbSpan ab_span(const AttnBatchArgs &a, uint32_t b, ui
     if (a.eights) s.lo &= ~7u;  // in the same page
     return s;
 }
+
+// A wave-uniform value that is there from here on: arguments are loaded together at a kernel's start, where the compiler
+// would put each in front of its first use, a chain of waits.
+#define AB_HERE(x) asm volatile("" : "+s"(x))
 
 template <int DB, bool PRECISE>
 __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
@@ -148,52 +151,53 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
 
     const uint32_t tid = threadIdx.x, lane = tid & 63u, h = lane >> 5, n = lane & 31u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t G = a.n_kv_heads, D = a.head_dim, group = a.group;
-    const uint32_t kvh = blockIdx.x % G, item = blockIdx.x / G;
-    const uint32_t b = a.n_slots > 1u ? ab_slot(a.item_begin, item) : 0u;
-    const uint32_t n_new = a.n_new[b], rows = n_new * group;
+    uint32_t G = a.n_kv_heads, kv_magic = a.kv_magic, kv_shift = a.kv_shift, n_slots = a.n_slots, n_heads = a.n_heads;
+    uint32_t D = a.head_dim, group = a.group, n_swa = a.n_swa, page_tokens = a.page_tokens, n_pages = a.n_pages;
+    const uint16_t *q_base = a.q;
+    const uint8_t *k_pool = (const uint8_t *) a.k_pages, *v_pool = (const uint8_t *) a.v_pages;
+    const float *sinks = a.sinks;
+    const uint32_t *row_table = a.block_tables;
+    uint64_t bt_stride = a.bt_stride;
+    AB_HERE(G); AB_HERE(kv_magic); AB_HERE(kv_shift); AB_HERE(n_slots); AB_HERE(n_heads); AB_HERE(D); AB_HERE(group); AB_HERE(n_swa);
+    AB_HERE(page_tokens); AB_HERE(n_pages); AB_HERE(q_base); AB_HERE(k_pool); AB_HERE(v_pool); AB_HERE(sinks); AB_HERE(row_table);
+    AB_HERE(bt_stride);
+    const uint32_t item = (uint32_t) ((uint64_t) blockIdx.x * kv_magic >> kv_shift), kvh = blockIdx.x - item * G;
+    const uint32_t b = n_slots > 1u ? ab_slot(a.item_begin, item) : 0u;
+    uint32_t n_new = a.slot[b].n_new, nt = a.slot[b].n_tiles, item0 = a.slot[b].item_begin, n_kv = a.slot[b].n_kv;
+    uint32_t seq = a.slot[b].seq, tok_row = a.slot[b].row0, pieces = a.slot[b].pieces, piece = a.slot[b].piece;
+    AB_HERE(n_new); AB_HERE(nt); AB_HERE(item0); AB_HERE(n_kv); AB_HERE(seq); AB_HERE(tok_row); AB_HERE(pieces); AB_HERE(piece);
+    const uint32_t rows = n_new * group, in_slot = item - item0;
     const bool few = rows <= MOEARC_AB_FEW;  // the four waves share 32 rows, each with keys of its own
     const uint32_t tile_rows = few ? 32u : MOEARC_AB_ROWS;
-    const uint32_t nt = a.n_tiles[b], in_slot = item - a.item_begin[b];
-    const uint32_t pieces = a.pieces[b], pc = pieces > 1u ? in_slot / nt : 0u;
+    const uint32_t pc = pieces > 1u ? in_slot / nt : 0u;
     const uint32_t tile = nt - 1u - (in_slot - pc * nt);  // the latest tile, which has the most keys, first
-    const AbSpan span = ab_span(a, b, tile, tile_rows);
-    const uint32_t lo = span.lo + pc * a.piece[b];  // with pages of eights a multiple of 8
-    const uint32_t hi = pieces > 1 ? min(span.hi, lo + a.piece[b]) : span.hi;
+    const AbSpan span = ab_span(a, n_new, n_kv, tile, tile_rows);
+    const uint32_t lo = span.lo + pc * piece;  // with pages of eights a multiple of 8
+    const uint32_t hi = pieces > 1 ? min(span.hi, lo + piece) : span.hi;
     if (pc && lo >= span.hi) return;  // an earlier tile's span has fewer pieces
+    row_table += seq * bt_stride;
 
-    // ---- this lane's query row ------------------------------------------------------------------
-    const int32_t shift = (int32_t) (a.n_kv[b] - n_new);
+    // ---- this lane's query row (rows behind the last are that one, and not stored) -------------------
+    const int32_t shift = (int32_t) (n_kv - n_new);
     const uint32_t row0 = tile * tile_rows + (few ? 0u : wave * 32u), row = row0 + n;
     const bool row_ok = row < rows;
     const uint32_t tok = ab_token(a, min(row, rows - 1u)), hd = kvh * group + min(row, rows - 1u) - tok * group;
     const int32_t pos = shift + (int32_t) tok;
     // visible keys j: j - row_lo <= row_len as unsigned numbers (an empty row: at 2^31, which no key has)
-    const uint32_t row_lo = pos < 0 ? 0x80000000u : a.n_swa && (uint32_t) pos + 1u > a.n_swa ? (uint32_t) pos + 1u - a.n_swa : 0u;
+    const uint32_t row_lo = pos < 0 ? 0x80000000u : n_swa && (uint32_t) pos + 1u > n_swa ? (uint32_t) pos + 1u - n_swa : 0u;
     const uint32_t row_len = pos < 0 ? 0u : (uint32_t) pos - row_lo;
     half8_t qop[2 * DB];
-    const uint16_t *q_row = a.q + (((uint64_t) a.row0[b] + tok) * a.n_heads + hd) * D;
+    {
+        const uint16_t *q_row = q_base + (((uint64_t) tok_row + tok) * n_heads + hd) * D;
 #pragma unroll
-    for (int t = 0; t < 2 * DB; ++t) {
-        u32x4_t v = {0u, 0u, 0u, 0u};
-        if (row_ok && 16u * t + 8u * h < D) v = *(const u32x4_t *) (q_row + 16u * t + 8u * h);
-        qop[t] = __builtin_bit_cast(half8_t, v);
+        for (int t = 0; t < 2 * DB; ++t)  // chunks behind the head's channels: any, for now
+            qop[t] = __builtin_bit_cast(half8_t, *(const u32x4_t *) (q_row + min(16u * t + 8u * h, D - 8u)));
     }
     float c = a.scale_log2e;
-    if (c < 0.f) {  // s * c = (-s) * (-c): then the row maximum of s * c is c times the maximum of s
-        c = -c;
-#pragma unroll
-        for (int t = 0; t < 2 * DB; ++t) qop[t] = -qop[t];
-    }
-    if (c == 0.f) {  // every score 0, and masked ones still -inf: q = 0
-        c = 1.f;
-#pragma unroll
-        for (int t = 0; t < 2 * DB; ++t) qop[t] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
-    }
     // positions of the wave's first and last row: which tiles cross a mask
     const int32_t w_first = shift + (int32_t) ab_token(a, min(row0, rows - 1u));
     const int32_t w_last = shift + (int32_t) ab_token(a, min(row0 + 31u, rows - 1u));
-    const int32_t w_lo_last = a.n_swa ? max(0, w_last + 1 - (int32_t) a.n_swa) : 0;
+    const int32_t w_lo_last = n_swa ? max(0, w_last + 1 - (int32_t) n_swa) : 0;
 
     // ---- LDS addresses and copies ----------------------------------------------------------------
     uint32_t v_at[DB];
@@ -229,30 +233,43 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     // Keys whose places fit `table` at a time (a segment); every thread of the work-group takes part.
     const uint32_t seg_keys = eights ? 8u * MOEARC_AB_PT : MOEARC_AB_PT;
     bool again_round = false;
-    const uint32_t *row_table = a.block_tables + a.seq[b] * a.bt_stride;
     auto load_places = [&](uint32_t seg, uint32_t last_key) {
         const uint32_t n_places = eights ? (last_key - seg) / 8u + 1u : last_key - seg + 1u;
-        if (seg != lo || again_round) __syncthreads();
         for (uint32_t i = tid; i < n_places; i += 256u) {
             const uint32_t key = seg + (eights ? 8u * i : i);
             const uint32_t page = (uint32_t) ((uint64_t) key * a.page_magic >> a.page_shift);
             uint32_t id = row_table[page];
-            if (id >= a.n_pages) {  // reported; what is read instead lies in the pool
+            if (id >= n_pages) {  // reported; what is read instead lies in the pool
                 *(volatile uint32_t *) a.err = 1u;
                 id = 0u;
             }
-            table[i] = id * a.page_tokens + (key - page * a.page_tokens);
+            table[i] = id * page_tokens + (key - page * page_tokens);
         }
-        // q has arrived, too: the compiler would wait for its loads in the key loop, and so for the copies issued after them
-#pragma unroll
-        for (int t = 0; t < 2 * DB; ++t) asm volatile("" : : "v"(qop[t]));
         __syncthreads();
     };
+    auto next_places = [&](uint32_t seg, uint32_t last_key) {  // of a later segment, or the first again
+        if (seg == lo && !again_round) return;
+        __syncthreads();
+        load_places(seg, last_key);
+    };
+    float sink2 = -INFINITY;
+    if (sinks) sink2 = sinks[hd];
+    if (lo < hi) load_places(lo, min(hi, lo + seg_keys) - 1u);
+    // q has arrived here: the compiler would wait for its loads in the key loop, and so for the copies issued after them
+#pragma unroll
+    for (int t = 0; t < 2 * DB; ++t) {
+        if (D < 32u * DB && 16u * t + 8u * h >= D) qop[t] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+        if (c < 0.f) qop[t] = -qop[t];  // s * c = (-s) * (-c): then the row maximum of s * c is c times the maximum of s
+        if (c == 0.f) qop[t] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};  // every score 0, and masked ones still -inf
+        asm volatile("" : "+v"(qop[t]));
+    }
+    c = c == 0.f ? 1.f : fabsf(c);
+    sink2 *= MOEARC_LOG2E;
+
     // Copies of eight keys: with pages of eights these share a page, and their base is wave-uniform; otherwise a lane looks
     // for its own key. Keys behind the last are that one: their scores are masked, and no slot is read that the cache has
     // not written.
     auto offset_of = [&](uint32_t place) { return (uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) place) * key_bytes; };
-    const uint8_t *const k_pool = (const uint8_t *) a.k_pages, *const v_pool = (const uint8_t *) a.v_pages;
     auto copy8_any = [&](const uint8_t *pool, const Lanes &l, uint32_t j, uint32_t seg, uint32_t last_key, uint32_t dst) {
 #pragma unroll
         for (uint32_t i = 0; i < COPIES; ++i) {
@@ -405,7 +422,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
         const Lanes k_own = k_lanes(8u * wave);
         for (uint32_t seg = lo; seg < hi; seg += seg_keys) {
             const uint32_t seg_hi = min(hi, seg + seg_keys), last_key = seg_hi - 1u;
-            load_places(seg, last_key);
+            next_places(seg, last_key);
             // a wave's copies of a tile: eight keys of K and of V
             auto place_of = [&](uint32_t j0) { return eights ? table[(min(j0 + 8u * wave, last_key) - seg) / 8u] : 0u; };
             const uint32_t lds_own = __builtin_amdgcn_readfirstlane(lds0 + 8u * wave * S::ROW);
@@ -461,7 +478,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
         const Lanes k0 = k_lanes(0u), k1 = k_lanes(16u);
         for (uint32_t seg = lo; seg < hi; seg += seg_keys) {
             const uint32_t seg_hi = min(hi, seg + seg_keys), last_key = seg_hi - 1u;
-            load_places(seg, last_key);
+            next_places(seg, last_key);
             const uint32_t lds = __builtin_amdgcn_readfirstlane(lds0 + wave * S::BUF);
             auto copy32 = [&](const uint8_t *pages, const Lanes &l0, const Lanes &l1, uint32_t j, uint32_t dst) {
                 if (eights && j + 31u <= last_key) {
@@ -498,7 +515,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
             }
         }
     };
-    const uint64_t rec = ((uint64_t) a.rec_begin[b] + (tile * pieces + pc) * tile_rows) * G + kvh * tile_rows;  // row 0's record
+    const uint64_t rec = ((uint64_t) a.slot[b].rec_begin + (tile * pieces + pc) * tile_rows) * G + kvh * tile_rows;  // row 0's record
     // Channels d .. d + 3 of out row `to`.
     auto store = [&](uint64_t to, uint32_t d, const float4_t &v) {
         if (a.out_f16) {
@@ -509,8 +526,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
         }
     };
     // 1 / (the row's sum with its sink), in the frame of m.
-    auto inverse = [&](float m, float sum, uint32_t head) {
-        const float sink2 = a.sinks ? a.sinks[head] * MOEARC_LOG2E : -INFINITY;
+    auto inverse = [&](float m, float sum, float sink2) {
         const float top = fmaxf(m, sink2), f = __builtin_amdgcn_exp2f(m - top);
         const float total = sum * f + __builtin_amdgcn_exp2f(sink2 - top + MOEARC_AB_LOG2_PSCALE);
         return total == 0.f ? 0.f : f / total;  // a row without keys and without a sink
@@ -525,6 +541,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
         float2_t *const ml = (float2_t *) table;
         __syncthreads();  // (with the places read)
         if (h == 0) ml[wave * 32u + n] = float2_t{m_run, L};
+        if (tid < 32u) ml[128u + tid] = float2_t{sink2, 0.f};
 #pragma unroll
         for (int mb = 0; mb < DB; ++mb)
 #pragma unroll
@@ -543,8 +560,8 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
             sum = fmaf(ml[32 * w + r][1], f[w], sum);
         }
         const uint32_t rt = ab_token(a, rr), head = kvh * group + rr - rt * group;
-        const uint64_t to = ((uint64_t) a.row0[b] + rt) * a.n_heads + head;
-        const float inv = pieces > 1 ? 1.f : inverse(m, sum, head);
+        const uint64_t to = ((uint64_t) tok_row + rt) * n_heads + head;
+        const float inv = pieces > 1 ? 1.f : inverse(m, sum, ml[128 + r][0]);
 #pragma unroll
         for (uint32_t k = 0; k < (uint32_t) DB; ++k) {
             const uint32_t quad = (tid & 7u) + 8u * k;
@@ -573,8 +590,8 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     const uint32_t rr = tile * MOEARC_AB_ROWS + r;
     if (rr >= rows) return;
     const uint32_t rt = ab_token(a, rr), head = kvh * group + rr - rt * group;
-    const uint64_t to = ((uint64_t) a.row0[b] + rt) * a.n_heads + head;
-    const float inv = pieces > 1 ? 1.f : inverse(m_run, L, head);
+    const uint64_t to = ((uint64_t) tok_row + rt) * n_heads + head;
+    const float inv = pieces > 1 ? 1.f : inverse(m_run, L, sink2);
 #pragma unroll
     for (int mb = 0; mb < DB; ++mb)
 #pragma unroll
@@ -591,16 +608,18 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
 // Joins the records of the tiles that were cut, in one pass over a row's pieces with the running maximum. A thread has
 // four channels of a row; work-groups are (tile and KV head, 256 / (head_dim / 4) rows of it).
 __device__ __forceinline__ void ab_merge_body(const AttnBatchArgs &a) {
-    const uint32_t G = a.n_kv_heads, D = a.head_dim, kvh = blockIdx.x % G, at = blockIdx.x / G;
+    const uint32_t G = a.n_kv_heads, D = a.head_dim;
+    const uint32_t at = (uint32_t) ((uint64_t) blockIdx.x * a.kv_magic >> a.kv_shift), kvh = blockIdx.x - at * G;
     const uint32_t b = a.n_slots > 1u ? ab_slot(a.merge_begin, at) : 0u;
-    const uint32_t tile = at - a.merge_begin[b], pieces = a.pieces[b];
-    const uint32_t rows = a.n_new[b] * a.group, tile_rows = rows <= MOEARC_AB_FEW ? 32u : MOEARC_AB_ROWS;
+    const AttnBatchSlot sl = a.slot[b];
+    const uint32_t tile = at - sl.merge_begin, pieces = sl.pieces;
+    const uint32_t rows = sl.n_new * a.group, tile_rows = rows <= MOEARC_AB_FEW ? 32u : MOEARC_AB_ROWS;
     const uint32_t quads = D / 4u, r = blockIdx.y * (256u / quads) + threadIdx.x / quads, d = 4u * (threadIdx.x % quads);
     const uint32_t row = tile * tile_rows + r;
     if (threadIdx.x / quads >= 256u / quads || r >= tile_rows || row >= rows) return;
-    const AbSpan span = ab_span(a, b, tile, tile_rows);
-    const uint32_t np = span.hi > span.lo ? (span.hi - span.lo + a.piece[b] - 1u) / a.piece[b] : 1u;
-    const uint64_t rec0 = ((uint64_t) a.rec_begin[b] + tile * pieces * tile_rows) * G + kvh * tile_rows + r;
+    const AbSpan span = ab_span(a, sl.n_new, sl.n_kv, tile, tile_rows);
+    const uint32_t np = span.hi > span.lo ? (span.hi - span.lo + sl.piece - 1u) / sl.piece : 1u;
+    const uint64_t rec0 = ((uint64_t) sl.rec_begin + tile * pieces * tile_rows) * G + kvh * tile_rows + r;
     const uint64_t step = (uint64_t) G * tile_rows;  // records from piece to piece
     const uint32_t tok = ab_token(a, row), hd = kvh * a.group + row - tok * a.group;
     const float sink2 = a.sinks ? a.sinks[hd] * MOEARC_LOG2E : -INFINITY;
@@ -633,7 +652,7 @@ __device__ __forceinline__ void ab_merge_body(const AttnBatchArgs &a) {
         }
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    const uint64_t to = (((uint64_t) a.row0[b] + tok) * a.n_heads + hd) * D + d;
+    const uint64_t to = (((uint64_t) sl.row0 + tok) * a.n_heads + hd) * D + d;
     if (a.out_f16) {
         const half2_t h0 = {(_Float16) (o[0] * inv), (_Float16) (o[1] * inv)}, h1 = {(_Float16) (o[2] * inv), (_Float16) (o[3] * inv)};
         *(u32x2_t *) ((_Float16 *) a.out + to) = u32x2_t{__builtin_bit_cast(uint32_t, h0), __builtin_bit_cast(uint32_t, h1)};

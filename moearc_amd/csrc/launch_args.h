@@ -387,28 +387,30 @@ struct QkvAppendArgs {
 #define MOEARC_AB_FEW 64u
 #define MOEARC_AB_PT 2044u        // keys' places that a work-group holds at a time (of eight keys each where pages allow)
 #define MOEARC_AB_LOG2_PSCALE 7.0f  // weights are 2^7 at the reference max: f16 keeps 21 bits below it
+struct AttnBatchSlot {
+    uint32_t item_begin, n_tiles, n_new, n_kv;
+    uint32_t seq, row0;             // block-table row; first token's row of q and out
+    uint32_t pieces, piece;         // of a tile's keys; keys each, a multiple of 32
+    uint32_t rec_begin, merge_begin;  // rows of records, per KV head; tiles that need a merge
+    uint32_t pad[2];
+};
 struct AttnBatchArgs {
     const uint16_t *q, *k_pages, *v_pages;
     const uint32_t *block_tables;
     const float *sinks;
+    uint64_t bt_stride;
+    uint32_t n_slots, n_kv_heads, kv_magic, kv_shift;  // x / n_kv_heads = x * magic >> shift for x < 2^31; so
+    uint32_t group, group_magic, group_shift;          // the group
+    uint32_t page_tokens, page_magic, page_shift;      // and page_tokens
+    uint32_t n_swa, n_heads, head_dim;
+    uint32_t eights;                // pages of a multiple of eight tokens
+    uint32_t n_pages;
+    float scale_log2e;
     void *out;
     float *rec_o, *rec_ml;
     uint32_t *err;
-    uint64_t bt_stride;
-    uint32_t n_swa, n_heads, n_kv_heads, group, head_dim;
-    uint32_t page_tokens, page_magic, page_shift;  // x / page_tokens = x * magic >> shift for x < 2^31; so the group
-    uint32_t group_magic, group_shift;
-    uint32_t eights;                // pages of a multiple of eight tokens
-    uint32_t n_pages, out_f16, n_slots, pad;
-    float scale_log2e;
-    uint32_t item_begin[MOEARC_BATCH_SEQS + 1];   // entries n_slots .. the end: the item count
-    uint32_t merge_begin[MOEARC_BATCH_SEQS + 1];  // tiles that need a merge
-    uint32_t seq[MOEARC_BATCH_SEQS];      // block-table row
-    uint32_t row0[MOEARC_BATCH_SEQS];     // first token's row of q and out
-    uint32_t n_new[MOEARC_BATCH_SEQS];
-    uint32_t n_kv[MOEARC_BATCH_SEQS];
-    uint32_t n_tiles[MOEARC_BATCH_SEQS];
-    uint32_t rec_begin[MOEARC_BATCH_SEQS];  // rows of records, per KV head
-    uint32_t piece[MOEARC_BATCH_SEQS];      // keys, a multiple of 32
-    uint32_t pieces[MOEARC_BATCH_SEQS];
+    uint32_t out_f16, pad;
+    uint32_t item_begin[MOEARC_BATCH_SEQS];   // entries n_slots .. the end: the item count
+    uint32_t merge_begin[MOEARC_BATCH_SEQS];
+    AttnBatchSlot slot[MOEARC_BATCH_SEQS];
 };

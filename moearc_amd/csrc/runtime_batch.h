@@ -311,6 +311,7 @@ int moearc_attn_prefill_batched(moearc_ctx *c, void *out, unsigned int out_type,
     a.page_tokens = (uint32_t) page_tokens;
     batch_divisor(page_tokens, a.page_magic, a.page_shift);
     batch_divisor(sh.group, a.group_magic, a.group_shift);
+    batch_divisor(n_kv_heads, a.kv_magic, a.kv_shift);
     a.eights = page_tokens % 8 == 0;
     a.n_pages = (uint32_t) n_pages;
     a.out_f16 = out_type;
@@ -326,18 +327,12 @@ int moearc_attn_prefill_batched(moearc_ctx *c, void *out, unsigned int out_type,
         a.n_slots = p.n;
         uint32_t item = 0, merge = 0;
         uint64_t rec = 0;
-        for (uint32_t i = 0; i <= MOEARC_BATCH_SEQS; ++i) {
+        for (uint32_t i = 0; i < MOEARC_BATCH_SEQS; ++i) {
             a.item_begin[i] = item;
             a.merge_begin[i] = merge;
             if (i >= p.n) continue;
-            a.seq[i] = p.s[i].seq;
-            a.row0[i] = p.s[i].row0;
-            a.n_new[i] = p.s[i].n_new;
-            a.n_kv[i] = p.s[i].n_kv;
-            a.n_tiles[i] = p.n_tiles[i];
-            a.rec_begin[i] = (uint32_t) rec;
-            a.piece[i] = p.piece[i];
-            a.pieces[i] = p.pieces[i];
+            a.slot[i] = AttnBatchSlot{item, p.n_tiles[i], p.s[i].n_new, p.s[i].n_kv, p.s[i].seq, p.s[i].row0,
+                                      p.pieces[i], p.piece[i], (uint32_t) rec, merge, {0u, 0u}};
             item += p.n_tiles[i] * p.pieces[i];
             if (p.pieces[i] > 1) {
                 rec += (uint64_t) p.n_tiles[i] * p.pieces[i] * p.tile_rows[i];
