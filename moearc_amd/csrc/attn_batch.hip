@@ -165,10 +165,11 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     const uint32_t b = n_slots > 1u ? ab_slot(a.item_begin, item) : 0u;
     uint32_t n_new = a.slot[b].n_new, nt = a.slot[b].n_tiles, item0 = a.slot[b].item_begin, n_kv = a.slot[b].n_kv;
     uint32_t seq = a.slot[b].seq, tok_row = a.slot[b].row0, pieces = a.slot[b].pieces, piece = a.slot[b].piece;
+    uint32_t tile_rows = a.slot[b].tile_rows;
     AB_HERE(n_new); AB_HERE(nt); AB_HERE(item0); AB_HERE(n_kv); AB_HERE(seq); AB_HERE(tok_row); AB_HERE(pieces); AB_HERE(piece);
+    AB_HERE(tile_rows);
     const uint32_t rows = n_new * group, in_slot = item - item0;
-    const bool few = rows <= MOEARC_AB_FEW;  // the four waves share 32 rows, each with keys of its own
-    const uint32_t tile_rows = few ? 32u : MOEARC_AB_ROWS;
+    const bool few = tile_rows == 32u;  // the four waves share the rows, each with keys of its own
     const uint32_t pc = pieces > 1u ? in_slot / nt : 0u;
     const uint32_t tile = nt - 1u - (in_slot - pc * nt);  // the latest tile, which has the most keys, first
     const AbSpan span = ab_span(a, n_new, n_kv, tile, tile_rows);
@@ -613,7 +614,7 @@ __device__ __forceinline__ void ab_merge_body(const AttnBatchArgs &a) {
     const uint32_t b = a.n_slots > 1u ? ab_slot(a.merge_begin, at) : 0u;
     const AttnBatchSlot sl = a.slot[b];
     const uint32_t tile = at - sl.merge_begin, pieces = sl.pieces;
-    const uint32_t rows = sl.n_new * a.group, tile_rows = rows <= MOEARC_AB_FEW ? 32u : MOEARC_AB_ROWS;
+    const uint32_t rows = sl.n_new * a.group, tile_rows = sl.tile_rows;
     const uint32_t quads = D / 4u, r = blockIdx.y * (256u / quads) + threadIdx.x / quads, d = 4u * (threadIdx.x % quads);
     const uint32_t row = tile * tile_rows + r;
     if (threadIdx.x / quads >= 256u / quads || r >= tile_rows || row >= rows) return;

@@ -377,14 +377,13 @@ struct QkvAppendArgs {
     uint32_t n_kv[MOEARC_BATCH_SEQS];
 };
 
-// Attention of a ragged batch. A sequence's rows (token, head of the KV head's group) are cut into tiles -- of 128
-// rows, or of 32 where there are at most MOEARC_AB_FEW -- and a tile's keys into pieces of piece[b]; a work-group takes one
-// piece of one tile for one KV head. Slot b's work items (tiles x pieces) start at item_begin[b]; a slot with more
-// than one piece to a tile leaves records that the merge kernel joins (rows of a tile: tr):
-//   rec_o[(rec_begin[b] + (tile * pieces + piece) * tr) * n_kv_heads + kvh * tr + row][head_dim]  un-normalised (f32)
+// Attention of a ragged batch. A sequence's rows (token, head of the KV head's group) are cut into tiles of 128 or 32
+// rows, a tile's keys into pieces; a work-group takes one piece of one tile for one KV head. A slot's work items (tiles x
+// pieces) start at item_begin; a slot with more than one piece to a tile leaves records that the merge kernel joins (tr:
+// rows of a tile):
+//   rec_o[(rec_begin + (tile * pieces + piece) * tr) * n_kv_heads + kvh * tr + row][head_dim]  un-normalised (f32)
 //   rec_ml[the same row index][2]   reference max (log2 domain), row sum in its frame
 #define MOEARC_AB_ROWS 128u       // rows of a tile: 32 to a wave
-#define MOEARC_AB_FEW 64u
 #define MOEARC_AB_PT 2044u        // keys' places that a work-group holds at a time (of eight keys each where pages allow)
 #define MOEARC_AB_LOG2_PSCALE 7.0f  // weights are 2^7 at the reference max: f16 keeps 21 bits below it
 struct AttnBatchSlot {
@@ -392,7 +391,7 @@ struct AttnBatchSlot {
     uint32_t seq, row0;             // block-table row; first token's row of q and out
     uint32_t pieces, piece;         // of a tile's keys; keys each, a multiple of 32
     uint32_t rec_begin, merge_begin;  // rows of records, per KV head; tiles that need a merge
-    uint32_t pad[2];
+    uint32_t tile_rows, pad;
 };
 struct AttnBatchArgs {
     const uint16_t *q, *k_pages, *v_pages;

@@ -6,7 +6,6 @@ namespace {
 
 constexpr unsigned long kBatchRows = 1ul << 20;  // new tokens of a call: launches stay below 2^32 threads
 constexpr unsigned long kBatchHeads = 1024;
-#define MOEARC_AB_MIN_CHUNKS 16  // of a piece of few rows' keys: four tiles a wave
 
 bool batch_load(moearc_ctx *c) {
     struct {
@@ -52,7 +51,7 @@ void batch_arm(moearc_ctx *c) {
 // What the plan of a group of sequences (at most MOEARC_BATCH_SEQS) needs to know of the call.
 struct BatchShape {
     unsigned long n_swa, group, n_kv_heads, head_dim;
-    unsigned wgs;  // work-groups that the device holds at once
+    unsigned cus, wgs;  // work-groups that the device holds at once
 };
 
 struct BatchSeq {
@@ -87,14 +86,22 @@ unsigned long batch_take(BatchPlan &p, const unsigned int *row_begin, const unsi
     return at;
 }
 
-// Tiles, and pieces where a tile's keys would keep one work-group longer than the whole work keeps the device: with
-// fewer, all work-groups run at once and the longest decides. Work is counted in 32-key chunks of a tile of few rows, whose
-// work-group takes four at a time; a full tile's takes one.
+// Tiles: of 128 rows, their waves in step on the same keys, or of 32, each wave with keys of its own, which read K and V
+// once per tile as well. The latter for a sequence of up to 64 rows, or of up to 256 where full tiles would leave half of the
+// CUs without work. Measured, full and small tiles, us: four sequences of 16 tokens behind 1500, 64 heads over 8 KV heads of 64
+// channels 20.2 and 16.8, of 32 tokens 21.0 and 19.5; 32 such sequences 45.4 and 47.4, 49.6 and 77.3; 64 behind 100, 13.9 and 23.5.
+// Pieces: where a tile's keys would keep one work-group longer than the whole work keeps the device; with fewer, all
+// work-groups run at once and the longest decides. Work is counted in 32-key chunks of a small tile, whose work-group takes four
+// at a time; a full tile's takes one. A piece has at least four of these steps, a full tile's sixteen: drafts of 3 to 7 tokens behind
+// 500 to 3000 take 15.5 us, 15.2 with half as many, 20.3 with twice; a full tile's pieces of eight chunks cost 2 us of 30.
 void batch_plan(BatchPlan &p, const BatchShape &sh, bool may_split) {
-    uint64_t total = 0, most = 0, longest[MOEARC_BATCH_SEQS];
+    uint64_t total = 0, most = 0, longest[MOEARC_BATCH_SEQS], full_wgs = 0;
+    for (uint32_t i = 0; i < p.n; ++i)
+        full_wgs += ((uint64_t) p.s[i].n_new * sh.group + MOEARC_AB_ROWS - 1) / MOEARC_AB_ROWS * sh.n_kv_heads;
+    const uint64_t few = 2 * full_wgs <= sh.cus ? 256 : 64;
     for (uint32_t i = 0; i < p.n; ++i) {
         const uint64_t rows = (uint64_t) p.s[i].n_new * sh.group;
-        p.tile_rows[i] = rows <= MOEARC_AB_FEW ? 32u : MOEARC_AB_ROWS;
+        p.tile_rows[i] = rows <= few ? 32u : MOEARC_AB_ROWS;
         p.n_tiles[i] = (uint32_t) ((rows + p.tile_rows[i] - 1) / p.tile_rows[i]);
         longest[i] = 1;
         uint64_t sum = 0;
@@ -107,9 +114,7 @@ void batch_plan(BatchPlan &p, const BatchShape &sh, bool may_split) {
         total += sum * cost;
         most = std::max(most, longest[i] * cost);
     }
-    static const uint64_t mn = getenv("AB_MIN") ? atoi(getenv("AB_MIN")) : MOEARC_AB_MIN_CHUNKS;
-    static const uint64_t R = getenv("AB_R") ? atoi(getenv("AB_R")) : 100;
-    uint64_t even = std::max<uint64_t>(mn, (total * sh.n_kv_heads + sh.wgs * R / 100 - 1) / (sh.wgs * R / 100));
+    uint64_t even = std::max<uint64_t>(16, (total * sh.n_kv_heads + sh.wgs - 1) / sh.wgs);
     const bool split = may_split && most > even + even / 4;
     // Pieces that together are a few more than the device holds at once would run in a second round: longer ones.
     auto cut = [&](uint32_t i) {
@@ -123,7 +128,7 @@ void batch_plan(BatchPlan &p, const BatchShape &sh, bool may_split) {
     for (int k = 0; k < 8; ++k) {
         uint64_t wgs = 0;
         for (uint32_t i = 0; i < p.n; ++i) wgs += cut(i) * sh.n_kv_heads;
-        if (!split || R != 100 || wgs <= sh.wgs || wgs >= 2 * sh.wgs) break;
+        if (!split || wgs <= sh.wgs || wgs >= 2 * sh.wgs) break;
         even += even / 16 + 1;
     }
     p.items = p.merge_tiles = p.merge_rows = 0;
@@ -159,7 +164,7 @@ int attn_batch_check(unsigned long n_heads, unsigned long n_kv_heads, unsigned l
 
 BatchShape batch_shape(const moearc_ctx *c, unsigned long n_heads, unsigned long n_kv_heads, unsigned long head_dim, unsigned long n_swa) {
     const unsigned cu = c->n_cu ? c->n_cu : 256;
-    return BatchShape{n_swa, n_heads / n_kv_heads, n_kv_heads, head_dim, cu * (head_dim <= 64 ? 3u : head_dim <= 128 ? 2u : 1u)};
+    return BatchShape{n_swa, n_heads / n_kv_heads, n_kv_heads, head_dim, cu, cu * (head_dim <= 64 ? 3u : head_dim <= 128 ? 2u : 1u)};
 }
 
 }  // namespace
@@ -332,7 +337,7 @@ int moearc_attn_prefill_batched(moearc_ctx *c, void *out, unsigned int out_type,
             a.merge_begin[i] = merge;
             if (i >= p.n) continue;
             a.slot[i] = AttnBatchSlot{item, p.n_tiles[i], p.s[i].n_new, p.s[i].n_kv, p.s[i].seq, p.s[i].row0,
-                                      p.pieces[i], p.piece[i], (uint32_t) rec, merge, {0u, 0u}};
+                                      p.pieces[i], p.piece[i], (uint32_t) rec, merge, p.tile_rows[i], 0u};
             item += p.n_tiles[i] * p.pieces[i];
             if (p.pieces[i] > 1) {
                 rec += (uint64_t) p.n_tiles[i] * p.pieces[i] * p.tile_rows[i];

@@ -178,9 +178,16 @@ def test_memory_of_the_context(cx, lib):
 
 
 def test_attention_grids(cx, lib):
-    # tiles of 128 (token, head) rows x KV heads; sequences without new tokens take no place in a launch
-    assert attend(cx, rows=(0, 100, 100, 132), n_kv=(100, 50, 40), n_heads=16, n_kv_heads=2, bt_stride=9) == 0
-    assert launches(lib) == [("moearc_attn_batch_d2_k", (7 + 2) * 2, 1, 1, 256)]
+    # tiles of 128 (token, head) rows x KV heads, of 32 for the few rows of a sequence; sequences without new tokens take no
+    # place in a launch
+    assert attend(cx, rows=(0, 100, 100, 132, 140), n_kv=(100, 50, 40, 9), n_heads=16, n_kv_heads=2, bt_stride=9) == 0
+    assert launches(lib) == [("moearc_attn_batch_d2_k", (7 + 8 + 2) * 2, 1, 1, 256)]
+    lib.host_hip_reset()  # full tiles give half of the CUs work: 64 rows are few, 65 are not
+    assert attend(cx, rows=(0, 1008, 1016, 1025), n_kv=(1008, 8, 9), n_heads=16, n_kv_heads=2, bt_stride=99) == 0
+    assert launches(lib) == [("moearc_attn_batch_d2_k", (63 + 1 + 3) * 2, 1, 1, 256)]
+    lib.host_hip_reset()
+    assert attend(cx, rows=(0, 1024, 1032, 1041), n_kv=(1024, 8, 9), n_heads=16, n_kv_heads=2, bt_stride=99) == 0
+    assert launches(lib) == [("moearc_attn_batch_d2_k", (64 + 2 + 1) * 2, 1, 1, 256)]
     lib.host_hip_reset()
     rows = np.concatenate([[0], np.cumsum([b % 2 for b in range(200)])]).tolist()
     assert attend(cx, rows=rows, n_kv=[60] * 200) == 0
