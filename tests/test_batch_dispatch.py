@@ -182,12 +182,11 @@ def test_attention_grids(cx, lib):
     # place in a launch
     assert attend(cx, rows=(0, 100, 100, 132, 140), n_kv=(100, 50, 40, 9), n_heads=16, n_kv_heads=2, bt_stride=9) == 0
     assert launches(lib) == [("moearc_attn_batch_d2_k", (7 + 8 + 2) * 2, 1, 1, 256)]
-    lib.host_hip_reset()  # full tiles give half of the CUs work: 64 rows are few, 65 are not
-    assert attend(cx, rows=(0, 1008, 1016, 1025), n_kv=(1008, 8, 9), n_heads=16, n_kv_heads=2, bt_stride=99) == 0
-    assert launches(lib) == [("moearc_attn_batch_d2_k", (63 + 1 + 3) * 2, 1, 1, 256)]
-    lib.host_hip_reset()
-    assert attend(cx, rows=(0, 1024, 1032, 1041), n_kv=(1024, 8, 9), n_heads=16, n_kv_heads=2, bt_stride=99) == 0
-    assert launches(lib) == [("moearc_attn_batch_d2_k", (64 + 2 + 1) * 2, 1, 1, 256)]
+    # up to 256 rows are few while full tiles would be work-groups for at most half of the CUs, 64 beyond
+    for tokens, want in ((992, 62 + 2 + 3), (1008, 63 + 2 + 1)):
+        lib.host_hip_reset()
+        assert attend(cx, rows=(0, tokens, tokens + 8, tokens + 17), n_kv=(tokens, 8, 9), n_heads=16, n_kv_heads=2, bt_stride=99, n_swa=16) == 0
+        assert launches(lib) == [("moearc_attn_batch_d2_k", want * 2, 1, 1, 256)]
     lib.host_hip_reset()
     rows = np.concatenate([[0], np.cumsum([b % 2 for b in range(200)])]).tolist()
     assert attend(cx, rows=rows, n_kv=[60] * 200) == 0
