@@ -430,7 +430,7 @@ int moearc_moe_ffn(moearc_ctx *c, const moearc_moe *m, void *y, const void *x, u
  * a decode step's one, a draft's few, a prompt chunk's many -- in one append and one attention call. Both take
  * the batch alike: rows row_begin[b] .. row_begin[b + 1] - 1 of q and out are sequence b's n new tokens
  * (none is allowed), row_begin HOST u32 [n_seqs + 1], ascending; n_kv HOST u32 [n_seqs] its keys with these among
- * them, below 2^31, so that new token i sits at position n_kv[b] - n + i; block_tables (device) row b at
+ * them, below 2^30, so that new token i sits at position n_kv[b] - n + i; block_tables (device) row b at
  * block_tables + b * bt_stride, ids below n_pages, the pages of each pool. Rows before row_begin[0] and from
  * row_begin[n_seqs] on are left as they are; at most 2^20 rows. A captured call keeps the lengths that it was
  * given. A block-table entry >= n_pages is never used as an address, and the next moearc_sync returns -1 (after any
@@ -479,8 +479,10 @@ int moearc_attn_prefill_batched_workspace(moearc_ctx *c, const unsigned int *row
 /* Attention of every new token over its sequence's keys up to itself (with n_swa the last n_swa of them), whose K and V
  * are in the cache: row i of sequence b is moearc_attn_decode at n_kv = p + 1, p its position. q f16
  * [row][n_heads][head_dim]; out the same, f32 or f16 by out_type; sinks f32 [n_heads] or NULL. A row at a negative position
- * is zero. K and V of keys that a row does not see do not reach it, infinities and NaN among them; slots from
- * n_kv[b] on are not read. Any group, any page size, head_dim a multiple of 8 up to 256; q, out and the pools 16-byte
+ * is zero. K and V of keys that a row does not see do not reach it, infinities and NaN among them (a call whose
+ * accumulators stop being finite runs twice); slots from n_kv[b] on are not read. A row that sees a NaN, or a score that is
+ * one or +infinity, is NaN; with a head_dim other than 64, 128 and 256 an infinity in the first eight channels of a key makes
+ * one. Scores, and scale times any, have to stay within f32. Any group, any page size, head_dim a multiple of 8 up to 256; q, out and the pools 16-byte
  * aligned; kv_type 1 (f16).
  * Precision: exact f16 products summed in f32. An f16 out rounds each softmax weight to f16 once, to 2^-11 of it
  * (the output's own rounding is as much, of a sum in which these average out); an f32 out carries it as f16 hi + lo,

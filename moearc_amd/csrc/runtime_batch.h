@@ -34,7 +34,7 @@ bool batch_load(moearc_ctx *c) {
 int batch_check(const unsigned int *row_begin, const unsigned int *n_kv, unsigned long n_seqs, unsigned long bt_stride,
                 unsigned long page_tokens) {
     for (unsigned long b = 0; b < n_seqs; ++b) {
-        if (row_begin[b + 1] < row_begin[b] || n_kv[b] >= (1u << 31)) return ERR_ARG;
+        if (row_begin[b + 1] < row_begin[b] || n_kv[b] >= (1u << 30)) return ERR_ARG;
         if (row_begin[b + 1] != row_begin[b] && (n_kv[b] + page_tokens - 1) / page_tokens > bt_stride) return ERR_ARG;
     }
     return n_seqs && row_begin[n_seqs] > kBatchRows ? ERR_ARG : OK;
@@ -65,14 +65,20 @@ struct BatchPlan {
     uint32_t tile_rows[MOEARC_BATCH_SEQS], n_tiles[MOEARC_BATCH_SEQS], pieces[MOEARC_BATCH_SEQS], piece[MOEARC_BATCH_SEQS];
 };
 
-// Keys of tile t's span, in 32-key chunks (attn_batch.hip's ab_span; it may start up to seven keys earlier).
-uint64_t batch_chunks(const BatchSeq &s, const BatchShape &sh, uint64_t tile_rows, uint64_t t) {
+// The 32-key chunks of a sequence's tiles (attn_batch.hip's ab_span): at most `longest` in one, about `sum` in all.
+struct BatchWork {
+    uint64_t longest, sum;
+};
+BatchWork batch_work(const BatchSeq &s, const BatchShape &sh, uint64_t tile_rows, uint64_t n_tiles) {
     const int64_t shift = (int64_t) s.n_kv - s.n_new;
-    const int64_t tok0 = (int64_t) (t * tile_rows / sh.group);
-    const int64_t tok1 = std::min<int64_t>((int64_t) ((t * tile_rows + tile_rows - 1) / sh.group), (int64_t) s.n_new - 1);
-    const int64_t hi = std::max<int64_t>(0, shift + tok1 + 1), first = std::max<int64_t>(0, shift + tok0);
-    const int64_t lo = sh.n_swa && first + 1 > (int64_t) sh.n_swa ? (first + 1 - (int64_t) sh.n_swa) / 8 * 8 : 0;
-    return hi > lo ? (uint64_t) (hi - lo + 31) / 32 : 0;
+    auto chunks = [&](uint64_t last_row) {  // without a window, up to this row's token
+        const int64_t hi = shift + std::min<int64_t>((int64_t) (last_row / sh.group), (int64_t) s.n_new - 1) + 1;
+        return hi > 0 ? (uint64_t) (hi + 31) / 32 : 0ull;
+    };
+    const uint64_t first = chunks(tile_rows - 1), last = chunks(n_tiles * tile_rows - 1);
+    // a window's keys, those of a tile's other tokens, and up to seven that the first page of eights has before them
+    const uint64_t window = sh.n_swa ? (sh.n_swa + (tile_rows + sh.group - 1) / sh.group + 7 + 31) / 32 : ~0ull;
+    return BatchWork{std::max<uint64_t>(1, std::min(last, window)), n_tiles * std::min((first + last + 1) / 2, window)};
 }
 
 // Sequences from `at` on that one launch carries; those without new tokens are passed over. The ones with the most keys
@@ -103,15 +109,10 @@ void batch_plan(BatchPlan &p, const BatchShape &sh, bool may_split) {
         const uint64_t rows = (uint64_t) p.s[i].n_new * sh.group;
         p.tile_rows[i] = rows <= few ? 32u : MOEARC_AB_ROWS;
         p.n_tiles[i] = (uint32_t) ((rows + p.tile_rows[i] - 1) / p.tile_rows[i]);
-        longest[i] = 1;
-        uint64_t sum = 0;
-        for (uint64_t t = 0; t < p.n_tiles[i]; ++t) {
-            const uint64_t n = batch_chunks(p.s[i], sh, p.tile_rows[i], t);
-            sum += n;
-            longest[i] = std::max(longest[i], n);
-        }
+        const BatchWork w = batch_work(p.s[i], sh, p.tile_rows[i], p.n_tiles[i]);
+        longest[i] = w.longest;
         const uint64_t cost = p.tile_rows[i] == MOEARC_AB_ROWS ? 4 : 1;
-        total += sum * cost;
+        total += w.sum * cost;
         most = std::max(most, longest[i] * cost);
     }
     uint64_t even = std::max<uint64_t>(16, (total * sh.n_kv_heads + sh.wgs - 1) / sh.wgs);

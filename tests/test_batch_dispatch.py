@@ -62,7 +62,8 @@ NAN, INF = float("nan"), float("inf")
     (dict(q_stride=255), -2), (dict(k_stride=127), -2), (dict(v_stride=127), -2), (dict(q_stride=1 << 40), -2), (dict(freq_base=0.0), -2),
     (dict(freq_base=NAN), -2), (dict(freq_base=INF), -2), (dict(freq_scale=0.0), -2), (dict(freq_scale=NAN), -2), (dict(eps=-1.0), 0),
     (dict(eps=-1.0, q_norm=64), -2), (dict(eps=NAN, k_norm=64), -2), (dict(eps=0.0, k_norm=64), 0), (dict(rows=(0, 3, 1)), -2),
-    (dict(n_kv=(1 << 31, 9)), -2), (dict(n_kv=(5, 65)), -2), (dict(n_kv=(5, 64)), 0), (dict(rows=(0, 1, 1), n_kv=(5, 65)), 0),
+    (dict(n_kv=(1 << 31, 9)), -2), (dict(n_kv=(1 << 30, 9), bt_stride=1 << 30), -2), (dict(n_kv=((1 << 30) - 1, 9), bt_stride=1 << 30), 0),
+    (dict(n_kv=(5, 65)), -2), (dict(n_kv=(5, 64)), 0), (dict(rows=(0, 1, 1), n_kv=(5, 65)), 0),
     (dict(rows=(0, 1, (1 << 20) + 1)), -2), (dict(rows=(0, 1, 1 << 20)), 0), (dict(rows=(3, 3, 3)), 0), (dict(rows=(0,), n_kv=()), 0)], ids=str)
 def test_append_refusals(cx, lib, kw, rc):
     assert append(cx, **kw) == rc
