@@ -93,9 +93,11 @@ unsigned long batch_take(BatchPlan &p, const unsigned int *row_begin, const unsi
 }
 
 // Tiles: of 128 rows, their waves in step on the same keys, or of 32, each wave with keys of its own, which read K and V
-// once per tile as well. The latter for a sequence of up to 64 rows, or of up to 256 where full tiles would leave half of the
-// CUs without work. Measured, full and small tiles, us: four sequences of 16 tokens behind 1500, 64 heads over 8 KV heads of 64
-// channels 20.2 and 16.8, of 32 tokens 21.0 and 19.5; 32 such sequences 45.4 and 47.4, 49.6 and 77.3; 64 behind 100, 13.9 and 23.5.
+// once per tile as well. The latter for a sequence of up to 64 rows, and where full tiles would leave half of the CUs
+// without work, for one of up to 256 rows or 2560 keys. Measured, full and small tiles, us: 64 heads over 8 KV heads of 64 channels,
+// four sequences of 16 tokens behind 1500 20.2 and 16.8, of 32 tokens 21.0 and 19.5; 32 such sequences 45.4 and 47.4, 49.6 and 77.3; 64
+// behind 100, 13.9 and 23.5; one of 200 behind 800 23.1 and 16.7. 32 heads over 4 of 128, one of 300 15.8 and 13.2, of 500 behind
+// 2000 44.6 and 40.5, of 100 behind 16,000 48.9 and 53.2, of 512 behind 32,700 304 and 390, two of 128 behind 4000 37.8 and 41.2.
 // Pieces: where a tile's keys would keep one work-group longer than the whole work keeps the device; with fewer, all
 // work-groups run at once and the longest decides. Work is counted in 32-key chunks of a small tile, whose work-group takes four
 // at a time; a full tile's takes one. A piece has at least four of these steps, a full tile's sixteen: drafts of 3 to 7 tokens behind
@@ -104,10 +106,10 @@ void batch_plan(BatchPlan &p, const BatchShape &sh, bool may_split) {
     uint64_t total = 0, most = 0, longest[MOEARC_BATCH_SEQS], full_wgs = 0;
     for (uint32_t i = 0; i < p.n; ++i)
         full_wgs += ((uint64_t) p.s[i].n_new * sh.group + MOEARC_AB_ROWS - 1) / MOEARC_AB_ROWS * sh.n_kv_heads;
-    const uint64_t few = 2 * full_wgs <= sh.cus ? 256 : 64;
+    const bool idle = 2 * full_wgs <= sh.cus;
     for (uint32_t i = 0; i < p.n; ++i) {
         const uint64_t rows = (uint64_t) p.s[i].n_new * sh.group;
-        p.tile_rows[i] = rows <= few ? 32u : MOEARC_AB_ROWS;
+        p.tile_rows[i] = rows <= 64 || (idle && (rows <= 256 || p.s[i].n_kv <= 2560)) ? 32u : MOEARC_AB_ROWS;
         p.n_tiles[i] = (uint32_t) ((rows + p.tile_rows[i] - 1) / p.tile_rows[i]);
         const BatchWork w = batch_work(p.s[i], sh, p.tile_rows[i], p.n_tiles[i]);
         longest[i] = w.longest;

@@ -60,27 +60,32 @@ class Batch:
         out, tol = (np.full((self.n_rows, self.heads, self.dim), np.nan) for _ in range(2))
         r = 2.0 ** -11 if out_type == OUT_F16 else 2.0 ** -22
         for b, (m, n) in enumerate(zip(self.new, self.n_kv)):
-            for i in range(m):
-                row, p = int(self.rows[b]) + i, n - m + i
-                if p < 0:
-                    out[row], tol[row] = 0.0, 0.0
-                    continue
-                lo = max(0, p + 1 - window) if window else 0
-                for h in range(self.heads):
-                    k, v = self.keys(b, h * self.kv_heads // self.heads, lo, p + 1)
-                    q = self.q[row, h].astype(np.float64)
-                    s = scale * (k @ q)
-                    size = abs(scale) * (np.abs(k) @ np.abs(q)).max()
-                    top = max(s.max(), self.sinks[h] if self.sinks is not None else -np.inf)
-                    w = np.exp(s - top)
-                    total = w.sum() + (np.exp(self.sinks[h] - top) if self.sinks is not None else 0.0)
-                    w /= total
-                    o = w @ v
-                    e = (self.dim + 8) * U * size + 8 * U * (np.abs(s).max() + abs(top) + 16) + r
-                    spread = w @ np.abs(v - o) + (1 - w.sum()) * np.abs(o)
-                    bound = 1.01 * e * spread + (len(s) + 8) * U * (w @ np.abs(v)) + len(s) * 2.0 ** -31 * np.abs(v).max()
-                    step = 2.0 ** -11 * np.abs(o) + 2.0 ** -25 if out_type == OUT_F16 else U * np.abs(o)
-                    out[row, h], tol[row, h] = o, bound + 1.01 * step
+            if m == 0:
+                continue
+            p = np.arange(n - m, n)[:, None]
+            first = max(0, n - m + 1 - window) if window else 0
+            j = np.arange(first, n)
+            sees = (j <= p) & ((p - j < window) if window else True) & (p >= 0)
+            count = sees.sum(1)[:, None]
+            at = slice(int(self.rows[b]), int(self.rows[b]) + m)
+            for h in range(self.heads):
+                k, v = self.keys(b, h * self.kv_heads // self.heads, first, n)
+                q = self.q[at, h].astype(np.float64)
+                s = np.where(sees, scale * (q @ k.T), -np.inf)
+                size = np.where(sees, abs(scale) * (np.abs(q) @ np.abs(k).T), 0).max(1, initial=0)[:, None]
+                sink = self.sinks[h] if self.sinks is not None else -np.inf
+                top = np.maximum(s.max(1, initial=-np.inf), sink)[:, None]
+                top = np.where(np.isfinite(top), top, 0)
+                w = np.exp(s - top)
+                total = w.sum(1, keepdims=True) + np.exp(sink - top)
+                w = w / np.where(total == 0, 1, total)
+                o, mass = w @ v, w.sum(1, keepdims=True)
+                e = (self.dim + 8) * U * size + 8 * U * (np.abs(np.where(sees, s, 0)).max(1, initial=0)[:, None] + np.abs(top) + 16) + r
+                # sum w|v - out| <= sqrt(sum w sum w (v - out)^2)
+                spread = np.sqrt(mass * np.maximum(0, w @ (v * v) - 2 * o * o + o * o * mass)) + (1 - mass) * np.abs(o)
+                bound = 1.01 * e * spread + (count + 8) * U * (w @ np.abs(v)) + count * 2.0 ** -31 * np.abs(v).max(initial=0)
+                step = 2.0 ** -11 * np.abs(o) + 2.0 ** -25 if out_type == OUT_F16 else U * np.abs(o)
+                out[at, h], tol[at, h] = o, np.where(count > 0, bound + 1.01 * step, 0)
         return out, tol
 
 

@@ -182,11 +182,11 @@ def test_attention_grids(cx, lib):
     # tiles of 128 (token, head) rows x KV heads, of 32 for the few rows of a sequence; sequences without new tokens take no
     # place in a launch
     assert attend(cx, rows=(0, 100, 100, 132, 140), n_kv=(100, 50, 40, 9), n_heads=16, n_kv_heads=2, bt_stride=9) == 0
-    assert launches(lib) == [("moearc_attn_batch_d2_k", (7 + 8 + 2) * 2, 1, 1, 256)]
-    # up to 256 rows are few while full tiles would be work-groups for at most half of the CUs, 64 beyond
-    for tokens, want in ((992, 62 + 2 + 3), (1008, 63 + 2 + 1)):
+    assert launches(lib) == [("moearc_attn_batch_d2_k", (25 + 8 + 2) * 2, 1, 1, 256)]
+    # up to 64 rows are few; while full tiles would be work-groups for at most half of the CUs, up to 256 or of up to 2560 keys
+    for tokens, keys, want in ((992, 2561, 62 + 2 + 3), (992, 2560, 248 + 2 + 3), (1008, 2560, 63 + 2 + 1)):
         lib.host_hip_reset()
-        assert attend(cx, rows=(0, tokens, tokens + 8, tokens + 17), n_kv=(tokens, 8, 9), n_heads=16, n_kv_heads=2, bt_stride=99, n_swa=16) == 0
+        assert attend(cx, rows=(0, tokens, tokens + 8, tokens + 17), n_kv=(keys, 8, 2570), n_heads=16, n_kv_heads=2, bt_stride=999, n_swa=16) == 0
         assert launches(lib) == [("moearc_attn_batch_d2_k", want * 2, 1, 1, 256)]
     lib.host_hip_reset()
     rows = np.concatenate([[0], np.cumsum([b % 2 for b in range(200)])]).tolist()
