@@ -482,8 +482,8 @@ int moearc_attn_prefill_batched_workspace(moearc_ctx *c, const unsigned int *row
  * is zero. K and V of keys that a row does not see do not reach it, infinities and NaN among them (a call whose
  * accumulators stop being finite runs twice); slots from n_kv[b] on are not read. A row that sees a NaN, or a score that is
  * one or +infinity, is NaN; with a head_dim other than 64, 128 and 256 an infinity in the first eight channels of a key makes
- * one. Scores, and scale times any, have to stay within f32. Any group, any page size, head_dim a multiple of 8 up to 256; q, out and the pools 16-byte
- * aligned; kv_type 1 (f16).
+ * one. q . k, and scale times it, have to stay below 10^29. Any group, any page size, head_dim a multiple of 8 up to 256; q, out
+ * and the pools 16-byte aligned; kv_type 1 (f16).
  * Precision: exact f16 products summed in f32. An f16 out rounds each softmax weight to f16 once, to 2^-11 of it
  * (the output's own rounding is as much, of a sum in which these average out); an f32 out carries it as f16 hi + lo,
  * to 2^-22 of it; either to 2^-32 of the row's largest weight where that is more.
@@ -491,8 +491,8 @@ int moearc_attn_prefill_batched_workspace(moearc_ctx *c, const unsigned int *row
  * done; NULL: the context's, grown on demand (calls that find none run without it, slower). A captured call whose
  * workspace is not 0 needs ws (else -1), and graphs that may run at the same time need one each. Refusals: a null
  * pointer other than sinks and ws -> -1; kv_type not 1, out_type not 0/1, n_heads 0 or above 1024, n_kv_heads 0 or no
- * divisor of it, head_dim as above, n_swa >= 2^31, page_tokens 0 or above 2^30, n_pages 0 or above 2^32 - 1, a scale that is
- * not finite (times log2 e), an address off its alignment, row_begin descending, more rows or keys than the above,
+ * divisor of it, head_dim as above, n_swa >= 2^31, page_tokens 0 or above 2^30, n_pages 0 or above (2^32 - 1) / page_tokens, a
+ * scale that is not finite (times log2 e), an address off its alignment, row_begin descending, more rows or keys than the above,
  * bt_stride < ceil(n_kv[b] / page_tokens) of a sequence with new tokens, a ws too small or misaligned -> -2. No rows -> 0. */
 int moearc_attn_prefill_batched(moearc_ctx *c, void *out, unsigned int out_type, const void *q, const void *k_pages,
                                 const void *v_pages, unsigned long n_pages, const unsigned int *block_tables,

@@ -380,10 +380,20 @@ class Context:
         self.finish(rc, "chunked prefill attention")
 
     # ---- ragged batches -----------------------------------------------------------------------
-    def _batch(self, block_tables: DeviceBuffer, bt_stride: int, row_begin, n_kv):
-        rb, nk = np.ascontiguousarray(row_begin, np.uint32), np.ascontiguousarray(n_kv, np.uint32)
+    @staticmethod
+    def _lengths(row_begin, n_kv):
+        rb, nk = (np.asarray(x) if len(x) else np.zeros(0, np.uint32) for x in (row_begin, n_kv))
+        for x in (rb, nk):  # a conversion to u32 would wrap what lies outside
+            if x.dtype.kind not in "iu" or x.ndim != 1 or (x.size and (x.min() < 0 or x.max() > 0xFFFFFFFF)):
+                raise BadArgument("row_begin and n_kv are sequences of 32-bit unsigned integers")
         if rb.size != nk.size + 1:
             raise BadArgument("row_begin has one entry more than n_kv")
+        return np.ascontiguousarray(rb, np.uint32), np.ascontiguousarray(nk, np.uint32)
+
+    def _batch(self, block_tables: DeviceBuffer, bt_stride: int, row_begin, n_kv):
+        rb, nk = self._lengths(row_begin, n_kv)
+        if bt_stride < 0:
+            raise BadArgument("a negative bt_stride")
         block_tables.require("block tables", nk.size * bt_stride * 4)
         return rb, nk, int(rb[-1])
 
@@ -399,9 +409,7 @@ class Context:
     def attn_prefill_batched_workspace(self, row_begin, n_kv, n_swa: int, n_heads: int, n_kv_heads: int,
                                        head_dim: int) -> int:
         """Bytes of working memory of attn_prefill_batched at these lengths (0: none)."""
-        rb, nk = np.ascontiguousarray(row_begin, np.uint32), np.ascontiguousarray(n_kv, np.uint32)
-        if rb.size != nk.size + 1:
-            raise BadArgument("row_begin has one entry more than n_kv")
+        rb, nk = self._lengths(row_begin, n_kv)
         n = ctypes.c_ulong()
         _check(self._lib.moearc_attn_prefill_batched_workspace(self.raw, rb.ctypes.data, nk.ctypes.data, nk.size, n_swa,
                                                                n_heads, n_kv_heads, head_dim, ctypes.byref(n)),

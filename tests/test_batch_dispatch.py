@@ -119,7 +119,8 @@ def attend(cx, rows=(0, 1, 3), n_kv=(5, 9), **kw):
     (dict(sinks=64), 0), (dict(kv_type=0), -2), (dict(out_type=2), -2), (dict(n_heads=0), -2), (dict(n_heads=5), -2), (dict(n_kv_heads=0), -2),
     (dict(n_heads=1026), -2), (dict(head_dim=0), -2), (dict(head_dim=60), -2), (dict(head_dim=264), -2), (dict(head_dim=8), 0),
     (dict(head_dim=256), 0), (dict(n_swa=1 << 31), -2), (dict(n_swa=(1 << 31) - 1), 0), (dict(page_tokens=0), -2),
-    (dict(page_tokens=(1 << 30) + 1), -2), (dict(n_pages=0), -2), (dict(n_pages=1 << 32), -2), (dict(scale=NAN), -2), (dict(scale=INF), -2),
+    (dict(page_tokens=(1 << 30) + 1), -2), (dict(n_pages=0), -2), (dict(n_pages=1 << 32), -2), (dict(n_pages=1 << 28), -2),
+    (dict(n_pages=(1 << 28) - 1), 0), (dict(scale=NAN), -2), (dict(scale=INF), -2),
     (dict(scale=2.9e38), -2), (dict(scale=-1.0), 0), (dict(scale=0.0), 0), (dict(out=(1 << 33) + 8), -2), (dict(q=(1 << 34) + 2), -2),
     (dict(k_pages=(1 << 35) + 4), -2), (dict(v_pages=(1 << 36) + 8), -2), (dict(rows=(0, 3, 1)), -2), (dict(n_kv=(1 << 31, 9)), -2),
     (dict(n_kv=(5, 65)), -2), (dict(n_kv=(5, 64)), 0), (dict(rows=(0, 1, 1), n_kv=(5, 65)), 0), (dict(rows=(0, 1, (1 << 20) + 1)), -2),
@@ -241,6 +242,31 @@ def test_wrapper_checks(cx, lib):
             attn(**kw)
     with pytest.raises(BadArgument):
         cx.attn_prefill_batched_workspace((0, 1, 2), (5,), 0, 4, 2, 64)
+
+
+def test_wrapper_lengths(cx, lib):
+    """What does not fit 32 bits is refused before it wraps into a length that the library would take."""
+    b = lambda n: at(cx, 1 << 34, n)
+    d = QkvAppendDesc.make(q=b(BIG), k=b(BIG), v=b(BIG), q_out=b(BIG), k_pages=b(BIG), v_pages=b(BIG), n_pages=4, n_heads=4,
+                           n_kv_heads=2, head_dim=64, page_tokens=16, n_rot=64, freq_base=1e4)
+
+    def calls(rows, kv, stride=1):
+        yield lambda: cx.rope_qkv_append_batched(d, b(BIG), stride, rows, kv)
+        yield lambda: cx.attn_prefill_batched(b(BIG), b(BIG), b(BIG), b(BIG), 4, b(BIG), stride, rows, kv, None, 0, 4, 2, 64, 16, 0.125)
+        if stride == 1:
+            yield lambda: cx.attn_prefill_batched_workspace(rows, kv, 0, 4, 2, 64)
+
+    i64 = lambda *x: np.array(x, np.int64)
+    for rows, kv in (((0, 2), (9,)), (i64(0, 2), i64(9)), (np.array([0, 2], np.uint32), [9]), ((0,), ()), (i64(0), i64())):
+        for call in calls(rows, kv):
+            call()
+    assert len(names(lib)) == 6
+    for args in ((i64(0, (1 << 32) + 2), i64(9)), (i64(0, 2), i64((1 << 32) + 9)), ((0, 2), (-1,)), (i64(0, 2), i64(-(1 << 32) + 9)), ((0, 2), (9.5,)),
+                 (np.array([[0, 2]]), (9,)), ((), ()), ((0, 2), (9,), -1)):
+        for call in calls(*args):
+            with pytest.raises(BadArgument):
+                call()
+    assert len(names(lib)) == 6
 
 
 def test_rust_descriptor_matches_the_header():
