@@ -4,10 +4,20 @@
 // [max(0, p + 1 - n_swa), p] (n_swa 0: [0, p]) with the head's sink in the denominator; a row at p < 0 sees
 // nothing and is zero.
 //
-// A work-group owns one KV head and a tile of 128 rows, a row being a (token, head of the KV head's group) pair, so
-// K and V are read once for all of a tile's heads; its four waves take 32 rows each. Keys stream through LDS in
-// 32-key tiles, four buffers, copies (LDS DMA, 16 bytes a lane) three tiles ahead, one barrier a tile. A tile whose
-// keys are cut into pieces (few rows, many keys) leaves records that the merge kernel joins.
+// A work-group owns one KV head and a tile of rows, a row being a (token, head of the KV head's group) pair, so K and V
+// are read once for all of a tile's heads. Full tiles have 128 rows, 32 to each of the four waves; keys stream through
+// LDS in 32-key tiles, four buffers, copies (LDS DMA, 16 bytes a lane) three tiles ahead, one barrier a tile. Small
+// tiles have 32 rows, which all waves hold, each with every fourth 32 keys in a buffer of its own, no barriers; the waves'
+// sums meet in LDS at the end. Tiles whose keys are cut into pieces (few rows, many keys) leave records that the merge
+// kernel joins. The host's plan chooses between these (batch_plan, with what each measured).
+//
+// Bounds and what it measured on MI355X (a 1 GiB copy there 5.15 TB/s, an 8192^3 f16 product 1.16 PFLOP/s):
+//   full tiles, 128 channels: power; 512 tokens behind 32,700, 32 heads over 4: 295 us, 937 TFLOP/s, the matrix cores busy for
+//     53% of the time at 1.73 GHz; 4096 tokens from the start 151 us, 910 TFLOP/s
+//   full tiles, 64 channels: the softmax's vector instructions, of which a score has as many beside half the products: four
+//     prompts of 2048, 64 heads over 8: 196 us, 702 TFLOP/s
+//   decode steps beside prompt pieces, 32 sequences: HBM; 46.7 us for 166 MB, 3.6 TB/s, and 5.4 for the merge
+//   few tokens: latency, a trip to the block table, to the keys, and the merge's launch; 18 tokens of four drafts 13.5 us
 //
 // Matrix layout (v_mfma_f32_32x32x16_f16, DB = channels / 32):
 //   S^T[32 keys x 32 rows] = K . Q^T          2 DB MFMAs
