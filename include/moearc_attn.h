@@ -478,8 +478,8 @@ int moearc_attn_prefill_batched_workspace(moearc_ctx *c, const unsigned int *row
 
 /* Attention of every new token over its sequence's keys up to itself (with n_swa the last n_swa of them), whose K and V
  * are in the cache: row i of sequence b is moearc_attn_decode at n_kv = p + 1, p its position. q f16
- * [row][n_heads][head_dim]; out the same, f32 or f16 by out_type; sinks f32 [n_heads] or NULL. A row at a negative position
- * is zero. K and V of keys that a row does not see do not reach it, infinities and NaN among them (a call whose
+ * [row][n_heads][head_dim]; out the same, f32 or f16 by out_type; sinks f32 [n_heads], below +infinity, or NULL. A row at a
+ * negative position is zero. K and V of keys that a row does not see do not reach it, infinities and NaN among them (a call whose
  * accumulators stop being finite runs twice); slots from n_kv[b] on are not read. A row that sees a NaN, or a score that is
  * one or +infinity, is NaN; with a head_dim other than 64, 128 and 256 an infinity in the first eight channels of a key makes
  * one. q . k, and scale times it, have to stay below 10^29. Any group, any page size, head_dim a multiple of 8 up to 256; q, out
