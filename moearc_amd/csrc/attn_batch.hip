@@ -241,7 +241,9 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
     auto k_lanes = [&](uint32_t first) { return lanes_of([](uint32_t k) { return S::fk(k); }, first); };
     const Lanes v_lanes = lanes_of([](uint32_t k) { return S::fv(k); }, 0u);
 
-    // Keys whose places fit `table` at a time (a segment); every thread of the work-group takes part.
+    // Keys whose places fit `table` at a time (a segment); every thread of the work-group takes part. A segment is whole tiles:
+    // masks go by what a row sees, so a tile's columns behind the segment's end would count, and again in the next one.
+    static_assert(MOEARC_AB_PT % 32u == 0u, "a segment of whole tiles");
     const uint32_t seg_keys = eights ? 8u * MOEARC_AB_PT : MOEARC_AB_PT;
     bool again_round = false;
     auto load_places = [&](uint32_t seg, uint32_t last_key) {

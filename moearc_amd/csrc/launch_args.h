@@ -384,7 +384,8 @@ struct QkvAppendArgs {
 //   rec_o[(rec_begin + (tile * pieces + piece) * tr) * n_kv_heads + kvh * tr + row][head_dim]  un-normalised (f32)
 //   rec_ml[the same row index][2]   reference max (log2 domain), row sum in its frame
 #define MOEARC_AB_ROWS 128u       // rows of a tile: 32 to a wave
-#define MOEARC_AB_PT 2044u        // keys' places that a work-group holds at a time (of eight keys each where pages allow)
+#define MOEARC_AB_PT 2016u        // keys' places that a work-group holds at a time (of eight keys each where pages allow): whole
+                                  // tiles of 32, or a segment's last tile would hold keys that the next one adds again
 #define MOEARC_AB_LOG2_PSCALE 7.0f  // weights are 2^7 at the reference max: f16 keeps 21 bits below it
 struct AttnBatchSlot {
     uint32_t item_begin, n_tiles, n_new, n_kv;

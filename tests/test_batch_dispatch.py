@@ -276,3 +276,21 @@ def test_rust_descriptor_matches_the_header():
     rs = open(os.path.join(ROOT, "crates", "moearc-hip", "src", "ffi.rs")).read()
     rs = rs[rs.index("pub struct MoearcQkvAppend {"):]
     assert c_fields == re.findall(r"pub (\w+):", rs[:rs.index("}")]) == [f[0] for f in QkvAppendDesc._fields_]
+
+
+@pytest.mark.parametrize("eights", [False, True])
+def test_a_segments_keys_are_whole_tiles(eights):
+    # the key loops (attn_batch.hip) take 32 keys at a time from a segment's start; copies behind its last key are that one again,
+    # and only what a row does not see is masked: each key must enter once
+    header = open(os.path.join(ROOT, "moearc_amd", "csrc", "launch_args.h")).read()
+    places = int(re.search(r"#define MOEARC_AB_PT (\d+)u", header).group(1))
+    seg_keys = places * (8 if eights else 1)
+    for lo, hi in ((0, 1), (8, 2048), (0, 4100), (16, 33000), (0, seg_keys), (0, seg_keys + 1), (40, 3 * seg_keys + 77)):
+        entered = np.zeros(hi, int)
+        for seg in range(lo, hi, seg_keys):
+            seg_hi = min(hi, seg + seg_keys)
+            for j0 in range(seg, seg_hi, 32):
+                for j in range(j0, j0 + 32):
+                    if j < hi:  # (the last row sees every key below)
+                        entered[min(j, seg_hi - 1)] += 1
+        assert (entered[lo:] == 1).all()
