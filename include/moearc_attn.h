@@ -481,9 +481,8 @@ int moearc_attn_prefill_batched_workspace(moearc_ctx *c, const unsigned int *row
  * [row][n_heads][head_dim]; out the same, f32 or f16 by out_type; sinks f32 [n_heads], below +infinity, or NULL. A row at a
  * negative position is zero. K and V of keys that a row does not see do not reach it, infinities and NaN among them (a call whose
  * accumulators stop being finite runs twice); slots from n_kv[b] on are not read. A row that sees a NaN, or a score that is
- * one or +infinity, is NaN; with a head_dim other than 64, 128 and 256 an infinity in the first eight channels of a key makes
- * one. q . k, and scale times it, have to stay below 10^29. Any group, any page size, head_dim a multiple of 8 up to 256; q, out
- * and the pools 16-byte aligned; kv_type 1 (f16).
+ * one or +infinity, is NaN; a score of -infinity is a weight of 0. Finite q . k, and scale times it, have to stay below 10^29.
+ * Any group, any page size, head_dim a multiple of 8 up to 256; q, out and the pools 16-byte aligned; kv_type 1 (f16).
  * Precision: exact f16 products summed in f32. An f16 out rounds each softmax weight to f16 once, to 2^-11 of it
  * (the output's own rounding is as much, of a sum in which these average out); an f32 out carries it as f16 hi + lo,
  * to 2^-22 of it; either to 2^-32 of the row's largest weight where that is more.

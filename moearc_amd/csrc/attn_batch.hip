@@ -37,7 +37,8 @@
 // averaging); precise ones, for f32 outputs, carry it as f16 hi + lo (2^-22).
 //
 // Infinities and NaN in V of keys that a row does not see must not reach it, but 0 * NaN would in the matrix cores.
-// A work-group that ends with a non-finite accumulator runs once more, with the tiles that cross a mask done key by key.
+// A work-group that ends with a non-finite accumulator runs once more, with the tiles that cross a mask done key by key and
+// without the chunks behind a narrower head's channels.
 #include "common.h"
 
 namespace {
@@ -306,13 +307,19 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) O[mb][i] = 0.f;
     };
-    // S^T of the tile at kt.
-    auto scores = [&](const uint8_t *kt) {
+    // S^T of the tile at kt. Chunks of K behind the head's channels hold its first one again: 0 * inf there is a NaN, which
+    // makes the row's accumulators one, so the second run leaves these chunks out.
+    auto scores = [&](auto by_key_c, const uint8_t *kt) {
         float16_t s;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
-        for (int t = 0; t < 2 * DB; ++t) s = pf_mfma(*(const half8_t *) (kt + (k_at ^ (uint32_t) t << 5)), qop[t], s);
+        for (int t = 0; t < 2 * DB; ++t) {
+            half8_t k = *(const half8_t *) (kt + (k_at ^ (uint32_t) t << 5));
+            if constexpr (decltype(by_key_c)::value)
+                if (16u * t + 8u * h >= D) k = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+            s = pf_mfma(k, qop[t], s);
+        }
         return s;
     };
     auto weights = [&](const float16_t &s, float bias, float l, half8_t (&phi)[2], half8_t (&plo)[2]) {
@@ -462,7 +469,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
             else if (steps > 1u) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(ONE) : "memory");
             else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
-            float16_t s = scores(tiles), next;
+            float16_t s = scores(by_key_c, tiles), next;
             auto open = [&](uint32_t r, uint32_t buf) {  // of tile r + 3
                 if (r + 2u < steps) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(ONE) : "memory");
                 else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
@@ -475,7 +482,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
             for (uint32_t r = 0; r < steps; ++r) {
                 open(r, (r + NBUF - 1u) % NBUF);
                 if (crosses(first_key(r))) mask(s, first_key(r));
-                next = scores(tiles + (r + 1u) % NBUF * S::BUF);  // beside the weights of this one
+                next = scores(by_key_c, tiles + (r + 1u) % NBUF * S::BUF);  // beside the weights of this one
                 absorb(by_key_c, s, first_key(r), tiles + r % NBUF * S::BUF, [] {});
                 s = next;
             }
@@ -515,7 +522,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
             for (; j0 < seg_hi; j0 += 128u) {
                 const bool more = j0 + 128u < seg_hi;
                 asm volatile("s_waitcnt vmcnt(%0)" : : "n"(4 * COPIES) : "memory");  // V's may be in flight
-                float16_t s = scores(own);
+                float16_t s = scores(by_key_c, own);
                 asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // K has been read
                 if (more) copy_k(j0 + 128u);
                 if (crosses(j0)) mask(s, j0);
