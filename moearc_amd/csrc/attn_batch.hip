@@ -148,6 +148,9 @@ __device__ __forceinline__ AbSpan ab_span(const AttnBatchArgs &a, uint32_t n, ui
     return s;
 }
 
+// A head's sink in the log2 domain. Above 2.3e38 the product overflows, and inf - inf would make NaN of a row that is zero.
+__device__ __forceinline__ float ab_sink(float sink) { return fminf(sink * MOEARC_LOG2E, 3.0e38f); }
+
 // A wave-uniform value that is there from here on: arguments are loaded together at a kernel's start, where the compiler
 // would put each in front of its first use, a chain of waits.
 #define AB_HERE(x) asm volatile("" : "+s"(x))
@@ -278,7 +281,7 @@ __device__ __forceinline__ void ab_body(const AttnBatchArgs &a) {
         asm volatile("" : "+v"(qop[t]));
     }
     c = c == 0.f ? 1.f : fabsf(c);
-    sink2 *= MOEARC_LOG2E;
+    sink2 = ab_sink(sink2);
 
     // Copies of eight keys: with pages of eights these share a page, and their base is wave-uniform; otherwise a lane looks
     // for its own key. Keys behind the last are that one: their scores are masked, and no slot is read that the cache has
@@ -642,7 +645,7 @@ __device__ __forceinline__ void ab_merge_body(const AttnBatchArgs &a) {
     const uint64_t rec0 = ((uint64_t) sl.rec_begin + tile * pieces * tile_rows) * G + kvh * tile_rows + r;
     const uint64_t step = (uint64_t) G * tile_rows;  // records from piece to piece
     const uint32_t tok = ab_token(a, row), hd = kvh * a.group + row - tok * a.group;
-    const float sink2 = a.sinks ? a.sinks[hd] * MOEARC_LOG2E : -INFINITY;
+    const float sink2 = a.sinks ? ab_sink(a.sinks[hd]) : -INFINITY;
     float top = fmaxf(sink2, PF_M_INIT), total = __builtin_amdgcn_exp2f(sink2 - top + MOEARC_AB_LOG2_PSCALE);
     float4_t o = {0.f, 0.f, 0.f, 0.f};
     for (uint32_t k0 = 0; k0 < np; k0 += 8u) {  // eight records' loads at a time

@@ -63,3 +63,20 @@ def test_a_score_of_plus_infinity_or_nan(cx, dim, page, form, bad):
         lo, hi = int(s.rows[b]), int(s.rows[b + 1])
         assert np.isnan(got[hi - 2:hi]).all()
         assert (np.abs(got - want) <= tol)[lo:hi - 2].all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_sinks_at_the_ends_of_f32(cx, dim, form):
+    # the lowest ones are none, the highest leave nothing of a row
+    s = Batch(*FORMS[form], dim, 16, dim + 2)
+    top = float(np.finfo(np.float32).max)
+    s.sinks[:7] = top, 2.4e38, 1e38, 1e6, -top, -2.4e38, -1e38
+    want, _ = s.expected(0, dim ** -0.5, OUT_F32)
+    assert (want[:, :4] == 0).all()
+    # (the bound of these heads without a sink: the formula's for an error of the weights has the sink's size in it)
+    bare = copy.copy(s)
+    bare.sinks = np.where(np.abs(s.sinks) > 1e5, -np.inf, s.sinks)
+    _, tol = bare.expected(0, dim ** -0.5, OUT_F32)
+    got = run(cx, s, out_type=OUT_F32).astype(np.float64)
+    assert np.isfinite(got).all() and (got[:, :4] == 0).all() and (np.abs(got - want) <= tol)[:, 4:].all()
