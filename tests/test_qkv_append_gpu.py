@@ -201,3 +201,68 @@ def test_many_sequences(cx):
 def test_a_page_outside_the_pool(cx, dim):
     check(cx, [3, 20], [40, 50], 4, 2, dim, 16, bad=(1, 2))
     check(cx, [3, 20], [40, 50], 4, 2, dim, 16)  # reported once
+
+
+# ---- long batches: three heads to a thread (more than eight work-groups to each of 256 CUs with one) ------------------
+LONG_NEW, LONG_CACHED = [200, 0, 333, 1, 170], [0, 9, 31, 4000, 260]
+LONG_KV = np.add(LONG_NEW, LONG_CACHED).tolist()
+# 256 / lanes heads to a work-group, times three: one with room to spare, and a second with few; threads whose three heads
+# are of q, k and v
+LONG_SHAPES = [(64, 8, 64, 64), (100, 9, 64, 32), (30, 33, 40, 40), (32, 4, 128, 128), (50, 7, 96, 48), (47, 1, 80, 80), (16, 2, 256, 256),
+               (21, 3, 136, 64), (2, 11, 200, 200)]
+
+
+def takes_three(heads, kv_heads, dim, rows):
+    at_a_time = 32 if dim <= 64 else 16 if dim <= 128 else 8
+    return -(-(heads + 2 * kv_heads) // at_a_time) * rows > 8 * 256
+
+
+@pytest.mark.parametrize("kind", list(RopeKind), ids=str)
+@pytest.mark.parametrize("heads,kv_heads,dim,n_rot", LONG_SHAPES, ids=str)
+def test_long_batches(cx, heads, kv_heads, dim, n_rot, kind):
+    new = np.array(LONG_NEW)
+    while not takes_three(heads, kv_heads, dim, new.sum()):
+        new = new * 2
+    kv = np.add(new, LONG_CACHED).tolist()
+    check(cx, new, kv, heads, kv_heads, dim, 16, n_rot, kind=kind, norm=True, q_type=OUT_F32, kv=KvType.F32)
+    check(cx, new, kv, heads, kv_heads, dim, 100, n_rot, kind=kind, in_type=OUT_F16, fused=8, seed=1)
+
+
+@pytest.mark.parametrize("in_type", [OUT_F32, OUT_F16], ids=["f32", "f16"])
+@pytest.mark.parametrize("q_type", [OUT_F32, OUT_F16], ids=["f32", "f16"])
+@pytest.mark.parametrize("kv", list(KvType), ids=str)
+def test_long_batches_types(cx, in_type, q_type, kv):
+    assert takes_three(80, 10, 64, sum(LONG_NEW))
+    check(cx, LONG_NEW, LONG_KV, 80, 10, 64, 16, in_type=in_type, q_type=q_type, kv=kv, norm=True, factors=True, scaling=YARN)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(64, 16, 64), (32, 8, 128), (17, 4, 256)], ids=str)
+def test_long_batches_of_few_positions_and_bad_pages(cx, heads, kv_heads, dim):
+    assert takes_three(heads, kv_heads, dim, 704)
+    check(cx, [300, 404], [0, 150], heads, kv_heads, dim, 16)  # most rows sit before the first position
+    check(cx, [300, 404], [400, 404], heads, kv_heads, dim, 16, bad=(1, 2), norm=True)
+
+
+def test_a_long_batch_in_place(cx):
+    check(cx, LONG_NEW, LONG_KV, 32, 8, 128, 16, norm=True, q_type=OUT_F32, in_place=True)
+
+
+@pytest.mark.parametrize("rows", [40, 704], ids=["one", "three"])
+@pytest.mark.parametrize("normed", ["q", "k"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(50, 30, 64), (31, 5, 128), (13, 7, 256)], ids=str)
+def test_a_norm_of_one_kind(cx, heads, kv_heads, dim, normed, rows):
+    # a wave's heads are of q, k and v, and only one kind's are normed
+    rng = np.random.default_rng(17)
+    assert takes_three(heads, kv_heads, dim, rows) == (rows == 704)
+    x = [rng.standard_normal((rows, n, dim)).astype(np.float32) for n in (heads, kv_heads, kv_heads)]
+    w = (1 + 0.3 * rng.standard_normal(dim)).astype(np.float32)
+    q_out, pools = cx.alloc(rows * heads * dim * 4), [cx.alloc(rows * kv_heads * dim * 4) for _ in range(2)]
+    d = QkvAppendDesc.make(*(cx.upload(a) for a in x), q_out, *pools, 1, heads, kv_heads, dim, rows, dim, 1e4, q_type=OUT_F32, kv=KvType.F32,
+                           **{normed + "_norm": cx.upload(w)})
+    cx.rope_qkv_append_batched(d, cx.upload(np.zeros(1, np.uint32)), 1, [0, rows], [rows])
+    cx.sync()
+    for a, kind, buf in ((x[0], "q", q_out), (x[1], "k", pools[0])):
+        want, tol = rotated(a.astype(np.float64), np.arange(rows), dim, 1e4, RopeScaling.NONE, RopeKind.NEOX, w if kind == normed else None, 1e-6, None)
+        got = cx.download(buf, np.float32, a.shape).astype(np.float64)
+        assert (np.abs(got - want) <= 1.01 * (tol + step(want, False))).all()
+    assert np.array_equal(cx.download(pools[1], np.float32, x[2].shape), x[2])
