@@ -10,9 +10,9 @@
 // quads that rotate into each other, so a head's norm is a sum over neighbouring lanes and every access is 16
 // bytes a lane (8 of f16). Work-groups are (token, group of 256 / LPH heads of q, k and v), or of three times as many
 // heads where there are more of these than the device holds at once: a work-group's life is mostly latency.
-// Measured on MI355X: a token of 80 heads of 64 takes 3.6 us, as long as any launch of one work-group does, 48 tokens of 40
-// normed heads of 128 4.1; 2048 tokens of one product's rows, f32 in and f16 out, 11.5 for 63 MB (5.5 TB/s, part of it from the
-// last-level cache); 3709 tokens with f16 rows and an f32 cache 27.1 for 106 MB (3.9 TB/s: an f16 quad is 8 bytes a load).
+// Measured on MI355X: a token of 80 heads of 64 takes 3.7 us, as long as any launch of one work-group does, 48 tokens of 40
+// normed heads of 128 4.2; 2048 tokens of one product's rows, f32 in and f16 out, 11.8 for 63 MB (5.3 TB/s, part of it from the
+// last-level cache); 3709 tokens with f16 rows and an f32 cache 27.2 for 106 MB (3.9 TB/s: an f16 quad is 8 bytes a load).
 #include "common.h"
 
 #define AP_MAX_PAIRS 128  // head_dim <= 256

@@ -11,13 +11,17 @@
 // sums meet in LDS at the end. Tiles whose keys are cut into pieces (few rows, many keys) leave records that the merge
 // kernel joins. The host's plan chooses between these (batch_plan, with what each measured).
 //
-// Bounds and what it measured on MI355X (a 1 GiB copy there 5.15 TB/s, an 8192^3 f16 product 1.16 PFLOP/s):
-//   full tiles, 128 channels: power; 512 tokens behind 32,700, 32 heads over 4: 295 us, 937 TFLOP/s, the matrix cores busy for
-//     53% of the time at 1.73 GHz; 4096 tokens from the start 151 us, 910 TFLOP/s
+// Bounds and what whole calls measured on MI355X, in a long run of them (a 1 GiB copy there 5.12 TB/s, an 8192^3 f16 product
+// 1.16 PFLOP/s):
+//   full tiles, 128 channels: power; 512 tokens behind 32,700, 32 heads over 4: 299 us, 924 TFLOP/s, the matrix cores busy for
+//     53% of the time at 1.73 GHz; 4096 tokens from the start 155 us, 886 TFLOP/s. Pages of no multiple of eight tokens: 361 and
+//     187, since each lane's copy takes an address of its own instead of a wave's base
 //   full tiles, 64 channels: the softmax's vector instructions, of which a score has as many beside half the products: four
-//     prompts of 2048, 64 heads over 8: 196 us, 702 TFLOP/s
-//   decode steps beside prompt pieces, 32 sequences: HBM; 46.7 us for 166 MB, 3.6 TB/s, and 5.4 for the merge
-//   few tokens: latency, a trip to the block table, to the keys, and the merge's launch; 18 tokens of four drafts 13.5 us
+//     prompts of 2048, 64 heads over 8: 198 us, 696 TFLOP/s
+//   full tiles, 256 channels: one work-group a CU, so nobody's products run beside a wave's softmax; 512 tokens behind 16,000,
+//     16 heads over 2: 217 us, 627 TFLOP/s; 4096 from the start 240 us, 573 TFLOP/s
+//   decode steps beside prompt pieces, 32 sequences: HBM; 46.6 us for 166 MB, 3.6 TB/s, and 5.5 for the merge
+//   few tokens: latency, a trip to the block table, to the keys, and the merge's launch; 18 tokens of four drafts 13.7 us
 //
 // Matrix layout (v_mfma_f32_32x32x16_f16, DB = channels / 32):
 //   S^T[32 keys x 32 rows] = K . Q^T          2 DB MFMAs

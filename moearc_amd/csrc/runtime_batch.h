@@ -98,6 +98,11 @@ unsigned long batch_take(BatchPlan &p, const unsigned int *row_begin, const unsi
 // four sequences of 16 tokens behind 1500 20.2 and 16.8, of 32 tokens 21.0 and 19.5; 32 such sequences 45.4 and 47.4, 49.6 and 77.3; 64
 // behind 100, 13.9 and 23.5; one of 200 behind 800 23.1 and 16.7. 32 heads over 4 of 128, one of 300 15.8 and 13.2, of 500 behind
 // 2000 44.6 and 40.5, of 100 behind 16,000 48.9 and 53.2, of 512 behind 32,700 304 and 390, two of 128 behind 4000 37.8 and 41.2.
+// The limit of 2560 keys, 32 heads over 4 of 128, one sequence of 200, 300 and 500 tokens: behind 1000 27.6 and 24.7, 28.6 and 23.6, 38.2 and 26.5; behind
+// 3000 33.5 and 34.7, 37.4 and 40.8, 50.3 and 49.5; behind 6000 45.8 and 47.4, 52.4 and 68.2, 75.0 and 82.1. Other heads put the
+// border elsewhere, 8 over 1 of 128 at 6000 and 16 over 2 of 256 at 2000 for 300 tokens. 33 to 64 rows, one half-empty full tile or
+// two small ones: 64 heads over 8 of 64, 5 to 8 tokens behind 2000, 8 sequences 18 and 18 to 22, 32 40 and 32, 64 66 and 73;
+// 32 behind 8000 124 and 137; 32 over 4 of 128, up to 32 sequences the same to 4%, 64 behind 2000 74 and 85.
 // Pieces: where a tile's keys would keep one work-group longer than the whole work keeps the device; with fewer, all
 // work-groups run at once and the longest decides. Work is counted in 32-key chunks of a small tile, whose work-group takes four
 // at a time; a full tile's takes one. A piece has at least four of these steps, a full tile's sixteen: drafts of 3 to 7 tokens behind
